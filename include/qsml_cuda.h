@@ -361,6 +361,22 @@ QSML_API qsml_status_t qsml_softmax(qsml_ctx* ctx, const qsml_tdesc* x, int32_t 
 QSML_API qsml_status_t qsml_layer_norm(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* gamma,
                                        const qsml_tdesc* beta, float eps, const qsml_tdesc* y);
 
+/* Gradients of qsml_layer_norm.  From x, gamma, eps as given to it and dy, the
+ * gradient of its y (x's shape and dtype):
+ *   dx = rstd * (h - mean(h) - xh * mean(h * xh)),  h = dy * gamma,
+ *        xh = (x - mean(x)) * rstd, the means along the last dim;
+ *   dgamma = sum over rows of dy * xh;  dbeta = sum over rows of dy.
+ * mean and rstd are computed again from x, so the forward pass keeps nothing.
+ * dx has x's shape and dtype, dgamma and dbeta [last dim] in F32 or x's dtype;
+ * each may be NULL when it is not wanted.  Binary32 arithmetic, each output
+ * rounded once; the sums over rows run in an order fixed by the shape, so
+ * results are run-to-run deterministic.  With no rows dgamma and dbeta are 0.
+ * Outputs may not overlap an input or each other (QSML_E_INVALID).  No
+ * reference counterpart (it has neither layer norm nor gradients). */
+QSML_API qsml_status_t qsml_layer_norm_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* gamma,
+                                                const qsml_tdesc* dy, float eps, const qsml_tdesc* dx,
+                                                const qsml_tdesc* dgamma, const qsml_tdesc* dbeta);
+
 /* C = A * B for rank-2 A[M,K], B[K,N] -> C[M,N], or batched rank-3
  * A[b,M,K], B[b,K,N] -> C[b,M,N] (batch strides may be 0).  A and B must have
  * unit stride in their last dim.  F32 inputs give F32 C; F16 inputs give

@@ -143,6 +143,8 @@ _SIGS = {
     "qsml_cast": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc)]),
     "qsml_softmax": (_c.c_int32, [_c.c_void_p, _P(TDesc), _c.c_int32, _P(TDesc)]),
     "qsml_layer_norm": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_float, _P(TDesc)]),
+    "qsml_layer_norm_backward": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_float, _P(TDesc),
+                                              _P(TDesc), _P(TDesc)]),
     "qsml_matmul": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_int32]),
     "qsml_reduce_noalloc": (_c.c_int32, [_c.c_void_p, _c.c_int32, _P(TDesc), _c.c_int32, _c.c_int32, _P(TDesc)]),
     "qsml_allreduce_partials": (_c.c_int32, [_c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int64]),
@@ -299,6 +301,11 @@ def torch_dtype_code(dt) -> int:
 def desc_of(t) -> TDesc:
     """Descriptor of a torch CUDA tensor (any strides; storage offset applied)."""
     return make_desc(t.data_ptr(), torch_dtype_code(t.dtype), tuple(t.shape), tuple(t.stride()))
+
+
+def _opt(d: Optional[TDesc]):
+    """An optional descriptor argument: None is NULL."""
+    return None if d is None else ctypes.byref(d)
 
 
 class Context:
@@ -461,6 +468,12 @@ class Context:
     def layer_norm(self, x: TDesc, g: TDesc, b: TDesc, eps: float, y: TDesc) -> None:
         self.check(self.lib.qsml_layer_norm(self.h, ctypes.byref(x), ctypes.byref(g), ctypes.byref(b),
                                             ctypes.c_float(eps), ctypes.byref(y)))
+
+    def layer_norm_backward(self, x: TDesc, g: TDesc, dy: TDesc, eps: float, dx: Optional[TDesc],
+                            dg: Optional[TDesc] = None, db: Optional[TDesc] = None) -> None:
+        """Gradients of layer_norm for x, gamma and beta (None: not wanted)."""
+        self.check(self.lib.qsml_layer_norm_backward(self.h, ctypes.byref(x), ctypes.byref(g), ctypes.byref(dy),
+                                                     ctypes.c_float(eps), _opt(dx), _opt(dg), _opt(db)))
 
     def matmul(self, a: TDesc, b: TDesc, c: TDesc, precision: int = MM_AUTO) -> None:
         self.check(self.lib.qsml_matmul(self.h, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c), precision))
