@@ -386,6 +386,70 @@ QSML_API qsml_status_t qsml_layer_norm_backward(qsml_ctx* ctx, const qsml_tdesc*
 QSML_API qsml_status_t qsml_matmul(qsml_ctx* ctx, const qsml_tdesc* a, const qsml_tdesc* b,
                                    const qsml_tdesc* c, int32_t precision);
 
+/* ---- linear layers ------------------------------------------------------ */
+
+/* Activations of the linear layers.  GELU is QSML_UN_GELU's tanh form;
+ * SILU(z) = z * sigmoid(z). */
+#define QSML_ACT_NONE 0
+#define QSML_ACT_RELU 1
+#define QSML_ACT_GELU 2
+#define QSML_ACT_SILU 3
+#define QSML_ACT_SIGMOID 4
+
+/* A linear layer in one kernel:  z = x w + bias,  y = act(z) + residual.
+ * x [.., K] (leading dims fold into rows of one stride; any stride in the last
+ * dim), w [K, N] with any strides (a transposed view of [N, K] is read in
+ * place), y [.., N].  bias [N] (F32 or x's dtype), residual [.., N] and pre
+ * [.., N] may be NULL; pre takes z for qsml_linear_backward.  x, w, residual,
+ * pre and y share one dtype, F32 or F16; y and pre are contiguous; residual has
+ * unit stride in its last dim and may be y itself (added in place).  Any other
+ * overlap of an output with an input or output returns QSML_E_INVALID.
+ * Products are summed in binary32 and everything after them is binary32,
+ * rounded once per output.  precision: QSML_MM_AUTO, or QSML_MM_FP16_F32ACC for
+ * F16 and QSML_MM_FP32_FFMA for F32 (CUDA-core fma, k ascending).
+ * With no rows nothing is written; with K = 0 the products are 0.
+ * Replaces a matmul followed by an add, an activation and an add
+ * (QuasarML/src/Ops/LinAlg.cpp:221-271, Ops/Elementwise.cpp:139-417), each a
+ * dispatch over the whole result. */
+QSML_API qsml_status_t qsml_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, const qsml_tdesc* bias,
+                                   int32_t act, const qsml_tdesc* residual, const qsml_tdesc* pre,
+                                   const qsml_tdesc* y, int32_t precision);
+
+/* Gradients of qsml_linear from dy, the gradient of its y:
+ *   dz = dy * act'(pre);  dx = dz w^T;  dw = x^T dz;  dbias = sum over rows of dz
+ * (the residual's gradient is dy itself).  pre is what the forward pass kept;
+ * with QSML_ACT_NONE it is not read and may be NULL.  dy has unit stride in its
+ * last dim and rows of one stride; dx [.., K] and dw [K, N] are contiguous, in
+ * x's dtype; dbias [N] in F32 or x's dtype; each may be NULL when it is not
+ * wanted.  dz is kept in x's dtype between its computation and the products
+ * (rounded once more: the products' operands are of that dtype), dbias is
+ * summed before that rounding.  With no rows dw and dbias are 0.  relu' is 0 at
+ * 0.  No reference counterpart (it has no gradients). */
+QSML_API qsml_status_t qsml_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,
+                                            const qsml_tdesc* pre, const qsml_tdesc* dy, const qsml_tdesc* dx,
+                                            const qsml_tdesc* dw, const qsml_tdesc* dbias, int32_t precision);
+
+/* A gated linear layer in one kernel, the two products sharing their reads of x:
+ *   g = x w_gate + b_gate,  u = x w_up + b_up,  y = act(g) * u.
+ * Arguments as in qsml_linear, w_gate and w_up both [K, N]; the biases (of one
+ * dtype) and gate, up (which take g and u for the backward pass) may each be
+ * NULL. */
+QSML_API qsml_status_t qsml_gated_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w_gate,
+                                         const qsml_tdesc* w_up, const qsml_tdesc* b_gate, const qsml_tdesc* b_up,
+                                         int32_t act, const qsml_tdesc* gate, const qsml_tdesc* up,
+                                         const qsml_tdesc* y, int32_t precision);
+
+/* Gradients of qsml_gated_linear from dy and the gate and up it kept:
+ *   dg = dy * u * act'(g);  du = dy * act(g);  dx = dg w_gate^T + du w_up^T;
+ *   dw_gate = x^T dg;  dw_up = x^T du;  db_gate, db_up: sums over rows.
+ * Arguments as in qsml_linear_backward. */
+QSML_API qsml_status_t qsml_gated_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w_gate,
+                                                  const qsml_tdesc* w_up, int32_t act, const qsml_tdesc* gate,
+                                                  const qsml_tdesc* up, const qsml_tdesc* dy, const qsml_tdesc* dx,
+                                                  const qsml_tdesc* dw_gate, const qsml_tdesc* dw_up,
+                                                  const qsml_tdesc* db_gate, const qsml_tdesc* db_up,
+                                                  int32_t precision);
+
 /* ---- Multi-GPU groups (NCCL) ------------------------------------------------
  * The reference is single-GPU; sharded execution combines per-GPU partial
  * results with an in-place all-reduce.  Two ways to form a group:

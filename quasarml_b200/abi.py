@@ -29,6 +29,7 @@ OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_POW = range(5)
 RED_SUM, RED_MEAN, RED_MAX, RED_MIN, RED_PROD = range(5)
 AXIS_ALL = -1000
 ARG_MAX, ARG_MIN = 0, 1
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU, ACT_SIGMOID = range(5)
 MM_AUTO, MM_FP32_FFMA, MM_FP32_3XTF32, MM_FP16_F32ACC = range(4)
 
 DTYPE_SIZE = {F32: 4, F16: 2, I32: 4, I16: 2, I8: 1, U32: 4, U16: 2, U8: 1}
@@ -146,6 +147,14 @@ _SIGS = {
     "qsml_layer_norm_backward": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_float, _P(TDesc),
                                               _P(TDesc), _P(TDesc)]),
     "qsml_matmul": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_int32]),
+    "qsml_linear": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _P(TDesc), _c.c_int32] + [_P(TDesc)] * 3
+                    + [_c.c_int32]),
+    "qsml_linear_backward": (_c.c_int32, [_c.c_void_p, _P(TDesc), _P(TDesc), _c.c_int32] + [_P(TDesc)] * 5
+                             + [_c.c_int32]),
+    "qsml_gated_linear": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 5 + [_c.c_int32] + [_P(TDesc)] * 3
+                          + [_c.c_int32]),
+    "qsml_gated_linear_backward": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 3 + [_c.c_int32] + [_P(TDesc)] * 8
+                                   + [_c.c_int32]),
     "qsml_reduce_noalloc": (_c.c_int32, [_c.c_void_p, _c.c_int32, _P(TDesc), _c.c_int32, _c.c_int32, _P(TDesc)]),
     "qsml_allreduce_partials": (_c.c_int32, [_c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int64]),
     "qsml_finish_partial": (_c.c_int32, [_c.c_void_p, _c.c_int32, _P(TDesc), _c.c_int64, _P(TDesc)]),
@@ -477,6 +486,36 @@ class Context:
 
     def matmul(self, a: TDesc, b: TDesc, c: TDesc, precision: int = MM_AUTO) -> None:
         self.check(self.lib.qsml_matmul(self.h, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c), precision))
+
+    def linear(self, x: TDesc, w: TDesc, bias: Optional[TDesc], act: int, residual: Optional[TDesc],
+               pre: Optional[TDesc], y: TDesc, precision: int = MM_AUTO) -> None:
+        """y = act(x w + bias) + residual; pre takes x w + bias (None: absent)."""
+        self.check(self.lib.qsml_linear(self.h, ctypes.byref(x), ctypes.byref(w), _opt(bias), int(act),
+                                        _opt(residual), _opt(pre), ctypes.byref(y), precision))
+
+    def linear_backward(self, x: TDesc, w: TDesc, act: int, pre: Optional[TDesc], dy: TDesc, dx: Optional[TDesc],
+                        dw: Optional[TDesc], dbias: Optional[TDesc] = None, precision: int = MM_AUTO) -> None:
+        """Gradients of linear for x, w and bias (None: not wanted)."""
+        self.check(self.lib.qsml_linear_backward(self.h, ctypes.byref(x), ctypes.byref(w), int(act), _opt(pre),
+                                                 ctypes.byref(dy), _opt(dx), _opt(dw), _opt(dbias), precision))
+
+    def gated_linear(self, x: TDesc, w_gate: TDesc, w_up: TDesc, b_gate: Optional[TDesc], b_up: Optional[TDesc],
+                     act: int, gate: Optional[TDesc], up: Optional[TDesc], y: TDesc,
+                     precision: int = MM_AUTO) -> None:
+        """y = act(x w_gate + b_gate) * (x w_up + b_up); gate and up take the two products."""
+        self.check(self.lib.qsml_gated_linear(self.h, ctypes.byref(x), ctypes.byref(w_gate), ctypes.byref(w_up),
+                                              _opt(b_gate), _opt(b_up), int(act), _opt(gate), _opt(up),
+                                              ctypes.byref(y), precision))
+
+    def gated_linear_backward(self, x: TDesc, w_gate: TDesc, w_up: TDesc, act: int, gate: TDesc, up: TDesc,
+                              dy: TDesc, dx: Optional[TDesc], dw_gate: Optional[TDesc], dw_up: Optional[TDesc],
+                              db_gate: Optional[TDesc] = None, db_up: Optional[TDesc] = None,
+                              precision: int = MM_AUTO) -> None:
+        """Gradients of gated_linear (None: not wanted)."""
+        self.check(self.lib.qsml_gated_linear_backward(
+            self.h, ctypes.byref(x), ctypes.byref(w_gate), ctypes.byref(w_up), int(act), ctypes.byref(gate),
+            ctypes.byref(up), ctypes.byref(dy), _opt(dx), _opt(dw_gate), _opt(dw_up), _opt(db_gate), _opt(db_up),
+            precision))
 
 
 def broadcast_shape(a: Iterable[int], b: Iterable[int]) -> tuple:

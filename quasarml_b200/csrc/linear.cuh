@@ -1,0 +1,214 @@
+// What the kernels of the linear layers share: the problem they are given and
+// the arithmetic behind the products (bias, activation, residual).
+//
+//   out = sum over segments s of A_s B_s          (LINEAR)
+//   (g, u) = (A B_0, A B_1)                        (DUAL: two products of one A)
+// LINEAR:  z = out + bias;  pre = z;  y = act(z) + residual
+// DUAL:    g += bias_0, u += bias_1;  pre_0 = g, pre_1 = u;  y = act(g) u
+// where every output that is null is left out.  All of it is binary32, each
+// output rounded once.
+#pragma once
+
+#include "workspace.cuh"
+
+namespace qsml {
+namespace linear {
+
+// A matrix as given: element (r, c) at p + r * rs + c * cs (elements).
+struct Mat {
+    const void* p = nullptr;
+    int64_t rows = 0, cols = 0, rs = 0, cs = 0;
+    Mat t() const { return Mat{p, cols, rows, cs, rs}; }
+};
+
+struct Epilogue {
+    const void* bias[2] = {nullptr, nullptr};
+    int bias_f32 = 1;              // else the dtype of the outputs
+    int act = QSML_ACT_NONE;
+    const void* residual = nullptr;
+    int64_t res_ld = 0;            // elements between residual rows
+    void* pre[2] = {nullptr, nullptr};
+    void* y = nullptr;             // y and pre: rows of N elements
+    int64_t N = 0;
+    int vec = 0;                   // groups of 8 columns are whole and 16-byte aligned everywhere
+};
+
+struct Problem {
+    int64_t M = 0, N = 0, K = 0;
+    int segments = 1;              // 2: a[0] b[0] + a[1] b[1]
+    bool dual = false;             // a[0] b[0] and a[0] b[1]
+    Mat a[2], b[2];
+    Epilogue e;
+};
+
+// CUDA-core products, binary32 fma with k ascending: any strides, any size.
+template <typename T> qsml_status_t run_simt(Context* ctx, const Problem& p);
+
+// ---- arithmetic shared by host-independent code --------------------------------
+__device__ __forceinline__ float ld1(const float* p) { return *p; }
+__device__ __forceinline__ float ld1(const __half* p) { return __half2float(*p); }
+
+// exp for the activations: binary16 results take the fast one (2 ulp and
+// 2^-24 |x|, far below half a step of binary16), binary32 ones expf.
+template <typename T> __device__ __forceinline__ float act_exp(float x) {
+    if constexpr (sizeof(T) == 2) return __expf(x);
+    else return expf(x);
+}
+// 1 / (1 + exp(-z)); 0 where exp(-z) overflows
+template <typename T> __device__ __forceinline__ float act_sigmoid(float z) {
+    const float d = __fadd_rn(1.0f, act_exp<T>(-z));
+    if constexpr (sizeof(T) == 2) return __fdividef(1.0f, d);
+    else return __frcp_rn(d);
+}
+
+constexpr float kGeluS = 0.7978845608f, kGeluC = 0.044715f;  // the constants of QSML_UN_GELU
+
+// act(z).  gelu: 0.5 z (1 + tanh v) = z sigmoid(2 v), v = s (z + c z^3).
+template <typename T> __device__ __forceinline__ float act_value(int act, float z) {
+    switch (act) {
+        case QSML_ACT_RELU: return z != z ? z : (z > 0.0f ? z : 0.0f);
+        case QSML_ACT_GELU: {
+            const float q = __fmul_rn(z, z);
+            const float v2 = __fmul_rn(__fmul_rn(2.0f * kGeluS, z), __fmaf_rn(kGeluC, q, 1.0f));
+            return __fmul_rn(z, act_sigmoid<T>(v2));
+        }
+        case QSML_ACT_SILU: return __fmul_rn(z, act_sigmoid<T>(z));
+        case QSML_ACT_SIGMOID: return act_sigmoid<T>(z);
+    }
+    return z;
+}
+
+// act(z) and its derivative.  With p the sigmoid:
+//   silu' = p + z p (1 - p);  sigmoid' = p (1 - p);
+//   gelu' = p + z p (1 - p) 2 v',  2 v' = 2 s (1 + 3 c z^2).
+template <typename T> __device__ __forceinline__ float act_grad(int act, float z, float& value) {
+    switch (act) {
+        case QSML_ACT_RELU:
+            value = z != z ? z : (z > 0.0f ? z : 0.0f);
+            return z != z ? z : (z > 0.0f ? 1.0f : 0.0f);
+        case QSML_ACT_GELU: {
+            const float q = __fmul_rn(z, z);
+            const float v2 = __fmul_rn(__fmul_rn(2.0f * kGeluS, z), __fmaf_rn(kGeluC, q, 1.0f));
+            const float p = act_sigmoid<T>(v2);
+            value = __fmul_rn(z, p);
+            const float dv = __fmul_rn(2.0f * kGeluS, __fmaf_rn(3.0f * kGeluC, q, 1.0f));
+            return __fmaf_rn(__fmul_rn(value, __fsub_rn(1.0f, p)), dv, p);
+        }
+        case QSML_ACT_SILU: {
+            const float p = act_sigmoid<T>(z);
+            value = __fmul_rn(z, p);
+            return __fmaf_rn(value, __fsub_rn(1.0f, p), p);
+        }
+        case QSML_ACT_SIGMOID: {
+            const float p = act_sigmoid<T>(z);
+            value = p;
+            return __fmul_rn(p, __fsub_rn(1.0f, p));
+        }
+    }
+    value = z;
+    return 1.0f;
+}
+
+// 8 consecutive elements of a row to binary32 and back; n of them are inside
+// (vec: all 8, 16-byte aligned).
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(h[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        } else {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? ld1(p + i) : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec) {
+            uint4 u;
+            __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<uint4*>(p) = u;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = __float2half_rn(v[i]);
+    } else {
+        if (vec) {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = v[i];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void add_bias8(const Epilogue& e, int which, int64_t col, int n, float (&z)[8]) {
+    if (!e.bias[which]) return;
+    float b[8];
+    if (e.bias_f32) load8(static_cast<const float*>(e.bias[which]) + col, n, e.vec, b);
+    else load8(static_cast<const T*>(e.bias[which]) + col, n, e.vec, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = __fadd_rn(z[i], b[i]);
+}
+
+// Columns col .. col + 7 of `row` from their products (u: DUAL only) to the
+// outputs.  col is a multiple of 8; columns from N on are not written.
+template <typename T, bool DUAL>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t col, float (&z)[8], float (&u)[8]) {
+    const int n = e.N - col < 8 ? static_cast<int>(e.N - col) : 8;
+    const int64_t at = row * e.N + col;
+    add_bias8<T>(e, 0, col, n, z);
+    if constexpr (DUAL) add_bias8<T>(e, 1, col, n, u);
+    if (e.pre[0]) store8(static_cast<T*>(e.pre[0]) + at, n, e.vec, z);
+    if constexpr (DUAL) {
+        if (e.pre[1]) store8(static_cast<T*>(e.pre[1]) + at, n, e.vec, u);
+    }
+    if (!e.y) return;
+    switch (e.act) {  // one branch for the eight
+        case QSML_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_RELU, z[i]);
+            break;
+        case QSML_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_GELU, z[i]);
+            break;
+        case QSML_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_SILU, z[i]);
+            break;
+        case QSML_ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_SIGMOID, z[i]);
+            break;
+    }
+    if constexpr (DUAL) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = __fmul_rn(z[i], u[i]);
+    } else if (e.residual) {
+        float r[8];
+        load8(static_cast<const T*>(e.residual) + row * e.res_ld + col, n, e.vec, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = __fadd_rn(z[i], r[i]);
+    }
+    store8(static_cast<T*>(e.y) + at, n, e.vec, z);
+}
+
+}  // namespace linear
+}  // namespace qsml

@@ -1,0 +1,113 @@
+// Gradients of the linear layers with respect to their products, and the
+// biases' gradients: one pass over dy and what the forward pass kept.
+//   LINEAR: dz = dy act'(pre)            db = column sums of dz
+//   DUAL:   dg = dy u act'(g), du = dy act(g), and the column sums of both
+// dz goes to a workspace that the two products of the backward pass read; the
+// sums are taken before it is rounded.  Bound by HBM: LINEAR reads 2 and writes
+// 1 element, DUAL reads 3 and writes 2.
+#include "linear_grad.cuh"
+
+namespace qsml {
+namespace linear {
+namespace {
+
+// A warp takes 256 columns (8 a lane), a CTA's 8 warps every 8th row of
+// [blockIdx.y * chunk, + chunk).  A thread keeps its columns and sums them in
+// registers; the warps' sums are added in warp order in shared memory.
+template <typename T, bool DUAL>
+__global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, bool vec) {
+    pdl_begin();
+    constexpr int NO = DUAL ? 2 : 1;
+    __shared__ float fold[NO][8][256 + 8];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 256 + lane * 8;
+    const int n = a.N - col < 8 ? static_cast<int>(a.N - col) : 8;  // may be <= 0
+    const int64_t r0 = blockIdx.y * chunk, r1 = r0 + chunk < a.M ? r0 + chunk : a.M;
+    float sum[NO][8];
+#pragma unroll
+    for (int o = 0; o < NO; ++o)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[o][i] = 0.0f;
+    if (n > 0) {
+#pragma unroll 2
+        for (int64_t r = r0 + w; r < r1; r += 8) {
+            float dy[8], z[8], u[8], d[NO][8];
+            load8(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec, dy);
+            if (a.pre[0]) load8(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec, z);
+            if constexpr (DUAL) load8(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!a.pre[0]) {
+                    d[0][i] = dy[i];
+                } else {
+                    float value;
+                    const float g = act_grad<T>(a.act, z[i], value);
+                    if constexpr (DUAL) {
+                        d[0][i] = __fmul_rn(__fmul_rn(dy[i], u[i]), g);
+                        d[1][i] = __fmul_rn(dy[i], value);
+                    } else {
+                        d[0][i] = __fmul_rn(dy[i], g);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 0; o < NO; ++o) {
+                if (a.dz[o]) store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[o][i] = __fadd_rn(sum[o][i], i < n ? d[o][i] : 0.0f);
+            }
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int o = 0; o < NO; ++o)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fold[o][w][lane * 8 + i] = sum[o][i];
+    __syncthreads();
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= a.N) return;
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+        float s = fold[o][0][threadIdx.x];
+        for (int k = 1; k < 8; ++k) s = __fadd_rn(s, fold[o][k][threadIdx.x]);
+        a.partial[(static_cast<int64_t>(o) * gridDim.y + blockIdx.y) * a.N + c] = s;
+    }
+}
+
+template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradArgs& given) {
+    GradArgs a = given;
+    const int64_t tiles = (a.N + 255) / 256;
+    // about eight CTAs an SM, at least 8 rows a warp where the bias's gradient is wanted
+    int64_t parts = (8 * ctx->num_sms + tiles - 1) / tiles;
+    const int64_t most = (a.M + 63) / 64;
+    if (parts > most) parts = most;
+    const int64_t chunk = (a.M + parts - 1) / parts;
+    parts = (a.M + chunk - 1) / chunk;
+    Workspace ws(ctx);
+    const bool sums = a.db[0].out || a.db[1].out;
+    void* partial = nullptr;
+    if (sums) QSML_TRY_STATUS(ws.get(static_cast<size_t>(DUAL ? 2 : 1) * parts * a.N * sizeof(float), &partial));
+    a.partial = static_cast<float*>(partial);
+    bool vec = a.N % 8 == 0 && a.dy_ld % 8 == 0 && aligned16(a.dy);
+    for (int i = 0; i < 2; ++i) vec = vec && (!a.pre[i] || aligned16(a.pre[i]));
+    const cudaError_t e = launch_pdl(k_linear_dz<T, DUAL>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
+                                     dim3(256), 0, ctx->stream, a, chunk, vec);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_dz");
+    QSML_TRY_STATUS(after_launch(ctx, "k_linear_dz"));
+    if (!sums) return QSML_OK;
+    ColumnSum s0 = a.db[0], s1 = a.db[1];
+    s0.partial = a.partial;
+    s1.partial = a.partial + parts * a.N;
+    return finish_column_sums(ctx, s0, s1, parts, a.N);
+}
+
+}  // namespace
+
+template <typename T> qsml_status_t run_grad(Context* ctx, const GradArgs& a, bool dual) {
+    return dual ? launch<T, true>(ctx, a) : launch<T, false>(ctx, a);
+}
+template qsml_status_t run_grad<float>(Context*, const GradArgs&, bool);
+template qsml_status_t run_grad<__half>(Context*, const GradArgs&, bool);
+
+}  // namespace linear
+}  // namespace qsml

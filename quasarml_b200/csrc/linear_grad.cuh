@@ -1,0 +1,24 @@
+// Gradients with respect to the products of the linear layers (linear_grad.cu).
+#pragma once
+
+#include "linear.cuh"
+
+namespace qsml {
+namespace linear {
+
+struct GradArgs {
+    int64_t M = 0, N = 0;
+    int act = QSML_ACT_NONE;
+    const void* dy = nullptr;
+    int64_t dy_ld = 0;
+    const void* pre[2] = {nullptr, nullptr};  // rows of N; pre[0] null: dz = dy
+    void* dz[2] = {nullptr, nullptr};         // rows of `pitch` (a multiple of 8), 16-byte aligned; null: not wanted
+    int64_t pitch = 0;
+    ColumnSum db[2];
+    float* partial = nullptr;
+};
+
+template <typename T> qsml_status_t run_grad(Context* ctx, const GradArgs& a, bool dual);
+
+}  // namespace linear
+}  // namespace qsml
