@@ -172,6 +172,7 @@ qsml_status_t run(Context* ctx, int32_t dtype, int32_t precision, Problem& p) {
     if (!p.e.y && !p.e.pre[0] && !p.e.pre[1]) return QSML_OK;
     p.e.N = p.N;
     set_vec(&p.e, dtype_size(dtype));
+    if (precision != QSML_MM_FP32_FFMA && p.K > 0) return run_tc(ctx, p, dtype == QSML_F32);
     return dtype == QSML_F32 ? run_simt<float>(ctx, p) : run_simt<__half>(ctx, p);
 }
 

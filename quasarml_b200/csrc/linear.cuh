@@ -44,7 +44,11 @@ struct Problem {
 // CUDA-core products, binary32 fma with k ascending: any strides, any size.
 template <typename T> qsml_status_t run_simt(Context* ctx, const Problem& p);
 
-// ---- arithmetic shared by host-independent code --------------------------------
+// Tensor-core products (linear_tc.cu), any strides, alignment and size with
+// K > 0: binary16, or binary32 as three bf16 parts.
+qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32);
+
+// ---- arithmetic shared by the kernels --------------------------------------------
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
 __device__ __forceinline__ float ld1(const __half* p) { return __half2float(*p); }
 
@@ -155,6 +159,39 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, bool v
         for (int i = 0; i < 8; ++i)
             if (i < n) p[i] = v[i];
     }
+}
+
+// x = x0 + x1 + x2 in bf16, exactly: each part the upper 8 bits of what is left,
+// truncated (a bf16 is the upper half of a binary32).  Below 2^-110 the last part
+// may fall under the smallest number and is cut.  Infinities and NaN are all x0.
+__device__ __forceinline__ void split3(float x, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    const uint32_t b = __float_as_uint(x), top = b & 0xffff0000u;
+    if ((b & 0x7f800000u) == 0x7f800000u) {
+        p0 = (b >> 16) | ((b & 0xffffu) ? 0x40u : 0u);  // a NaN stays one
+        p1 = p2 = 0;
+        return;
+    }
+    const float r1 = __fsub_rn(x, __uint_as_float(top));
+    const uint32_t t1 = __float_as_uint(r1) & 0xffff0000u;
+    const float r2 = __fsub_rn(r1, __uint_as_float(t1));
+    p0 = top >> 16;
+    p1 = t1 >> 16;
+    p2 = __float_as_uint(r2) >> 16;
+}
+// Eight of them to three rows of bf16, `plane` elements apart (16-byte aligned).
+__device__ __forceinline__ void split8(const float (&v)[8], uint16_t* dst, int64_t plane) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t a[3], b[3];
+        split3(v[2 * i], a[0], a[1], a[2]);
+        split3(v[2 * i + 1], b[0], b[1], b[2]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) w[p][i] = a[p] | (b[p] << 16);
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 
 template <typename T>

@@ -1,0 +1,564 @@
+// The linear layers' products on the tensor cores (tcgen05.mma, accumulators in
+// TMEM, operands staged by TMA in 128-byte swizzled shared memory).
+//
+// Operands are tiles of 128 rows (of the result's rows or columns) by 64 k in
+// 16-bit elements, 16 KiB, in whichever order they lie in memory: K-major (k
+// contiguous: one box of 64 k x 128) or MN-major (two boxes of 64 x 64 k).  So x
+// and x^T, w and w^T are read in place by the forward product, dz w^T and x^T dz.
+// Operands that TMA cannot read (a row pitch or start off 16 bytes, strides in
+// both dims) are copied once to a workspace.
+//
+// binary16: one product, kind::f16, binary32 accumulators.
+// binary32: x = x0 + x1 + x2 exactly, three bf16 parts of 8 bits each (the upper
+// bits by truncation, so no part overflows and all have x's sign); the six
+// products x_i w_j with i + j <= 2 are formed on the bf16 pipe, the dropped ones
+// being below 3 * 2^-24 |x w|.  A tensor-core accumulator is truncated at each
+// step, so the main product x0 w0 is drained every 256 k into binary32 registers
+// (rounded to nearest there); the other five, 2^-8 of it and less, have an
+// accumulator of their own for the whole sum.  Cost: six times binary16's.
+//
+// k_linear_tc: 128 x 128 of the result a CTA (64 columns of each weight for a dual
+// product).  Where the tiles do not fill the GPU, a cluster of up to 8 CTAs splits
+// the sum over k: each leaves its binary32 tile in shared memory, and all of them
+// add the cluster's tiles, in rank order, for a share of the outputs (distributed
+// shared memory: no workspace, no atomics, one launch).
+#include "linear.cuh"
+#include "tcgen05.cuh"
+
+namespace qsml {
+namespace linear {
+namespace {
+
+using namespace tc;
+
+constexpr int TILE_BYTES = 128 * 128;     // one operand tile: 128 rows x 64 k
+constexpr int CHUNK = 4;                  // binary32: k-blocks between drains
+constexpr int THREADS = 192;              // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int MAX_SPLIT = 8;              // portable cluster size
+
+struct TcArgs {
+    CUtensorMap a[2], b[2];
+    Epilogue e;
+    int M, N;
+    int tiles_m, tiles_n;
+    int kb;                  // k-blocks of 64 a segment
+    int segments;
+    int splits;
+    int a_mn[2], b_mn[2];    // MN-major operands, by segment
+    int* status;
+};
+
+template <bool F32> struct Shape {
+    static constexpr int PARTS = F32 ? 3 : 1;
+    static constexpr int STAGES = F32 ? 2 : 3;
+    static constexpr int STAGE = 2 * PARTS * TILE_BYTES;
+    static constexpr int TMEM = F32 ? 512 : 128;
+    static constexpr size_t SMEM = size_t(STAGES) * STAGE + 1024 + 128;
+    static constexpr int CTAS = F32 ? 1 : 2;  // a SM
+};
+
+// D f32; A and B f16 (0) or bf16 (1); their major-ness; N, M.
+__device__ __forceinline__ uint32_t idesc(bool bf16, int a_mn, int b_mn, int m, int n) {
+    const uint32_t f = bf16 ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) |
+           (uint32_t(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+
+// The k16 slice k of a tile: K-major rows of 128 bytes (32 bytes a slice), or
+// MN-major chunks of 64 with 128 bytes a k (2048 bytes a slice, chunks 8 KiB apart).
+__device__ __forceinline__ uint64_t slice_desc(uint32_t tile, int mn, int k) {
+    return mn ? smem_desc(tile + k * 2048, 8192, 1024) : smem_desc(tile + k * 32, 16, 1024);
+}
+
+__device__ __forceinline__ void cluster_arrive_wait() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+template <bool F32, bool DUAL>
+__global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const __grid_constant__ TcArgs g) {
+    using T = std::conditional_t<F32, float, __half>;
+    using S = Shape<F32>;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = smem_raw + (base - raw);
+    const uint32_t bars = base + S::STAGES * S::STAGE;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * S::STAGES + 4);
+    unsigned char* misc = gbase + S::STAGES * S::STAGE + 8 * (2 * S::STAGES + 5);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 4);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(S::TMEM)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_begin();  // everything above needed no memory of the kernels before
+    const long long limit = wait_limit(g.status);
+
+    const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
+    const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
+    constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
+    // this CTA's share of the k-blocks (binary32: of the chunks between drains)
+    const int per_seg = F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb;
+    const int units = per_seg * g.segments;
+    const int u0 = static_cast<int>(static_cast<int64_t>(units) * rank / g.splits);
+    const int u1 = static_cast<int>(static_cast<int64_t>(units) * (rank + 1) / g.splits);
+    // blocks [k0, k1) of segment seg that unit u covers
+    auto unit = [&](int u, int& seg, int& k0, int& k1) {
+        seg = u / per_seg;
+        k0 = (u - seg * per_seg) * (F32 ? CHUNK : 1);
+        k1 = F32 ? min(k0 + CHUNK, g.kb) : k0 + 1;
+    };
+    auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
+    auto b_tile = [&](int s, int p) { return base + s * S::STAGE + (S::PARTS + p) * TILE_BYTES; };
+
+    bool done = true;  // epilogue warps: the CTA's sums are complete
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            int issued[S::STAGES];
+            for (int s = 0; s < S::STAGES; ++s) issued[s] = -1;
+            bool ok = true;
+            for (int u = u0; u < u1 && ok; ++u) {
+                int seg, k0, k1;
+                unit(u, seg, k0, k1);
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = full_bar(stage);
+                    mbar_expect_tx(bar, S::STAGE);
+#pragma unroll
+                    for (int p = 0; p < S::PARTS; ++p) {
+                        const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
+                        if (g.a_mn[seg]) {
+                            tma_load_3d(at, &g.a[seg], bar, mt * 128, kb * 64, p);
+                            tma_load_3d(at + 8192, &g.a[seg], bar, mt * 128 + 64, kb * 64, p);
+                        } else {
+                            tma_load_3d(at, &g.a[seg], bar, kb * 64, mt * 128, p);
+                        }
+                        if constexpr (DUAL) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                if (g.b_mn[0]) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
+                                else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, p);
+                            }
+                        } else if (g.b_mn[seg]) {
+                            tma_load_3d(bt, &g.b[seg], bar, nt * 128, kb * 64, p);
+                            tma_load_3d(bt + 8192, &g.b[seg], bar, nt * 128 + 64, kb * 64, p);
+                        } else {
+                            tma_load_3d(bt, &g.b[seg], bar, kb * 64, nt * 128, p);
+                        }
+                    }
+                    issued[stage] = static_cast<int>(phase);
+                    if (++stage == S::STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // every copy this thread started lands before the memory has another use
+            for (int s = 0; s < S::STAGES; ++s) {
+                if (issued[s] < 0) continue;
+                const long long t0 = clock64();
+                while (!mbar_test(full_bar(s), static_cast<uint32_t>(issued[s])) && clock64() - t0 < WAIT_CYCLES) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            const uint32_t small = tmem + 256;  // binary32: the five lesser products
+            for (int u = u0; u < u1 && ok; ++u) {
+                int seg, k0, k1;
+                unit(u, seg, k0, k1);
+                const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
+                const uint32_t id = idesc(F32, a_mn, b_mn, 128, 128);
+                if (F32) {
+                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
+                    tc_fence_after();
+                }
+                const uint32_t d = F32 ? tmem + acc * 128 : tmem;
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma_f16(dst, slice_desc(a_tile(stage, pa), a_mn, k), slice_desc(b_tile(stage, pb), b_mn, k), id,
+                                    fresh && k == 0 ? 0u : 1u);
+                    };
+                    if constexpr (F32) {
+                        product(0, 2, small, u == u0 && kb == k0);
+                        product(2, 0, small, false);
+                        product(1, 1, small, false);
+                        product(0, 1, small, false);
+                        product(1, 0, small, false);
+                        product(0, 0, d, kb == k0);
+                    } else {
+                        product(0, 0, d, u == u0);
+                    }
+                    mma_commit(empty_bar(stage));
+                    if (++stage == S::STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if (F32 || u + 1 == u1) {
+                    mma_commit(tfull_bar(acc));
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1u;
+                    }
+                }
+            }
+            mma_commit(drain_bar);
+            const long long t0 = clock64();
+            while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        const int row = quarter * 32 + lane;
+        // the row's 16-byte unit u of the CTA's binary32 tile: units swapped by
+        // row, so that 32 rows' stores of one unit meet different banks
+        auto put = [&](int c, const float (&v)[32]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t at = base + row * 512 + (((c / 4 + j) ^ lane) << 4);
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[4 * j]), "f"(v[4 * j + 1]),
+                             "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                             : "memory");
+            }
+        };
+        auto ready = [&](int acc, uint32_t phase) {
+            int r = 0;
+            if (lane == 0) r = mbar_wait(tfull_bar(acc), phase, abort_flag, limit) ? 1 : 0;
+            r = __shfl_sync(0xffffffffu, r, 0);
+            tc_fence_after();
+            return r != 0;
+        };
+        const bool rows_here = mt * 128 + quarter * 32 < g.M;
+        if constexpr (F32) {
+            float sum[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
+            int acc = 0;
+            uint32_t phase = 0;
+            for (int u = u0; u < u1; ++u) {
+                if (!ready(acc, phase)) {
+                    done = false;
+                    break;
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(lanes + acc * 128 + c * 32, r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty_bar(acc));
+                if (++acc == 2) {
+                    acc = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (done && rows_here) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(lanes + 256 + c * 32, r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                    put(c * 32, sum[c]);
+                }
+            }
+        } else {
+            done = ready(0, 0);
+            if (done && rows_here) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    float v[32];
+                    tmem_ld32(lanes + c * 32, r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                    put(c * 32, v);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    // all of the cluster's tiles are in shared memory
+    if (g.splits > 1) cluster_arrive_wait();
+    else __syncthreads();
+    tc_fence_after();
+    if (!*abort_flag) {
+        const int rows = min(128, g.M - mt * 128);
+        constexpr int UNITS = BN / 8;
+        for (int i = rank * THREADS + static_cast<int>(threadIdx.x); i < rows * UNITS; i += g.splits * THREADS) {
+            const int r = i / UNITS, c = (i % UNITS) * 8;
+            const int64_t col = static_cast<int64_t>(nt) * BN + c;
+            if (col >= g.N) continue;
+            float z[8], u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = u[j] = 0.0f;
+            auto add = [&](uint32_t tile_base, int cc, float (&v)[8]) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 q = ld_cluster(tile_base + r * 512 + (((cc / 4 + h) ^ (r & 31)) << 4));
+                    v[4 * h] = __fadd_rn(v[4 * h], q.x);
+                    v[4 * h + 1] = __fadd_rn(v[4 * h + 1], q.y);
+                    v[4 * h + 2] = __fadd_rn(v[4 * h + 2], q.z);
+                    v[4 * h + 3] = __fadd_rn(v[4 * h + 3], q.w);
+                }
+            };
+            for (int s = 0; s < g.splits; ++s) {
+                const uint32_t from = map_to_rank(base, s);
+                add(from, c, z);
+                if constexpr (DUAL) add(from, 64 + c, u);
+            }
+            finish8<T, DUAL>(g.e, static_cast<int64_t>(mt) * 128 + r, col, z, u);
+        }
+    } else if (threadIdx.x == 0) {
+        atomicExch(g.status, QSML_E_TIMEOUT);
+    }
+    // no CTA leaves while another reads its tile
+    if (g.splits > 1) cluster_arrive_wait();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Operands for TMA
+// ---------------------------------------------------------------------------
+
+// Eight consecutive elements of the stored order at a time, any strides, to
+// 16-bit rows of `pitch`: binary16 as it is, binary32 as its three bf16 parts
+// (`plane` elements apart).  Bound by HBM: binary32 reads 4 and writes 6 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_linear_stage(const T* __restrict__ src, int64_t outer, int64_t inner, int64_t os, int64_t is, bool vec,
+                   uint16_t* __restrict__ dst, int64_t pitch, int64_t plane) {
+    pdl_begin();
+    const int64_t groups = pitch / 8;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < outer * groups;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t o = i / groups, c = (i - o * groups) * 8;
+        const int n = inner - c < 8 ? static_cast<int>(inner - c) : 8;
+        const T* p = src + o * os + c * is;
+        float v[8];
+        if (vec && n == 8) {
+            load8(p, 8, true, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < n ? ld1(p + j * is) : 0.0f;
+        }
+        if constexpr (sizeof(T) == 2) {
+            store8(reinterpret_cast<__half*>(dst + o * pitch + c), 8, true, v);
+        } else {
+            split8(v, dst + o * pitch + c, plane);
+        }
+    }
+}
+
+struct Staged {
+    const void* p = nullptr;
+    int64_t inner = 0, outer = 0, pitch = 0, plane = 0;  // 16-bit elements
+    bool trans = false;  // stored as the matrix's transpose
+};
+
+// The matrix as TMA reads it, copied only where it has to be.  want: 0 rows, 1
+// columns contiguous, -1 as it lies.
+qsml_status_t stage(Context* ctx, Workspace& ws, const Mat& m, bool f32, int want, Staged* s) {
+    const bool by_rows = m.cs == 1 || m.cols == 1, by_cols = m.rs == 1 || m.rows == 1;
+    s->trans = want >= 0 ? want == 1 : !by_rows && by_cols;
+    s->inner = s->trans ? m.rows : m.cols;
+    s->outer = s->trans ? m.cols : m.rows;
+    int64_t os = s->trans ? m.cs : m.rs, is = s->trans ? m.rs : m.cs;
+    if (s->inner == 1) is = 1;
+    if (s->outer == 1) os = (s->inner + 7) / 8 * 8;
+    s->p = m.p;
+    s->pitch = os;
+    s->plane = 0;
+    const int es = f32 ? 4 : 2;
+    if (!f32 && is == 1 && aligned16(m.p) && os % 8 == 0 && os >= s->inner && os < (int64_t(1) << 38)) return QSML_OK;
+    const int64_t pitch = (s->inner + 7) / 8 * 8;
+    const int64_t plane = pitch * s->outer;
+    void* dst = nullptr;
+    QSML_TRY_STATUS(ws.get(static_cast<size_t>(plane) * 2 * (f32 ? 3 : 1), &dst));
+    const bool vec = is == 1 && aligned16(m.p) && (os * es) % 16 == 0;
+    const int64_t work = s->outer * (pitch / 8);
+    int64_t grid = (work + 255) / 256;
+    if (grid > int64_t(ctx->num_sms) * 16) grid = int64_t(ctx->num_sms) * 16;
+    cudaError_t e;
+    if (f32)
+        e = launch_pdl(k_linear_stage<float>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream,
+                       static_cast<const float*>(m.p), s->outer, s->inner, os, is, vec, static_cast<uint16_t*>(dst), pitch,
+                       plane);
+    else
+        e = launch_pdl(k_linear_stage<__half>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream,
+                       static_cast<const __half*>(m.p), s->outer, s->inner, os, is, vec, static_cast<uint16_t*>(dst), pitch,
+                       plane);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_stage");
+    QSML_TRY_STATUS(after_launch(ctx, "k_linear_stage"));
+    s->p = dst;
+    s->pitch = pitch;
+    s->plane = plane;
+    return QSML_OK;
+}
+
+// mn: MN-major boxes of 64 x 64 k, else K-major boxes of 64 k x `rows`.
+bool operand_map(CUtensorMap* map, const Staged& s, bool f32, bool mn, uint32_t rows) {
+    const uint64_t planes = f32 ? 3 : 1;
+    return make_map(map, s.p, s.inner, s.outer, planes, s.pitch * 2, (s.plane ? s.plane : s.pitch * s.outer) * 2, 64,
+                    mn ? 64 : rows, f32 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+}
+
+template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem& p, TcArgs& g) {
+    using S = Shape<F32>;
+    constexpr int BN = DUAL ? 64 : 128;
+    auto kernel = k_linear_tc<F32, DUAL>;
+    {
+        static std::mutex mu;
+        static uint64_t done = 0;
+        std::lock_guard<std::mutex> lk(mu);
+        const uint64_t bit = uint64_t(1) << (ctx->device & 63);
+        if (!(done & bit)) {
+            QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                                 static_cast<int>(S::SMEM)),
+                                       "linear: shared-memory attribute"));
+            done |= bit;
+        }
+    }
+    g.tiles_m = static_cast<int>((p.M + 127) / 128);
+    g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
+    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
+    if (tiles * MAX_SPLIT > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
+    // split the sum while that leaves no more CTAs than the SMs take at once
+    const int64_t units = static_cast<int64_t>(F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb) * g.segments;
+    int splits = 1;
+    while (splits < MAX_SPLIT && tiles * splits * 2 <= int64_t(ctx->num_sms) * S::CTAS && units >= splits * 4) splits *= 2;
+    g.splits = splits;
+
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = ctx->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = splits > 1 ? 2 : 1;
+    const char* name = F32 ? "k_linear_tc<f32>" : "k_linear_tc<f16>";
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
+    if (e != cudaSuccess) return check_cuda(ctx, e, name);
+    return after_launch(ctx, name);
+}
+
+}  // namespace
+
+qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
+    Workspace ws(ctx);
+    TcArgs g;
+    g.e = p.e;
+    g.M = static_cast<int>(p.M);
+    g.N = static_cast<int>(p.N);
+    g.kb = static_cast<int>((p.K + 63) / 64);
+    g.segments = p.segments;
+    g.status = ctx->status;
+    bool ok = true;
+    Staged b0;
+    for (int i = 0; i < 2; ++i) {
+        g.a_mn[i] = g.b_mn[i] = 0;
+        if (i < p.segments) {
+            Staged s;
+            QSML_TRY_STATUS(stage(ctx, ws, p.a[i], f32, -1, &s));
+            g.a_mn[i] = s.trans ? 1 : 0;  // stored [K, M]
+            ok = ok && operand_map(&g.a[i], s, f32, s.trans, 128);
+        } else {
+            g.a[i] = g.a[0];
+        }
+        if (i < (p.dual ? 2 : p.segments)) {
+            // a dual product's weights share an order: they meet in one MMA
+            Staged s;
+            QSML_TRY_STATUS(stage(ctx, ws, p.b[i], f32, p.dual && i ? (b0.trans ? 1 : 0) : -1, &s));
+            if (i == 0) b0 = s;
+            g.b_mn[i] = s.trans ? 0 : 1;  // stored [K, N]
+            ok = ok && operand_map(&g.b[i], s, f32, !s.trans, p.dual ? 64 : 128);
+        } else {
+            g.b[i] = g.b[0];
+        }
+    }
+    if (!ok) return set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
+    if (f32) return p.dual ? launch<true, true>(ctx, p, g) : launch<true, false>(ctx, p, g);
+    return p.dual ? launch<false, true>(ctx, p, g) : launch<false, false>(ctx, p, g);
+}
+
+}  // namespace linear
+}  // namespace qsml
