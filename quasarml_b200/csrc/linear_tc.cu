@@ -390,6 +390,374 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 }
 
 // ---------------------------------------------------------------------------
+// Large products: persistent pairs of SMs (cta_group::2), the epilogue of a tile
+// under the products of the next.
+//   binary16: 256 x 256 of the result a pair (dual: 128 columns of each weight, one
+//     from each CTA), six stages of 32 KiB a CTA, two accumulators of 256 columns;
+//   binary32: 256 x 128 (dual: 64 of each), three stages of all parts (72 KiB a CTA),
+//     two accumulators for the drains of the main product and two, by tile, for the
+//     lesser ones.
+// Each CTA loads its own 128 rows of A and half of the tile's columns of B; the
+// leader issues the MMAs of both.  Roles and barriers as in k_linear_tc, the
+// leader's full barrier counting both CTAs' bytes.
+// ---------------------------------------------------------------------------
+template <bool F32> struct PairShape {
+    static constexpr int PARTS = F32 ? 3 : 1;
+    static constexpr int STAGES = F32 ? 3 : 6;
+    static constexpr int BCOLS = F32 ? 64 : 128;              // columns of B a CTA
+    static constexpr int B_BYTES = BCOLS * 128;
+    static constexpr int STAGE = PARTS * (TILE_BYTES + B_BYTES);
+    static constexpr int NACC = 2 * BCOLS;                    // accumulator columns
+    static constexpr int OUT = F32 ? 0 : 4 * 8192;            // epilogue staging, 8 KiB a warp
+    static constexpr size_t SMEM = size_t(STAGES) * STAGE + OUT + 1024 + 256;
+    static_assert(SMEM <= 232448, "shared memory");
+};
+constexpr int PAIR_GROUP_M = 16;  // tiles of 16 row blocks run together: A and B panels stay in L2
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+
+template <bool F32, bool DUAL>
+__global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constant__ TcArgs g) {
+    using T = std::conditional_t<F32, float, __half>;
+    using S = PairShape<F32>;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = smem_raw + (base - raw);
+    const uint32_t out_stage = base + S::STAGES * S::STAGE;
+    const uint32_t bars = out_stage + S::OUT;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 + a); };
+    auto sempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 4 + a); };  // binary32: lesser products read
+    const uint32_t drain_bar = bars + 8u * (2 * S::STAGES + 6);
+    unsigned char* misc = gbase + S::STAGES * S::STAGE + S::OUT + 8 * (2 * S::STAGES + 7);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
+
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 8);  // 4 epilogue warps in each CTA
+            mbar_init(sempty_bar(a), 8);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_begin();
+    const long long limit = wait_limit(g.status);
+
+    constexpr int BN = DUAL ? S::BCOLS : 2 * S::BCOLS;  // result columns a tile
+    const int total = g.tiles_m * g.tiles_n;
+    const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
+    auto decode = [&](int t, int& mt, int& nt) {
+        const int group = t / (PAIR_GROUP_M * g.tiles_n);
+        const int first = group * PAIR_GROUP_M;
+        const int gm = min(PAIR_GROUP_M, g.tiles_m - first);
+        const int within = t - first * g.tiles_n;
+        mt = first + within % gm;
+        nt = within / gm;
+    };
+    const int per_seg = F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb;
+    const int units = per_seg * g.segments;
+    auto unit = [&](int u, int& seg, int& k0, int& k1) {
+        seg = u / per_seg;
+        k0 = (u - seg * per_seg) * (F32 ? CHUNK : 1);
+        k1 = F32 ? min(k0 + CHUNK, g.kb) : k0 + 1;
+    };
+    auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
+    auto b_tile = [&](int s, int p) { return base + s * S::STAGE + S::PARTS * TILE_BYTES + p * S::B_BYTES; };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += pairs) {
+                int mt, nt;
+                decode(t, mt, nt);
+                const int row = mt * 256 + static_cast<int>(rank) * 128;
+                const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
+                for (int u = 0; u < units && ok; ++u) {
+                    int seg, k0, k1;
+                    unit(u, seg, k0, k1);
+                    const CUtensorMap* mb = &g.b[DUAL ? rank : seg];
+                    const int b_mn = g.b_mn[DUAL ? 0 : seg];
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        if (leader) mbar_expect_tx(full_bar(stage), 2 * S::STAGE);
+                        const uint32_t bar = map_to_rank(full_bar(stage), 0);
+#pragma unroll
+                        for (int p = 0; p < S::PARTS; ++p) {
+                            const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
+                            if (g.a_mn[seg]) {
+                                tma_load_3d_pair(at, &g.a[seg], bar, row, kb * 64, p);
+                                tma_load_3d_pair(at + 8192, &g.a[seg], bar, row + 64, kb * 64, p);
+                            } else {
+                                tma_load_3d_pair(at, &g.a[seg], bar, kb * 64, row, p);
+                            }
+                            if (b_mn) {
+#pragma unroll
+                                for (int j = 0; j < S::BCOLS / 64; ++j)
+                                    tma_load_3d_pair(bt + j * 8192, mb, bar, col + j * 64, kb * 64, p);
+                            } else {
+                                tma_load_3d_pair(bt, mb, bar, kb * 64, col, p);
+                            }
+                        }
+                        if (++stage == S::STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            int stage = 0, acc = 0, par = 0;
+            uint32_t phase = 0, acc_phase = 0, par_phase = 0;
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += pairs) {
+                if (F32) {
+                    if (!mbar_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) break;
+                    tc_fence_after();
+                }
+                const uint32_t small = tmem + 256 + par * 128;
+                for (int u = 0; u < units && ok; ++u) {
+                    int seg, k0, k1;
+                    unit(u, seg, k0, k1);
+                    const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
+                    const uint32_t id = idesc(F32, a_mn, b_mn, 256, S::NACC);
+                    if (F32 || u == 0) {
+                        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
+                    const uint32_t d = tmem + acc * S::NACC;
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_f16_pair(dst, slice_desc(a_tile(stage, pa), a_mn, k),
+                                             slice_desc(b_tile(stage, pb), b_mn, k), id, fresh && k == 0 ? 0u : 1u);
+                        };
+                        if constexpr (F32) {
+                            product(0, 2, small, u == 0 && kb == k0);
+                            product(2, 0, small, false);
+                            product(1, 1, small, false);
+                            product(0, 1, small, false);
+                            product(1, 0, small, false);
+                            product(0, 0, d, kb == k0);
+                        } else {
+                            product(0, 0, d, u == 0);
+                        }
+                        mma_commit_pair(empty_bar(stage));
+                        if (++stage == S::STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    if (F32 || u + 1 == units) {
+                        mma_commit_pair(tfull_bar(acc));
+                        if (++acc == 2) {
+                            acc = 0;
+                            acc_phase ^= 1u;
+                        }
+                    }
+                }
+                if (++par == 2) {
+                    par = 0;
+                    par_phase ^= 1u;
+                }
+            }
+            mma_commit_pair_local(drain_bar);
+            const long long t0 = clock64();
+            while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        int acc = 0, par = 0;
+        uint32_t phase = 0;
+        auto ready = [&]() {
+            int r = 0;
+            if (lane == 0) r = mbar_wait(tfull_bar(acc), phase, abort_flag, limit) ? 1 : 0;
+            r = __shfl_sync(0xffffffffu, r, 0);
+            tc_fence_after();
+            return r != 0;
+        };
+        auto release = [&](uint32_t bar) {  // this warp is done with an accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(bar, 0));
+        };
+        auto next_acc = [&]() {
+            if (++acc == 2) {
+                acc = 0;
+                phase ^= 1u;
+            }
+        };
+        bool ok = true;
+        for (int t = pair; t < total && ok; t += pairs) {
+            int mt, nt;
+            decode(t, mt, nt);
+            const int row0 = mt * 256 + static_cast<int>(rank) * 128 + quarter * 32;  // first of the warp's 32 rows
+            const int64_t col0 = static_cast<int64_t>(nt) * BN;
+            if constexpr (F32) {
+                // a thread has a row of the tile in registers (128 columns)
+                float sum[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
+                for (int u = 0; u < units; ++u) {
+                    if (!ready()) {
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(lanes + acc * 128 + c * 32, r);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                    }
+                    release(tempty_bar(acc));
+                    next_acc();
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(lanes + 256 + par * 128 + c * 32, r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                }
+                release(sempty_bar(par));
+                par ^= 1;
+                // 32-byte groups, whole sectors, straight from the registers
+                if (row0 + lane < g.M) {
+#pragma unroll
+                    for (int c = 0; c < BN / 8; ++c) {
+                        if (col0 + c * 8 >= g.N) break;
+                        float z[8], v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            z[i] = sum[c / 4][(c % 4) * 8 + i];
+                            v[i] = DUAL ? sum[c / 4 + 2 * (DUAL ? 1 : 0)][(c % 4) * 8 + i] : 0.0f;
+                        }
+                        finish8<T, DUAL>(g.e, row0 + lane, col0 + c * 8, z, v);
+                    }
+                }
+            } else {
+                if (!ready()) break;
+                const uint32_t stage = out_stage + quarter * 8192;  // 32 rows of 64 binary32, units swapped by row
+                const uint32_t d = lanes + acc * S::NACC;
+                constexpr int STEP = DUAL ? 32 : 64;
+                const int cend = static_cast<int>(g.N - col0 < BN ? g.N - col0 : BN);
+                for (int c0 = 0; c0 < cend; c0 += STEP) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t r[32];
+                        tmem_ld32(d + (DUAL ? c0 + h * 128 : c0 + h * 32), r);
+                        if (h == 1 && c0 + STEP >= cend) release(tempty_bar(acc));
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t at = stage + lane * 256 + (((h * 8 + j) ^ (lane & 15)) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[4 * j]),
+                                         "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                                         : "memory");
+                        }
+                    }
+                    __syncwarp();
+                    // rows of 64 (dual: 32) columns, 8 a lane: whole lines of the outputs
+                    constexpr int UNITS = STEP / 8, ROWS = 32 / UNITS;
+                    const int un = lane % UNITS;
+                    const int64_t col = col0 + c0 + un * 8;
+                    auto take = [&](int row, int unit, float (&v)[8]) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t at = stage + row * 256 + (((unit + h) ^ (row & 15)) << 4);
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3])
+                                         : "r"(at)
+                                         : "memory");
+                        }
+                    };
+                    if (col < g.N) {
+#pragma unroll 2
+                        for (int r = lane / UNITS; r < 32; r += ROWS) {
+                            if (row0 + r >= g.M) break;
+                            float z[8], v[8];
+                            take(r, un * 2, z);
+                            if constexpr (DUAL) take(r, 8 + un * 2, v);
+                            finish8<T, DUAL>(g.e, row0 + r, col, z, v);
+                        }
+                    }
+                    __syncwarp();
+                }
+                next_acc();
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        if (threadIdx.x == 0) atomicExch(g.status, QSML_E_TIMEOUT);
+        // copies still in flight complete on the leader's barrier: give them time
+        // to land before the pair's shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000LL) {
+        }
+    }
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Operands for TMA
 // ---------------------------------------------------------------------------
 
@@ -475,6 +843,65 @@ bool operand_map(CUtensorMap* map, const Staged& s, bool f32, bool mn, uint32_t 
                     mn ? 64 : rows, f32 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
 }
 
+// Pairs of SMs that the device holds at once (0: none), once per device and kernel.
+template <bool F32, bool DUAL> qsml_status_t max_pairs(Context* ctx, int* pairs) {
+    static std::mutex mu;
+    static int known[64] = {};
+    std::lock_guard<std::mutex> lk(mu);
+    int& n = known[ctx->device & 63];
+    if (n == 0) {
+        auto kernel = k_linear_pair<F32, DUAL>;
+        QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                             static_cast<int>(PairShape<F32>::SMEM)),
+                                   "linear: shared-memory attribute"));
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(2 * (ctx->num_sms / 2));
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = PairShape<F32>::SMEM;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = -1;
+        }
+    }
+    *pairs = n < 0 ? 0 : n;
+    return QSML_OK;
+}
+
+template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Problem& p, TcArgs& g, int pairs) {
+    using S = PairShape<F32>;
+    constexpr int BN = DUAL ? S::BCOLS : 2 * S::BCOLS;
+    g.tiles_m = static_cast<int>((p.M + 255) / 256);
+    g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
+    g.splits = 1;
+    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
+    if (tiles > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = ctx->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const char* name = F32 ? "k_linear_pair<f32>" : "k_linear_pair<f16>";
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_linear_pair<F32, DUAL>, g);
+    if (e != cudaSuccess) return check_cuda(ctx, e, name);
+    return after_launch(ctx, name);
+}
+
 template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem& p, TcArgs& g) {
     using S = Shape<F32>;
     constexpr int BN = DUAL ? 64 : 128;
@@ -524,6 +951,14 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
 }  // namespace
 
 qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
+    // pairs of SMs where the tiles fill them, else 128 x 128 tiles and split sums
+    int pairs = 0;
+    if (f32) QSML_TRY_STATUS((p.dual ? max_pairs<true, true>(ctx, &pairs) : max_pairs<true, false>(ctx, &pairs)));
+    else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &pairs) : max_pairs<false, false>(ctx, &pairs)));
+    const int64_t bn = (f32 ? 128 : 256) / (p.dual ? 2 : 1);
+    const int64_t tiles = ((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
+    const bool pair = pairs > 0 && tiles >= pairs;
+
     Workspace ws(ctx);
     TcArgs g;
     g.e = p.e;
@@ -534,6 +969,7 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
     g.status = ctx->status;
     bool ok = true;
     Staged b0;
+    const uint32_t b_rows = pair ? (f32 ? 64 : 128) : (p.dual ? 64 : 128);  // of a K-major box
     for (int i = 0; i < 2; ++i) {
         g.a_mn[i] = g.b_mn[i] = 0;
         if (i < p.segments) {
@@ -550,12 +986,16 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
             QSML_TRY_STATUS(stage(ctx, ws, p.b[i], f32, p.dual && i ? (b0.trans ? 1 : 0) : -1, &s));
             if (i == 0) b0 = s;
             g.b_mn[i] = s.trans ? 0 : 1;  // stored [K, N]
-            ok = ok && operand_map(&g.b[i], s, f32, !s.trans, p.dual ? 64 : 128);
+            ok = ok && operand_map(&g.b[i], s, f32, !s.trans, b_rows);
         } else {
             g.b[i] = g.b[0];
         }
     }
     if (!ok) return set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
+    if (pair) {
+        if (f32) return p.dual ? launch_pair<true, true>(ctx, p, g, pairs) : launch_pair<true, false>(ctx, p, g, pairs);
+        return p.dual ? launch_pair<false, true>(ctx, p, g, pairs) : launch_pair<false, false>(ctx, p, g, pairs);
+    }
     if (f32) return p.dual ? launch<true, true>(ctx, p, g) : launch<true, false>(ctx, p, g);
     return p.dual ? launch<false, true>(ctx, p, g) : launch<false, false>(ctx, p, g);
 }

@@ -227,6 +227,19 @@ def test_activations(ctx, act, dt, gated):
     check_backward(c, act, kept, *backward(ctx, c, act, kept))
 
 
+# the forward product, dx and dw in turn large enough for pairs of SMs, ragged in every size
+@pytest.mark.parametrize("size", [(2200, 136, 2500), (2200, 2500, 136), (136, 2200, 2500)])
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+def test_pairs_of_sms(ctx, size, dt, gated):
+    c = Case(*size, dt, gated=gated)
+    y, pre = forward(ctx, c, "silu", True)
+    assert ctx.last_kernel().startswith("k_linear_pair") == (size[1] == 136), ctx.last_kernel()
+    check_forward(c, "silu", y, pre, True)
+    kept = c.kept()
+    check_backward(c, "silu", kept, *backward(ctx, c, "silu", kept))
+
+
 def strided(a, how):
     """A device view with the values of `a`: transposed storage, an odd row pitch, columns of a
     wider matrix, every other column, a start off the 16-byte boundary."""
