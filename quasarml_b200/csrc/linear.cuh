@@ -194,24 +194,39 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint16_t* dst, int64
         *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 
-template <typename T>
-__device__ __forceinline__ void add_bias8(const Epilogue& e, int which, int64_t col, int n, float (&z)[8]) {
-    if (!e.bias[which]) return;
-    float b[8];
-    if (e.bias_f32) load8(static_cast<const float*>(e.bias[which]) + col, n, e.vec, b);
-    else load8(static_cast<const T*>(e.bias[which]) + col, n, e.vec, b);
+// The biases of columns col .. col + 7 (0 where there is none), for finish8.
+template <typename T, bool DUAL>
+__device__ __forceinline__ void bias8(const Epilogue& e, int64_t col, float (&b)[DUAL ? 2 : 1][8]) {
+    const int n = e.N - col < 8 ? static_cast<int>(e.N - col) : 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = __fadd_rn(z[i], b[i]);
+    for (int w = 0; w < (DUAL ? 2 : 1); ++w) {
+        if (!e.bias[w]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[w][i] = 0.0f;
+        } else if (e.bias_f32) {
+            load8(static_cast<const float*>(e.bias[w]) + col, n, e.vec, b[w]);
+        } else {
+            load8(static_cast<const T*>(e.bias[w]) + col, n, e.vec, b[w]);
+        }
+    }
 }
 
 // Columns col .. col + 7 of `row` from their products (u: DUAL only) to the
 // outputs.  col is a multiple of 8; columns from N on are not written.
 template <typename T, bool DUAL>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t col, float (&z)[8], float (&u)[8]) {
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t col, const float (&b)[DUAL ? 2 : 1][8],
+                                        float (&z)[8], float (&u)[8]) {
     const int n = e.N - col < 8 ? static_cast<int>(e.N - col) : 8;
     const int64_t at = row * e.N + col;
-    add_bias8<T>(e, 0, col, n, z);
-    if constexpr (DUAL) add_bias8<T>(e, 1, col, n, u);
+    float r[8];
+    if constexpr (!DUAL) {  // first, so that it is in flight under the rest
+        if (e.residual) load8(static_cast<const T*>(e.residual) + row * e.res_ld + col, n, e.vec, r);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        z[i] = __fadd_rn(z[i], b[0][i]);
+        if constexpr (DUAL) u[i] = __fadd_rn(u[i], b[DUAL ? 1 : 0][i]);
+    }
     if (e.pre[0]) store8(static_cast<T*>(e.pre[0]) + at, n, e.vec, z);
     if constexpr (DUAL) {
         if (e.pre[1]) store8(static_cast<T*>(e.pre[1]) + at, n, e.vec, u);
@@ -239,8 +254,6 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t 
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[i] = __fmul_rn(z[i], u[i]);
     } else if (e.residual) {
-        float r[8];
-        load8(static_cast<const T*>(e.residual) + row * e.res_ld + col, n, e.vec, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[i] = __fadd_rn(z[i], r[i]);
     }

@@ -93,10 +93,12 @@ __global__ void __launch_bounds__(256) k_linear_simt(const __grid_constant__ Pro
     }
     const int64_t col = col0 + tx * 8;
     if (col >= p.N) return;
+    float bias[NB][8];
+    bias8<T, DUAL>(p.e, col, bias);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = row0 + ty * 4 + i;
-        if (row < p.M) finish8<T, DUAL>(p.e, row, col, acc[0][i], acc[NB - 1][i]);
+        if (row < p.M) finish8<T, DUAL>(p.e, row, col, bias, acc[0][i], acc[NB - 1][i]);
     }
 }
 

@@ -79,6 +79,16 @@ __device__ __forceinline__ uint64_t slice_desc(uint32_t tile, int mn, int k) {
     return mn ? smem_desc(tile + k * 2048, 8192, 1024) : smem_desc(tile + k * 32, 16, 1024);
 }
 
+// What the MMA thread needs of an operand's order: it issues an MMA every 64 to 128
+// cycles alone, so a descriptor is one addition to these.
+struct Walk {
+    uint64_t first;  // descriptor of the tile at address 0 of the ring, k slice 0
+    uint32_t step;   // from a k slice to the next (16-byte units)
+};
+__device__ __forceinline__ Walk walk_of(uint32_t tile, int mn) {
+    return Walk{slice_desc(tile, mn, 0), mn ? 2048u >> 4 : 32u >> 4};
+}
+
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
@@ -141,16 +151,15 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
     const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
     constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
-    // this CTA's share of the k-blocks (binary32: of the chunks between drains)
+    // this CTA's share of the sum, in units of k-blocks (binary32: of the CHUNK
+    // k-blocks between drains), and of it the part [lo, hi) in segment seg
     const int per_seg = F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb;
     const int units = per_seg * g.segments;
     const int u0 = static_cast<int>(static_cast<int64_t>(units) * rank / g.splits);
     const int u1 = static_cast<int>(static_cast<int64_t>(units) * (rank + 1) / g.splits);
-    // blocks [k0, k1) of segment seg that unit u covers
-    auto unit = [&](int u, int& seg, int& k0, int& k1) {
-        seg = u / per_seg;
-        k0 = (u - seg * per_seg) * (F32 ? CHUNK : 1);
-        k1 = F32 ? min(k0 + CHUNK, g.kb) : k0 + 1;
+    auto part = [&](int seg, int& lo, int& hi) {
+        lo = max(u0 - seg * per_seg, 0) * (F32 ? CHUNK : 1);
+        hi = min(max(u1 - seg * per_seg, 0) * (F32 ? CHUNK : 1), g.kb);
     };
     auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
     auto b_tile = [&](int s, int p) { return base + s * S::STAGE + (S::PARTS + p) * TILE_BYTES; };
@@ -163,10 +172,12 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             int issued[S::STAGES];
             for (int s = 0; s < S::STAGES; ++s) issued[s] = -1;
             bool ok = true;
-            for (int u = u0; u < u1 && ok; ++u) {
-                int seg, k0, k1;
-                unit(u, seg, k0, k1);
-                for (int kb = k0; kb < k1; ++kb) {
+            for (int seg = 0; seg < g.segments && ok; ++seg) {
+                int lo, hi;
+                part(seg, lo, hi);
+                const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
+                const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? 0 : seg];
+                for (int kb = lo; kb < hi; ++kb) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
                         ok = false;
                         break;
@@ -176,23 +187,23 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 #pragma unroll
                     for (int p = 0; p < S::PARTS; ++p) {
                         const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
-                        if (g.a_mn[seg]) {
-                            tma_load_3d(at, &g.a[seg], bar, mt * 128, kb * 64, p);
-                            tma_load_3d(at + 8192, &g.a[seg], bar, mt * 128 + 64, kb * 64, p);
+                        if (a_mn) {
+                            tma_load_3d(at, ma, bar, mt * 128, kb * 64, p);
+                            tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, p);
                         } else {
-                            tma_load_3d(at, &g.a[seg], bar, kb * 64, mt * 128, p);
+                            tma_load_3d(at, ma, bar, kb * 64, mt * 128, p);
                         }
                         if constexpr (DUAL) {
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                if (g.b_mn[0]) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
+                                if (b_mn) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
                                 else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, p);
                             }
-                        } else if (g.b_mn[seg]) {
-                            tma_load_3d(bt, &g.b[seg], bar, nt * 128, kb * 64, p);
-                            tma_load_3d(bt + 8192, &g.b[seg], bar, nt * 128 + 64, kb * 64, p);
+                        } else if (b_mn) {
+                            tma_load_3d(bt, mb, bar, nt * 128, kb * 64, p);
+                            tma_load_3d(bt + 8192, mb, bar, nt * 128 + 64, kb * 64, p);
                         } else {
-                            tma_load_3d(bt, &g.b[seg], bar, kb * 64, nt * 128, p);
+                            tma_load_3d(bt, mb, bar, kb * 64, nt * 128, p);
                         }
                     }
                     issued[stage] = static_cast<int>(phase);
@@ -216,53 +227,66 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             const uint32_t small = tmem + 256;  // binary32: the five lesser products
-            for (int u = u0; u < u1 && ok; ++u) {
-                int seg, k0, k1;
-                unit(u, seg, k0, k1);
+            bool begun = false;
+            for (int seg = 0; seg < g.segments && ok; ++seg) {
+                int lo, hi;
+                part(seg, lo, hi);
                 const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
                 const uint32_t id = idesc(F32, a_mn, b_mn, 128, 128);
-                if (F32) {
-                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
-                    tc_fence_after();
-                }
-                const uint32_t d = F32 ? tmem + acc * 128 : tmem;
-                for (int kb = k0; kb < k1; ++kb) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
-                        ok = false;
-                        break;
+                const Walk wa = walk_of(a_tile(0, 0), a_mn), wb = walk_of(b_tile(0, 0), b_mn);
+                // binary32: a drain every CHUNK k-blocks; else none inside
+                for (int k0 = lo; k0 < hi && ok; k0 += F32 ? CHUNK : hi) {
+                    const int k1 = F32 ? min(k0 + CHUNK, hi) : hi;
+                    if (F32) {
+                        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
                     }
-                    tc_fence_after();
-                    auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+                    const uint32_t d = F32 ? tmem + acc * 128 : tmem;
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t as = wa.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                        const uint64_t bs = wb.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                        auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_f16(dst, slice_desc(a_tile(stage, pa), a_mn, k), slice_desc(b_tile(stage, pb), b_mn, k), id,
-                                    fresh && k == 0 ? 0u : 1u);
-                    };
-                    if constexpr (F32) {
-                        product(0, 2, small, u == u0 && kb == k0);
-                        product(2, 0, small, false);
-                        product(1, 1, small, false);
-                        product(0, 1, small, false);
-                        product(1, 0, small, false);
-                        product(0, 0, d, kb == k0);
-                    } else {
-                        product(0, 0, d, u == u0);
+                            for (int k = 0; k < 4; ++k)
+                                mma_f16(dst, as + static_cast<uint32_t>(pa * (TILE_BYTES >> 4)) + k * wa.step,
+                                        bs + static_cast<uint32_t>(pb * (TILE_BYTES >> 4)) + k * wb.step, id,
+                                        fresh && k == 0 ? 0u : 1u);
+                        };
+                        if constexpr (F32) {
+                            product(0, 2, small, !begun);
+                            product(2, 0, small, false);
+                            product(1, 1, small, false);
+                            product(0, 1, small, false);
+                            product(1, 0, small, false);
+                            product(0, 0, d, kb == k0);
+                        } else {
+                            product(0, 0, d, !begun);
+                        }
+                        begun = true;
+                        mma_commit(empty_bar(stage));
+                        if (++stage == S::STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
-                    mma_commit(empty_bar(stage));
-                    if (++stage == S::STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-                if (!ok) break;
-                if (F32 || u + 1 == u1) {
-                    mma_commit(tfull_bar(acc));
-                    if (++acc == 2) {
-                        acc = 0;
-                        acc_phase ^= 1u;
+                    if (F32 && ok) {
+                        mma_commit(tfull_bar(acc));
+                        if (++acc == 2) {
+                            acc = 0;
+                            acc_phase ^= 1u;
+                        }
                     }
                 }
             }
+            if (!F32 && ok) mma_commit(tfull_bar(0));
             mma_commit(drain_bar);
             const long long t0 = clock64();
             while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
@@ -375,7 +399,9 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 add(from, c, z);
                 if constexpr (DUAL) add(from, 64 + c, u);
             }
-            finish8<T, DUAL>(g.e, static_cast<int64_t>(mt) * 128 + r, col, z, u);
+            float bias[DUAL ? 2 : 1][8];
+            bias8<T, DUAL>(g.e, col, bias);
+            finish8<T, DUAL>(g.e, static_cast<int64_t>(mt) * 128 + r, col, bias, z, u);
         }
     } else if (threadIdx.x == 0) {
         atomicExch(g.status, QSML_E_TIMEOUT);
@@ -403,12 +429,14 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 // ---------------------------------------------------------------------------
 template <bool F32> struct PairShape {
     static constexpr int PARTS = F32 ? 3 : 1;
-    static constexpr int STAGES = F32 ? 3 : 6;
+    static constexpr int STAGES = F32 ? 3 : 5;
+    static constexpr int EPI = F32 ? 4 : 8;                   // epilogue warps
+    static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BCOLS = F32 ? 64 : 128;              // columns of B a CTA
     static constexpr int B_BYTES = BCOLS * 128;
     static constexpr int STAGE = PARTS * (TILE_BYTES + B_BYTES);
     static constexpr int NACC = 2 * BCOLS;                    // accumulator columns
-    static constexpr int OUT = F32 ? 0 : 4 * 8192;            // epilogue staging, 8 KiB a warp
+    static constexpr int OUT = F32 ? 0 : EPI * 8192;          // epilogue staging, 8 KiB a warp
     static constexpr size_t SMEM = size_t(STAGES) * STAGE + OUT + 1024 + 256;
     static_assert(SMEM <= 232448, "shared memory");
 };
@@ -424,7 +452,7 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b,
 }
 
 template <bool F32, bool DUAL>
-__global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constant__ TcArgs g) {
+__global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(const __grid_constant__ TcArgs g) {
     using T = std::conditional_t<F32, float, __half>;
     using S = PairShape<F32>;
     extern __shared__ unsigned char smem_raw[];
@@ -453,8 +481,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 8);  // 4 epilogue warps in each CTA
-            mbar_init(sempty_bar(a), 8);
+            mbar_init(tempty_bar(a), 2 * S::EPI);  // the epilogue warps of both CTAs
+            mbar_init(sempty_bar(a), 2 * S::EPI);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -485,13 +513,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
         mt = first + within % gm;
         nt = within / gm;
     };
-    const int per_seg = F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb;
-    const int units = per_seg * g.segments;
-    auto unit = [&](int u, int& seg, int& k0, int& k1) {
-        seg = u / per_seg;
-        k0 = (u - seg * per_seg) * (F32 ? CHUNK : 1);
-        k1 = F32 ? min(k0 + CHUNK, g.kb) : k0 + 1;
-    };
+    // binary32: drains a tile (the CHUNK k-blocks between them counted by segment)
+    const int drains = (g.kb + CHUNK - 1) / CHUNK * g.segments;
     auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
     auto b_tile = [&](int s, int p) { return base + s * S::STAGE + S::PARTS * TILE_BYTES + p * S::B_BYTES; };
 
@@ -505,12 +528,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
                 decode(t, mt, nt);
                 const int row = mt * 256 + static_cast<int>(rank) * 128;
                 const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
-                for (int u = 0; u < units && ok; ++u) {
-                    int seg, k0, k1;
-                    unit(u, seg, k0, k1);
-                    const CUtensorMap* mb = &g.b[DUAL ? rank : seg];
-                    const int b_mn = g.b_mn[DUAL ? 0 : seg];
-                    for (int kb = k0; kb < k1; ++kb) {
+                for (int seg = 0; seg < g.segments && ok; ++seg) {
+                    const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
+                    const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
+                    for (int kb = 0; kb < g.kb; ++kb) {
                         if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
                             ok = false;
                             break;
@@ -520,11 +541,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
                             const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
-                            if (g.a_mn[seg]) {
-                                tma_load_3d_pair(at, &g.a[seg], bar, row, kb * 64, p);
-                                tma_load_3d_pair(at + 8192, &g.a[seg], bar, row + 64, kb * 64, p);
+                            if (a_mn) {
+                                tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
+                                tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
                             } else {
-                                tma_load_3d_pair(at, &g.a[seg], bar, kb * 64, row, p);
+                                tma_load_3d_pair(at, ma, bar, kb * 64, row, p);
                             }
                             if (b_mn) {
 #pragma unroll
@@ -553,54 +574,72 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
                     tc_fence_after();
                 }
                 const uint32_t small = tmem + 256 + par * 128;
-                for (int u = 0; u < units && ok; ++u) {
-                    int seg, k0, k1;
-                    unit(u, seg, k0, k1);
+                if (!F32) {
+                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
+                    tc_fence_after();
+                }
+                bool begun = false;
+                for (int seg = 0; seg < g.segments && ok; ++seg) {
                     const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
                     const uint32_t id = idesc(F32, a_mn, b_mn, 256, S::NACC);
-                    if (F32 || u == 0) {
-                        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
-                            ok = false;
-                            break;
+                    const Walk wa = walk_of(a_tile(0, 0), a_mn), wb = walk_of(b_tile(0, 0), b_mn);
+                    for (int k0 = 0; k0 < g.kb && ok; k0 += F32 ? CHUNK : g.kb) {
+                        const int k1 = F32 ? min(k0 + CHUNK, g.kb) : g.kb;
+                        if (F32) {
+                            if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
                         }
-                        tc_fence_after();
-                    }
-                    const uint32_t d = tmem + acc * S::NACC;
-                    for (int kb = k0; kb < k1; ++kb) {
-                        if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+                        const uint32_t d = tmem + acc * S::NACC;
+                        for (int kb = k0; kb < k1; ++kb) {
+                            if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const uint64_t as = wa.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                            const uint64_t bs = wb.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                            auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma_f16_pair(dst, slice_desc(a_tile(stage, pa), a_mn, k),
-                                             slice_desc(b_tile(stage, pb), b_mn, k), id, fresh && k == 0 ? 0u : 1u);
-                        };
-                        if constexpr (F32) {
-                            product(0, 2, small, u == 0 && kb == k0);
-                            product(2, 0, small, false);
-                            product(1, 1, small, false);
-                            product(0, 1, small, false);
-                            product(1, 0, small, false);
-                            product(0, 0, d, kb == k0);
-                        } else {
-                            product(0, 0, d, u == 0);
+                                for (int k = 0; k < 4; ++k)
+                                    mma_f16_pair(dst, as + static_cast<uint32_t>(pa * (TILE_BYTES >> 4)) + k * wa.step,
+                                                 bs + static_cast<uint32_t>(pb * (S::B_BYTES >> 4)) + k * wb.step, id,
+                                                 fresh && k == 0 ? 0u : 1u);
+                            };
+                            if constexpr (F32) {
+                                product(0, 2, small, !begun);
+                                product(2, 0, small, false);
+                                product(1, 1, small, false);
+                                product(0, 1, small, false);
+                                product(1, 0, small, false);
+                                product(0, 0, d, kb == k0);
+                            } else {
+                                product(0, 0, d, !begun);
+                            }
+                            begun = true;
+                            mma_commit_pair(empty_bar(stage));
+                            if (++stage == S::STAGES) {
+                                stage = 0;
+                                phase ^= 1u;
+                            }
                         }
-                        mma_commit_pair(empty_bar(stage));
-                        if (++stage == S::STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
+                        if (F32 && ok) {
+                            mma_commit_pair(tfull_bar(acc));
+                            if (++acc == 2) {
+                                acc = 0;
+                                acc_phase ^= 1u;
+                            }
                         }
                     }
-                    if (!ok) break;
-                    if (F32 || u + 1 == units) {
-                        mma_commit_pair(tfull_bar(acc));
-                        if (++acc == 2) {
-                            acc = 0;
-                            acc_phase ^= 1u;
-                        }
+                }
+                if (!ok) break;
+                if (!F32) {
+                    mma_commit_pair(tfull_bar(acc));
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1u;
                     }
                 }
                 if (++par == 2) {
@@ -649,7 +688,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
-                for (int u = 0; u < units; ++u) {
+                for (int u = 0; u < drains; ++u) {
                     if (!ready()) {
                         ok = false;
                         break;
@@ -685,16 +724,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
                             z[i] = sum[c / 4][(c % 4) * 8 + i];
                             v[i] = DUAL ? sum[c / 4 + 2 * (DUAL ? 1 : 0)][(c % 4) * 8 + i] : 0.0f;
                         }
-                        finish8<T, DUAL>(g.e, row0 + lane, col0 + c * 8, z, v);
+                        float bias[DUAL ? 2 : 1][8];
+                        bias8<T, DUAL>(g.e, col0 + c * 8, bias);
+                        finish8<T, DUAL>(g.e, row0 + lane, col0 + c * 8, bias, z, v);
                     }
                 }
             } else {
                 if (!ready()) break;
-                const uint32_t stage = out_stage + quarter * 8192;  // 32 rows of 64 binary32, units swapped by row
+                // two warps a quarter of the rows, each half of the columns
+                const uint32_t stage = out_stage + (warp - 2) * 8192;  // 32 rows of 64 binary32, units swapped by row
                 const uint32_t d = lanes + acc * S::NACC;
                 constexpr int STEP = DUAL ? 32 : 64;
-                const int cend = static_cast<int>(g.N - col0 < BN ? g.N - col0 : BN);
-                for (int c0 = 0; c0 < cend; c0 += STEP) {
+                const int cbegin = warp >= 6 ? BN / 2 : 0;
+                const int cend = static_cast<int>(min(g.N - col0, static_cast<int64_t>(cbegin + BN / 2)));
+                if (cbegin >= cend) release(tempty_bar(acc));
+                for (int c0 = cbegin; c0 < cend; c0 += STEP) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t r[32];
@@ -724,13 +768,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_pair(const __grid_constan
                         }
                     };
                     if (col < g.N) {
+                        float bias[DUAL ? 2 : 1][8];
+                        bias8<T, DUAL>(g.e, col, bias);
 #pragma unroll 2
                         for (int r = lane / UNITS; r < 32; r += ROWS) {
                             if (row0 + r >= g.M) break;
                             float z[8], v[8];
                             take(r, un * 2, z);
                             if constexpr (DUAL) take(r, 8 + un * 2, v);
-                            finish8<T, DUAL>(g.e, row0 + r, col, z, v);
+                            finish8<T, DUAL>(g.e, row0 + r, col, bias, z, v);
                         }
                     }
                     __syncwarp();
@@ -861,7 +907,7 @@ template <bool F32, bool DUAL> qsml_status_t max_pairs(Context* ctx, int* pairs)
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.gridDim = dim3(2 * (ctx->num_sms / 2));
-        cfg.blockDim = dim3(THREADS);
+        cfg.blockDim = dim3(PairShape<F32>::THREADS);
         cfg.dynamicSmemBytes = PairShape<F32>::SMEM;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
@@ -891,7 +937,7 @@ template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Pro
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
@@ -957,7 +1003,7 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
     else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &pairs) : max_pairs<false, false>(ctx, &pairs)));
     const int64_t bn = (f32 ? 128 : 256) / (p.dual ? 2 : 1);
     const int64_t tiles = ((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
-    const bool pair = pairs > 0 && tiles >= pairs;
+    const bool pair = pairs > 0 && p.M > 128 && tiles >= pairs;
 
     Workspace ws(ctx);
     TcArgs g;
