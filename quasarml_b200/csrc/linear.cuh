@@ -136,6 +136,27 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, b
         for (int i = 0; i < 8; ++i) v[i] = i < n ? ld1(p + i) : 0.0f;
     }
 }
+// The same through the read-only path, for inputs that nothing writes meanwhile.
+template <typename T> __device__ __forceinline__ void ldg8(const T* p, int n, bool vec, float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(h[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        } else {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+    } else {
+        load8(p, n, false, v);
+    }
+}
 template <typename T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
     if constexpr (sizeof(T) == 2) {
         if (vec) {

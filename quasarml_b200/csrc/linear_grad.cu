@@ -14,7 +14,7 @@ namespace {
 // A warp takes 256 columns (8 a lane), a CTA's 8 warps every 8th row of
 // [blockIdx.y * chunk, + chunk).  A thread keeps its columns and sums them in
 // registers; the warps' sums are added in warp order in shared memory.
-template <typename T, bool DUAL>
+template <typename T, bool DUAL, int ACT>
 __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, bool vec) {
     pdl_begin();
     constexpr int NO = DUAL ? 2 : 1;
@@ -29,19 +29,20 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[o][i] = 0.0f;
     if (n > 0) {
+        // inputs by the read-only path: no output of the call overlaps them
 #pragma unroll 2
         for (int64_t r = r0 + w; r < r1; r += 8) {
             float dy[8], z[8], u[8], d[NO][8];
-            load8(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec, dy);
-            if (a.pre[0]) load8(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec, z);
-            if constexpr (DUAL) load8(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec, u);
+            ldg8(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec, dy);
+            if (DUAL || ACT != QSML_ACT_NONE) ldg8(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec, z);
+            if constexpr (DUAL) ldg8(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (!a.pre[0]) {
+                if constexpr (!DUAL && ACT == QSML_ACT_NONE) {
                     d[0][i] = dy[i];
                 } else {
                     float value;
-                    const float g = act_grad<T>(a.act, z[i], value);
+                    const float g = act_grad<T>(ACT, z[i], value);
                     if constexpr (DUAL) {
                         d[0][i] = __fmul_rn(__fmul_rn(dy[i], u[i]), g);
                         d[1][i] = __fmul_rn(dy[i], value);
@@ -90,7 +91,14 @@ template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradAr
     a.partial = static_cast<float*>(partial);
     bool vec = a.N % 8 == 0 && a.dy_ld % 8 == 0 && aligned16(a.dy);
     for (int i = 0; i < 2; ++i) vec = vec && (!a.pre[i] || aligned16(a.pre[i]));
-    const cudaError_t e = launch_pdl(k_linear_dz<T, DUAL>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
+    auto kernel = k_linear_dz<T, DUAL, QSML_ACT_NONE>;
+    switch (a.act) {
+        case QSML_ACT_RELU: kernel = k_linear_dz<T, DUAL, QSML_ACT_RELU>; break;
+        case QSML_ACT_GELU: kernel = k_linear_dz<T, DUAL, QSML_ACT_GELU>; break;
+        case QSML_ACT_SILU: kernel = k_linear_dz<T, DUAL, QSML_ACT_SILU>; break;
+        case QSML_ACT_SIGMOID: kernel = k_linear_dz<T, DUAL, QSML_ACT_SIGMOID>; break;
+    }
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
                                      dim3(256), 0, ctx->stream, a, chunk, vec);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_dz");
     QSML_TRY_STATUS(after_launch(ctx, "k_linear_dz"));

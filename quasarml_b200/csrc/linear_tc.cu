@@ -44,16 +44,20 @@ struct TcArgs {
     int kb;                  // k-blocks of 64 a segment
     int segments;
     int splits;
+    int a_bytes;             // k_linear_tc: of an operand tile of A (fewer than 128 rows where M has fewer)
+    int slots;               // k_linear_tc: operand tiles of A and B in the ring
     int a_mn[2], b_mn[2];    // MN-major operands, by segment
     int* status;
 };
 
+// A ring of slots in shared memory, each a tile of A and one of B (of one part, for
+// binary32: a k-block takes three).  Binary16 has two CTAs a SM.
 template <bool F32> struct Shape {
     static constexpr int PARTS = F32 ? 3 : 1;
-    static constexpr int STAGES = F32 ? 2 : 3;
-    static constexpr int STAGE = 2 * PARTS * TILE_BYTES;
+    static constexpr int MAX_SLOTS = F32 ? 6 : 5;
     static constexpr int TMEM = F32 ? 512 : 128;
-    static constexpr size_t SMEM = size_t(STAGES) * STAGE + 1024 + 128;
+    static constexpr size_t RING = F32 ? 6 * 32768 : 3 * 32768;
+    static constexpr size_t SMEM = RING + 1024 + 144;
     static constexpr int CTAS = F32 ? 1 : 2;  // a SM
 };
 
@@ -110,19 +114,20 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* gbase = smem_raw + (base - raw);
-    const uint32_t bars = base + S::STAGES * S::STAGE;
+    const uint32_t bars = base + S::RING;
     auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };
-    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + a); };
-    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 + a); };
-    const uint32_t drain_bar = bars + 8u * (2 * S::STAGES + 4);
-    unsigned char* misc = gbase + S::STAGES * S::STAGE + 8 * (2 * S::STAGES + 5);
+    auto empty_bar = [&](int s) { return bars + 8u * (S::MAX_SLOTS + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::MAX_SLOTS + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::MAX_SLOTS + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * S::MAX_SLOTS + 4);
+    unsigned char* misc = gbase + S::RING + 8 * (2 * S::MAX_SLOTS + 5);
+    static_assert(8 * (2 * S::MAX_SLOTS + 5) + 8 <= 144, "barriers");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) {
+        for (int s = 0; s < g.slots; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
@@ -161,32 +166,30 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         lo = max(u0 - seg * per_seg, 0) * (F32 ? CHUNK : 1);
         hi = min(max(u1 - seg * per_seg, 0) * (F32 ? CHUNK : 1), g.kb);
     };
-    auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
-    auto b_tile = [&](int s, int p) { return base + s * S::STAGE + (S::PARTS + p) * TILE_BYTES; };
+    // A's tile comes first: where it has fewer than 128 rows the MMA takes the rest
+    // from B's, for rows of the result that are not there
+    const uint32_t slot_bytes = g.a_bytes + TILE_BYTES;
 
     bool done = true;  // epilogue warps: the CTA's sums are complete
     if (warp == 0) {
         if (lane == 0) {
-            int stage = 0;
+            int slot = 0, filled = 0;
             uint32_t phase = 0;
-            int issued[S::STAGES];
-            for (int s = 0; s < S::STAGES; ++s) issued[s] = -1;
             bool ok = true;
             for (int seg = 0; seg < g.segments && ok; ++seg) {
                 int lo, hi;
                 part(seg, lo, hi);
                 const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
                 const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? 0 : seg];
-                for (int kb = lo; kb < hi; ++kb) {
-                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t bar = full_bar(stage);
-                    mbar_expect_tx(bar, S::STAGE);
+                for (int kb = lo; kb < hi && ok; ++kb) {
 #pragma unroll
                     for (int p = 0; p < S::PARTS; ++p) {
-                        const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
+                        if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t bar = full_bar(slot), at = base + slot * slot_bytes, bt = at + g.a_bytes;
+                        mbar_expect_tx(bar, slot_bytes);
                         if (a_mn) {
                             tma_load_3d(at, ma, bar, mt * 128, kb * 64, p);
                             tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, p);
@@ -205,25 +208,26 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         } else {
                             tma_load_3d(bt, mb, bar, kb * 64, nt * 128, p);
                         }
-                    }
-                    issued[stage] = static_cast<int>(phase);
-                    if (++stage == S::STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
+                        ++filled;
+                        if (++slot == g.slots) {
+                            slot = 0;
+                            phase ^= 1u;
+                        }
                     }
                 }
             }
-            // every copy this thread started lands before the memory has another use
-            for (int s = 0; s < S::STAGES; ++s) {
-                if (issued[s] < 0) continue;
+            // every copy this thread started lands before the memory has another use:
+            // the last fill of each slot (fill i is in slot i % slots, phase i / slots)
+            for (int i = max(0, filled - g.slots); i < filled; ++i) {
+                const uint32_t parity = static_cast<uint32_t>((i / g.slots) & 1);
                 const long long t0 = clock64();
-                while (!mbar_test(full_bar(s), static_cast<uint32_t>(issued[s])) && clock64() - t0 < WAIT_CYCLES) {
+                while (!mbar_test(full_bar(i % g.slots), parity) && clock64() - t0 < WAIT_CYCLES) {
                 }
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            int stage = 0, acc = 0;
+            int slot = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             const uint32_t small = tmem + 256;  // binary32: the five lesser products
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 part(seg, lo, hi);
                 const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
                 const uint32_t id = idesc(F32, a_mn, b_mn, 128, 128);
-                const Walk wa = walk_of(a_tile(0, 0), a_mn), wb = walk_of(b_tile(0, 0), b_mn);
+                const Walk wa = walk_of(base, a_mn), wb = walk_of(base + g.a_bytes, b_mn);
                 // binary32: a drain every CHUNK k-blocks; else none inside
                 for (int k0 = lo; k0 < hi && ok; k0 += F32 ? CHUNK : hi) {
                     const int k1 = F32 ? min(k0 + CHUNK, hi) : hi;
@@ -245,37 +249,46 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         tc_fence_after();
                     }
                     const uint32_t d = F32 ? tmem + acc * 128 : tmem;
-                    for (int kb = k0; kb < k1; ++kb) {
-                        if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint64_t as = wa.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
-                        const uint64_t bs = wb.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                    for (int kb = k0; kb < k1 && ok; ++kb) {
+                        int at[S::PARTS] = {};  // the parts' slots
                         auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+                            const uint64_t as = wa.first + static_cast<uint32_t>(at[pa] * (slot_bytes >> 4));
+                            const uint64_t bs = wb.first + static_cast<uint32_t>(at[pb] * (slot_bytes >> 4));
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                mma_f16(dst, as + static_cast<uint32_t>(pa * (TILE_BYTES >> 4)) + k * wa.step,
-                                        bs + static_cast<uint32_t>(pb * (TILE_BYTES >> 4)) + k * wb.step, id,
-                                        fresh && k == 0 ? 0u : 1u);
+                                mma_f16(dst, as + k * wa.step, bs + k * wb.step, id, fresh && k == 0 ? 0u : 1u);
                         };
-                        if constexpr (F32) {
-                            product(0, 2, small, !begun);
-                            product(2, 0, small, false);
-                            product(1, 1, small, false);
-                            product(0, 1, small, false);
-                            product(1, 0, small, false);
-                            product(0, 0, d, kb == k0);
-                        } else {
-                            product(0, 0, d, !begun);
+#pragma unroll
+                        for (int p = 0; p < S::PARTS; ++p) {
+                            if (!mbar_wait(full_bar(slot), phase, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            at[p] = slot;
+                            if (++slot == g.slots) {
+                                slot = 0;
+                                phase ^= 1u;
+                            }
+                            if constexpr (F32) {
+                                if (p == 0) {
+                                    product(0, 0, d, kb == k0);
+                                } else if (p == 1) {
+                                    product(1, 1, small, !begun);
+                                    product(0, 1, small, false);
+                                    product(1, 0, small, false);
+                                } else {
+                                    product(0, 2, small, false);
+                                    product(2, 0, small, false);
+                                }
+                            } else {
+                                product(0, 0, d, !begun);
+                            }
                         }
+                        if (!ok) break;
                         begun = true;
-                        mma_commit(empty_bar(stage));
-                        if (++stage == S::STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+#pragma unroll
+                        for (int p = 0; p < S::PARTS; ++p) mma_commit(empty_bar(at[p]));
                     }
                     if (F32 && ok) {
                         mma_commit(tfull_bar(acc));
@@ -382,23 +395,31 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             const int64_t col = static_cast<int64_t>(nt) * BN + c;
             if (col >= g.N) continue;
             float z[8], u[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = u[j] = 0.0f;
-            auto add = [&](uint32_t tile_base, int cc, float (&v)[8]) {
+            // the cluster's tiles, all loads under way together, added in rank order
+            auto sum = [&](int cc, float (&v)[8]) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float4 q = ld_cluster(tile_base + r * 512 + (((cc / 4 + h) ^ (r & 31)) << 4));
-                    v[4 * h] = __fadd_rn(v[4 * h], q.x);
-                    v[4 * h + 1] = __fadd_rn(v[4 * h + 1], q.y);
-                    v[4 * h + 2] = __fadd_rn(v[4 * h + 2], q.z);
-                    v[4 * h + 3] = __fadd_rn(v[4 * h + 3], q.w);
+                    float4 q[MAX_SPLIT];
+#pragma unroll
+                    for (int s = 0; s < MAX_SPLIT; ++s)
+                        if (s < g.splits) q[s] = ld_cluster(map_to_rank(base, s) + r * 512 + (((cc / 4 + h) ^ (r & 31)) << 4));
+                    float4 t = q[0];
+#pragma unroll
+                    for (int s = 1; s < MAX_SPLIT; ++s)
+                        if (s < g.splits) {
+                            t.x = __fadd_rn(t.x, q[s].x);
+                            t.y = __fadd_rn(t.y, q[s].y);
+                            t.z = __fadd_rn(t.z, q[s].z);
+                            t.w = __fadd_rn(t.w, q[s].w);
+                        }
+                    v[4 * h] = t.x;
+                    v[4 * h + 1] = t.y;
+                    v[4 * h + 2] = t.z;
+                    v[4 * h + 3] = t.w;
                 }
             };
-            for (int s = 0; s < g.splits; ++s) {
-                const uint32_t from = map_to_rank(base, s);
-                add(from, c, z);
-                if constexpr (DUAL) add(from, 64 + c, u);
-            }
+            sum(c, z);
+            if constexpr (DUAL) sum(64 + c, u);
             float bias[DUAL ? 2 : 1][8];
             bias8<T, DUAL>(g.e, col, bias);
             finish8<T, DUAL>(g.e, static_cast<int64_t>(mt) * 128 + r, col, bias, z, u);
@@ -420,8 +441,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 // under the products of the next.
 //   binary16: 256 x 256 of the result a pair (dual: 128 columns of each weight, one
 //     from each CTA), six stages of 32 KiB a CTA, two accumulators of 256 columns;
-//   binary32: 256 x 128 (dual: 64 of each), three stages of all parts (72 KiB a CTA),
-//     two accumulators for the drains of the main product and two, by tile, for the
+//   binary32: 256 x 128 (dual: 64 of each), eight slots of one part (24 KiB a CTA), two accumulators for the drains of the main product and two, by tile, for the
 //     lesser ones.
 // Each CTA loads its own 128 rows of A and half of the tile's columns of B; the
 // leader issues the MMAs of both.  Roles and barriers as in k_linear_tc, the
@@ -429,15 +449,15 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 // ---------------------------------------------------------------------------
 template <bool F32> struct PairShape {
     static constexpr int PARTS = F32 ? 3 : 1;
-    static constexpr int STAGES = F32 ? 3 : 5;
-    static constexpr int EPI = F32 ? 4 : 8;                   // epilogue warps
+    static constexpr int SLOTS = F32 ? 8 : 5;                 // a tile of A and one of B each, of one part
+    static constexpr int EPI = 8;                             // epilogue warps
     static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BCOLS = F32 ? 64 : 128;              // columns of B a CTA
-    static constexpr int B_BYTES = BCOLS * 128;
-    static constexpr int STAGE = PARTS * (TILE_BYTES + B_BYTES);
+    static constexpr int SLOT = TILE_BYTES + BCOLS * 128;
     static constexpr int NACC = 2 * BCOLS;                    // accumulator columns
-    static constexpr int OUT = F32 ? 0 : EPI * 8192;          // epilogue staging, 8 KiB a warp
-    static constexpr size_t SMEM = size_t(STAGES) * STAGE + OUT + 1024 + 256;
+    static constexpr int OUT_WARP = F32 ? 4096 : 8192;        // epilogue staging: 32 rows of 32 (64) binary32
+    static constexpr int OUT = EPI * OUT_WARP;
+    static constexpr size_t SMEM = size_t(SLOTS) * SLOT + OUT + 1024 + 256;
     static_assert(SMEM <= 232448, "shared memory");
 };
 constexpr int PAIR_GROUP_M = 16;  // tiles of 16 row blocks run together: A and B panels stay in L2
@@ -459,15 +479,15 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* gbase = smem_raw + (base - raw);
-    const uint32_t out_stage = base + S::STAGES * S::STAGE;
+    const uint32_t out_stage = base + S::SLOTS * S::SLOT;
     const uint32_t bars = out_stage + S::OUT;
     auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };
-    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + a); };
-    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 + a); };
-    auto sempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 4 + a); };  // binary32: lesser products read
-    const uint32_t drain_bar = bars + 8u * (2 * S::STAGES + 6);
-    unsigned char* misc = gbase + S::STAGES * S::STAGE + S::OUT + 8 * (2 * S::STAGES + 7);
+    auto empty_bar = [&](int s) { return bars + 8u * (S::SLOTS + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::SLOTS + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::SLOTS + 2 + a); };
+    auto sempty_bar = [&](int a) { return bars + 8u * (2 * S::SLOTS + 4 + a); };  // binary32: lesser products read
+    const uint32_t drain_bar = bars + 8u * (2 * S::SLOTS + 6);
+    unsigned char* misc = gbase + S::SLOTS * S::SLOT + S::OUT + 8 * (2 * S::SLOTS + 7);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
@@ -475,7 +495,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     const bool leader = rank == 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) {
+        for (int s = 0; s < S::SLOTS; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
@@ -515,12 +535,9 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     };
     // binary32: drains a tile (the CHUNK k-blocks between them counted by segment)
     const int drains = (g.kb + CHUNK - 1) / CHUNK * g.segments;
-    auto a_tile = [&](int s, int p) { return base + s * S::STAGE + p * TILE_BYTES; };
-    auto b_tile = [&](int s, int p) { return base + s * S::STAGE + S::PARTS * TILE_BYTES + p * S::B_BYTES; };
-
     if (warp == 0) {
         if (lane == 0) {
-            int stage = 0;
+            int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += pairs) {
@@ -531,16 +548,16 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 for (int seg = 0; seg < g.segments && ok; ++seg) {
                     const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
                     const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
-                    for (int kb = 0; kb < g.kb; ++kb) {
-                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, limit)) {
-                            ok = false;
-                            break;
-                        }
-                        if (leader) mbar_expect_tx(full_bar(stage), 2 * S::STAGE);
-                        const uint32_t bar = map_to_rank(full_bar(stage), 0);
+                    for (int kb = 0; kb < g.kb && ok; ++kb) {
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
-                            const uint32_t at = a_tile(stage, p), bt = b_tile(stage, p);
+                            if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            if (leader) mbar_expect_tx(full_bar(slot), 2 * S::SLOT);
+                            const uint32_t bar = map_to_rank(full_bar(slot), 0);
+                            const uint32_t at = base + slot * S::SLOT, bt = at + TILE_BYTES;
                             if (a_mn) {
                                 tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
                                 tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
@@ -554,10 +571,10 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             } else {
                                 tma_load_3d_pair(bt, mb, bar, kb * 64, col, p);
                             }
-                        }
-                        if (++stage == S::STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
+                            if (++slot == S::SLOTS) {
+                                slot = 0;
+                                phase ^= 1u;
+                            }
                         }
                     }
                 }
@@ -565,7 +582,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
-            int stage = 0, acc = 0, par = 0;
+            int slot = 0, acc = 0, par = 0;
             uint32_t phase = 0, acc_phase = 0, par_phase = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += pairs) {
@@ -582,7 +599,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 for (int seg = 0; seg < g.segments && ok; ++seg) {
                     const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
                     const uint32_t id = idesc(F32, a_mn, b_mn, 256, S::NACC);
-                    const Walk wa = walk_of(a_tile(0, 0), a_mn), wb = walk_of(b_tile(0, 0), b_mn);
+                    const Walk wa = walk_of(base, a_mn), wb = walk_of(base + TILE_BYTES, b_mn);
                     for (int k0 = 0; k0 < g.kb && ok; k0 += F32 ? CHUNK : g.kb) {
                         const int k1 = F32 ? min(k0 + CHUNK, g.kb) : g.kb;
                         if (F32) {
@@ -593,37 +610,46 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             tc_fence_after();
                         }
                         const uint32_t d = tmem + acc * S::NACC;
-                        for (int kb = k0; kb < k1; ++kb) {
-                            if (!mbar_wait(full_bar(stage), phase, abort_flag, limit)) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            const uint64_t as = wa.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
-                            const uint64_t bs = wb.first + static_cast<uint32_t>(stage * (S::STAGE >> 4));
+                        for (int kb = k0; kb < k1 && ok; ++kb) {
+                            int at[S::PARTS] = {};  // the parts' slots
                             auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+                                const uint64_t as = wa.first + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
+                                const uint64_t bs = wb.first + static_cast<uint32_t>(at[pb] * (S::SLOT >> 4));
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
-                                    mma_f16_pair(dst, as + static_cast<uint32_t>(pa * (TILE_BYTES >> 4)) + k * wa.step,
-                                                 bs + static_cast<uint32_t>(pb * (S::B_BYTES >> 4)) + k * wb.step, id,
-                                                 fresh && k == 0 ? 0u : 1u);
+                                    mma_f16_pair(dst, as + k * wa.step, bs + k * wb.step, id, fresh && k == 0 ? 0u : 1u);
                             };
-                            if constexpr (F32) {
-                                product(0, 2, small, !begun);
-                                product(2, 0, small, false);
-                                product(1, 1, small, false);
-                                product(0, 1, small, false);
-                                product(1, 0, small, false);
-                                product(0, 0, d, kb == k0);
-                            } else {
-                                product(0, 0, d, !begun);
+#pragma unroll
+                            for (int p = 0; p < S::PARTS; ++p) {
+                                if (!mbar_wait(full_bar(slot), phase, abort_flag, limit)) {
+                                    ok = false;
+                                    break;
+                                }
+                                tc_fence_after();
+                                at[p] = slot;
+                                if (++slot == S::SLOTS) {
+                                    slot = 0;
+                                    phase ^= 1u;
+                                }
+                                if constexpr (F32) {
+                                    if (p == 0) {
+                                        product(0, 0, d, kb == k0);
+                                    } else if (p == 1) {
+                                        product(1, 1, small, !begun);
+                                        product(0, 1, small, false);
+                                        product(1, 0, small, false);
+                                    } else {
+                                        product(0, 2, small, false);
+                                        product(2, 0, small, false);
+                                    }
+                                } else {
+                                    product(0, 0, d, !begun);
+                                }
                             }
+                            if (!ok) break;
                             begun = true;
-                            mma_commit_pair(empty_bar(stage));
-                            if (++stage == S::STAGES) {
-                                stage = 0;
-                                phase ^= 1u;
-                            }
+#pragma unroll
+                            for (int p = 0; p < S::PARTS; ++p) mma_commit_pair(empty_bar(at[p]));
                         }
                         if (F32 && ok) {
                             mma_commit_pair(tfull_bar(acc));
@@ -681,62 +707,94 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
             decode(t, mt, nt);
             const int row0 = mt * 256 + static_cast<int>(rank) * 128 + quarter * 32;  // first of the warp's 32 rows
             const int64_t col0 = static_cast<int64_t>(nt) * BN;
-            if constexpr (F32) {
-                // a thread has a row of the tile in registers (128 columns)
-                float sum[4][32];
+            // two warps a quarter of the rows, each half of the columns (dual: of both weights')
+            const uint32_t stage = out_stage + (warp - 2) * S::OUT_WARP;
+            const int cbegin = warp >= 6 ? BN / 2 : 0;
+            const int cend = static_cast<int>(min(g.N - col0, static_cast<int64_t>(cbegin + BN / 2)));
+            constexpr int WORDS = S::OUT_WARP / 128;       // binary32 a staged row
+            constexpr int STEP = DUAL ? WORDS / 2 : WORDS;  // result columns a round
+            // 16-byte unit j of the lane's row: units swapped by row against bank conflicts
+            auto unit_at = [&](int row, int j) {
+                return stage + row * (WORDS * 4) + ((j ^ (row & (WORDS / 4 - 1))) << 4);
+            };
+            auto put = [&](int j, float a, float b, float c, float d) {
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at(lane, j)), "f"(a), "f"(b), "f"(c),
+                             "f"(d)
+                             : "memory");
+            };
+            auto take = [&](int row, int j, float (&v)[8]) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int h = 0; h < 2; ++h)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3])
+                                 : "r"(unit_at(row, j + h))
+                                 : "memory");
+            };
+            // the staged round's outputs: 8 columns a lane, whole rows of STEP together
+            auto finish = [&](int c0) {
+                __syncwarp();
+                constexpr int UNITS = STEP / 8, ROWS = 32 / UNITS;
+                const int un = lane % UNITS;
+                const int64_t col = col0 + c0 + un * 8;
+                if (col < g.N) {
+                    float bias[DUAL ? 2 : 1][8];
+                    bias8<T, DUAL>(g.e, col, bias);
+#pragma unroll 2
+                    for (int r = lane / UNITS; r < 32; r += ROWS) {
+                        if (row0 + r >= g.M) break;
+                        float z[8], v[8];
+                        take(r, un * 2, z);
+                        if constexpr (DUAL) take(r, WORDS / 8 + un * 2, v);
+                        finish8<T, DUAL>(g.e, row0 + r, col, bias, z, v);
+                    }
+                }
+                __syncwarp();
+            };
+            if constexpr (F32) {
+                // the drains, added in registers: 64 columns of a row a thread, those of
+                // the accumulator from `from(c)` on
+                auto from = [&](int c) { return DUAL ? (c < 1 ? cbegin : 64 + cbegin) : cbegin + c * 32; };
+                float sum[2][32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
+                auto drain = [&](uint32_t d) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(d + from(c), r);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                    }
+                };
                 for (int u = 0; u < drains; ++u) {
                     if (!ready()) {
                         ok = false;
                         break;
                     }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t r[32];
-                        tmem_ld32(lanes + acc * 128 + c * 32, r);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
-                    }
+                    drain(lanes + acc * 128);
                     release(tempty_bar(acc));
                     next_acc();
                 }
                 if (!ok) break;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(lanes + 256 + par * 128 + c * 32, r);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
-                }
+                drain(lanes + 256 + par * 128);
                 release(sempty_bar(par));
                 par ^= 1;
-                // 32-byte groups, whole sectors, straight from the registers
-                if (row0 + lane < g.M) {
 #pragma unroll
-                    for (int c = 0; c < BN / 8; ++c) {
-                        if (col0 + c * 8 >= g.N) break;
-                        float z[8], v[8];
+                for (int round = 0; round < 2; ++round) {
+                    if (cbegin + round * STEP >= cend) break;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            z[i] = sum[c / 4][(c % 4) * 8 + i];
-                            v[i] = DUAL ? sum[c / 4 + 2 * (DUAL ? 1 : 0)][(c % 4) * 8 + i] : 0.0f;
-                        }
-                        float bias[DUAL ? 2 : 1][8];
-                        bias8<T, DUAL>(g.e, col0 + c * 8, bias);
-                        finish8<T, DUAL>(g.e, row0 + lane, col0 + c * 8, bias, z, v);
+                    for (int j = 0; j < 8; ++j) {
+                        // dual: columns 16 round .. + 15 of both weights', else 32 of one
+                        const float* v = DUAL ? &sum[j / 4][round * 16 + (j % 4) * 4] : &sum[round][j * 4];
+                        put(j, v[0], v[1], v[2], v[3]);
                     }
+                    finish(cbegin + round * STEP);
                 }
             } else {
                 if (!ready()) break;
-                // two warps a quarter of the rows, each half of the columns
-                const uint32_t stage = out_stage + (warp - 2) * 8192;  // 32 rows of 64 binary32, units swapped by row
                 const uint32_t d = lanes + acc * S::NACC;
-                constexpr int STEP = DUAL ? 32 : 64;
-                const int cbegin = warp >= 6 ? BN / 2 : 0;
-                const int cend = static_cast<int>(min(g.N - col0, static_cast<int64_t>(cbegin + BN / 2)));
                 if (cbegin >= cend) release(tempty_bar(acc));
                 for (int c0 = cbegin; c0 < cend; c0 += STEP) {
 #pragma unroll
@@ -745,41 +803,11 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                         tmem_ld32(d + (DUAL ? c0 + h * 128 : c0 + h * 32), r);
                         if (h == 1 && c0 + STEP >= cend) release(tempty_bar(acc));
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t at = stage + lane * 256 + (((h * 8 + j) ^ (lane & 15)) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[4 * j]),
-                                         "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
-                                         : "memory");
-                        }
+                        for (int j = 0; j < 8; ++j)
+                            put(h * 8 + j, __uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
                     }
-                    __syncwarp();
-                    // rows of 64 (dual: 32) columns, 8 a lane: whole lines of the outputs
-                    constexpr int UNITS = STEP / 8, ROWS = 32 / UNITS;
-                    const int un = lane % UNITS;
-                    const int64_t col = col0 + c0 + un * 8;
-                    auto take = [&](int row, int unit, float (&v)[8]) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t at = stage + row * 256 + (((unit + h) ^ (row & 15)) << 4);
-                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3])
-                                         : "r"(at)
-                                         : "memory");
-                        }
-                    };
-                    if (col < g.N) {
-                        float bias[DUAL ? 2 : 1][8];
-                        bias8<T, DUAL>(g.e, col, bias);
-#pragma unroll 2
-                        for (int r = lane / UNITS; r < 32; r += ROWS) {
-                            if (row0 + r >= g.M) break;
-                            float z[8], v[8];
-                            take(r, un * 2, z);
-                            if constexpr (DUAL) take(r, 8 + un * 2, v);
-                            finish8<T, DUAL>(g.e, row0 + r, col, bias, z, v);
-                        }
-                    }
-                    __syncwarp();
+                    finish(c0);
                 }
                 next_acc();
             }
@@ -973,6 +1001,8 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     int splits = 1;
     while (splits < MAX_SPLIT && tiles * splits * 2 <= int64_t(ctx->num_sms) * S::CTAS && units >= splits * 4) splits *= 2;
     g.splits = splits;
+    g.slots = static_cast<int>(S::RING / (g.a_bytes + TILE_BYTES));
+    if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
 
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -1013,29 +1043,24 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
     g.kb = static_cast<int>((p.K + 63) / 64);
     g.segments = p.segments;
     g.status = ctx->status;
-    bool ok = true;
-    Staged b0;
+    const int na = p.segments, nb = p.dual ? 2 : p.segments;
+    Staged sa[2], sb[2];
+    for (int i = 0; i < na; ++i) QSML_TRY_STATUS(stage(ctx, ws, p.a[i], f32, -1, &sa[i]));
+    // a dual product's weights share an order: they meet in one MMA
+    for (int i = 0; i < nb; ++i)
+        QSML_TRY_STATUS(stage(ctx, ws, p.b[i], f32, p.dual && i ? (sb[0].trans ? 1 : 0) : -1, &sb[i]));
+    // few rows: a K-major tile of A holds no more than them, in whole groups of 8
+    int a_rows = !pair && p.M <= 64 ? static_cast<int>((p.M + 7) / 8 * 8) : 128;
+    for (int i = 0; i < na; ++i)
+        if (sa[i].trans) a_rows = 128;
+    g.a_bytes = a_rows * 128;
     const uint32_t b_rows = pair ? (f32 ? 64 : 128) : (p.dual ? 64 : 128);  // of a K-major box
+    bool ok = true;
     for (int i = 0; i < 2; ++i) {
-        g.a_mn[i] = g.b_mn[i] = 0;
-        if (i < p.segments) {
-            Staged s;
-            QSML_TRY_STATUS(stage(ctx, ws, p.a[i], f32, -1, &s));
-            g.a_mn[i] = s.trans ? 1 : 0;  // stored [K, M]
-            ok = ok && operand_map(&g.a[i], s, f32, s.trans, 128);
-        } else {
-            g.a[i] = g.a[0];
-        }
-        if (i < (p.dual ? 2 : p.segments)) {
-            // a dual product's weights share an order: they meet in one MMA
-            Staged s;
-            QSML_TRY_STATUS(stage(ctx, ws, p.b[i], f32, p.dual && i ? (b0.trans ? 1 : 0) : -1, &s));
-            if (i == 0) b0 = s;
-            g.b_mn[i] = s.trans ? 0 : 1;  // stored [K, N]
-            ok = ok && operand_map(&g.b[i], s, f32, !s.trans, b_rows);
-        } else {
-            g.b[i] = g.b[0];
-        }
+        g.a_mn[i] = sa[i < na ? i : 0].trans ? 1 : 0;  // stored [K, M]
+        g.b_mn[i] = sb[i < nb ? i : 0].trans ? 0 : 1;  // stored [K, N]
+        ok = ok && operand_map(&g.a[i], sa[i < na ? i : 0], f32, g.a_mn[i], static_cast<uint32_t>(a_rows)) &&
+             operand_map(&g.b[i], sb[i < nb ? i : 0], f32, g.b_mn[i], b_rows);
     }
     if (!ok) return set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
     if (pair) {
