@@ -52,20 +52,24 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32);
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
 __device__ __forceinline__ float ld1(const __half* p) { return __half2float(*p); }
 
-// exp for the activations: binary16 results take the fast one (2 ulp and
-// 2^-24 |x|, far below half a step of binary16), binary32 ones expf.
-template <typename T> __device__ __forceinline__ float act_exp(float x) {
-    if constexpr (sizeof(T) == 2) return __expf(x);
-    else return expf(x);
-}
-// 1 / (1 + exp(-z)); 0 where exp(-z) overflows
-template <typename T> __device__ __forceinline__ float act_sigmoid(float z) {
-    const float d = __fadd_rn(1.0f, act_exp<T>(-z));
-    if constexpr (sizeof(T) == 2) return __fdividef(1.0f, d);
-    else return __frcp_rn(d);
-}
-
 constexpr float kGeluS = 0.7978845608f, kGeluC = 0.044715f;  // the constants of QSML_UN_GELU
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + exp(-z)); 0 where exp(-z) overflows.  Binary32 results take expf and a
+// correctly rounded reciprocal.  Binary16 ones take 2^t and 1/d of the hardware
+// (2 ulp and 1 ulp; t = -z log2(e) is off by 2^-24 |t|): far below half a step of
+// binary16, and a third of the instructions, which bounded the epilogue and the
+// gradient's pass.
+template <typename T> __device__ __forceinline__ float act_sigmoid(float z) {
+    if constexpr (sizeof(T) == 2) {
+        float e, p;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(-kLog2e, z)));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(__fadd_rn(1.0f, e)));
+        return p;
+    } else {
+        return __frcp_rn(__fadd_rn(1.0f, expf(-z)));
+    }
+}
 
 // act(z).  gelu: 0.5 z (1 + tanh v) = z sigmoid(2 v), v = s (z + c z^3).
 template <typename T> __device__ __forceinline__ float act_value(int act, float z) {

@@ -83,14 +83,152 @@ __device__ __forceinline__ uint64_t slice_desc(uint32_t tile, int mn, int k) {
     return mn ? smem_desc(tile + k * 2048, 8192, 1024) : smem_desc(tile + k * 32, 16, 1024);
 }
 
-// What the MMA thread needs of an operand's order: it issues an MMA every 64 to 128
-// cycles alone, so a descriptor is one addition to these.
-struct Walk {
-    uint64_t first;  // descriptor of the tile at address 0 of the ring, k slice 0
-    uint32_t step;   // from a k slice to the next (16-byte units)
+// ---- the binary16 epilogue of a row, 32 columns in registers -----------------------
+// z += bias of columns col .. col + 31 (the warp's lanes have one row each and read
+// the same 32 values)
+__device__ __forceinline__ void add_bias32(const Epilogue& e, int which, int64_t col, float (&z)[32]) {
+    if (!e.bias[which]) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t c = col + 8 * j;
+        if (c >= e.N) break;
+        const int n = e.N - c < 8 ? static_cast<int>(e.N - c) : 8;
+        float b[8];
+        if (e.bias_f32) ldg8(static_cast<const float*>(e.bias[which]) + c, n, e.vec, b);
+        else ldg8(static_cast<const __half*>(e.bias[which]) + c, n, e.vec, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[8 * j + i] = __fadd_rn(z[8 * j + i], b[i]);
+    }
+}
+
+__device__ __forceinline__ void act32(int act, float (&z)[32]) {
+    switch (act) {
+        case QSML_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_RELU, z[i]);
+            break;
+        case QSML_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_GELU, z[i]);
+            break;
+        case QSML_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_SILU, z[i]);
+            break;
+        case QSML_ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_SIGMOID, z[i]);
+            break;
+    }
+}
+
+// A warp's staging buffer: 32 rows of COLS binary16 in 16-byte units, swapped by
+// row so that a column of units and a row of them both meet every bank.
+template <int COLS> struct HalfRows {
+    static constexpr int UNITS = COLS / 8;
+    static constexpr int BYTES = 32 * COLS * 2;
+    uint32_t base;
+    __device__ uint32_t at(int row, int unit) const {
+        return base + row * (COLS * 2) + ((unit ^ ((COLS == 64 ? row : row >> 1) & (UNITS - 1))) << 4);
+    }
+    // 32 columns of the lane's row, from column 32 * h of the buffer on
+    __device__ void put(int lane, int h, const float (&z)[32]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 v = __floats2half2_rn(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(lane, 4 * h + j)), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+    }
+    __device__ void add(int lane, int h, float (&z)[32]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(at(lane, 4 * h + j))
+                         : "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                z[8 * j + 2 * i] = __fadd_rn(z[8 * j + 2 * i], f.x);
+                z[8 * j + 2 * i + 1] = __fadd_rn(z[8 * j + 2 * i + 1], f.y);
+            }
+        }
+    }
+    // The buffer's rows to or from a matrix of N columns, rows of `ld`, whose element
+    // (0, 0) lies at p; a row's units by neighbouring lanes.  `rows` of the 32 exist.
+    template <bool LOAD>
+    __device__ void copy(__half* p, int64_t ld, int64_t col, int64_t N, int64_t row0, int rows, bool vec) const {
+        const int lane = threadIdx.x & 31, unit = lane % UNITS;
+        const int64_t c = col + unit * 8;
+        if (c >= N) return;
+        const int n = N - c < 8 ? static_cast<int>(N - c) : 8;
+#pragma unroll 4
+        for (int r = lane / UNITS; r < rows; r += 32 / UNITS) {
+            __half* q = p + (row0 + r) * ld + c;
+            uint4 u;
+            __half* h = reinterpret_cast<__half*>(&u);
+            if constexpr (LOAD) {
+                if (vec) {
+                    u = *reinterpret_cast<const uint4*>(q);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[i] = i < n ? q[i] : __float2half_rn(0.0f);
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(r, unit)), "r"(u.x), "r"(u.y), "r"(u.z),
+                             "r"(u.w)
+                             : "memory");
+            } else {
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                             : "r"(at(r, unit))
+                             : "memory");
+                if (vec) {
+                    *reinterpret_cast<uint4*>(q) = u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < n) q[i] = h[i];
+                }
+            }
+        }
+    }
 };
-__device__ __forceinline__ Walk walk_of(uint32_t tile, int mn) {
-    return Walk{slice_desc(tile, mn, 0), mn ? 2048u >> 4 : 32u >> 4};
+
+// From a k slice's descriptor to the next.
+__device__ __forceinline__ constexpr uint32_t slice_step(int mn) { return mn ? 2048u >> 4 : 32u >> 4; }
+
+// f(a_mn, b_mn) with the orders as constants: the MMA thread issues an MMA every 64
+// to 128 cycles alone, and descriptors whose steps it has to look up cost 10 % of a
+// large product (227 us against 205 at 8192 x 4096 x 4096).
+template <class F> __device__ __forceinline__ void by_order(int a_mn, int b_mn, F&& f) {
+    using No = std::integral_constant<int, 0>;
+    using Yes = std::integral_constant<int, 1>;
+    if (a_mn) {
+        if (b_mn) f(Yes{}, Yes{});
+        else f(Yes{}, No{});
+    } else {
+        if (b_mn) f(No{}, Yes{});
+        else f(No{}, No{});
+    }
+}
+
+// The producer and MMA warps run their loops with all lanes, so that addresses and
+// descriptors stay in uniform registers; one lane of them issues.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)) != 0;
 }
 
 __device__ __forceinline__ void cluster_arrive_wait() {
@@ -125,7 +263,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < g.slots; ++s) {
             mbar_init(full_bar(s), 1);
@@ -172,41 +310,45 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 
     bool done = true;  // epilogue warps: the CTA's sums are complete
     if (warp == 0) {
-        if (lane == 0) {
+        {
+            const bool issue = elect_one();
             int slot = 0, filled = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int seg = 0; seg < g.segments && ok; ++seg) {
                 int lo, hi;
                 part(seg, lo, hi);
-                const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
-                const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? 0 : seg];
+                by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+                const CUtensorMap* ma = &g.a[seg];
+                [[maybe_unused]] const CUtensorMap* mb = &g.b[DUAL ? 0 : seg];
                 for (int kb = lo; kb < hi && ok; ++kb) {
 #pragma unroll
                     for (int p = 0; p < S::PARTS; ++p) {
-                        if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
+                        if (!warp_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
                             ok = false;
                             break;
                         }
                         const uint32_t bar = full_bar(slot), at = base + slot * slot_bytes, bt = at + g.a_bytes;
-                        mbar_expect_tx(bar, slot_bytes);
-                        if (a_mn) {
-                            tma_load_3d(at, ma, bar, mt * 128, kb * 64, p);
-                            tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, p);
-                        } else {
-                            tma_load_3d(at, ma, bar, kb * 64, mt * 128, p);
-                        }
-                        if constexpr (DUAL) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                if (b_mn) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
-                                else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, p);
+                        if (issue) {
+                            mbar_expect_tx(bar, slot_bytes);
+                            if (a_mn.value) {
+                                tma_load_3d(at, ma, bar, mt * 128, kb * 64, p);
+                                tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, p);
+                            } else {
+                                tma_load_3d(at, ma, bar, kb * 64, mt * 128, p);
                             }
-                        } else if (b_mn) {
-                            tma_load_3d(bt, mb, bar, nt * 128, kb * 64, p);
-                            tma_load_3d(bt + 8192, mb, bar, nt * 128 + 64, kb * 64, p);
-                        } else {
-                            tma_load_3d(bt, mb, bar, kb * 64, nt * 128, p);
+                            if constexpr (DUAL) {
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    if (b_mn.value) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
+                                    else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, p);
+                                }
+                            } else if (b_mn.value) {
+                                tma_load_3d(bt, mb, bar, nt * 128, kb * 64, p);
+                                tma_load_3d(bt + 8192, mb, bar, nt * 128 + 64, kb * 64, p);
+                            } else {
+                                tma_load_3d(bt, mb, bar, kb * 64, nt * 128, p);
+                            }
                         }
                         ++filled;
                         if (++slot == g.slots) {
@@ -215,6 +357,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         }
                     }
                 }
+                });
             }
             // every copy this thread started lands before the memory has another use:
             // the last fill of each slot (fill i is in slot i % slots, phase i / slots)
@@ -226,7 +369,8 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
+            const bool issue = elect_one();
             int slot = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
@@ -235,14 +379,14 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             for (int seg = 0; seg < g.segments && ok; ++seg) {
                 int lo, hi;
                 part(seg, lo, hi);
-                const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
-                const uint32_t id = idesc(F32, a_mn, b_mn, 128, 128);
-                const Walk wa = walk_of(base, a_mn), wb = walk_of(base + g.a_bytes, b_mn);
+                by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+                const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 128, 128);
+                const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + g.a_bytes, b_mn.value, 0);
                 // binary32: a drain every CHUNK k-blocks; else none inside
                 for (int k0 = lo; k0 < hi && ok; k0 += F32 ? CHUNK : hi) {
                     const int k1 = F32 ? min(k0 + CHUNK, hi) : hi;
                     if (F32) {
-                        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                        if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
                             ok = false;
                             break;
                         }
@@ -252,15 +396,15 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                     for (int kb = k0; kb < k1 && ok; ++kb) {
                         int at[S::PARTS] = {};  // the parts' slots
                         auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
-                            const uint64_t as = wa.first + static_cast<uint32_t>(at[pa] * (slot_bytes >> 4));
-                            const uint64_t bs = wb.first + static_cast<uint32_t>(at[pb] * (slot_bytes >> 4));
+                            const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (slot_bytes >> 4));
+                            const uint64_t bs = wb + static_cast<uint32_t>(at[pb] * (slot_bytes >> 4));
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                mma_f16(dst, as + k * wa.step, bs + k * wb.step, id, fresh && k == 0 ? 0u : 1u);
+                                if (issue) mma_f16(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value), id, fresh && k == 0 ? 0u : 1u);
                         };
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
-                            if (!mbar_wait(full_bar(slot), phase, abort_flag, limit)) {
+                            if (!warp_wait(full_bar(slot), phase, abort_flag, limit)) {
                                 ok = false;
                                 break;
                             }
@@ -288,19 +432,20 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         if (!ok) break;
                         begun = true;
 #pragma unroll
-                        for (int p = 0; p < S::PARTS; ++p) mma_commit(empty_bar(at[p]));
+                        for (int p = 0; p < S::PARTS; ++p) if (issue) mma_commit(empty_bar(at[p]));
                     }
                     if (F32 && ok) {
-                        mma_commit(tfull_bar(acc));
+                        if (issue) mma_commit(tfull_bar(acc));
                         if (++acc == 2) {
                             acc = 0;
                             acc_phase ^= 1u;
                         }
                     }
                 }
+                });
             }
-            if (!F32 && ok) mma_commit(tfull_bar(0));
-            mma_commit(drain_bar);
+            if (!F32 && ok && issue) mma_commit(tfull_bar(0));
+            if (issue) mma_commit(drain_bar);
             const long long t0 = clock64();
             while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
             }
@@ -455,7 +600,7 @@ template <bool F32> struct PairShape {
     static constexpr int BCOLS = F32 ? 64 : 128;              // columns of B a CTA
     static constexpr int SLOT = TILE_BYTES + BCOLS * 128;
     static constexpr int NACC = 2 * BCOLS;                    // accumulator columns
-    static constexpr int OUT_WARP = F32 ? 4096 : 8192;        // epilogue staging: 32 rows of 32 (64) binary32
+    static constexpr int OUT_WARP = F32 ? 4096 : 8192;        // epilogue staging of a warp's 32 rows
     static constexpr int OUT = EPI * OUT_WARP;
     static constexpr size_t SMEM = size_t(SLOTS) * SLOT + OUT + 1024 + 256;
     static_assert(SMEM <= 232448, "shared memory");
@@ -493,7 +638,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
 
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::SLOTS; ++s) {
             mbar_init(full_bar(s), 1);
@@ -536,7 +681,8 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     // binary32: drains a tile (the CHUNK k-blocks between them counted by segment)
     const int drains = (g.kb + CHUNK - 1) / CHUNK * g.segments;
     if (warp == 0) {
-        if (lane == 0) {
+        {
+            const bool issue = elect_one();
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -547,29 +693,31 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
                 for (int seg = 0; seg < g.segments && ok; ++seg) {
                     const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
-                    const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
+                    by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                     for (int kb = 0; kb < g.kb && ok; ++kb) {
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
-                            if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
+                            if (!warp_wait(empty_bar(slot), phase ^ 1u, abort_flag, limit)) {
                                 ok = false;
                                 break;
                             }
-                            if (leader) mbar_expect_tx(full_bar(slot), 2 * S::SLOT);
+                            if (issue && leader) mbar_expect_tx(full_bar(slot), 2 * S::SLOT);
                             const uint32_t bar = map_to_rank(full_bar(slot), 0);
                             const uint32_t at = base + slot * S::SLOT, bt = at + TILE_BYTES;
-                            if (a_mn) {
-                                tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
-                                tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
-                            } else {
-                                tma_load_3d_pair(at, ma, bar, kb * 64, row, p);
-                            }
-                            if (b_mn) {
+                            if (issue) {
+                            if (a_mn.value) {
+                                    tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
+                                    tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
+                                } else {
+                                    tma_load_3d_pair(at, ma, bar, kb * 64, row, p);
+                                }
+                                if (b_mn.value) {
 #pragma unroll
-                                for (int j = 0; j < S::BCOLS / 64; ++j)
-                                    tma_load_3d_pair(bt + j * 8192, mb, bar, col + j * 64, kb * 64, p);
-                            } else {
-                                tma_load_3d_pair(bt, mb, bar, kb * 64, col, p);
+                                    for (int j = 0; j < S::BCOLS / 64; ++j)
+                                        tma_load_3d_pair(bt + j * 8192, mb, bar, col + j * 64, kb * 64, p);
+                                } else {
+                                    tma_load_3d_pair(bt, mb, bar, kb * 64, col, p);
+                                }
                             }
                             if (++slot == S::SLOTS) {
                                 slot = 0;
@@ -577,33 +725,35 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             }
                         }
                     }
+                    });
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
+            const bool issue = elect_one();
             int slot = 0, acc = 0, par = 0;
             uint32_t phase = 0, acc_phase = 0, par_phase = 0;
             bool ok = true;
             for (int t = pair; t < total && ok; t += pairs) {
                 if (F32) {
-                    if (!mbar_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) break;
+                    if (!warp_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) break;
                     tc_fence_after();
                 }
                 const uint32_t small = tmem + 256 + par * 128;
                 if (!F32) {
-                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
+                    if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
                     tc_fence_after();
                 }
                 bool begun = false;
                 for (int seg = 0; seg < g.segments && ok; ++seg) {
-                    const int a_mn = g.a_mn[seg], b_mn = g.b_mn[DUAL ? 0 : seg];
-                    const uint32_t id = idesc(F32, a_mn, b_mn, 256, S::NACC);
-                    const Walk wa = walk_of(base, a_mn), wb = walk_of(base + TILE_BYTES, b_mn);
+                    by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+                    const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 256, S::NACC);
+                    const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + TILE_BYTES, b_mn.value, 0);
                     for (int k0 = 0; k0 < g.kb && ok; k0 += F32 ? CHUNK : g.kb) {
                         const int k1 = F32 ? min(k0 + CHUNK, g.kb) : g.kb;
                         if (F32) {
-                            if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                            if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
                                 ok = false;
                                 break;
                             }
@@ -613,15 +763,15 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                         for (int kb = k0; kb < k1 && ok; ++kb) {
                             int at[S::PARTS] = {};  // the parts' slots
                             auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
-                                const uint64_t as = wa.first + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
-                                const uint64_t bs = wb.first + static_cast<uint32_t>(at[pb] * (S::SLOT >> 4));
+                                const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
+                                const uint64_t bs = wb + static_cast<uint32_t>(at[pb] * (S::SLOT >> 4));
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
-                                    mma_f16_pair(dst, as + k * wa.step, bs + k * wb.step, id, fresh && k == 0 ? 0u : 1u);
+                                    if (issue) mma_f16_pair(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value), id, fresh && k == 0 ? 0u : 1u);
                             };
 #pragma unroll
                             for (int p = 0; p < S::PARTS; ++p) {
-                                if (!mbar_wait(full_bar(slot), phase, abort_flag, limit)) {
+                                if (!warp_wait(full_bar(slot), phase, abort_flag, limit)) {
                                     ok = false;
                                     break;
                                 }
@@ -649,20 +799,21 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             if (!ok) break;
                             begun = true;
 #pragma unroll
-                            for (int p = 0; p < S::PARTS; ++p) mma_commit_pair(empty_bar(at[p]));
+                            for (int p = 0; p < S::PARTS; ++p) if (issue) mma_commit_pair(empty_bar(at[p]));
                         }
                         if (F32 && ok) {
-                            mma_commit_pair(tfull_bar(acc));
+                            if (issue) mma_commit_pair(tfull_bar(acc));
                             if (++acc == 2) {
                                 acc = 0;
                                 acc_phase ^= 1u;
                             }
                         }
                     }
+                    });
                 }
                 if (!ok) break;
                 if (!F32) {
-                    mma_commit_pair(tfull_bar(acc));
+                    if (issue) mma_commit_pair(tfull_bar(acc));
                     if (++acc == 2) {
                         acc = 0;
                         acc_phase ^= 1u;
@@ -673,7 +824,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     par_phase ^= 1u;
                 }
             }
-            mma_commit_pair_local(drain_bar);
+            if (issue) mma_commit_pair_local(drain_bar);
             const long long t0 = clock64();
             while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
             }
@@ -711,7 +862,8 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
             const uint32_t stage = out_stage + (warp - 2) * S::OUT_WARP;
             const int cbegin = warp >= 6 ? BN / 2 : 0;
             const int cend = static_cast<int>(min(g.N - col0, static_cast<int64_t>(cbegin + BN / 2)));
-            constexpr int WORDS = S::OUT_WARP / 128;       // binary32 a staged row
+            if constexpr (F32) {
+            constexpr int WORDS = 32;                       // binary32 a staged row
             constexpr int STEP = DUAL ? WORDS / 2 : WORDS;  // result columns a round
             // 16-byte unit j of the lane's row: units swapped by row against bank conflicts
             auto unit_at = [&](int row, int j) {
@@ -750,7 +902,6 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 }
                 __syncwarp();
             };
-            if constexpr (F32) {
                 // the drains, added in registers: 64 columns of a row a thread, those of
                 // the accumulator from `from(c)` on
                 auto from = [&](int c) { return DUAL ? (c < 1 ? cbegin : 64 + cbegin) : cbegin + c * 32; };
@@ -793,21 +944,61 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     finish(cbegin + round * STEP);
                 }
             } else {
+                // registers to binary16 staging to whole row segments: staging costs the
+                // shared-memory bandwidth that the operands' loads and reads use up
+                constexpr int COLS = DUAL ? 32 : 64;  // a round
+                using Rows = HalfRows<COLS>;
+                const Rows out{stage}, kept0{stage + Rows::BYTES}, kept1{stage + 2 * Rows::BYTES};
+                static_assert((DUAL ? 3 : 2) * Rows::BYTES <= S::OUT_WARP, "staging");
+                const int rows = max(0, min(32, g.M - row0));
+                const Epilogue& e = g.e;
+                const bool vec = e.vec;
                 if (!ready()) break;
                 const uint32_t d = lanes + acc * S::NACC;
                 if (cbegin >= cend) release(tempty_bar(acc));
-                for (int c0 = cbegin; c0 < cend; c0 += STEP) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t r[32];
-                        tmem_ld32(d + (DUAL ? c0 + h * 128 : c0 + h * 32), r);
-                        if (h == 1 && c0 + STEP >= cend) release(tempty_bar(acc));
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            put(h * 8 + j, __uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                for (int c0 = cbegin; c0 < cend; c0 += COLS) {
+                    const int64_t col = col0 + c0;
+                    if (!DUAL && e.residual && e.y) {
+                        out.template copy<true>(static_cast<__half*>(const_cast<void*>(e.residual)), e.res_ld, col, g.N,
+                                                row0, rows, vec);
+                        __syncwarp();
                     }
-                    finish(c0);
+#pragma unroll
+                    for (int h = 0; h < COLS / 32; ++h) {
+                        if (c0 + h * 32 >= cend) break;
+                        float z[32], u[32];
+                        auto load = [&](uint32_t from, float (&v)[32]) {
+                            uint32_t r[32];
+                            tmem_ld32(from, r);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                        };
+                        load(d + c0 + h * 32, z);
+                        if constexpr (DUAL) load(d + 128 + c0, u);
+                        if (c0 + h * 32 + 32 >= cend) release(tempty_bar(acc));
+                        add_bias32(e, 0, col + h * 32, z);
+                        if constexpr (DUAL) add_bias32(e, 1, col, u);
+                        if (e.pre[0]) kept0.put(lane, h, z);
+                        if constexpr (DUAL) {
+                            if (e.pre[1]) kept1.put(lane, h, u);
+                        }
+                        if (e.y) {
+                            act32(e.act, z);
+                            if constexpr (DUAL) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) z[i] = __fmul_rn(z[i], u[i]);
+                            } else if (e.residual) {
+                                out.add(lane, h, z);
+                            }
+                            out.put(lane, h, z);
+                        }
+                    }
+                    __syncwarp();
+                    if (e.y) out.template copy<false>(static_cast<__half*>(e.y), g.N, col, g.N, row0, rows, vec);
+                    if (e.pre[0]) kept0.template copy<false>(static_cast<__half*>(e.pre[0]), g.N, col, g.N, row0, rows, vec);
+                    if (DUAL && e.pre[1])
+                        kept1.template copy<false>(static_cast<__half*>(e.pre[1]), g.N, col, g.N, row0, rows, vec);
+                    __syncwarp();
                 }
                 next_acc();
             }
