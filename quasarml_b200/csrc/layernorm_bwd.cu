@@ -7,15 +7,21 @@
 // the row, which has to be read for xh anyway.  The reference has no layer
 // norm and no gradients.
 //
-// k_layer_norm_bwd: a CTA (or, for narrow rows, a warp) holds a row of x and dy
-// in registers, so both are read once and dx is written once (3 elements of
-// traffic, the floor).  Row sums take two steps: the row sum, then together
-// the squared deviations, sum(h) and sum(h (x - mean)), all about the mean, so
-// nothing is lost by cancellation.  A thread keeps its columns for every row
-// it meets and so sums dgamma and dbeta in registers (binary32); the CTAs'
-// sums are joined by k_column_finish in a fixed order.
+// k_layer_norm_bwd: a CTA holds a row of x and dy in registers, so both are read
+// once and dx is written once (3 elements of traffic, the floor).  Rows of whole
+// 16-byte groups come through a ring of shared-memory slots filled by bulk copies
+// (bounded waits), other rows through registers one row ahead.  Row sums take two
+// steps: the row sum, then together the squared deviations, sum(h) and
+// sum(h (x - mean)), all about the mean, so nothing is lost by cancellation.  A
+// thread keeps its columns for every row it meets and so sums dgamma and dbeta in
+// registers (binary32); the CTAs' sums are joined by k_column_finish in a fixed
+// order.  Arithmetic is in packed pairs (fma.rn.f32x2 and the like, each lane
+// rounded as the scalar instruction): the kernel was bound by instructions, 32 an
+// element, before it was by HBM.
+// k_layer_norm_bwd_groups: rows narrower than a CTA's, 4 to 32 lanes a row.
 // k_layer_norm_bwd_rows + k_layer_norm_bwd_cols: rows wider than the registers
 // hold, in two kernels (5 elements of traffic and the row statistics).
+#include "row_pipe.cuh"
 #include "workspace.cuh"
 
 namespace qsml {
@@ -36,154 +42,426 @@ __device__ __forceinline__ float warp_add(float v) {
     return v;
 }
 
-// Sums of `n` values over the threads that share a row: a warp (WARP) or the
-// CTA, every thread ending with the same bits.  `slot` (n x 32 floats) is not
-// written again before every thread has read it: callers alternate two.
-template <bool WARP, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float* slot) {
+// Sums of N values over the CTA, every thread ending with the same bits.  `slot`
+// (N x 32 floats) is not written again before every thread has read it: callers
+// alternate two.
+template <int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* slot) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_add(v[i]);
-    if constexpr (!WARP) {
-        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-        if (lane == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) slot[i * 32 + w] = v[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = warp_add(lane < nw ? slot[i * 32 + lane] : 0.0f);
+    for (int i = 0; i < N; ++i) {
+        v[i] = warp_add(v[i]);
+        if (lane == 0) slot[i * 32 + w] = v[i];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_add(lane < nw ? slot[i * 32 + lane] : 0.0f);
 }
 
-// PV elements a load, NV loads a thread.  partial: [gridDim.x][cols] of dgamma
-// followed by the same of dbeta (null: not wanted).  dx may be null.
-template <typename T, typename GT, int PV, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512)
-    k_layer_norm_bwd(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
-                     T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int cols, float eps) {
-    pdl_begin();
-    constexpr int E = NV * PV;
+// Two binary32 values in one register pair and the packed arithmetic of sm_100.
+struct P2 {
+    uint64_t v;
+};
+__device__ __forceinline__ P2 pack(float a, float b) {
+    P2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack(P2 p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ P2 add2(P2 a, P2 b) {
+    P2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ P2 mul2(P2 a, P2 b) {
+    P2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ P2 fma2(P2 a, P2 b, P2 c) {
+    P2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float sum2(P2 p) {
+    const float2 f = unpack(p);
+    return __fadd_rn(f.x, f.y);
+}
+
+// A thread's columns: NV groups of PV elements, group i at column
+// (t + i * th) * PV of the row, as E / 2 pairs.
+template <typename T, int PV, int NV> struct Cols {
+    static constexpr int E = PV * NV, H = E / 2;
     using V = Vec<T, PV>;
-    __shared__ float slots[4 * 32];
-    extern __shared__ float fold[];  // WARP: the warps' column sums, [2][cols]
-    const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const int th = WARP ? 32 : blockDim.x;
-    const int per = WARP ? blockDim.x >> 5 : 1;  // rows a CTA has at a time
-    const int packs = cols / PV;
-    float g[E], sg[E], sb[E];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int p = t + i * th;
-#pragma unroll
-        for (int e = 0; e < PV; ++e) {
-            g[i * PV + e] = p < packs ? to_f(gamma[p * PV + e]) : 0.0f;
-            sg[i * PV + e] = 0.0f;
-            sb[i * PV + e] = 0.0f;
+    V v[NV];
+    __device__ P2 pair(int j) const {  // elements 2 j and 2 j + 1
+        if constexpr (sizeof(T) == 2 && PV >= 2) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[2 * j / PV].v[2 * j % PV]));
+            return pack(f.x, f.y);
+        } else {
+            return pack(to_f(v[2 * j / PV].v[2 * j % PV]), to_f(v[(2 * j + 1) / PV].v[(2 * j + 1) % PV]));
         }
     }
-    const float inv_n = __frcp_rn(static_cast<float>(cols));
-    const int64_t step = static_cast<int64_t>(gridDim.x) * per;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0);
-    V nx[NV], ny[NV];
-    auto load = [&](int64_t r) {
-        const V* xr = reinterpret_cast<const V*>(x + r * cols);
-        const V* yr = reinterpret_cast<const V*>(dy + r * cols);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int p = t + i * th;
-            if (p < packs) {
-                nx[i] = xr[p];
-                ny[i] = yr[p];
-            }
+    __device__ void set(int j, P2 p) {
+        const float2 f = unpack(p);
+        if constexpr (sizeof(T) == 2 && PV >= 2) {
+            *reinterpret_cast<__half2*>(&v[2 * j / PV].v[2 * j % PV]) = __floats2half2_rn(f.x, f.y);
+        } else {
+            from_f(f.x, v[2 * j / PV].v[2 * j % PV]);
+            from_f(f.y, v[(2 * j + 1) / PV].v[(2 * j + 1) % PV]);
         }
-    };
-    if (row < rows) load(row);
-    for (; row < rows; row += step) {
-        float d[E], y[E];
-        float s1[1] = {0.0f};
+    }
+};
+
+// What a thread keeps of its columns over the rows, and the arithmetic of a row
+// between the sums.  Columns past the row's end (not FULL) have gamma, x and dy
+// 0; only their deviations need a mask.
+template <typename T, int PV, int NV, bool FULL> struct RowWork {
+    using C = Cols<T, PV, NV>;
+    static constexpr int H = C::H;
+    P2 g[H], sg[H], sb[H];
+    P2 d[H], y[H];
+    bool in[NV];
+
+    template <typename GT> __device__ void begin(const GT* gamma, int t, int th, int packs) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = t + i * th < packs;
-#pragma unroll
-            for (int e = 0; e < PV; ++e) {
-                d[i * PV + e] = in ? to_f(nx[i].v[e]) : 0.0f;
-                y[i * PV + e] = in ? to_f(ny[i].v[e]) : 0.0f;
-                s1[0] = __fadd_rn(s1[0], d[i * PV + e]);
-            }
-        }
-        if (row + step < rows) load(row + step);  // in flight while this row is reduced
-        row_sums<WARP>(s1, slots);
-        const float mean = __fmul_rn(s1[0], inv_n);
-        float s3[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = t + i * th < packs;
-#pragma unroll
-            for (int e = 0; e < PV; ++e) {
-                const int k = i * PV + e;
-                d[k] = in ? __fsub_rn(d[k], mean) : 0.0f;
-                const float h = __fmul_rn(y[k], g[k]);
-                s3[0] = __fmaf_rn(d[k], d[k], s3[0]);
-                s3[1] = __fadd_rn(s3[1], h);
-                s3[2] = __fmaf_rn(h, d[k], s3[2]);
-            }
-        }
-        row_sums<WARP>(s3, slots + 32);
-        const float rstd = rsqrtf(__fmaf_rn(s3[0], inv_n, eps));
-        // dx = rstd h - rstd c1 - d (rstd^2 c2),  c2 = mean(h d) rstd
-        const float a = __fmul_rn(__fmul_rn(s3[1], inv_n), rstd);
-        const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), __fmul_rn(rstd, rstd));
-        V out[NV];
+        for (int i = 0; i < NV; ++i) in[i] = FULL || t + i * th < packs;
+        float f[C::E];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < PV; ++e) {
-                const int k = i * PV + e;
-                const float h = __fmul_rn(y[k], g[k]);
-                from_f(__fmaf_rn(h, rstd, -__fmaf_rn(d[k], b, a)), out[i].v[e]);
-                sg[k] = __fmaf_rn(y[k], __fmul_rn(d[k], rstd), sg[k]);
-                sb[k] = __fadd_rn(sb[k], y[k]);
+            for (int e = 0; e < PV; ++e) f[i * PV + e] = in[i] ? to_f(gamma[(t + i * th) * PV + e]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            g[j] = pack(f[2 * j], f[2 * j + 1]);
+            sg[j].v = sb[j].v = 0;
+        }
+    }
+    // the row's values; their sum
+    __device__ float take(const C& x, const C& dy) {
+        P2 s;
+        s.v = 0;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            d[j] = x.pair(j);
+            y[j] = dy.pair(j);
+            s = add2(s, d[j]);
+        }
+        return sum2(s);
+    }
+    // x - mean; sums of its square, of h = dy gamma and of h (x - mean)
+    __device__ void deviations(float mean, float (&s3)[3]) {
+        const P2 m = pack(-mean, -mean);
+        P2 q, a, b;
+        q.v = a.v = b.v = 0;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            d[j] = add2(d[j], m);
+            if (!FULL) {
+                const float2 f = unpack(d[j]);
+                d[j] = pack(in[2 * j / PV] ? f.x : 0.0f, in[(2 * j + 1) / PV] ? f.y : 0.0f);
             }
+            const P2 h = mul2(y[j], g[j]);
+            q = fma2(d[j], d[j], q);
+            a = add2(a, h);
+            b = fma2(h, d[j], b);
+        }
+        s3[0] = sum2(q);
+        s3[1] = sum2(a);
+        s3[2] = sum2(b);
+    }
+    // dx = rstd h - (rstd c1 + (x - mean) rstd^2 c2),  c2 = mean(h (x - mean)) rstd
+    __device__ void outputs(const float (&s3)[3], float inv_n, float eps, C& out) {
+        const float rstd = rsqrtf(__fmaf_rn(s3[0], inv_n, eps));
+        const float a = __fmul_rn(__fmul_rn(s3[1], inv_n), -rstd);
+        const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), -__fmul_rn(rstd, rstd));
+        const P2 r2 = pack(rstd, rstd), a2 = pack(a, a), b2 = pack(b, b);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            const P2 h = mul2(y[j], g[j]);
+            out.set(j, fma2(h, r2, fma2(d[j], b2, a2)));
+            sg[j] = fma2(y[j], mul2(d[j], r2), sg[j]);
+            sb[j] = add2(sb[j], y[j]);
+        }
+    }
+};
+
+// Three values' sums over a warp, six exchanges instead of fifteen: two values
+// change places by half warps, then by quarters, so that a lane goes on with one
+// of them.  Lanes 0-7 end with v[0]'s sum, 8-15 with v[1]'s, 16-23 with v[2]'s.
+__device__ __forceinline__ float warp_sum3(const float (&v)[3]) {
+    const int lane = threadIdx.x & 31;
+    const bool b4 = lane & 16, b3 = lane & 8;
+    const float r0 = __fadd_rn(b4 ? v[2] : v[0], __shfl_xor_sync(0xffffffffu, b4 ? v[0] : v[2], 16));
+    const float r1 = __fadd_rn(b4 ? 0.0f : v[1], __shfl_xor_sync(0xffffffffu, b4 ? v[1] : 0.0f, 16));
+    float r = __fadd_rn(b3 ? r1 : r0, __shfl_xor_sync(0xffffffffu, b3 ? r0 : r1, 8));
+#pragma unroll
+    for (int m = 4; m >= 1; m >>= 1) r = __fadd_rn(r, __shfl_xor_sync(0xffffffffu, r, m));
+    return r;
+}
+
+constexpr int kMaxSlots = 4;
+
+// PV elements a load, NV loads a thread; FULL: the threads' groups are exactly the
+// row's.  slots > 0: rows come through a ring of that many slots of x and dy.
+// partial: [gridDim.x][cols] of dgamma followed by the same of dbeta (null: not
+// wanted).  dx may be null.
+template <typename T, typename GT, int PV, int NV, bool RING, bool FULL>
+__global__ void __launch_bounds__(512)
+    k_layer_norm_bwd(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
+                     T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int cols, float eps, int slots,
+                     int* status) {
+    pdl_begin();
+    using C = Cols<T, PV, NV>;
+    using V = typename C::V;
+    extern __shared__ __align__(16) unsigned char ring[];  // slots x (a row of x, a row of dy)
+    __shared__ uint64_t bars[kMaxSlots];
+    __shared__ float sum1[16], sum3[3][16];  // by warp; those past the last one stay 0
+    const int t = threadIdx.x, th = blockDim.x, lane = t & 31, w = t >> 5;
+    const int packs = cols / PV;
+    int span = 1;  // the warps, up to a power of two
+    while (span < th >> 5) span *= 2;
+    if (t < 16) {
+        sum1[t] = 0.0f;
+        sum3[0][t] = sum3[1][t] = sum3[2][t] = 0.0f;
+    }
+    const int64_t G = gridDim.x;
+    const uint32_t row_bytes = static_cast<uint32_t>(cols * sizeof(T));
+    const uint32_t bar0 = rowpipe::smem_addr(bars), ring0 = rowpipe::smem_addr(ring);
+    auto fill = [&](int slot, int64_t row) {
+        const uint32_t bar = bar0 + 8u * slot, at = ring0 + slot * 2 * row_bytes;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * row_bytes) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at),
+                     "l"(x + row * cols), "r"(row_bytes), "r"(bar)
+                     : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         at + row_bytes),
+                     "l"(dy + row * cols), "r"(row_bytes), "r"(bar)
+                     : "memory");
+    };
+    long long limit = 0;
+    if constexpr (RING) {
+        limit = wait_limit(status);
+        if (t == 0) {
+            for (int s = 0; s < slots; ++s)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8u * s) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            for (int s = 0; s < slots; ++s)
+                if (blockIdx.x + s * G < rows) fill(s, blockIdx.x + s * G);
+        }
+    }
+    RowWork<T, PV, NV, FULL> work;
+    work.begin(gamma, t, th, packs);
+    const float inv_n = __frcp_rn(static_cast<float>(cols));
+    __syncthreads();
+    C nx, ny;  // !RING: the next row; columns past the end stay 0
+    auto load = [&](const V* xr, const V* yr, C& a, C& b) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (work.in[i]) {
+                a.v[i] = xr[t + i * th];
+                b.v[i] = yr[t + i * th];
+            }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+            from_f(0.0f, nx.v[i].v[e]);
+            from_f(0.0f, ny.v[i].v[e]);
+        }
+    auto row_at = [&](const T* p, int64_t r) { return reinterpret_cast<const V*>(p + r * cols); };
+    if (!RING) load(row_at(x, blockIdx.x), row_at(dy, blockIdx.x), nx, ny);
+    int slot = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (int64_t row = blockIdx.x; row < rows; row += G) {
+        bool landed = true;
+        if constexpr (RING) {
+            landed = rowpipe::bar_wait(bar0 + 8u * slot, parity, limit);
+            const V* at = reinterpret_cast<const V*>(ring + slot * 2 * row_bytes);
+            if (landed) load(at, at + packs, nx, ny);
+        }
+        const float s = warp_add(work.take(nx, ny));
+        if (!RING && row + G < rows) load(row_at(x, row + G), row_at(dy, row + G), nx, ny);
+        if (lane == 0) sum1[w] = s;
+        // every thread has its part of the row, and of the row before it all sums
+        if constexpr (RING) {
+            if (__syncthreads_or(!landed)) {
+                ok = false;
+                break;
+            }
+            const int64_t next = row + slots * G;
+            if (t == 0 && next < rows) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                fill(slot, next);
+            }
+        } else {
+            __syncthreads();
+        }
+        float mean = sum1[lane & (span - 1)];
+        for (int m = span / 2; m >= 1; m >>= 1) mean = __fadd_rn(mean, __shfl_xor_sync(0xffffffffu, mean, m));
+        mean = __fmul_rn(mean, inv_n);
+        float s3[3];
+        work.deviations(mean, s3);
+        const float mine = warp_sum3(s3);
+        if ((lane & 7) == 0 && lane < 24) sum3[lane >> 3][w] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            s3[k] = sum3[k][lane & (span - 1)];
+            for (int m = span / 2; m >= 1; m >>= 1) s3[k] = __fadd_rn(s3[k], __shfl_xor_sync(0xffffffffu, s3[k], m));
+        }
+        C out;
+        work.outputs(s3, inv_n, eps, out);
         if (dx) {
             V* dr = reinterpret_cast<V*>(dx + row * cols);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (t + i * th < packs) dr[t + i * th] = out[i];
+                if (work.in[i]) dr[t + i * th] = out.v[i];
+        }
+        if (RING && ++slot == slots) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+    if (RING && !ok) {
+        // the copies still in flight -- of this slot's row and those after it -- land first
+        if (t == 0) {
+            atomicExch(status, QSML_E_TIMEOUT);
+            for (int k = 0; k < slots; ++k) {
+                rowpipe::bar_drain(bar0 + 8u * slot, parity);
+                if (++slot == slots) {
+                    slot = 0;
+                    parity ^= 1u;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (!partial) return;
+    float* pg = partial + blockIdx.x * static_cast<int64_t>(cols);
+    float* pb = pg + G * cols;
+#pragma unroll
+    for (int j = 0; j < C::H; ++j) {
+        const float2 a = unpack(work.sg[j]), b = unpack(work.sb[j]);
+        const int i0 = 2 * j / PV, i1 = (2 * j + 1) / PV;
+        const int c0 = (t + i0 * th) * PV + 2 * j % PV, c1 = (t + i1 * th) * PV + (2 * j + 1) % PV;
+        if (work.in[i0]) {
+            pg[c0] = a.x;
+            pb[c0] = b.x;
+        }
+        if (work.in[i1]) {
+            pg[c1] = a.y;
+            pb[c1] = b.y;
+        }
+    }
+}
+
+// Narrow rows: L lanes a row, so 32 / L rows a warp and 8 warps a CTA, no barrier
+// between them; the next row's loads are in flight while this one is reduced.
+template <typename T, typename GT, int PV, int NV, int L>
+__global__ void __launch_bounds__(256)
+    k_layer_norm_bwd_groups(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
+                            T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int cols, float eps) {
+    pdl_begin();
+    using C = Cols<T, PV, NV>;
+    using V = typename C::V;
+    extern __shared__ float fold[];  // the warps' column sums, [2][cols]
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, t = lane % L;
+    const int packs = cols / PV;
+    RowWork<T, PV, NV, false> work;
+    work.begin(gamma, t, L, packs);
+    const float inv_n = __frcp_rn(static_cast<float>(cols));
+    C nx, ny;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+            from_f(0.0f, nx.v[i].v[e]);
+            from_f(0.0f, ny.v[i].v[e]);
+        }
+    auto load = [&](int64_t r) {
+        const V* xr = reinterpret_cast<const V*>(x + r * cols);
+        const V* yr = reinterpret_cast<const V*>(dy + r * cols);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (work.in[i]) {
+                nx.v[i] = xr[t + i * L];
+                ny.v[i] = yr[t + i * L];
+            }
+    };
+    auto group_sum = [](float v) {
+#pragma unroll
+        for (int m = L / 2; m >= 1; m >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, m));
+        return v;
+    };
+    constexpr int PER = 32 / L;  // rows a warp
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * PER;
+    // the warp's first row decides the trips, so that all lanes take part in the sums
+    int64_t first = (static_cast<int64_t>(blockIdx.x) * 8 + w) * PER;
+    if (first + lane / L < rows) load(first + lane / L);
+    for (; first < rows; first += step) {
+        const int64_t row = first + lane / L;
+        const bool here = row < rows;
+        float s3[3];
+        const float s = work.take(nx, ny);
+        if (row + step < rows) load(row + step);
+        work.deviations(__fmul_rn(group_sum(s), inv_n), s3);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s3[k] = group_sum(s3[k]);
+        C out;
+        // a group past the last row must not add to the columns' sums: its dy is 0
+        if (!here) {
+#pragma unroll
+            for (int j = 0; j < C::H; ++j) work.y[j].v = work.d[j].v = 0;
+        }
+        work.outputs(s3, inv_n, eps, out);
+        if (dx && here) {
+            V* dr = reinterpret_cast<V*>(dx + row * cols);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (work.in[i]) dr[t + i * L] = out.v[i];
         }
     }
     if (!partial) return;
-    float* pg = partial + static_cast<int64_t>(blockIdx.x) * cols;
-    float* pb = pg + static_cast<int64_t>(gridDim.x) * cols;
-    if constexpr (WARP) {
-        // the warps' sums, one warp after another
-        for (int w = 0; w < per; ++w) {
-            if (static_cast<int>(threadIdx.x >> 5) == w) {
+    // the groups of a warp by exchanges, then the warps one after another
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (t + i * th < packs)
+    for (int m = L; m < 32; m <<= 1)
 #pragma unroll
-                        for (int e = 0; e < PV; ++e) {
-                            const int c = (t + i * th) * PV + e, k = i * PV + e;
-                            fold[c] = w ? __fadd_rn(fold[c], sg[k]) : sg[k];
-                            fold[cols + c] = w ? __fadd_rn(fold[cols + c], sb[k]) : sb[k];
-                        }
-            }
-            __syncthreads();
+        for (int j = 0; j < C::H; ++j) {
+            P2 a, b;
+            a.v = __shfl_xor_sync(0xffffffffu, work.sg[j].v, m);
+            b.v = __shfl_xor_sync(0xffffffffu, work.sb[j].v, m);
+            work.sg[j] = add2(work.sg[j], a);
+            work.sb[j] = add2(work.sb[j], b);
         }
-        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-            pg[c] = fold[c];
-            pb[c] = fold[cols + c];
-        }
-    } else {
+    for (int k = 0; k < 8; ++k) {
+        if (w == k && lane < L) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (t + i * th < packs)
+            for (int j = 0; j < C::H; ++j) {
+                const float2 a = unpack(work.sg[j]), b = unpack(work.sb[j]);
+                const float va[2] = {a.x, a.y}, vb[2] = {b.x, b.y};
 #pragma unroll
-                for (int e = 0; e < PV; ++e) {
-                    const int c = (t + i * th) * PV + e;
-                    pg[c] = sg[i * PV + e];
-                    pb[c] = sb[i * PV + e];
+                for (int h = 0; h < 2; ++h) {
+                    const int i = (2 * j + h) / PV, c = (t + i * L) * PV + (2 * j + h) % PV;
+                    if (work.in[i]) {
+                        fold[c] = k ? __fadd_rn(fold[c], va[h]) : va[h];
+                        fold[cols + c] = k ? __fadd_rn(fold[cols + c], vb[h]) : vb[h];
+                    }
                 }
+            }
+        }
+        __syncthreads();
+    }
+    float* pg = partial + blockIdx.x * static_cast<int64_t>(cols);
+    float* pb = pg + gridDim.x * static_cast<int64_t>(cols);
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+        pg[c] = fold[c];
+        pb[c] = fold[cols + c];
     }
 }
 
@@ -201,7 +479,7 @@ __global__ void __launch_bounds__(512)
         const T* yr = dy + row * cols;
         float s1[1] = {0.0f};
         for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) s1[0] = __fadd_rn(s1[0], to_f(xr[c]));
-        row_sums<false>(s1, slots);
+        row_sums(s1, slots);
         const float mean = __fmul_rn(s1[0], inv_n);
         float s3[3] = {0.0f, 0.0f, 0.0f};
         for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
@@ -210,7 +488,7 @@ __global__ void __launch_bounds__(512)
             s3[1] = __fadd_rn(s3[1], h);
             s3[2] = __fmaf_rn(h, d, s3[2]);
         }
-        row_sums<false>(s3, slots + 32);
+        row_sums(s3, slots + 32);
         const float rstd = rsqrtf(__fmaf_rn(s3[0], inv_n, eps));
         if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
         if (!dx) continue;
@@ -261,27 +539,71 @@ qsml_status_t finish(Context* ctx, const Args& a, float* partial, int64_t parts)
     return finish_column_sums(ctx, g, b, parts, a.cols);
 }
 
-template <typename T, typename GT, int PV, int NV, bool WARP>
-qsml_status_t launch_bwd(Context* ctx, const Args& a, int th) {
-    auto kernel = k_layer_norm_bwd<T, GT, PV, NV, WARP>;
-    const int per = WARP ? 8 : 1;
-    const int block = WARP ? 256 : th;
-    const size_t smem = WARP && a.sums() ? static_cast<size_t>(a.cols) * 2 * sizeof(float) : 0;
+// CTAs of `kernel` a SM, once per device, block size and shared memory; opts in to
+// that much dynamic shared memory.
+qsml_status_t resident(Context* ctx, const void* kernel, int block, size_t smem, int* per_sm) {
+    static std::mutex mu;
+    static std::map<std::pair<std::pair<const void*, int>, std::pair<int, size_t>>, int> known;
+    static std::map<std::pair<const void*, int>, size_t> opted;
+    std::lock_guard<std::mutex> lk(mu);
+    size_t& have = opted[{kernel, ctx->device}];
+    if (smem > 40 * 1024 && smem > have) {  // 48 KiB without it, static memory included
+        QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                             static_cast<int>(smem)),
+                                   "layer norm backward: shared-memory attribute"));
+        have = smem;
+    }
+    int& n = known[{{kernel, ctx->device}, {block, smem}}];
+    if (n == 0) {
+        QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, smem),
+                                   "layer norm backward: occupancy"));
+        if (n < 1) n = 1;
+    }
+    *per_sm = n;
+    return QSML_OK;
+}
+
+template <typename T, typename GT, int PV, int NV, bool RING, bool FULL>
+qsml_status_t launch_cta(Context* ctx, const Args& a, int th) {
+    auto kernel = k_layer_norm_bwd<T, GT, PV, NV, RING, FULL>;
+    // three rows in flight a CTA: two CTAs a SM up to rows of 16 KiB
+    const size_t slot = 2 * static_cast<size_t>(a.cols) * sizeof(T);
+    int slots = RING ? 3 : 0;
+    while (slots > 2 && slots * slot > 108 * 1024) --slots;
+    const size_t smem = slots * slot;
     int per_sm = 0;
-    QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem),
-                               "layer norm backward: occupancy"));
-    int64_t grid = static_cast<int64_t>(ctx->num_sms) * (per_sm < 1 ? 1 : per_sm);
-    const int64_t most = (a.rows + per - 1) / per;
+    QSML_TRY_STATUS(resident(ctx, reinterpret_cast<const void*>(kernel), th, smem, &per_sm));
+    int64_t grid = static_cast<int64_t>(ctx->num_sms) * per_sm;
+    if (grid > a.rows) grid = a.rows;
+    Workspace ws(ctx);
+    void* partial = nullptr;
+    if (a.sums()) QSML_TRY_STATUS(ws.get(static_cast<size_t>(grid) * a.cols * 2 * sizeof(float), &partial));
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(th), smem, ctx->stream,
+                                     static_cast<const T*>(a.x), static_cast<const GT*>(a.gamma),
+                                     static_cast<const T*>(a.dy), static_cast<T*>(a.dx), static_cast<float*>(partial),
+                                     a.rows, static_cast<int>(a.cols), a.eps, slots, ctx->status);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd");
+    QSML_TRY_STATUS(after_launch(ctx, "k_layer_norm_bwd"));
+    return a.sums() ? finish(ctx, a, static_cast<float*>(partial), grid) : QSML_OK;
+}
+
+template <typename T, typename GT, int PV, int NV, int L> qsml_status_t launch_groups(Context* ctx, const Args& a) {
+    auto kernel = k_layer_norm_bwd_groups<T, GT, PV, NV, L>;
+    const size_t smem = a.sums() ? static_cast<size_t>(a.cols) * 2 * sizeof(float) : 0;
+    int per_sm = 0;
+    QSML_TRY_STATUS(resident(ctx, reinterpret_cast<const void*>(kernel), 256, smem, &per_sm));
+    int64_t grid = static_cast<int64_t>(ctx->num_sms) * per_sm;
+    const int64_t most = (a.rows + 8 * (32 / L) - 1) / (8 * (32 / L));
     if (grid > most) grid = most;
     Workspace ws(ctx);
     void* partial = nullptr;
     if (a.sums()) QSML_TRY_STATUS(ws.get(static_cast<size_t>(grid) * a.cols * 2 * sizeof(float), &partial));
-    const cudaError_t e = launch_pdl(
-        kernel, dim3(static_cast<unsigned>(grid)), dim3(block), smem, ctx->stream, static_cast<const T*>(a.x),
-        static_cast<const GT*>(a.gamma), static_cast<const T*>(a.dy), static_cast<T*>(a.dx),
-        static_cast<float*>(partial), a.rows, static_cast<int>(a.cols), a.eps);
-    if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd");
-    QSML_TRY_STATUS(after_launch(ctx, "k_layer_norm_bwd"));
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), smem, ctx->stream,
+                                     static_cast<const T*>(a.x), static_cast<const GT*>(a.gamma),
+                                     static_cast<const T*>(a.dy), static_cast<T*>(a.dx), static_cast<float*>(partial),
+                                     a.rows, static_cast<int>(a.cols), a.eps);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd_groups");
+    QSML_TRY_STATUS(after_launch(ctx, "k_layer_norm_bwd_groups"));
     return a.sums() ? finish(ctx, a, static_cast<float*>(partial), grid) : QSML_OK;
 }
 
@@ -315,17 +637,27 @@ qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
     return finish(ctx, a, static_cast<float*>(partial), parts);
 }
 
-// Columns by loads of PV elements: a warp a row while its lanes hold the row in
-// 16 elements each, else a CTA with up to 16 elements a thread and 512 threads.
-template <typename T, typename GT, int PV>
-qsml_status_t pick(Context* ctx, const Args& a) {
-    constexpr int MAXV = 16 / PV;
+// Loads of PV elements, 16 elements a thread: 4 to 32 lanes hold a row, else a CTA
+// of up to 512 threads does.
+template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, const Args& a) {
+    constexpr int NV = 16 / PV;
+    constexpr bool RING = PV > 1;
     const int64_t packs = a.cols / PV;
-    if (packs <= 32) return launch_bwd<T, GT, PV, 1, true>(ctx, a, 32);
-    if (packs <= 32 * MAXV) return launch_bwd<T, GT, PV, MAXV, true>(ctx, a, 32);
-    if (packs <= 512 * MAXV) {
-        const int th = static_cast<int>(((packs + MAXV - 1) / MAXV + 31) / 32 * 32);
-        return launch_bwd<T, GT, PV, MAXV, false>(ctx, a, th);
+    if (packs <= 4 * NV) return launch_groups<T, GT, PV, NV, 4>(ctx, a);
+    if (packs <= 8 * NV) return launch_groups<T, GT, PV, NV, 8>(ctx, a);
+    if (packs <= 16 * NV) return launch_groups<T, GT, PV, NV, 16>(ctx, a);
+    if (packs <= 32 * NV) return launch_groups<T, GT, PV, NV, 32>(ctx, a);
+    if constexpr (PV == 1) {
+        // single elements: 8 a thread while that suffices (registers for two rows' loads)
+        if (packs <= 512 * 8) {
+            const int th = static_cast<int>(((packs + 7) / 8 + 31) / 32 * 32);
+            return launch_cta<T, GT, 1, 8, false, false>(ctx, a, th);
+        }
+    }
+    if (packs <= 512 * NV) {
+        const int th = static_cast<int>(((packs + NV - 1) / NV + 31) / 32 * 32);
+        if (RING && packs == th * NV) return launch_cta<T, GT, PV, NV, RING, RING>(ctx, a, th);
+        return launch_cta<T, GT, PV, NV, RING, false>(ctx, a, th);
     }
     return launch_wide_bwd<T, GT>(ctx, a);
 }
