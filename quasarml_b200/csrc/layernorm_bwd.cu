@@ -117,37 +117,73 @@ template <typename T, int PV, int NV> struct Cols {
 };
 
 // What a thread keeps of its columns over the rows, and the arithmetic of a row
-// between the sums.  Columns past the row's end (not FULL) have gamma, x and dy
-// 0; only their deviations need a mask.
+// between the sums.  Columns past the row's end (not FULL) have x and dy 0; only
+// their deviations need a mask.  With 32 elements a thread (WIDE) the registers
+// go to the sums and the deviations: dy stays as it was loaded and gamma is read
+// from shared memory, group p's quad k as float4 k * packs + p.
 template <typename T, int PV, int NV, bool FULL> struct RowWork {
     using C = Cols<T, PV, NV>;
     static constexpr int H = C::H;
-    P2 g[H], sg[H], sb[H];
-    P2 d[H], y[H];
-    bool in[NV];
+    static constexpr bool WIDE = C::E > 16;
+    P2 g[WIDE ? 1 : H], sg[H], sb[H];
+    P2 d[H], y[WIDE ? 1 : H];
+    C raw;
+    const float4* sgam;
+    int t, th, packs;
 
-    template <typename GT> __device__ void begin(const GT* gamma, int t, int th, int packs) {
+    __device__ bool in(int i) const { return FULL || t + i * th < packs; }
+    template <typename GT> __device__ void begin(const GT* gamma, float4* shared, int t_, int th_, int packs_) {
+        t = t_;
+        th = th_;
+        packs = packs_;
+        sgam = shared;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) in[i] = FULL || t + i * th < packs;
-        float f[C::E];
+        for (int i = 0; i < NV; ++i) {
+            float f[PV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int e = 0; e < PV; ++e) f[e] = in(i) ? to_f(gamma[(t + i * th) * PV + e]) : 0.0f;
+            if constexpr (WIDE) {
+                if (in(i))
 #pragma unroll
-            for (int e = 0; e < PV; ++e) f[i * PV + e] = in[i] ? to_f(gamma[(t + i * th) * PV + e]) : 0.0f;
+                    for (int k = 0; k < PV / 4; ++k)
+                        shared[k * packs + t + i * th] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            } else {
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            g[j] = pack(f[2 * j], f[2 * j + 1]);
-            sg[j].v = sb[j].v = 0;
+                for (int e = 0; e < PV; ++e) {
+                    const int k = i * PV + e;
+                    const float2 u = unpack(g[k / 2]);
+                    g[k / 2] = k % 2 ? pack(u.x, f[e]) : pack(f[e], 0.0f);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < H; ++j) sg[j].v = sb[j].v = 0;
+    }
+    __device__ P2 dy(int j) const {
+        if constexpr (WIDE) return raw.pair(j);
+        else return y[j];
+    }
+    // gamma of pairs 2 q and 2 q + 1
+    __device__ void gam(int q, P2 (&o)[2]) const {
+        if constexpr (WIDE) {
+            const int i = q / (PV / 4);
+            const float4 f = sgam[q % (PV / 4) * packs + (in(i) ? t + i * th : 0)];
+            o[0] = pack(f.x, f.y);
+            o[1] = pack(f.z, f.w);
+        } else {
+            o[0] = g[2 * q];
+            o[1] = g[2 * q + 1];
         }
     }
     // the row's values; their sum
-    __device__ float take(const C& x, const C& dy) {
+    __device__ float take(const C& x, const C& dyv) {
         P2 s;
         s.v = 0;
+        if constexpr (WIDE) raw = dyv;
 #pragma unroll
         for (int j = 0; j < H; ++j) {
             d[j] = x.pair(j);
-            y[j] = dy.pair(j);
+            if constexpr (!WIDE) y[j] = dyv.pair(j);
             s = add2(s, d[j]);
         }
         return sum2(s);
@@ -158,16 +194,22 @@ template <typename T, int PV, int NV, bool FULL> struct RowWork {
         P2 q, a, b;
         q.v = a.v = b.v = 0;
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            d[j] = add2(d[j], m);
-            if (!FULL) {
-                const float2 f = unpack(d[j]);
-                d[j] = pack(in[2 * j / PV] ? f.x : 0.0f, in[(2 * j + 1) / PV] ? f.y : 0.0f);
+        for (int k = 0; k < H / 2; ++k) {
+            P2 gg[2];
+            gam(k, gg);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = 2 * k + u;
+                d[j] = add2(d[j], m);
+                if (!FULL) {
+                    const float2 f = unpack(d[j]);
+                    d[j] = pack(in(2 * j / PV) ? f.x : 0.0f, in((2 * j + 1) / PV) ? f.y : 0.0f);
+                }
+                const P2 h = mul2(dy(j), gg[u]);
+                q = fma2(d[j], d[j], q);
+                a = add2(a, h);
+                b = fma2(h, d[j], b);
             }
-            const P2 h = mul2(y[j], g[j]);
-            q = fma2(d[j], d[j], q);
-            a = add2(a, h);
-            b = fma2(h, d[j], b);
         }
         s3[0] = sum2(q);
         s3[1] = sum2(a);
@@ -180,11 +222,17 @@ template <typename T, int PV, int NV, bool FULL> struct RowWork {
         const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), -__fmul_rn(rstd, rstd));
         const P2 r2 = pack(rstd, rstd), a2 = pack(a, a), b2 = pack(b, b);
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            const P2 h = mul2(y[j], g[j]);
-            out.set(j, fma2(h, r2, fma2(d[j], b2, a2)));
-            sg[j] = fma2(y[j], mul2(d[j], r2), sg[j]);
-            sb[j] = add2(sb[j], y[j]);
+        for (int k = 0; k < H / 2; ++k) {
+            P2 gg[2];
+            gam(k, gg);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = 2 * k + u;
+                const P2 v = dy(j), h = mul2(v, gg[u]);
+                out.set(j, fma2(h, r2, fma2(d[j], b2, a2)));
+                sg[j] = fma2(v, mul2(d[j], r2), sg[j]);
+                sb[j] = add2(sb[j], v);
+            }
         }
     }
 };
@@ -210,21 +258,21 @@ constexpr int kMaxSlots = 4;
 // partial: [gridDim.x][cols] of dgamma followed by the same of dbeta (null: not
 // wanted).  dx may be null.
 template <typename T, typename GT, int PV, int NV, bool RING, bool FULL>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(PV * NV > 16 ? 256 : 512)
     k_layer_norm_bwd(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
                      T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int cols, float eps, int slots,
                      int* status) {
     pdl_begin();
     using C = Cols<T, PV, NV>;
     using V = typename C::V;
-    extern __shared__ __align__(16) unsigned char ring[];  // slots x (a row of x, a row of dy)
+    extern __shared__ __align__(16) unsigned char ring[];  // slots x (a row of x, a row of dy), then gamma (WIDE)
     __shared__ uint64_t bars[kMaxSlots];
-    __shared__ float sum1[16], sum3[3][16];  // by warp; those past the last one stay 0
+    __shared__ float sum1[32], sum3[3][32];  // by warp; those past the last one stay 0
     const int t = threadIdx.x, th = blockDim.x, lane = t & 31, w = t >> 5;
     const int packs = cols / PV;
     int span = 1;  // the warps, up to a power of two
     while (span < th >> 5) span *= 2;
-    if (t < 16) {
+    if (t < 32) {
         sum1[t] = 0.0f;
         sum3[0][t] = sum3[1][t] = sum3[2][t] = 0.0f;
     }
@@ -254,14 +302,14 @@ __global__ void __launch_bounds__(512)
         }
     }
     RowWork<T, PV, NV, FULL> work;
-    work.begin(gamma, t, th, packs);
+    work.begin(gamma, reinterpret_cast<float4*>(ring + 2 * slots * row_bytes), t, th, packs);
     const float inv_n = __frcp_rn(static_cast<float>(cols));
     __syncthreads();
     C nx, ny;  // !RING: the next row; columns past the end stay 0
     auto load = [&](const V* xr, const V* yr, C& a, C& b) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (work.in[i]) {
+            if (work.in(i)) {
                 a.v[i] = xr[t + i * th];
                 b.v[i] = yr[t + i * th];
             }
@@ -321,7 +369,7 @@ __global__ void __launch_bounds__(512)
             V* dr = reinterpret_cast<V*>(dx + row * cols);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (work.in[i]) dr[t + i * th] = out.v[i];
+                if (work.in(i)) dr[t + i * th] = out.v[i];
         }
         if (RING && ++slot == slots) {
             slot = 0;
@@ -345,18 +393,32 @@ __global__ void __launch_bounds__(512)
     if (!partial) return;
     float* pg = partial + blockIdx.x * static_cast<int64_t>(cols);
     float* pb = pg + G * cols;
+    if constexpr (PV >= 4) {
 #pragma unroll
-    for (int j = 0; j < C::H; ++j) {
-        const float2 a = unpack(work.sg[j]), b = unpack(work.sb[j]);
-        const int i0 = 2 * j / PV, i1 = (2 * j + 1) / PV;
-        const int c0 = (t + i0 * th) * PV + 2 * j % PV, c1 = (t + i1 * th) * PV + (2 * j + 1) % PV;
-        if (work.in[i0]) {
-            pg[c0] = a.x;
-            pb[c0] = b.x;
-        }
-        if (work.in[i1]) {
-            pg[c1] = a.y;
-            pb[c1] = b.y;
+        for (int i = 0; i < NV; ++i)
+            if (work.in(i))
+#pragma unroll
+                for (int q = 0; q < PV / 4; ++q) {
+                    const int j = (i * PV + q * 4) / 2, c = (t + i * th) * PV + q * 4;
+                    const float2 a0 = unpack(work.sg[j]), a1 = unpack(work.sg[j + 1]);
+                    const float2 b0 = unpack(work.sb[j]), b1 = unpack(work.sb[j + 1]);
+                    *reinterpret_cast<float4*>(pg + c) = make_float4(a0.x, a0.y, a1.x, a1.y);
+                    *reinterpret_cast<float4*>(pb + c) = make_float4(b0.x, b0.y, b1.x, b1.y);
+                }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C::H; ++j) {
+            const float2 a = unpack(work.sg[j]), b = unpack(work.sb[j]);
+            const int i0 = 2 * j / PV, i1 = (2 * j + 1) / PV;
+            const int c0 = (t + i0 * th) * PV + 2 * j % PV, c1 = (t + i1 * th) * PV + (2 * j + 1) % PV;
+            if (work.in(i0)) {
+                pg[c0] = a.x;
+                pb[c0] = b.x;
+            }
+            if (work.in(i1)) {
+                pg[c1] = a.y;
+                pb[c1] = b.y;
+            }
         }
     }
 }
@@ -374,7 +436,7 @@ __global__ void __launch_bounds__(256)
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, t = lane % L;
     const int packs = cols / PV;
     RowWork<T, PV, NV, false> work;
-    work.begin(gamma, t, L, packs);
+    work.begin(gamma, nullptr, t, L, packs);
     const float inv_n = __frcp_rn(static_cast<float>(cols));
     C nx, ny;
 #pragma unroll
@@ -389,7 +451,7 @@ __global__ void __launch_bounds__(256)
         const V* yr = reinterpret_cast<const V*>(dy + r * cols);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (work.in[i]) {
+            if (work.in(i)) {
                 nx.v[i] = xr[t + i * L];
                 ny.v[i] = yr[t + i * L];
             }
@@ -424,7 +486,7 @@ __global__ void __launch_bounds__(256)
             V* dr = reinterpret_cast<V*>(dx + row * cols);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (work.in[i]) dr[t + i * L] = out.v[i];
+                if (work.in(i)) dr[t + i * L] = out.v[i];
         }
     }
     if (!partial) return;
@@ -448,7 +510,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int i = (2 * j + h) / PV, c = (t + i * L) * PV + (2 * j + h) % PV;
-                    if (work.in[i]) {
+                    if (work.in(i)) {
                         fold[c] = k ? __fadd_rn(fold[c], va[h]) : va[h];
                         fold[cols + c] = k ? __fadd_rn(fold[cols + c], vb[h]) : vb[h];
                     }
@@ -566,11 +628,10 @@ qsml_status_t resident(Context* ctx, const void* kernel, int block, size_t smem,
 template <typename T, typename GT, int PV, int NV, bool RING, bool FULL>
 qsml_status_t launch_cta(Context* ctx, const Args& a, int th) {
     auto kernel = k_layer_norm_bwd<T, GT, PV, NV, RING, FULL>;
-    // three rows in flight a CTA: two CTAs a SM up to rows of 16 KiB
+    // two rows in flight a CTA (about four CTAs a SM)
     const size_t slot = 2 * static_cast<size_t>(a.cols) * sizeof(T);
-    int slots = RING ? 3 : 0;
-    while (slots > 2 && slots * slot > 108 * 1024) --slots;
-    const size_t smem = slots * slot;
+    const int slots = RING ? 2 : 0;
+    const size_t smem = slots * slot + (PV * NV > 16 ? a.cols * sizeof(float) : 0);
     int per_sm = 0;
     QSML_TRY_STATUS(resident(ctx, reinterpret_cast<const void*>(kernel), th, smem, &per_sm));
     int64_t grid = static_cast<int64_t>(ctx->num_sms) * per_sm;
@@ -637,29 +698,30 @@ qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
     return finish(ctx, a, static_cast<float*>(partial), parts);
 }
 
-// Loads of PV elements, 16 elements a thread: 4 to 32 lanes hold a row, else a CTA
-// of up to 512 threads does.
-template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, const Args& a) {
-    constexpr int NV = 16 / PV;
-    constexpr bool RING = PV > 1;
+// The threads of a CTA that hold a row's groups, NV each, and whether exactly.
+template <typename T, typename GT, int PV, int NV, bool RING> qsml_status_t run_cta(Context* ctx, const Args& a) {
     const int64_t packs = a.cols / PV;
-    if (packs <= 4 * NV) return launch_groups<T, GT, PV, NV, 4>(ctx, a);
-    if (packs <= 8 * NV) return launch_groups<T, GT, PV, NV, 8>(ctx, a);
-    if (packs <= 16 * NV) return launch_groups<T, GT, PV, NV, 16>(ctx, a);
-    if (packs <= 32 * NV) return launch_groups<T, GT, PV, NV, 32>(ctx, a);
-    if constexpr (PV == 1) {
-        // single elements: 8 a thread while that suffices (registers for two rows' loads)
-        if (packs <= 512 * 8) {
-            const int th = static_cast<int>(((packs + 7) / 8 + 31) / 32 * 32);
-            return launch_cta<T, GT, 1, 8, false, false>(ctx, a, th);
-        }
+    const int th = static_cast<int>(((packs + NV - 1) / NV + 31) / 32 * 32);
+    if (RING && packs == th * NV) return launch_cta<T, GT, PV, NV, RING, RING>(ctx, a, th);
+    return launch_cta<T, GT, PV, NV, RING, false>(ctx, a, th);
+}
+
+// Loads of PV elements.  Rows of up to 512 columns: 4 to 32 lanes with 16 elements
+// each.  Up to 8192: a CTA, whose threads hold 32 elements of binary16 rows (fewer
+// warps meet at the row's two barriers and more rows are on a SM: 16384 x 4096 took
+// 98 us with 16 elements and 124 with 8), 16 of binary32 ones, 8 or 16 single ones.
+template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, const Args& a) {
+    const int64_t packs = a.cols / PV;
+    if (a.cols <= 512) {
+        constexpr int NV = 16 / PV;
+        if (packs <= 4 * NV) return launch_groups<T, GT, PV, NV, 4>(ctx, a);
+        if (packs <= 8 * NV) return launch_groups<T, GT, PV, NV, 8>(ctx, a);
+        if (packs <= 16 * NV) return launch_groups<T, GT, PV, NV, 16>(ctx, a);
+        return launch_groups<T, GT, PV, NV, 32>(ctx, a);
     }
-    if (packs <= 512 * NV) {
-        const int th = static_cast<int>(((packs + NV - 1) / NV + 31) / 32 * 32);
-        if (RING && packs == th * NV) return launch_cta<T, GT, PV, NV, RING, RING>(ctx, a, th);
-        return launch_cta<T, GT, PV, NV, RING, false>(ctx, a, th);
-    }
-    return launch_wide_bwd<T, GT>(ctx, a);
+    if (a.cols > 8192) return launch_wide_bwd<T, GT>(ctx, a);
+    if constexpr (PV == 1) return a.cols <= 4096 ? run_cta<T, GT, 1, 8, false>(ctx, a) : run_cta<T, GT, 1, 16, false>(ctx, a);
+    else return run_cta<T, GT, PV, (sizeof(T) == 2 ? 32 : 16) / PV, true>(ctx, a);
 }
 
 template <typename T, typename GT>

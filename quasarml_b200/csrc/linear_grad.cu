@@ -11,6 +11,24 @@ namespace qsml {
 namespace linear {
 namespace {
 
+// Eight consecutive elements as they were loaded, by the read-only path (no output
+// of the call overlaps an input).
+template <typename T> struct alignas(16) Raw8 {
+    T v[8];
+    __device__ void load(const T* p, int n, bool vec) {
+        if (vec) {
+            constexpr int Q = sizeof(T) * 8 / 16;
+            uint4* d = reinterpret_cast<uint4*>(v);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) d[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.0f);
+        }
+    }
+    __device__ float get(int i) const { return ld1(v + i); }
+};
+
 // A warp takes 256 columns (8 a lane), a CTA's 8 warps every 8th row of
 // [blockIdx.y * chunk, + chunk).  A thread keeps its columns and sums them in
 // registers; the warps' sums are added in warp order in shared memory.
@@ -29,33 +47,51 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[o][i] = 0.0f;
     if (n > 0) {
-        // inputs by the read-only path: no output of the call overlaps them
-#pragma unroll 2
-        for (int64_t r = r0 + w; r < r1; r += 8) {
-            float dy[8], z[8], u[8], d[NO][8];
-            ldg8(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec, dy);
-            if (DUAL || ACT != QSML_ACT_NONE) ldg8(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec, z);
-            if constexpr (DUAL) ldg8(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec, u);
+        // two rows in flight under the one at hand
+        constexpr bool PRE = DUAL || ACT != QSML_ACT_NONE;
+        Raw8<T> ry[3], rz[3], ru[3];
+        auto load = [&](int64_t r, Raw8<T>& y, Raw8<T>& z, Raw8<T>& u) {
+            if (r >= r1) return;
+            y.load(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec);
+            if constexpr (PRE) z.load(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec);
+            if constexpr (DUAL) u.load(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec);
+        };
+        auto work = [&](int64_t r, const Raw8<T>& y, const Raw8<T>& z, const Raw8<T>& u) {
+            float d[NO][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if constexpr (!DUAL && ACT == QSML_ACT_NONE) {
-                    d[0][i] = dy[i];
+                if constexpr (!PRE) {
+                    d[0][i] = y.get(i);
                 } else {
                     float value;
-                    const float g = act_grad<T>(ACT, z[i], value);
+                    const float g = act_grad<T>(ACT, z.get(i), value);
                     if constexpr (DUAL) {
-                        d[0][i] = __fmul_rn(__fmul_rn(dy[i], u[i]), g);
-                        d[1][i] = __fmul_rn(dy[i], value);
+                        d[0][i] = __fmul_rn(__fmul_rn(y.get(i), u.get(i)), g);
+                        d[1][i] = __fmul_rn(y.get(i), value);
                     } else {
-                        d[0][i] = __fmul_rn(dy[i], g);
+                        d[0][i] = __fmul_rn(y.get(i), g);
                     }
                 }
             }
 #pragma unroll
             for (int o = 0; o < NO; ++o) {
                 if (a.dz[o]) store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
+                if (a.partial) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[o][i] = __fadd_rn(sum[o][i], i < n ? d[o][i] : 0.0f);
+                    for (int i = 0; i < 8; ++i) sum[o][i] = __fadd_rn(sum[o][i], i < n ? d[o][i] : 0.0f);
+                }
+            }
+        };
+        int64_t r = r0 + w;
+        load(r, ry[0], rz[0], ru[0]);
+        load(r + 8, ry[1], rz[1], ru[1]);
+        while (r < r1) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                if (r >= r1) break;
+                load(r + 16, ry[(i + 2) % 3], rz[(i + 2) % 3], ru[(i + 2) % 3]);
+                work(r, ry[i], rz[i], ru[i]);
+                r += 8;
             }
         }
     }

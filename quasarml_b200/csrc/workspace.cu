@@ -32,34 +32,38 @@ qsml_status_t Workspace::get(size_t bytes, void** ptr) {
 
 namespace {
 
-// A CTA takes 32 columns; its 32 warps take every 32nd partial row, each lane
-// one column (128-byte rows), then warp 0 adds the 32 warps' sums in order.
-// Bound by L2 latency: a few thousand rows of 32 columns per CTA at most.
-__global__ void __launch_bounds__(1024) k_column_finish(ColumnSum s0, ColumnSum s1, int64_t parts, int64_t cols) {
+// A CTA takes 8 columns (one 32-byte sector a row), its 64 groups of 8 lanes every
+// 64th partial row, 8 rows in flight each; then a tree over the groups.  Bound by
+// L2 latency: with 32 columns a CTA, 1184 rows of 1024 columns took 18 us.
+constexpr int kFinishGroups = 64;
+
+__global__ void __launch_bounds__(8 * kFinishGroups) k_column_finish(ColumnSum s0, ColumnSum s1, int64_t parts, int64_t cols) {
     pdl_begin();
     const ColumnSum s = blockIdx.y == 0 ? s0 : s1;
-    __shared__ float acc[32][33];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+    __shared__ float acc[kFinishGroups][9];
+    const int k = threadIdx.x & 7, group = threadIdx.x >> 3;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + k;
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = 0.0f;
     if (c < cols) {
         const float* p = s.partial + c;
-        int64_t r = w;
-        for (; r + 96 < parts; r += 128) {
-            a0 = __fadd_rn(a0, p[r * cols]);
-            a1 = __fadd_rn(a1, p[(r + 32) * cols]);
-            a2 = __fadd_rn(a2, p[(r + 64) * cols]);
-            a3 = __fadd_rn(a3, p[(r + 96) * cols]);
+        for (int64_t r = group; r < parts; r += 8 * kFinishGroups) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (r + i * kFinishGroups < parts) a[i] = __fadd_rn(a[i], p[(r + i * kFinishGroups) * cols]);
         }
-        for (; r < parts; r += 32) a0 = __fadd_rn(a0, p[r * cols]);
     }
-    acc[w][lane] = __fadd_rn(__fadd_rn(a0, a1), __fadd_rn(a2, a3));
+    acc[group][k] = __fadd_rn(__fadd_rn(__fadd_rn(a[0], a[1]), __fadd_rn(a[2], a[3])),
+                              __fadd_rn(__fadd_rn(a[4], a[5]), __fadd_rn(a[6], a[7])));
     __syncthreads();
-    // warp w now owns column w: its lanes hold the 32 partial sums
-    float v = acc[lane][w];
+    // warp w < 8 owns column w: two of the 64 sums a lane
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (w >= 8) return;
+    float v = __fadd_rn(acc[lane][w], acc[lane + 32][w]);
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, m));
-    const int64_t oc = static_cast<int64_t>(blockIdx.x) * 32 + w;
+    const int64_t oc = static_cast<int64_t>(blockIdx.x) * 8 + w;
     if (lane == 0 && oc < cols) {
         if (s.out_dtype == QSML_F16)
             static_cast<__half*>(s.out)[oc] = __float2half_rn(v);
@@ -74,8 +78,8 @@ qsml_status_t finish_column_sums(Context* ctx, const ColumnSum& s0, const Column
     const ColumnSum first = s0.out ? s0 : s1;
     const unsigned n = (s0.out ? 1u : 0u) + (s1.out ? 1u : 0u);
     if (n == 0 || cols == 0) return QSML_OK;
-    const dim3 grid(static_cast<unsigned>((cols + 31) / 32), n);
-    const cudaError_t e = launch_pdl(k_column_finish, grid, dim3(1024), 0, ctx->stream, first, s1, parts, cols);
+    const dim3 grid(static_cast<unsigned>((cols + 7) / 8), n);
+    const cudaError_t e = launch_pdl(k_column_finish, grid, dim3(8 * kFinishGroups), 0, ctx->stream, first, s1, parts, cols);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_column_finish");
     return after_launch(ctx, "k_column_finish");
 }
