@@ -406,7 +406,12 @@ QSML_API qsml_status_t qsml_matmul(qsml_ctx* ctx, const qsml_tdesc* a, const qsm
  * overlap of an output with an input or output returns QSML_E_INVALID.
  * Products are summed in binary32 and everything after them is binary32,
  * rounded once per output.  precision: QSML_MM_AUTO, or QSML_MM_FP16_F32ACC for
- * F16 and QSML_MM_FP32_FFMA for F32 (CUDA-core fma, k ascending).
+ * F16 and QSML_MM_FP32_FFMA for F32 (CUDA-core fma).  F32 under QSML_MM_AUTO runs
+ * on the tensor cores as three bf16 parts of each operand (exact) and six of
+ * their nine products, the others being below 2^-22 of |x| |w|: binary32
+ * accuracy for finite operands, but an infinite operand gives NaN where the
+ * CUDA cores give an infinity; a few rows (16, or 8 of a gated layer) run on
+ * the CUDA cores.
  * With no rows nothing is written; with K = 0 the products are 0.
  * Replaces a matmul followed by an add, an activation and an add
  * (QuasarML/src/Ops/LinAlg.cpp:221-271, Ops/Elementwise.cpp:139-417), each a

@@ -166,14 +166,30 @@ void set_vec(Epilogue* e, int es) {
     e->vec = v ? 1 : 0;
 }
 
-// The products of a problem, by the kernel that takes them.
+bool on_tensor_cores(int32_t precision, const Problem& p) { return precision != QSML_MM_FP32_FFMA && p.K > 0; }
+
+// The products of n problems (at most 2), by the kernels that take them.
+qsml_status_t run(Context* ctx, int32_t dtype, int32_t precision, Problem* const* all, int n) {
+    const Problem* tc[2];
+    int ntc = 0;
+    for (int i = 0; i < n; ++i) {
+        Problem& p = *all[i];
+        if (p.M == 0 || p.N == 0) continue;
+        if (!p.e.y && !p.e.pre[0] && !p.e.pre[1]) continue;
+        p.e.N = p.N;
+        set_vec(&p.e, dtype_size(dtype));
+        if (dtype == QSML_F32 && few_rows(p))
+            QSML_TRY_STATUS(run_few(ctx, p));
+        else if (on_tensor_cores(precision, p))
+            tc[ntc++] = &p;
+        else
+            QSML_TRY_STATUS(dtype == QSML_F32 ? run_simt<float>(ctx, p) : run_simt<__half>(ctx, p));
+    }
+    return ntc ? run_tc(ctx, tc, ntc, dtype == QSML_F32) : QSML_OK;
+}
 qsml_status_t run(Context* ctx, int32_t dtype, int32_t precision, Problem& p) {
-    if (p.M == 0 || p.N == 0) return QSML_OK;
-    if (!p.e.y && !p.e.pre[0] && !p.e.pre[1]) return QSML_OK;
-    p.e.N = p.N;
-    set_vec(&p.e, dtype_size(dtype));
-    if (precision != QSML_MM_FP32_FFMA && p.K > 0) return run_tc(ctx, p, dtype == QSML_F32);
-    return dtype == QSML_F32 ? run_simt<float>(ctx, p) : run_simt<__half>(ctx, p);
+    Problem* one = &p;
+    return run(ctx, dtype, precision, &one, 1);
 }
 
 template <typename F> qsml_status_t by_dtype(int32_t dtype, F&& f) {
@@ -192,8 +208,11 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
         want_dw = want_dw || dw[i];
         want_db = want_db || db[i];
     }
-    // dz = dy needs no copy
-    const bool plain = nw == 1 && act == QSML_ACT_NONE;
+    // dz = dy needs no copy, but binary32 operands of the tensor cores are split once
+    // for both products (which have terms to sum: M and N are not 0 where they run); a few
+    // rows may go to the kernel that takes binary32 as it is
+    const bool split = dtype == QSML_F32 && precision != QSML_MM_FP32_FFMA && M > 16 && (dx || want_dw);
+    const bool plain = nw == 1 && act == QSML_ACT_NONE && !split;
     Mat dz[2];
     Workspace ws(ctx);
     GradArgs g;
@@ -202,13 +221,14 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
     g.act = act;
     g.dy = dy->data;
     g.dy_ld = dy_ld;
-    g.pitch = (N + 7) / 8 * 8;
+    g.pitch = line_pitch(N);
+    g.plane = split ? g.pitch * M : 0;
     for (int i = 0; i < nw; ++i) {
         if (!plain) {
-            g.pre[i] = pre[i]->data;
+            if (act != QSML_ACT_NONE || nw == 2) g.pre[i] = pre[i]->data;
             if ((dx || want_dw) && M * N > 0) {
-                QSML_TRY_STATUS(ws.get(static_cast<size_t>(M) * g.pitch * es, &g.dz[i]));
-                dz[i] = Mat{g.dz[i], M, N, g.pitch, 1};
+                QSML_TRY_STATUS(ws.get(static_cast<size_t>(M) * g.pitch * (split ? 6 : es), &g.dz[i]));
+                dz[i] = Mat{g.dz[i], M, N, g.pitch, 1, g.plane};
             }
         } else {
             dz[i] = Mat{dy->data, M, N, dy_ld, 1};
@@ -225,8 +245,12 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
     } else if (N > 0 && (want_db || (!plain && (dx || want_dw)))) {
         QSML_TRY_STATUS(by_dtype(dtype, [&](auto* t) { return run_grad<std::remove_pointer_t<decltype(t)>>(ctx, g, nw == 2); }));
     }
+    Problem products[2];
+    Problem* wanted[2];
+    int n = 0;
     if (dx) {  // dz w^T, summed over the weights
-        Problem p;
+        Problem& p = *(wanted[n] = &products[n]);
+        ++n;
         p.M = M;
         p.N = K;
         p.K = N;
@@ -236,10 +260,10 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
             p.b[i] = w[i].t();
         }
         p.e.y = dx->data;
-        QSML_TRY_STATUS(run(ctx, dtype, precision, p));
     }
     if (want_dw) {  // x^T dz
-        Problem p;
+        Problem& p = *(wanted[n] = &products[n]);
+        ++n;
         p.M = K;
         p.N = N;
         p.K = M;
@@ -255,9 +279,8 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
             p.b[0] = dz[i];
             p.e.y = dw[i]->data;
         }
-        QSML_TRY_STATUS(run(ctx, dtype, precision, p));
     }
-    return QSML_OK;
+    return run(ctx, dtype, precision, wanted, n);
 }
 
 }  // namespace

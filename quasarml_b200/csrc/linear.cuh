@@ -14,12 +14,18 @@
 namespace qsml {
 namespace linear {
 
-// A matrix as given: element (r, c) at p + r * rs + c * cs (elements).
+// A matrix as given: element (r, c) at p + r * rs + c * cs (elements).  plane > 0:
+// binary32 values already split into three bf16 parts, `plane` elements apart
+// (split8), one of the strides being 1 and the other a multiple of 8.
 struct Mat {
     const void* p = nullptr;
-    int64_t rows = 0, cols = 0, rs = 0, cs = 0;
-    Mat t() const { return Mat{p, cols, rows, cs, rs}; }
+    int64_t rows = 0, cols = 0, rs = 0, cs = 0, plane = 0;
+    Mat t() const { return Mat{p, cols, rows, cs, rs, plane}; }
 };
+
+// Elements between the rows of a 16-bit workspace matrix: whole 128-byte lines, so
+// that a 128-byte box row is one (a pitch of 1032 doubled the L2 traffic).
+inline int64_t line_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }
 
 struct Epilogue {
     const void* bias[2] = {nullptr, nullptr};
@@ -44,9 +50,15 @@ struct Problem {
 // CUDA-core products, binary32 fma with k ascending: any strides, any size.
 template <typename T> qsml_status_t run_simt(Context* ctx, const Problem& p);
 
+// Binary32 products of at most 16 rows (8 for a dual product) with weights that are
+// contiguous along one dim: whether p is one, and its kernel (linear_few.cu).
+bool few_rows(const Problem& p);
+qsml_status_t run_few(Context* ctx, const Problem& p);
+
 // Tensor-core products (linear_tc.cu), any strides, alignment and size with
-// K > 0: binary16, or binary32 as three bf16 parts.
-qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32);
+// K > 0: binary16, or binary32 as three bf16 parts.  The operands of all n (at
+// most 2) problems that have to be copied are copied in one launch.
+qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32);
 
 // ---- arithmetic shared by the kernels --------------------------------------------
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
@@ -84,6 +96,28 @@ template <typename T> __device__ __forceinline__ float act_value(int act, float 
         case QSML_ACT_SIGMOID: return act_sigmoid<T>(z);
     }
     return z;
+}
+
+// act of N values, one branch for all of them
+template <typename T, int N> __device__ __forceinline__ void act_all(int act, float (&z)[N]) {
+    switch (act) {
+        case QSML_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_RELU, z[i]);
+            break;
+        case QSML_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_GELU, z[i]);
+            break;
+        case QSML_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_SILU, z[i]);
+            break;
+        case QSML_ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_SIGMOID, z[i]);
+            break;
+    }
 }
 
 // act(z) and its derivative.  With p the sigmoid:
@@ -257,24 +291,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t 
         if (e.pre[1]) store8(static_cast<T*>(e.pre[1]) + at, n, e.vec, u);
     }
     if (!e.y) return;
-    switch (e.act) {  // one branch for the eight
-        case QSML_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_RELU, z[i]);
-            break;
-        case QSML_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_GELU, z[i]);
-            break;
-        case QSML_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_SILU, z[i]);
-            break;
-        case QSML_ACT_SIGMOID:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = act_value<T>(QSML_ACT_SIGMOID, z[i]);
-            break;
-    }
+    act_all<T>(e.act, z);
     if constexpr (DUAL) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[i] = __fmul_rn(z[i], u[i]);
@@ -284,6 +301,13 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t 
     }
     store8(static_cast<T*>(e.y) + at, n, e.vec, z);
 }
+
+template <typename T> __device__ __forceinline__ float bias1(const Epilogue& e, int which, int64_t col) {
+    if (!e.bias[which]) return 0.0f;
+    return e.bias_f32 ? static_cast<const float*>(e.bias[which])[col] : ld1(static_cast<const T*>(e.bias[which]) + col);
+}
+__device__ __forceinline__ void st1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st1(__half* p, float v) { *p = __float2half_rn(v); }
 
 }  // namespace linear
 }  // namespace qsml

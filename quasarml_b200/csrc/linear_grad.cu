@@ -2,8 +2,9 @@
 // biases' gradients: one pass over dy and what the forward pass kept.
 //   LINEAR: dz = dy act'(pre)            db = column sums of dz
 //   DUAL:   dg = dy u act'(g), du = dy act(g), and the column sums of both
-// dz goes to a workspace that the two products of the backward pass read; the
-// sums are taken before it is rounded.  Bound by HBM: LINEAR reads 2 and writes
+// dz goes to a workspace that the two products of the backward pass read (binary32:
+// as the three bf16 parts that the tensor cores take); the sums are taken before it
+// is rounded.  Bound by HBM: LINEAR reads 2 and writes
 // 1 element, DUAL reads 3 and writes 2.
 #include "linear_grad.cuh"
 
@@ -75,7 +76,15 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
             }
 #pragma unroll
             for (int o = 0; o < NO; ++o) {
-                if (a.dz[o]) store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
+                if (a.dz[o]) {
+                    if (sizeof(T) == 4 && a.plane) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) d[o][i] = i < n ? d[o][i] : 0.0f;
+                        split8(d[o], static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col, a.plane);
+                    } else {
+                        store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
+                    }
+                }
                 if (a.partial) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum[o][i] = __fadd_rn(sum[o][i], i < n ? d[o][i] : 0.0f);
@@ -114,9 +123,10 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
 template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradArgs& given) {
     GradArgs a = given;
     const int64_t tiles = (a.N + 255) / 256;
-    // about eight CTAs an SM, at least 8 rows a warp where the bias's gradient is wanted
+    // about eight CTAs an SM, at least 2 rows a warp (8 left most SMs without a CTA at
+    // 515 x 1366: 23 us)
     int64_t parts = (8 * ctx->num_sms + tiles - 1) / tiles;
-    const int64_t most = (a.M + 63) / 64;
+    const int64_t most = (a.M + 15) / 16;
     if (parts > most) parts = most;
     const int64_t chunk = (a.M + parts - 1) / parts;
     parts = (a.M + chunk - 1) / chunk;

@@ -101,27 +101,6 @@ __device__ __forceinline__ void add_bias32(const Epilogue& e, int which, int64_t
     }
 }
 
-__device__ __forceinline__ void act32(int act, float (&z)[32]) {
-    switch (act) {
-        case QSML_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_RELU, z[i]);
-            break;
-        case QSML_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_GELU, z[i]);
-            break;
-        case QSML_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_SILU, z[i]);
-            break;
-        case QSML_ACT_SIGMOID:
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = act_value<__half>(QSML_ACT_SIGMOID, z[i]);
-            break;
-    }
-}
-
 // A warp's staging buffer: 32 rows of COLS binary16 in 16-byte units, swapped by
 // row so that a column of units and a row of them both meet every bank.
 template <int COLS> struct HalfRows {
@@ -244,6 +223,20 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ float lds1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 template <bool F32, bool DUAL>
 __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const __grid_constant__ TcArgs g) {
     using T = std::conditional_t<F32, float, __half>;
@@ -294,15 +287,13 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
     const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
     constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
-    // this CTA's share of the sum, in units of k-blocks (binary32: of the CHUNK
-    // k-blocks between drains), and of it the part [lo, hi) in segment seg
-    const int per_seg = F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb;
-    const int units = per_seg * g.segments;
-    const int u0 = static_cast<int>(static_cast<int64_t>(units) * rank / g.splits);
-    const int u1 = static_cast<int>(static_cast<int64_t>(units) * (rank + 1) / g.splits);
+    // this CTA's share of the k-blocks, and of it the part [lo, hi) in segment seg
+    const int total = g.kb * g.segments;
+    const int u0 = static_cast<int>(static_cast<int64_t>(total) * rank / g.splits);
+    const int u1 = static_cast<int>(static_cast<int64_t>(total) * (rank + 1) / g.splits);
     auto part = [&](int seg, int& lo, int& hi) {
-        lo = max(u0 - seg * per_seg, 0) * (F32 ? CHUNK : 1);
-        hi = min(max(u1 - seg * per_seg, 0) * (F32 ? CHUNK : 1), g.kb);
+        lo = min(max(u0 - seg * g.kb, 0), g.kb);
+        hi = min(max(u1 - seg * g.kb, 0), g.kb);
     };
     // A's tile comes first: where it has fewer than 128 rows the MMA takes the rest
     // from B's, for rows of the result that are not there
@@ -481,7 +472,13 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
             int acc = 0;
             uint32_t phase = 0;
-            for (int u = u0; u < u1; ++u) {
+            int drains = 0;  // as the MMA warp's loops make them
+            for (int seg = 0; seg < g.segments; ++seg) {
+                int lo, hi;
+                part(seg, lo, hi);
+                drains += (hi - lo + CHUNK - 1) / CHUNK;
+            }
+            for (int u = 0; u < drains; ++u) {
                 if (!ready(acc, phase)) {
                     done = false;
                     break;
@@ -534,40 +531,111 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     tc_fence_after();
     if (!*abort_flag) {
         const int rows = min(128, g.M - mt * 128);
-        constexpr int UNITS = BN / 8;
-        for (int i = rank * THREADS + static_cast<int>(threadIdx.x); i < rows * UNITS; i += g.splits * THREADS) {
-            const int r = i / UNITS, c = (i % UNITS) * 8;
-            const int64_t col = static_cast<int64_t>(nt) * BN + c;
-            if (col >= g.N) continue;
-            float z[8], u[8];
-            // the cluster's tiles, all loads under way together, added in rank order
-            auto sum = [&](int cc, float (&v)[8]) {
+        const int64_t row0 = static_cast<int64_t>(mt) * 128, col0 = static_cast<int64_t>(nt) * BN;
+        // 16-byte unit `unit` of row r of the tiles, added over the cluster in rank order, all loads under way together
+        auto sum4 = [&](int r, int unit) {
+            const uint32_t at = r * 512 + ((unit ^ (r & 31)) << 4);
+            if (g.splits == 1) return lds4(base + at);
+            float4 q[MAX_SPLIT];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float4 q[MAX_SPLIT];
+            for (int s = 0; s < MAX_SPLIT; ++s)
+                if (s < g.splits) q[s] = ld_cluster(map_to_rank(base, s) + at);
+            float4 t = q[0];
 #pragma unroll
-                    for (int s = 0; s < MAX_SPLIT; ++s)
-                        if (s < g.splits) q[s] = ld_cluster(map_to_rank(base, s) + r * 512 + (((cc / 4 + h) ^ (r & 31)) << 4));
-                    float4 t = q[0];
-#pragma unroll
-                    for (int s = 1; s < MAX_SPLIT; ++s)
-                        if (s < g.splits) {
-                            t.x = __fadd_rn(t.x, q[s].x);
-                            t.y = __fadd_rn(t.y, q[s].y);
-                            t.z = __fadd_rn(t.z, q[s].z);
-                            t.w = __fadd_rn(t.w, q[s].w);
-                        }
-                    v[4 * h] = t.x;
-                    v[4 * h + 1] = t.y;
-                    v[4 * h + 2] = t.z;
-                    v[4 * h + 3] = t.w;
+            for (int s = 1; s < MAX_SPLIT; ++s)
+                if (s < g.splits) {
+                    t.x = __fadd_rn(t.x, q[s].x);
+                    t.y = __fadd_rn(t.y, q[s].y);
+                    t.z = __fadd_rn(t.z, q[s].z);
+                    t.w = __fadd_rn(t.w, q[s].w);
                 }
-            };
-            sum(c, z);
-            if constexpr (DUAL) sum(64 + c, u);
-            float bias[DUAL ? 2 : 1][8];
-            bias8<T, DUAL>(g.e, col, bias);
-            finish8<T, DUAL>(g.e, static_cast<int64_t>(mt) * 128 + r, col, bias, z, u);
+            return t;
+        };
+        if (g.e.vec) {
+            // 8 columns a thread, always the same ones
+            constexpr int UNITS = BN / 8;
+            static_assert(THREADS % UNITS == 0, "a thread keeps its columns");
+            const int id = rank * THREADS + static_cast<int>(threadIdx.x);
+            const int c = id % UNITS * 8;
+            if (col0 + c < g.N) {
+                float bias[DUAL ? 2 : 1][8];
+                bias8<T, DUAL>(g.e, col0 + c, bias);
+#pragma unroll(DUAL ? 1 : 2)
+                for (int r = id / UNITS; r < rows; r += g.splits * (THREADS / UNITS)) {
+                    float z[8], u[8];
+                    auto sum = [&](int unit, float (&v)[8]) {
+                        const float4 lo = sum4(r, unit), hi = sum4(r, unit + 1);
+                        v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+                        v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+                    };
+                    sum(c / 4, z);
+                    if constexpr (DUAL) sum(16 + c / 4, u);
+                    finish8<T, DUAL>(g.e, row0 + r, col0 + c, bias, z, u);
+                }
+            }
+        } else {
+            // rows off 16 bytes: a warp a row, every 32nd column a lane, ROWS rows together
+            constexpr int STEPS = BN / 32, ROWS = 4, WARPS = THREADS / 32;
+            auto sum1 = [&](int r, int c) { return lds1(base + r * 512 + (((c / 4) ^ (r & 31)) << 4) + (c & 3) * 4); };
+            const Epilogue& e = g.e;
+            float b0[STEPS], b1[STEPS];
+            bool in[STEPS];
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                const int64_t col = col0 + j * 32 + lane;
+                in[j] = col < g.N;
+                b0[j] = in[j] ? bias1<T>(e, 0, col) : 0.0f;
+                b1[j] = DUAL && in[j] ? bias1<T>(e, 1, col) : 0.0f;
+            }
+            const int step = g.splits * WARPS;
+            for (int r0 = rank * WARPS + warp; r0 < rows; r0 += ROWS * step) {
+                if (g.splits > 1) {  // the cluster's sums of these rows, in place of this CTA's part
+#pragma unroll
+                    for (int i = 0; i < ROWS; ++i) {
+                        const int r = r0 + i * step;
+                        if (r >= rows) break;
+                        const float4 t = sum4(r, lane);
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(base + r * 512 + ((lane ^ (r & 31)) << 4)),
+                                     "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w)
+                                     : "memory");
+                    }
+                    __syncwarp();
+                }
+                float z[ROWS * STEPS], u[DUAL ? ROWS * STEPS : 1], res[DUAL ? 1 : ROWS * STEPS];
+                // element k of the ROWS rows: whether it exists, and where
+                auto here = [&](int k) { return in[k % STEPS] && r0 + k / STEPS * step < rows; };
+                auto at = [&](int k, int64_t ld) {
+                    return (row0 + r0 + k / STEPS * step) * ld + col0 + k % STEPS * 32 + lane;
+                };
+                if (!DUAL && e.residual && e.y) {
+#pragma unroll
+                    for (int k = 0; k < ROWS * STEPS; ++k)
+                        if (here(k)) res[DUAL ? 0 : k] = ld1(static_cast<const T*>(e.residual) + at(k, e.res_ld));
+                }
+#pragma unroll
+                for (int k = 0; k < ROWS * STEPS; ++k) {
+                    const int r = min(r0 + k / STEPS * step, rows - 1), c = k % STEPS * 32 + lane;
+                    z[k] = __fadd_rn(sum1(r, c), b0[k % STEPS]);
+                    if constexpr (DUAL) u[k] = __fadd_rn(sum1(r, 64 + c), b1[k % STEPS]);
+                }
+                auto store = [&](void* p, const float* v) {
+#pragma unroll
+                    for (int k = 0; k < ROWS * STEPS; ++k)
+                        if (here(k)) st1(static_cast<T*>(p) + at(k, e.N), v[k]);
+                };
+                if (e.pre[0]) store(e.pre[0], z);
+                if (DUAL && e.pre[1]) store(e.pre[1], u);
+                if (!e.y) continue;
+                act_all<T>(e.act, z);
+                if constexpr (DUAL) {
+#pragma unroll
+                    for (int k = 0; k < ROWS * STEPS; ++k) z[k] = __fmul_rn(z[k], u[k]);
+                } else if (e.residual) {
+#pragma unroll
+                    for (int k = 0; k < ROWS * STEPS; ++k) z[k] = __fadd_rn(z[k], res[k]);
+                }
+                store(e.y, z);
+            }
         }
     } else if (threadIdx.x == 0) {
         atomicExch(g.status, QSML_E_TIMEOUT);
@@ -983,7 +1051,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             if (e.pre[1]) kept1.put(lane, h, u);
                         }
                         if (e.y) {
-                            act32(e.act, z);
+                            act_all<__half>(e.act, z);
                             if constexpr (DUAL) {
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) z[i] = __fmul_rn(z[i], u[i]);
@@ -1026,32 +1094,45 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
 // Operands for TMA
 // ---------------------------------------------------------------------------
 
-// Eight consecutive elements of the stored order at a time, any strides, to
-// 16-bit rows of `pitch`: binary16 as it is, binary32 as its three bf16 parts
-// (`plane` elements apart).  Bound by HBM: binary32 reads 4 and writes 6 bytes.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    k_linear_stage(const T* __restrict__ src, int64_t outer, int64_t inner, int64_t os, int64_t is, bool vec,
-                   uint16_t* __restrict__ dst, int64_t pitch, int64_t plane) {
+// A copy to 16-bit rows of `pitch`: binary16 as it is, binary32 as its three bf16
+// parts (`plane` elements apart); `outer` rows of `inner` from any strides.
+struct StageJob {
+    const void* src;
+    uint16_t* dst;
+    int64_t outer, inner, os, is, pitch, plane;
+    int64_t first;  // block of the launch that begins it
+    int vec;        // 16-byte aligned rows of unit stride
+};
+constexpr int MAX_JOBS = 8;
+struct StageJobs {
+    StageJob job[MAX_JOBS];
+    int n = 0;
+    int64_t blocks = 0;
+};
+
+// Eight consecutive elements of the stored order a thread.  Bound by HBM: binary32
+// reads 4 and writes 6 bytes an element.
+template <typename T> __global__ void __launch_bounds__(256) k_linear_stage(const __grid_constant__ StageJobs jobs) {
     pdl_begin();
-    const int64_t groups = pitch / 8;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < outer * groups;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
+    int k = 0;
+    while (k + 1 < jobs.n && static_cast<int64_t>(blockIdx.x) >= jobs.job[k + 1].first) ++k;
+    const StageJob& j = jobs.job[k];
+    const int64_t groups = (j.inner + 7) / 8, total = j.outer * groups;
+    const int64_t blocks = (k + 1 < jobs.n ? jobs.job[k + 1].first : jobs.blocks) - j.first;
+    for (int64_t i = (blockIdx.x - j.first) * 256 + threadIdx.x; i < total; i += blocks * 256) {
         const int64_t o = i / groups, c = (i - o * groups) * 8;
-        const int n = inner - c < 8 ? static_cast<int>(inner - c) : 8;
-        const T* p = src + o * os + c * is;
+        const int n = j.inner - c < 8 ? static_cast<int>(j.inner - c) : 8;
+        const T* p = static_cast<const T*>(j.src) + o * j.os + c * j.is;
         float v[8];
-        if (vec && n == 8) {
-            load8(p, 8, true, v);
+        if (j.vec && n == 8) {
+            ldg8(p, 8, true, v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < n ? ld1(p + j * is) : 0.0f;
+            for (int q = 0; q < 8; ++q) v[q] = q < n ? ld1(p + q * j.is) : 0.0f;
         }
-        if constexpr (sizeof(T) == 2) {
-            store8(reinterpret_cast<__half*>(dst + o * pitch + c), 8, true, v);
-        } else {
-            split8(v, dst + o * pitch + c, plane);
-        }
+        uint16_t* d = j.dst + o * j.pitch + c;
+        if constexpr (sizeof(T) == 2) store8(reinterpret_cast<__half*>(d), 8, true, v);
+        else split8(v, d, j.plane);
     }
 }
 
@@ -1061,44 +1142,51 @@ struct Staged {
     bool trans = false;  // stored as the matrix's transpose
 };
 
-// The matrix as TMA reads it, copied only where it has to be.  want: 0 rows, 1
-// columns contiguous, -1 as it lies.
-qsml_status_t stage(Context* ctx, Workspace& ws, const Mat& m, bool f32, int want, Staged* s) {
+// The matrix as TMA will read it; a copy, where there has to be one, is added to
+// `jobs`.  want: 0 rows, 1 columns contiguous, -1 as it lies.
+qsml_status_t stage(Context* ctx, Workspace& ws, StageJobs* jobs, const Mat& m, bool f32, int want, Staged* s) {
     const bool by_rows = m.cs == 1 || m.cols == 1, by_cols = m.rs == 1 || m.rows == 1;
     s->trans = want >= 0 ? want == 1 : !by_rows && by_cols;
     s->inner = s->trans ? m.rows : m.cols;
     s->outer = s->trans ? m.cols : m.rows;
     int64_t os = s->trans ? m.cs : m.rs, is = s->trans ? m.rs : m.cs;
     if (s->inner == 1) is = 1;
-    if (s->outer == 1) os = (s->inner + 7) / 8 * 8;
+    if (s->outer == 1) os = line_pitch(s->inner);
     s->p = m.p;
     s->pitch = os;
-    s->plane = 0;
+    s->plane = m.plane;
+    if (m.plane) return QSML_OK;
     const int es = f32 ? 4 : 2;
     if (!f32 && is == 1 && aligned16(m.p) && os % 8 == 0 && os >= s->inner && os < (int64_t(1) << 38)) return QSML_OK;
-    const int64_t pitch = (s->inner + 7) / 8 * 8;
-    const int64_t plane = pitch * s->outer;
+    StageJob& j = jobs->job[jobs->n];
+    j.src = m.p;
+    j.outer = s->outer;
+    j.inner = s->inner;
+    j.os = os;
+    j.is = is;
+    j.pitch = line_pitch(s->inner);
+    j.plane = j.pitch * s->outer;
+    j.vec = is == 1 && aligned16(m.p) && (os * es) % 16 == 0;
     void* dst = nullptr;
-    QSML_TRY_STATUS(ws.get(static_cast<size_t>(plane) * 2 * (f32 ? 3 : 1), &dst));
-    const bool vec = is == 1 && aligned16(m.p) && (os * es) % 16 == 0;
-    const int64_t work = s->outer * (pitch / 8);
-    int64_t grid = (work + 255) / 256;
-    if (grid > int64_t(ctx->num_sms) * 16) grid = int64_t(ctx->num_sms) * 16;
-    cudaError_t e;
-    if (f32)
-        e = launch_pdl(k_linear_stage<float>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream,
-                       static_cast<const float*>(m.p), s->outer, s->inner, os, is, vec, static_cast<uint16_t*>(dst), pitch,
-                       plane);
-    else
-        e = launch_pdl(k_linear_stage<__half>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream,
-                       static_cast<const __half*>(m.p), s->outer, s->inner, os, is, vec, static_cast<uint16_t*>(dst), pitch,
-                       plane);
-    if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_stage");
-    QSML_TRY_STATUS(after_launch(ctx, "k_linear_stage"));
+    QSML_TRY_STATUS(ws.get(static_cast<size_t>(j.plane) * 2 * (f32 ? 3 : 1), &dst));
+    j.dst = static_cast<uint16_t*>(dst);
+    j.first = jobs->blocks;
+    int64_t blocks = (s->outer * ((s->inner + 7) / 8) + 255) / 256;
+    if (blocks > int64_t(ctx->num_sms) * 16) blocks = int64_t(ctx->num_sms) * 16;
+    jobs->blocks += blocks;
+    ++jobs->n;
     s->p = dst;
-    s->pitch = pitch;
-    s->plane = plane;
+    s->pitch = j.pitch;
+    s->plane = f32 ? j.plane : 0;
     return QSML_OK;
+}
+
+qsml_status_t run_jobs(Context* ctx, const StageJobs& jobs, bool f32) {
+    if (jobs.n == 0) return QSML_OK;
+    const cudaError_t e = launch_pdl(f32 ? k_linear_stage<float> : k_linear_stage<__half>,
+                                     dim3(static_cast<unsigned>(jobs.blocks)), dim3(256), 0, ctx->stream, jobs);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_stage");
+    return after_launch(ctx, "k_linear_stage");
 }
 
 // mn: MN-major boxes of 64 x 64 k, else K-major boxes of 64 k x `rows`.
@@ -1167,6 +1255,57 @@ template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Pro
     return after_launch(ctx, name);
 }
 
+// CTAs that share a tile's sum.
+// One row of tiles: every operand of weight is read once, HBM bounds the whole, and
+// as many as the device holds at once pull it fastest (a second turn costs: the gated
+// 5 x 4096 x 11008 took 35 us unsplit in one turn and 41 us in three parts and two).
+// More rows: the tensor pipe of a SM bounds.  A SM works off its CTAs' k-blocks, and
+// each turn has about OVER blocks' time of beginning and end, a joint sum half of it
+// again; the fewest such blocks win, fewer splits on a tie (512 x 11008 x 4096, one
+// tile a SM: 54 us unsplit, 68 us split in two).
+template <bool F32, bool DUAL>
+qsml_status_t best_split(Context* ctx, int64_t tiles, bool one_row, int64_t blocks, int* splits) {
+    using S = Shape<F32>;
+    static std::mutex mu;
+    static int held[64][MAX_SPLIT + 1] = {};  // clusters of each size that the device holds
+    std::lock_guard<std::mutex> lk(mu);
+    int* n = held[ctx->device & 63];
+    constexpr int64_t OVER = F32 ? 2 : 8;
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= MAX_SPLIT && s <= blocks; ++s) {
+        if (n[s] == 0) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = s;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(static_cast<unsigned>(s * ctx->num_sms));
+            cfg.blockDim = dim3(THREADS);
+            cfg.dynamicSmemBytes = S::SMEM;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n[s], k_linear_tc<F32, DUAL>, &cfg) != cudaSuccess || n[s] <= 0) {
+                cudaGetLastError();
+                n[s] = s == 1 ? ctx->num_sms : -1;
+            }
+        }
+        if (n[s] < 0) continue;
+        const int64_t turns = (tiles + n[s] - 1) / n[s];
+        if (one_row) {
+            if (turns == 1 && blocks >= 2 * s) *splits = s;
+            continue;
+        }
+        const int64_t on_a_sm = (tiles * s + ctx->num_sms - 1) / ctx->num_sms;
+        const int64_t cost = on_a_sm * ((blocks + s - 1) / s) + OVER * turns + (s > 1 ? OVER / 2 : 0);
+        if (cost < best) {
+            best = cost;
+            *splits = s;
+        }
+    }
+    return QSML_OK;
+}
+
 template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem& p, TcArgs& g) {
     using S = Shape<F32>;
     constexpr int BN = DUAL ? 64 : 128;
@@ -1187,10 +1326,8 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
     const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
     if (tiles * MAX_SPLIT > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
-    // split the sum while that leaves no more CTAs than the SMs take at once
-    const int64_t units = static_cast<int64_t>(F32 ? (g.kb + CHUNK - 1) / CHUNK : g.kb) * g.segments;
     int splits = 1;
-    while (splits < MAX_SPLIT && tiles * splits * 2 <= int64_t(ctx->num_sms) * S::CTAS && units >= splits * 4) splits *= 2;
+    QSML_TRY_STATUS((best_split<F32, DUAL>(ctx, tiles, g.tiles_m == 1, static_cast<int64_t>(g.kb) * g.segments, &splits)));
     g.splits = splits;
     g.slots = static_cast<int>(S::RING / (g.a_bytes + TILE_BYTES));
     if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
@@ -1217,16 +1354,30 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
 
 }  // namespace
 
-qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
-    // pairs of SMs where the tiles fill them, else 128 x 128 tiles and split sums
+namespace {
+
+// A problem whose operands are known to TMA.
+struct Ready {
+    Staged a[2], b[2];
+    bool pair = false;
     int pairs = 0;
-    if (f32) QSML_TRY_STATUS((p.dual ? max_pairs<true, true>(ctx, &pairs) : max_pairs<true, false>(ctx, &pairs)));
-    else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &pairs) : max_pairs<false, false>(ctx, &pairs)));
+};
+
+qsml_status_t prepare(Context* ctx, Workspace& ws, StageJobs* jobs, const Problem& p, bool f32, Ready* r) {
+    // pairs of SMs where the tiles fill them, else 128 x 128 tiles and split sums
+    if (f32) QSML_TRY_STATUS((p.dual ? max_pairs<true, true>(ctx, &r->pairs) : max_pairs<true, false>(ctx, &r->pairs)));
+    else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &r->pairs) : max_pairs<false, false>(ctx, &r->pairs)));
     const int64_t bn = (f32 ? 128 : 256) / (p.dual ? 2 : 1);
     const int64_t tiles = ((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
-    const bool pair = pairs > 0 && p.M > 128 && tiles >= pairs;
+    r->pair = r->pairs > 0 && p.M > 128 && tiles >= r->pairs;
+    for (int i = 0; i < p.segments; ++i) QSML_TRY_STATUS(stage(ctx, ws, jobs, p.a[i], f32, -1, &r->a[i]));
+    // a dual product's weights share an order: they meet in one MMA
+    for (int i = 0; i < (p.dual ? 2 : p.segments); ++i)
+        QSML_TRY_STATUS(stage(ctx, ws, jobs, p.b[i], f32, p.dual && i ? (r->b[0].trans ? 1 : 0) : -1, &r->b[i]));
+    return QSML_OK;
+}
 
-    Workspace ws(ctx);
+qsml_status_t run_ready(Context* ctx, const Problem& p, bool f32, const Ready& r) {
     TcArgs g;
     g.e = p.e;
     g.M = static_cast<int>(p.M);
@@ -1235,31 +1386,41 @@ qsml_status_t run_tc(Context* ctx, const Problem& p, bool f32) {
     g.segments = p.segments;
     g.status = ctx->status;
     const int na = p.segments, nb = p.dual ? 2 : p.segments;
-    Staged sa[2], sb[2];
-    for (int i = 0; i < na; ++i) QSML_TRY_STATUS(stage(ctx, ws, p.a[i], f32, -1, &sa[i]));
-    // a dual product's weights share an order: they meet in one MMA
-    for (int i = 0; i < nb; ++i)
-        QSML_TRY_STATUS(stage(ctx, ws, p.b[i], f32, p.dual && i ? (sb[0].trans ? 1 : 0) : -1, &sb[i]));
     // few rows: a K-major tile of A holds no more than them, in whole groups of 8
-    int a_rows = !pair && p.M <= 64 ? static_cast<int>((p.M + 7) / 8 * 8) : 128;
+    int a_rows = !r.pair && p.M <= 64 ? static_cast<int>((p.M + 7) / 8 * 8) : 128;
     for (int i = 0; i < na; ++i)
-        if (sa[i].trans) a_rows = 128;
+        if (r.a[i].trans) a_rows = 128;
     g.a_bytes = a_rows * 128;
-    const uint32_t b_rows = pair ? (f32 ? 64 : 128) : (p.dual ? 64 : 128);  // of a K-major box
+    const uint32_t b_rows = r.pair ? (f32 ? 64 : 128) : (p.dual ? 64 : 128);  // of a K-major box
     bool ok = true;
     for (int i = 0; i < 2; ++i) {
-        g.a_mn[i] = sa[i < na ? i : 0].trans ? 1 : 0;  // stored [K, M]
-        g.b_mn[i] = sb[i < nb ? i : 0].trans ? 0 : 1;  // stored [K, N]
-        ok = ok && operand_map(&g.a[i], sa[i < na ? i : 0], f32, g.a_mn[i], static_cast<uint32_t>(a_rows)) &&
-             operand_map(&g.b[i], sb[i < nb ? i : 0], f32, g.b_mn[i], b_rows);
+        const Staged &a = r.a[i < na ? i : 0], &b = r.b[i < nb ? i : 0];
+        g.a_mn[i] = a.trans ? 1 : 0;  // stored [K, M]
+        g.b_mn[i] = b.trans ? 0 : 1;  // stored [K, N]
+        if (i < na) ok = ok && operand_map(&g.a[i], a, f32, g.a_mn[i], static_cast<uint32_t>(a_rows));
+        else g.a[i] = g.a[0];
+        if (i < nb) ok = ok && operand_map(&g.b[i], b, f32, g.b_mn[i], b_rows);
+        else g.b[i] = g.b[0];
     }
     if (!ok) return set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
-    if (pair) {
-        if (f32) return p.dual ? launch_pair<true, true>(ctx, p, g, pairs) : launch_pair<true, false>(ctx, p, g, pairs);
-        return p.dual ? launch_pair<false, true>(ctx, p, g, pairs) : launch_pair<false, false>(ctx, p, g, pairs);
+    if (r.pair) {
+        if (f32) return p.dual ? launch_pair<true, true>(ctx, p, g, r.pairs) : launch_pair<true, false>(ctx, p, g, r.pairs);
+        return p.dual ? launch_pair<false, true>(ctx, p, g, r.pairs) : launch_pair<false, false>(ctx, p, g, r.pairs);
     }
     if (f32) return p.dual ? launch<true, true>(ctx, p, g) : launch<true, false>(ctx, p, g);
     return p.dual ? launch<false, true>(ctx, p, g) : launch<false, false>(ctx, p, g);
+}
+
+}  // namespace
+
+qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32) {
+    Workspace ws(ctx);
+    StageJobs jobs;
+    Ready r[2];
+    for (int i = 0; i < n; ++i) QSML_TRY_STATUS(prepare(ctx, ws, &jobs, *p[i], f32, &r[i]));
+    QSML_TRY_STATUS(run_jobs(ctx, jobs, f32));
+    for (int i = 0; i < n; ++i) QSML_TRY_STATUS(run_ready(ctx, *p[i], f32, r[i]));
+    return QSML_OK;
 }
 
 }  // namespace linear

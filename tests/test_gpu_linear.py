@@ -275,6 +275,22 @@ def test_strides(ctx, how, dt, size):
     check_backward(c, "relu", kept, *backward(ctx, c, "relu", kept, tx=tx, tw=tw, tdy=tdy))
 
 
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 16])
+@pytest.mark.parametrize("how", ["plain", "transposed", "odd", "step"])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_few_rows(ctx, m, how, dt):
+    """A handful of rows, both orders of the weight, loads that fit and loads that do not; a long sum
+    that several CTAs share, and columns past the last whole tile."""
+    for k, n in ((1100, 332), (515, 37)):
+        for gated in (False, True):
+            c = Case(m, k, n, dt, gated=gated)
+            tw = [dev(w) if how == "plain" else strided(w, how) for w in c.w]
+            y, pre = forward(ctx, c, "silu", True, tw=tw)
+            check_forward(c, "silu", y, pre, True)
+            kept = c.kept()
+            check_backward(c, "silu", kept, *backward(ctx, c, "silu", kept, tw=tw))
+
+
 def test_one_row_for_all_and_reversed_rows(ctx):
     """Stride 0 (a broadcast input) and a negative stride."""
     for dt in DTYPES:
