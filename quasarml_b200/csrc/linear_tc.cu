@@ -45,19 +45,23 @@ struct TcArgs {
     int segments;
     int splits;
     int a_bytes;             // k_linear_tc: of an operand tile of A (fewer than 128 rows where M has fewer)
-    int slots;               // k_linear_tc: operand tiles of A and B in the ring
+    int slots, ring;         // k_linear_tc: operand tiles of A and B in the ring, and its bytes
     int a_mn[2], b_mn[2];    // MN-major operands, by segment
     int* status;
 };
 
 // A ring of slots in shared memory, each a tile of A and one of B (of one part, for
-// binary32: a k-block takes three).  Binary16 has two CTAs a SM.
+// binary32: a k-block takes three).  Binary16 has two CTAs a SM with 96 KiB each, or
+// one with 192 KiB where there are no more CTAs than SMs (three slots do not cover
+// L2's latency: 512 x 11008 x 4096 took 68 us).
 template <bool F32> struct Shape {
     static constexpr int PARTS = F32 ? 3 : 1;
-    static constexpr int MAX_SLOTS = F32 ? 6 : 5;
+    static constexpr int MAX_SLOTS = F32 ? 6 : 10;
     static constexpr int TMEM = F32 ? 512 : 128;
-    static constexpr size_t RING = F32 ? 6 * 32768 : 3 * 32768;
-    static constexpr size_t SMEM = RING + 1024 + 144;
+    static constexpr int RING = F32 ? 6 * 32768 : 3 * 32768;
+    static constexpr int DEEP_RING = 6 * 32768;
+    static constexpr int BARS = 8 * (2 * MAX_SLOTS + 5) + 8;
+    static constexpr size_t smem(int ring) { return size_t(ring) + 1024 + BARS; }
     static constexpr int CTAS = F32 ? 1 : 2;  // a SM
 };
 
@@ -245,14 +249,13 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* gbase = smem_raw + (base - raw);
-    const uint32_t bars = base + S::RING;
+    const uint32_t bars = base + g.ring;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S::MAX_SLOTS + s); };
     auto tfull_bar = [&](int a) { return bars + 8u * (2 * S::MAX_SLOTS + a); };
     auto tempty_bar = [&](int a) { return bars + 8u * (2 * S::MAX_SLOTS + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (2 * S::MAX_SLOTS + 4);
-    unsigned char* misc = gbase + S::RING + 8 * (2 * S::MAX_SLOTS + 5);
-    static_assert(8 * (2 * S::MAX_SLOTS + 5) + 8 <= 144, "barriers");
+    unsigned char* misc = gbase + g.ring + 8 * (2 * S::MAX_SLOTS + 5);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
@@ -1282,7 +1285,7 @@ qsml_status_t best_split(Context* ctx, int64_t tiles, bool one_row, int64_t bloc
             attr[0].val.clusterDim.z = 1;
             cfg.gridDim = dim3(static_cast<unsigned>(s * ctx->num_sms));
             cfg.blockDim = dim3(THREADS);
-            cfg.dynamicSmemBytes = S::SMEM;
+            cfg.dynamicSmemBytes = S::smem(S::RING);
             cfg.attrs = attr;
             cfg.numAttrs = 1;
             if (cudaOccupancyMaxActiveClusters(&n[s], k_linear_tc<F32, DUAL>, &cfg) != cudaSuccess || n[s] <= 0) {
@@ -1317,7 +1320,7 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
         const uint64_t bit = uint64_t(1) << (ctx->device & 63);
         if (!(done & bit)) {
             QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                                 static_cast<int>(S::SMEM)),
+                                                                 static_cast<int>(S::smem(S::DEEP_RING))),
                                        "linear: shared-memory attribute"));
             done |= bit;
         }
@@ -1329,7 +1332,8 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     int splits = 1;
     QSML_TRY_STATUS((best_split<F32, DUAL>(ctx, tiles, g.tiles_m == 1, static_cast<int64_t>(g.kb) * g.segments, &splits)));
     g.splits = splits;
-    g.slots = static_cast<int>(S::RING / (g.a_bytes + TILE_BYTES));
+    g.ring = tiles * splits <= ctx->num_sms ? S::DEEP_RING : S::RING;
+    g.slots = g.ring / (g.a_bytes + TILE_BYTES);
     if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
 
     cudaLaunchConfig_t cfg = {};
@@ -1342,7 +1346,7 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.dynamicSmemBytes = S::smem(g.ring);
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
     cfg.numAttrs = splits > 1 ? 2 : 1;
