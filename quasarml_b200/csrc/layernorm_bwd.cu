@@ -527,28 +527,41 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Rows of any width, a CTA a row in three sweeps over global memory (L2 holds a
-// row between them); leaves the row's mean and rstd for the column kernel.
-template <typename T, typename GT>
+// Rows of any width, a CTA a row in three sweeps over global memory by loads of PV
+// elements (L2 holds a row between them); leaves the row's mean and rstd for the
+// column kernel.
+template <typename T, typename GT, int PV>
 __global__ void __launch_bounds__(512)
     k_layer_norm_bwd_rows(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
-                          T* __restrict__ dx, float2* __restrict__ stats, int64_t rows, int64_t cols, float eps) {
+                          T* __restrict__ dx, float2* __restrict__ stats, int64_t rows, int cols, float eps) {
     pdl_begin();
+    using V = Vec<T, PV>;
     __shared__ float slots[4 * 32];
     const float inv_n = __frcp_rn(static_cast<float>(cols));
+    const int packs = cols / PV;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        const T* xr = x + row * cols;
-        const T* yr = dy + row * cols;
+        const V* xr = reinterpret_cast<const V*>(x + row * cols);
+        const V* yr = reinterpret_cast<const V*>(dy + row * cols);
         float s1[1] = {0.0f};
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) s1[0] = __fadd_rn(s1[0], to_f(xr[c]));
+#pragma unroll 4
+        for (int p = threadIdx.x; p < packs; p += 512) {
+            const V v = xr[p];
+#pragma unroll
+            for (int e = 0; e < PV; ++e) s1[0] = __fadd_rn(s1[0], to_f(v.v[e]));
+        }
         row_sums(s1, slots);
         const float mean = __fmul_rn(s1[0], inv_n);
         float s3[3] = {0.0f, 0.0f, 0.0f};
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-            const float d = __fsub_rn(to_f(xr[c]), mean), h = __fmul_rn(to_f(yr[c]), to_f(gamma[c]));
-            s3[0] = __fmaf_rn(d, d, s3[0]);
-            s3[1] = __fadd_rn(s3[1], h);
-            s3[2] = __fmaf_rn(h, d, s3[2]);
+#pragma unroll 2
+        for (int p = threadIdx.x; p < packs; p += 512) {
+            const V v = xr[p], y = yr[p];
+#pragma unroll
+            for (int e = 0; e < PV; ++e) {
+                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), to_f(gamma[p * PV + e]));
+                s3[0] = __fmaf_rn(d, d, s3[0]);
+                s3[1] = __fadd_rn(s3[1], h);
+                s3[2] = __fmaf_rn(h, d, s3[2]);
+            }
         }
         row_sums(s3, slots + 32);
         const float rstd = rsqrtf(__fmaf_rn(s3[0], inv_n, eps));
@@ -556,33 +569,53 @@ __global__ void __launch_bounds__(512)
         if (!dx) continue;
         const float a = __fmul_rn(__fmul_rn(s3[1], inv_n), rstd);
         const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), __fmul_rn(rstd, rstd));
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
-            const float d = __fsub_rn(to_f(xr[c]), mean), h = __fmul_rn(to_f(yr[c]), to_f(gamma[c]));
-            from_f(__fmaf_rn(h, rstd, -__fmaf_rn(d, b, a)), dx[row * cols + c]);
+        V* dr = reinterpret_cast<V*>(dx + row * cols);
+#pragma unroll 2
+        for (int p = threadIdx.x; p < packs; p += 512) {
+            const V v = xr[p], y = yr[p];
+            V o;
+#pragma unroll
+            for (int e = 0; e < PV; ++e) {
+                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), to_f(gamma[p * PV + e]));
+                from_f(__fmaf_rn(h, rstd, -__fmaf_rn(d, b, a)), o.v[e]);
+            }
+            dr[p] = o;
         }
     }
 }
 
 // Column sums of dy xh and dy over the rows [blockIdx.y * chunk, + chunk): a
-// thread a column.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// thread PV columns.
+template <typename T, int PV>
+__global__ void __launch_bounds__(128)
     k_layer_norm_bwd_cols(const T* __restrict__ x, const T* __restrict__ dy, const float2* __restrict__ stats,
-                          float* __restrict__ partial, int64_t rows, int64_t cols, int64_t chunk) {
+                          float* __restrict__ partial, int64_t rows, int cols, int64_t chunk) {
     pdl_begin();
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    using V = Vec<T, PV>;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x) * PV;
     if (c >= cols) return;
     const int64_t r0 = blockIdx.y * chunk, r1 = r0 + chunk < rows ? r0 + chunk : rows;
-    float sg = 0.0f, sb = 0.0f;
+    float sg[PV], sb[PV];
+#pragma unroll
+    for (int e = 0; e < PV; ++e) sg[e] = sb[e] = 0.0f;
 #pragma unroll 4
     for (int64_t r = r0; r < r1; ++r) {
         const float2 st = stats[r];
-        const float y = to_f(dy[r * cols + c]);
-        sg = __fmaf_rn(y, __fmul_rn(__fsub_rn(to_f(x[r * cols + c]), st.x), st.y), sg);
-        sb = __fadd_rn(sb, y);
+        const V v = *reinterpret_cast<const V*>(x + r * cols + c), y = *reinterpret_cast<const V*>(dy + r * cols + c);
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+            const float f = to_f(y.v[e]);
+            sg[e] = __fmaf_rn(f, __fmul_rn(__fsub_rn(to_f(v.v[e]), st.x), st.y), sg[e]);
+            sb[e] = __fadd_rn(sb[e], f);
+        }
     }
-    partial[blockIdx.y * cols + c] = sg;
-    partial[(gridDim.y + static_cast<int64_t>(blockIdx.y)) * cols + c] = sb;
+    float* pg = partial + blockIdx.y * static_cast<int64_t>(cols) + c;
+    float* pb = pg + gridDim.y * static_cast<int64_t>(cols);
+#pragma unroll
+    for (int e = 0; e < PV; ++e) {
+        pg[e] = sg[e];
+        pb[e] = sb[e];
+    }
 }
 
 struct Args {
@@ -668,13 +701,13 @@ template <typename T, typename GT, int PV, int NV, int L> qsml_status_t launch_g
     return a.sums() ? finish(ctx, a, static_cast<float*>(partial), grid) : QSML_OK;
 }
 
-template <typename T, typename GT>
+template <typename T, typename GT, int PV>
 qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
     Workspace ws(ctx);
     void *stats = nullptr, *partial = nullptr;
-    // a chunk of rows for each CTA of the column kernel, about four CTAs an SM
-    const int64_t tiles = (a.cols + 255) / 256;
-    int64_t parts = (4 * ctx->num_sms + tiles - 1) / tiles;
+    // a chunk of rows for each CTA of the column kernel, about eight CTAs an SM
+    const int64_t tiles = (a.cols / PV + 127) / 128;
+    int64_t parts = (8 * ctx->num_sms + tiles - 1) / tiles;
     if (parts > a.rows) parts = a.rows;
     const int64_t chunk = (a.rows + parts - 1) / parts;
     parts = (a.rows + chunk - 1) / chunk;
@@ -683,16 +716,16 @@ qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
         QSML_TRY_STATUS(ws.get(static_cast<size_t>(parts) * a.cols * 2 * sizeof(float), &partial));
     }
     const int64_t grid = a.rows < 4 * ctx->num_sms ? a.rows : 4 * ctx->num_sms;
-    cudaError_t e = launch_pdl(k_layer_norm_bwd_rows<T, GT>, dim3(static_cast<unsigned>(grid)), dim3(512), 0,
+    cudaError_t e = launch_pdl(k_layer_norm_bwd_rows<T, GT, PV>, dim3(static_cast<unsigned>(grid)), dim3(512), 0,
                                ctx->stream, static_cast<const T*>(a.x), static_cast<const GT*>(a.gamma),
                                static_cast<const T*>(a.dy), static_cast<T*>(a.dx), static_cast<float2*>(stats), a.rows,
-                               a.cols, a.eps);
+                               static_cast<int>(a.cols), a.eps);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd_rows");
     QSML_TRY_STATUS(after_launch(ctx, "k_layer_norm_bwd_rows"));
     if (!a.sums()) return QSML_OK;
-    e = launch_pdl(k_layer_norm_bwd_cols<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
-                   dim3(256), 0, ctx->stream, static_cast<const T*>(a.x), static_cast<const T*>(a.dy),
-                   static_cast<const float2*>(stats), static_cast<float*>(partial), a.rows, a.cols, chunk);
+    e = launch_pdl(k_layer_norm_bwd_cols<T, PV>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
+                   dim3(128), 0, ctx->stream, static_cast<const T*>(a.x), static_cast<const T*>(a.dy),
+                   static_cast<const float2*>(stats), static_cast<float*>(partial), a.rows, static_cast<int>(a.cols), chunk);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd_cols");
     QSML_TRY_STATUS(after_launch(ctx, "k_layer_norm_bwd_cols"));
     return finish(ctx, a, static_cast<float*>(partial), parts);
@@ -719,7 +752,7 @@ template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, cons
         if (packs <= 16 * NV) return launch_groups<T, GT, PV, NV, 16>(ctx, a);
         return launch_groups<T, GT, PV, NV, 32>(ctx, a);
     }
-    if (a.cols > 8192) return launch_wide_bwd<T, GT>(ctx, a);
+    if (a.cols > 8192) return launch_wide_bwd<T, GT, PV>(ctx, a);
     if constexpr (PV == 1) return a.cols <= 4096 ? run_cta<T, GT, 1, 8, false>(ctx, a) : run_cta<T, GT, 1, 16, false>(ctx, a);
     else return run_cta<T, GT, PV, (sizeof(T) == 2 ? 32 : 16) / PV, true>(ctx, a);
 }
