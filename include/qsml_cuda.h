@@ -150,8 +150,9 @@ QSML_API qsml_status_t qsml_get_stream(qsml_ctx* ctx, void** stream);
 QSML_API qsml_status_t qsml_synchronize(qsml_ctx* ctx);
 
 /* Limit, in SM clock cycles, after which a kernel that waits for data on an
- * mbarrier (the one-SM tensor-core GEMM, the layer-norm and softmax row
- * pipelines) gives up: it stops, lets every copy and MMA it already issued
+ * mbarrier (the one-SM tensor-core GEMM, the one-SM kernel of the linear
+ * layers, the layer-norm and softmax row pipelines, the layer norm's backward
+ * pass) gives up: it stops, lets every copy and MMA it already issued
  * finish, records QSML_E_TIMEOUT for the next qsml_synchronize and returns,
  * so the context stays usable.  0 restores the default (2e9 cycles, about
  * 1 s).  Stream-ordered: applies to kernels enqueued after the call.  Meant
@@ -370,7 +371,10 @@ QSML_API qsml_status_t qsml_layer_norm(qsml_ctx* ctx, const qsml_tdesc* x, const
  * dx has x's shape and dtype, dgamma and dbeta [last dim] in F32 or x's dtype;
  * each may be NULL when it is not wanted.  Binary32 arithmetic, each output
  * rounded once; the sums over rows run in an order fixed by the shape, so
- * results are run-to-run deterministic.  With no rows dgamma and dbeta are 0.
+ * results are run-to-run deterministic.  Workspace (binary32 column sums of the
+ * CTAs) comes from the context's allocator; a call that is captured into a graph
+ * takes it from the graph (cudaMallocAsync nodes), so graphs and later calls
+ * never share it.  With no rows dgamma and dbeta are 0.
  * Outputs may not overlap an input or each other (QSML_E_INVALID).  No
  * reference counterpart (it has neither layer norm nor gradients). */
 QSML_API qsml_status_t qsml_layer_norm_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* gamma,
@@ -412,7 +416,10 @@ QSML_API qsml_status_t qsml_matmul(qsml_ctx* ctx, const qsml_tdesc* a, const qsm
  * accuracy for finite operands, but an infinite operand gives NaN where the
  * CUDA cores give an infinity; a few rows (16, or 8 of a gated layer) run on
  * the CUDA cores.
- * With no rows nothing is written; with K = 0 the products are 0.
+ * With no rows nothing is written; with K = 0 the products are 0.  Operands that
+ * TMA cannot read (F32, a row pitch or start off 16 bytes, strides in both dims)
+ * are copied once a call to a workspace, taken as qsml_layer_norm_backward takes
+ * its.
  * Replaces a matmul followed by an add, an activation and an add
  * (QuasarML/src/Ops/LinAlg.cpp:221-271, Ops/Elementwise.cpp:139-417), each a
  * dispatch over the whole result. */

@@ -2,7 +2,8 @@
 // names and signatures, over the B200 backend.  Additions: pow, axis-aware
 // slice with a step, transpose(x, d0, d1) as a view, contiguous, cast,
 // layer_norm, batch_matmul, matmul with an output dtype, cpu_fallback_count,
-// row-sharded reductions over several devices.
+// row-sharded reductions over several devices, linear and gated linear layers
+// with their backward passes, layer_norm_backward.
 // The Vulkan-only Kernel type (GLSL pipelines) has no counterpart.
 #pragma once
 
@@ -19,6 +20,7 @@
 #include "Core/Tensor.h"
 #include "Ops/Distributed.h"
 #include "Ops/Elementwise.h"
+#include "Ops/FeedForward.h"
 #include "Ops/LinAlg.h"
 #include "Ops/Manipulation.h"
 #include "Ops/Reduction.h"
@@ -159,6 +161,33 @@ inline TensorPtr transpose(TensorPtr x) { return QuasarML::Ops::transpose(device
 inline TensorPtr transpose(TensorPtr x, i32 d0, i32 d1) { return QuasarML::Ops::transpose(device(), x, d0, d1); }
 inline TensorPtr layer_norm(TensorPtr x, TensorPtr gamma, TensorPtr beta, f32 eps = 1e-5f) {
     return QuasarML::Ops::layer_norm(device(), x, gamma, beta, eps);
+}
+
+// Linear layers (bias, activation and residual in the product's kernel) and the
+// gradients of a feed-forward sublayer.
+using QuasarML::Activation;
+using QuasarML::GatedLinearGrads;
+using QuasarML::LayerNormGrads;
+using QuasarML::LinearGrads;
+inline LayerNormGrads layer_norm_backward(TensorPtr x, TensorPtr gamma, TensorPtr dy, f32 eps = 1e-5f) {
+    return QuasarML::Ops::layer_norm_backward(device(), x, gamma, dy, eps);
+}
+inline TensorPtr linear(TensorPtr x, TensorPtr w, TensorPtr bias = nullptr, Activation act = Activation::None,
+                        TensorPtr residual = nullptr, TensorPtr* keep = nullptr) {
+    return QuasarML::Ops::linear(device(), x, w, bias, act, residual, keep);
+}
+inline LinearGrads linear_backward(TensorPtr x, TensorPtr w, Activation act, TensorPtr pre, TensorPtr dy,
+                                   bool want_dbias = false) {
+    return QuasarML::Ops::linear_backward(device(), x, w, act, pre, dy, want_dbias);
+}
+inline TensorPtr gated_linear(TensorPtr x, TensorPtr w_gate, TensorPtr w_up, Activation act = Activation::Silu,
+                              TensorPtr b_gate = nullptr, TensorPtr b_up = nullptr, TensorPtr* keep_gate = nullptr,
+                              TensorPtr* keep_up = nullptr) {
+    return QuasarML::Ops::gated_linear(device(), x, w_gate, w_up, act, b_gate, b_up, keep_gate, keep_up);
+}
+inline GatedLinearGrads gated_linear_backward(TensorPtr x, TensorPtr w_gate, TensorPtr w_up, Activation act, TensorPtr gate,
+                                              TensorPtr up, TensorPtr dy, bool want_dbias = false) {
+    return QuasarML::Ops::gated_linear_backward(device(), x, w_gate, w_up, act, gate, up, dy, want_dbias);
 }
 
 inline TensorPtr reshape(TensorPtr x, const std::vector<u32>& new_shape) { return QuasarML::Ops::reshape(device(), x, new_shape); }

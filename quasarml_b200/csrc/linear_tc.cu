@@ -304,15 +304,14 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 
     bool done = true;  // epilogue warps: the CTA's sums are complete
     if (warp == 0) {
-        {
-            const bool issue = elect_one();
-            int slot = 0, filled = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int seg = 0; seg < g.segments && ok; ++seg) {
-                int lo, hi;
-                part(seg, lo, hi);
-                by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+        const bool issue = elect_one();
+        int slot = 0, filled = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int seg = 0; seg < g.segments && ok; ++seg) {
+            int lo, hi;
+            part(seg, lo, hi);
+            by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                 const CUtensorMap* ma = &g.a[seg];
                 [[maybe_unused]] const CUtensorMap* mb = &g.b[DUAL ? 0 : seg];
                 for (int kb = lo; kb < hi && ok; ++kb) {
@@ -351,29 +350,27 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         }
                     }
                 }
-                });
-            }
-            // every copy this thread started lands before the memory has another use:
-            // the last fill of each slot (fill i is in slot i % slots, phase i / slots)
-            for (int i = max(0, filled - g.slots); i < filled; ++i) {
-                const uint32_t parity = static_cast<uint32_t>((i / g.slots) & 1);
-                const long long t0 = clock64();
-                while (!mbar_test(full_bar(i % g.slots), parity) && clock64() - t0 < WAIT_CYCLES) {
-                }
+            });
+        }
+        // every copy this thread started lands before the memory has another use:
+        // the last fill of each slot (fill i is in slot i % slots, phase i / slots)
+        for (int i = max(0, filled - g.slots); i < filled; ++i) {
+            const uint32_t parity = static_cast<uint32_t>((i / g.slots) & 1);
+            const long long t0 = clock64();
+            while (!mbar_test(full_bar(i % g.slots), parity) && clock64() - t0 < WAIT_CYCLES) {
             }
         }
     } else if (warp == 1) {
-        {
-            const bool issue = elect_one();
-            int slot = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
-            const uint32_t small = tmem + 256;  // binary32: the five lesser products
-            bool begun = false;
-            for (int seg = 0; seg < g.segments && ok; ++seg) {
-                int lo, hi;
-                part(seg, lo, hi);
-                by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+        const bool issue = elect_one();
+        int slot = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        const uint32_t small = tmem + 256;  // binary32: the five lesser products
+        bool begun = false;
+        for (int seg = 0; seg < g.segments && ok; ++seg) {
+            int lo, hi;
+            part(seg, lo, hi);
+            by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                 const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 128, 128);
                 const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + g.a_bytes, b_mn.value, 0);
                 // binary32: a drain every CHUNK k-blocks; else none inside
@@ -394,7 +391,9 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                             const uint64_t bs = wb + static_cast<uint32_t>(at[pb] * (slot_bytes >> 4));
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                if (issue) mma_f16(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value), id, fresh && k == 0 ? 0u : 1u);
+                                if (issue)
+                                    mma_f16(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value), id,
+                                            fresh && k == 0 ? 0u : 1u);
                         };
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
@@ -426,7 +425,8 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         if (!ok) break;
                         begun = true;
 #pragma unroll
-                        for (int p = 0; p < S::PARTS; ++p) if (issue) mma_commit(empty_bar(at[p]));
+                        for (int p = 0; p < S::PARTS; ++p)
+                            if (issue) mma_commit(empty_bar(at[p]));
                     }
                     if (F32 && ok) {
                         if (issue) mma_commit(tfull_bar(acc));
@@ -436,13 +436,12 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         }
                     }
                 }
-                });
-            }
-            if (!F32 && ok && issue) mma_commit(tfull_bar(0));
-            if (issue) mma_commit(drain_bar);
-            const long long t0 = clock64();
-            while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
-            }
+            });
+        }
+        if (!F32 && ok && issue) mma_commit(tfull_bar(0));
+        if (issue) mma_commit(drain_bar);
+        const long long t0 = clock64();
+        while (!mbar_test(drain_bar, 0) && clock64() - t0 < WAIT_CYCLES) {
         }
     } else {
         const int quarter = warp & 3;
@@ -736,7 +735,9 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_begin();
-    const long long limit = wait_limit(g.status);
+    // not the context's limit: copies in flight complete on the other CTA's barrier, so
+    // a pair gives up only when something is wrong
+    constexpr long long limit = WAIT_CYCLES;
 
     constexpr int BN = DUAL ? S::BCOLS : 2 * S::BCOLS;  // result columns a tile
     const int total = g.tiles_m * g.tiles_n;
@@ -752,19 +753,18 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     // binary32: drains a tile (the CHUNK k-blocks between them counted by segment)
     const int drains = (g.kb + CHUNK - 1) / CHUNK * g.segments;
     if (warp == 0) {
-        {
-            const bool issue = elect_one();
-            int slot = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = pair; t < total && ok; t += pairs) {
-                int mt, nt;
-                decode(t, mt, nt);
-                const int row = mt * 256 + static_cast<int>(rank) * 128;
-                const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
-                for (int seg = 0; seg < g.segments && ok; ++seg) {
-                    const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
-                    by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+        const bool issue = elect_one();
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = pair; t < total && ok; t += pairs) {
+            int mt, nt;
+            decode(t, mt, nt);
+            const int row = mt * 256 + static_cast<int>(rank) * 128;
+            const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
+            for (int seg = 0; seg < g.segments && ok; ++seg) {
+                const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
+                by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                     for (int kb = 0; kb < g.kb && ok; ++kb) {
 #pragma unroll
                         for (int p = 0; p < S::PARTS; ++p) {
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             const uint32_t bar = map_to_rank(full_bar(slot), 0);
                             const uint32_t at = base + slot * S::SLOT, bt = at + TILE_BYTES;
                             if (issue) {
-                            if (a_mn.value) {
+                                if (a_mn.value) {
                                     tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
                                     tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
                                 } else {
@@ -796,8 +796,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             }
                         }
                     }
-                    });
-                }
+                });
             }
         }
     } else if (warp == 1) {
@@ -819,67 +818,70 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 bool begun = false;
                 for (int seg = 0; seg < g.segments && ok; ++seg) {
                     by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
-                    const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 256, S::NACC);
-                    const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + TILE_BYTES, b_mn.value, 0);
-                    for (int k0 = 0; k0 < g.kb && ok; k0 += F32 ? CHUNK : g.kb) {
-                        const int k1 = F32 ? min(k0 + CHUNK, g.kb) : g.kb;
-                        if (F32) {
-                            if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                        }
-                        const uint32_t d = tmem + acc * S::NACC;
-                        for (int kb = k0; kb < k1 && ok; ++kb) {
-                            int at[S::PARTS] = {};  // the parts' slots
-                            auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
-                                const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
-                                const uint64_t bs = wb + static_cast<uint32_t>(at[pb] * (S::SLOT >> 4));
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    if (issue) mma_f16_pair(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value), id, fresh && k == 0 ? 0u : 1u);
-                            };
-#pragma unroll
-                            for (int p = 0; p < S::PARTS; ++p) {
-                                if (!warp_wait(full_bar(slot), phase, abort_flag, limit)) {
+                        const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 256, S::NACC);
+                        const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + TILE_BYTES, b_mn.value, 0);
+                        for (int k0 = 0; k0 < g.kb && ok; k0 += F32 ? CHUNK : g.kb) {
+                            const int k1 = F32 ? min(k0 + CHUNK, g.kb) : g.kb;
+                            if (F32) {
+                                if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
                                     ok = false;
                                     break;
                                 }
                                 tc_fence_after();
-                                at[p] = slot;
-                                if (++slot == S::SLOTS) {
-                                    slot = 0;
-                                    phase ^= 1u;
-                                }
-                                if constexpr (F32) {
-                                    if (p == 0) {
-                                        product(0, 0, d, kb == k0);
-                                    } else if (p == 1) {
-                                        product(1, 1, small, !begun);
-                                        product(0, 1, small, false);
-                                        product(1, 0, small, false);
-                                    } else {
-                                        product(0, 2, small, false);
-                                        product(2, 0, small, false);
-                                    }
-                                } else {
-                                    product(0, 0, d, !begun);
-                                }
                             }
-                            if (!ok) break;
-                            begun = true;
+                            const uint32_t d = tmem + acc * S::NACC;
+                            for (int kb = k0; kb < k1 && ok; ++kb) {
+                                int at[S::PARTS] = {};  // the parts' slots
+                                auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
+                                    const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
+                                    const uint64_t bs = wb + static_cast<uint32_t>(at[pb] * (S::SLOT >> 4));
 #pragma unroll
-                            for (int p = 0; p < S::PARTS; ++p) if (issue) mma_commit_pair(empty_bar(at[p]));
-                        }
-                        if (F32 && ok) {
-                            if (issue) mma_commit_pair(tfull_bar(acc));
-                            if (++acc == 2) {
-                                acc = 0;
-                                acc_phase ^= 1u;
+                                    for (int k = 0; k < 4; ++k)
+                                        if (issue)
+                                            mma_f16_pair(dst, as + k * slice_step(a_mn.value), bs + k * slice_step(b_mn.value),
+                                                         id, fresh && k == 0 ? 0u : 1u);
+                                };
+#pragma unroll
+                                for (int p = 0; p < S::PARTS; ++p) {
+                                    if (!warp_wait(full_bar(slot), phase, abort_flag, limit)) {
+                                        ok = false;
+                                        break;
+                                    }
+                                    tc_fence_after();
+                                    at[p] = slot;
+                                    if (++slot == S::SLOTS) {
+                                        slot = 0;
+                                        phase ^= 1u;
+                                    }
+                                    if constexpr (F32) {
+                                        if (p == 0) {
+                                            product(0, 0, d, kb == k0);
+                                        } else if (p == 1) {
+                                            product(1, 1, small, !begun);
+                                            product(0, 1, small, false);
+                                            product(1, 0, small, false);
+                                        } else {
+                                            product(0, 2, small, false);
+                                            product(2, 0, small, false);
+                                        }
+                                    } else {
+                                        product(0, 0, d, !begun);
+                                    }
+                                }
+                                if (!ok) break;
+                                begun = true;
+#pragma unroll
+                                for (int p = 0; p < S::PARTS; ++p)
+                                    if (issue) mma_commit_pair(empty_bar(at[p]));
+                            }
+                            if (F32 && ok) {
+                                if (issue) mma_commit_pair(tfull_bar(acc));
+                                if (++acc == 2) {
+                                    acc = 0;
+                                    acc_phase ^= 1u;
+                                }
                             }
                         }
-                    }
                     });
                 }
                 if (!ok) break;
