@@ -433,9 +433,9 @@ QSML_API qsml_status_t qsml_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsm
  * with QSML_ACT_NONE it is not read and may be NULL.  dy has unit stride in its
  * last dim and rows of one stride; dx [.., K] and dw [K, N] are contiguous, in
  * x's dtype; dbias [N] in F32 or x's dtype; each may be NULL when it is not
- * wanted.  dz is kept in x's dtype between its computation and the products
- * (rounded once more: the products' operands are of that dtype), dbias is
- * summed before that rounding.  With no rows dw and dbias are 0.  relu' is 0 at
+ * wanted.  Between its computation and the products an F16 dz is rounded to
+ * F16, the type of the products' operands, where it has more than 2^16 elements
+ * (smaller ones keep 22 bits); dbias is summed before that.  With no rows dw and dbias are 0.  relu' is 0 at
  * 0.  No reference counterpart (it has no gradients). */
 QSML_API qsml_status_t qsml_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,
                                             const qsml_tdesc* pre, const qsml_tdesc* dy, const qsml_tdesc* dx,

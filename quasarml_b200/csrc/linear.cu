@@ -208,11 +208,20 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
         want_dw = want_dw || dw[i];
         want_db = want_db || db[i];
     }
-    // dz = dy needs no copy, but binary32 operands of the tensor cores are split once
-    // for both products (which have terms to sum: M and N are not 0 where they run); a few
-    // rows may go to the kernel that takes binary32 as it is
-    const bool split = dtype == QSML_F32 && precision != QSML_MM_FP32_FFMA && M > 16 && (dx || want_dw);
-    const bool plain = nw == 1 && act == QSML_ACT_NONE && !split;
+    // How dz lies between its computation and the products.
+    // binary32: in the three parts of the tensor cores, split once for both products; as
+    // it is where the CUDA cores take it (FFMA, few rows).
+    // binary16: rounding dz adds to dx and dw an error of the size of their own rounding
+    // (1.4 times the error in all).  A dz of up to 2^16 elements is kept in two parts, 22
+    // bits: its products are short (20 x 39 x 35: 17 us either way), and so few roundings
+    // do not even out.  Beyond, two parts would double the products' time (16384 x 1024 x
+    // 2048: 125 us to 250).
+    // Without an activation dz = dy and needs no copy, binary32's split apart.
+    const bool exact = act == QSML_ACT_NONE && nw == 1;
+    const bool split = (dx || want_dw) && (dtype == QSML_F32 ? precision != QSML_MM_FP32_FFMA && M > 16
+                                                             : !exact && M * N <= 65536);
+    const bool plain = exact && !split;
+    const size_t dz_bytes = !split ? es : dtype == QSML_F32 ? 6 : 4;  // an element
     Mat dz[2];
     Workspace ws(ctx);
     GradArgs g;
@@ -227,7 +236,7 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
         if (!plain) {
             if (act != QSML_ACT_NONE || nw == 2) g.pre[i] = pre[i]->data;
             if ((dx || want_dw) && M * N > 0) {
-                QSML_TRY_STATUS(ws.get(static_cast<size_t>(M) * g.pitch * (split ? 6 : es), &g.dz[i]));
+                QSML_TRY_STATUS(ws.get(static_cast<size_t>(M) * g.pitch * dz_bytes, &g.dz[i]));
                 dz[i] = Mat{g.dz[i], M, N, g.pitch, 1, g.plane};
             }
         } else {

@@ -15,8 +15,9 @@ namespace qsml {
 namespace linear {
 
 // A matrix as given: element (r, c) at p + r * rs + c * cs (elements).  plane > 0:
-// binary32 values already split into three bf16 parts, `plane` elements apart
-// (split8), one of the strides being 1 and the other a multiple of 8.
+// values in parts for the tensor cores, `plane` elements apart, one of the strides
+// being 1 and the other a multiple of 8: binary32 as three bf16 (split8), or binary32
+// values of a binary16 problem as two binary16 (halve8).
 struct Mat {
     const void* p = nullptr;
     int64_t rows = 0, cols = 0, rs = 0, cs = 0, plane = 0;
@@ -251,6 +252,19 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint16_t* dst, int64
 #pragma unroll
     for (int p = 0; p < 3; ++p)
         *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// x = h0 + h1 + (below 2^-22 |x|, or 2^-25), h0 and h1 binary16; an x beyond their
+// range is h0 = infinity and h1 = 0.  Eight of them to two rows, `plane` elements apart.
+__device__ __forceinline__ void halve8(const float (&v)[8], __half* dst, int64_t plane) {
+    float hi[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = __half2float(__float2half_rn(v[i]));
+        lo[i] = fabsf(hi[i]) < 65536.0f ? __fsub_rn(v[i], hi[i]) : 0.0f;
+    }
+    store8(dst, 8, true, hi);
+    store8(dst + plane, 8, true, lo);
 }
 
 // The biases of columns col .. col + 7 (0 where there is none), for finish8.

@@ -2,9 +2,8 @@
 // biases' gradients: one pass over dy and what the forward pass kept.
 //   LINEAR: dz = dy act'(pre)            db = column sums of dz
 //   DUAL:   dg = dy u act'(g), du = dy act(g), and the column sums of both
-// dz goes to a workspace that the two products of the backward pass read (binary32:
-// as the three bf16 parts that the tensor cores take); the sums are taken before it
-// is rounded.  Bound by HBM: LINEAR reads 2 and writes
+// dz goes to a workspace that the two products of the backward pass read (in the parts that
+// the tensor cores take, see GradArgs); the sums are taken before it is rounded.  Bound by HBM: LINEAR reads 2 and writes
 // 1 element, DUAL reads 3 and writes 2.
 #include "linear_grad.cuh"
 
@@ -77,10 +76,12 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
 #pragma unroll
             for (int o = 0; o < NO; ++o) {
                 if (a.dz[o]) {
-                    if (sizeof(T) == 4 && a.plane) {
+                    if (a.plane) {
+                        uint16_t* to = static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) d[o][i] = i < n ? d[o][i] : 0.0f;
-                        split8(d[o], static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col, a.plane);
+                        if constexpr (sizeof(T) == 4) split8(d[o], to, a.plane);
+                        else halve8(d[o], reinterpret_cast<__half*>(to), a.plane);
                     } else {
                         store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
                     }

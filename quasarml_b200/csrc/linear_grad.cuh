@@ -14,7 +14,7 @@ struct GradArgs {
     const void* pre[2] = {nullptr, nullptr};  // rows of N; pre[0] null: dz = dy
     void* dz[2] = {nullptr, nullptr};         // rows of `pitch` (a multiple of 8), 16-byte aligned; null: not wanted
     int64_t pitch = 0;
-    int64_t plane = 0;                        // binary32: > 0, dz as three bf16 parts `plane` elements apart
+    int64_t plane = 0;                        // > 0: dz in parts `plane` elements apart (Mat::plane)
     ColumnSum db[2];
     float* partial = nullptr;
 };

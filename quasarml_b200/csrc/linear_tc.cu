@@ -8,7 +8,8 @@
 // Operands that TMA cannot read (a row pitch or start off 16 bytes, strides in
 // both dims) are copied once to a workspace.
 //
-// binary16: one product, kind::f16, binary32 accumulators.
+// binary16: one product, kind::f16, binary32 accumulators; an operand that comes in
+// two parts (its value their sum) is two segments of the sum.
 // binary32: x = x0 + x1 + x2 exactly, three bf16 parts of 8 bits each (the upper
 // bits by truncation, so no part overflows and all have x's sign); the six
 // products x_i w_j with i + j <= 2 are formed on the bf16 pipe, the dropped ones
@@ -42,7 +43,9 @@ struct TcArgs {
     int M, N;
     int tiles_m, tiles_n;
     int kb;                  // k-blocks of 64 a segment
-    int segments;
+    int segments;            // binary16 with an operand in two parts: twice the problem's
+    int halves;              // then 2, else 1
+    int a_halves, b_halves;  // which operand it is
     int splits;
     int a_bytes;             // k_linear_tc: of an operand tile of A (fewer than 128 rows where M has fewer)
     int slots, ring;         // k_linear_tc: operand tiles of A and B in the ring, and its bytes
@@ -308,10 +311,12 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         int slot = 0, filled = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int seg = 0; seg < g.segments && ok; ++seg) {
+        for (int sp = 0; sp < g.segments && ok; ++sp) {
+            const int seg = sp / g.halves, half = sp - seg * g.halves;
             int lo, hi;
-            part(seg, lo, hi);
+            part(sp, lo, hi);
             by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
+                const int ha = g.a_halves ? half : 0, hb = g.b_halves ? half : 0;
                 const CUtensorMap* ma = &g.a[seg];
                 [[maybe_unused]] const CUtensorMap* mb = &g.b[DUAL ? 0 : seg];
                 for (int kb = lo; kb < hi && ok; ++kb) {
@@ -325,22 +330,22 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                         if (issue) {
                             mbar_expect_tx(bar, slot_bytes);
                             if (a_mn.value) {
-                                tma_load_3d(at, ma, bar, mt * 128, kb * 64, p);
-                                tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, p);
+                                tma_load_3d(at, ma, bar, mt * 128, kb * 64, F32 ? p : ha);
+                                tma_load_3d(at + 8192, ma, bar, mt * 128 + 64, kb * 64, F32 ? p : ha);
                             } else {
-                                tma_load_3d(at, ma, bar, kb * 64, mt * 128, p);
+                                tma_load_3d(at, ma, bar, kb * 64, mt * 128, F32 ? p : ha);
                             }
                             if constexpr (DUAL) {
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
-                                    if (b_mn.value) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, p);
-                                    else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, p);
+                                    if (b_mn.value) tma_load_3d(bt + j * 8192, &g.b[j], bar, nt * 64, kb * 64, F32 ? p : hb);
+                                    else tma_load_3d(bt + j * 8192, &g.b[j], bar, kb * 64, nt * 64, F32 ? p : hb);
                                 }
                             } else if (b_mn.value) {
-                                tma_load_3d(bt, mb, bar, nt * 128, kb * 64, p);
-                                tma_load_3d(bt + 8192, mb, bar, nt * 128 + 64, kb * 64, p);
+                                tma_load_3d(bt, mb, bar, nt * 128, kb * 64, F32 ? p : hb);
+                                tma_load_3d(bt + 8192, mb, bar, nt * 128 + 64, kb * 64, F32 ? p : hb);
                             } else {
-                                tma_load_3d(bt, mb, bar, kb * 64, nt * 128, p);
+                                tma_load_3d(bt, mb, bar, kb * 64, nt * 128, F32 ? p : hb);
                             }
                         }
                         ++filled;
@@ -367,9 +372,10 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         bool ok = true;
         const uint32_t small = tmem + 256;  // binary32: the five lesser products
         bool begun = false;
-        for (int seg = 0; seg < g.segments && ok; ++seg) {
+        for (int sp = 0; sp < g.segments && ok; ++sp) {
+            const int seg = sp / g.halves;
             int lo, hi;
-            part(seg, lo, hi);
+            part(sp, lo, hi);
             by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                 const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 128, 128);
                 const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + g.a_bytes, b_mn.value, 0);
@@ -762,8 +768,10 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
             decode(t, mt, nt);
             const int row = mt * 256 + static_cast<int>(rank) * 128;
             const int col = DUAL ? nt * BN : nt * BN + static_cast<int>(rank) * S::BCOLS;
-            for (int seg = 0; seg < g.segments && ok; ++seg) {
+            for (int sp = 0; sp < g.segments && ok; ++sp) {
+                const int seg = sp / g.halves, half = sp - seg * g.halves;
                 const CUtensorMap *ma = &g.a[seg], *mb = &g.b[DUAL ? rank : seg];
+                const int ha = g.a_halves ? half : 0, hb = g.b_halves ? half : 0;
                 by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                     for (int kb = 0; kb < g.kb && ok; ++kb) {
 #pragma unroll
@@ -777,17 +785,17 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             const uint32_t at = base + slot * S::SLOT, bt = at + TILE_BYTES;
                             if (issue) {
                                 if (a_mn.value) {
-                                    tma_load_3d_pair(at, ma, bar, row, kb * 64, p);
-                                    tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, p);
+                                    tma_load_3d_pair(at, ma, bar, row, kb * 64, F32 ? p : ha);
+                                    tma_load_3d_pair(at + 8192, ma, bar, row + 64, kb * 64, F32 ? p : ha);
                                 } else {
-                                    tma_load_3d_pair(at, ma, bar, kb * 64, row, p);
+                                    tma_load_3d_pair(at, ma, bar, kb * 64, row, F32 ? p : ha);
                                 }
                                 if (b_mn.value) {
 #pragma unroll
                                     for (int j = 0; j < S::BCOLS / 64; ++j)
-                                        tma_load_3d_pair(bt + j * 8192, mb, bar, col + j * 64, kb * 64, p);
+                                        tma_load_3d_pair(bt + j * 8192, mb, bar, col + j * 64, kb * 64, F32 ? p : hb);
                                 } else {
-                                    tma_load_3d_pair(bt, mb, bar, kb * 64, col, p);
+                                    tma_load_3d_pair(bt, mb, bar, kb * 64, col, F32 ? p : hb);
                                 }
                             }
                             if (++slot == S::SLOTS) {
@@ -816,7 +824,8 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     tc_fence_after();
                 }
                 bool begun = false;
-                for (int seg = 0; seg < g.segments && ok; ++seg) {
+                for (int sp = 0; sp < g.segments && ok; ++sp) {
+                    const int seg = sp / g.halves;
                     by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
                         const uint32_t id = idesc(F32, a_mn.value, b_mn.value, 256, S::NACC);
                         const uint64_t wa = slice_desc(base, a_mn.value, 0), wb = slice_desc(base + TILE_BYTES, b_mn.value, 0);
@@ -1196,7 +1205,7 @@ qsml_status_t run_jobs(Context* ctx, const StageJobs& jobs, bool f32) {
 
 // mn: MN-major boxes of 64 x 64 k, else K-major boxes of 64 k x `rows`.
 bool operand_map(CUtensorMap* map, const Staged& s, bool f32, bool mn, uint32_t rows) {
-    const uint64_t planes = f32 ? 3 : 1;
+    const uint64_t planes = f32 ? 3 : s.plane ? 2 : 1;
     return make_map(map, s.p, s.inner, s.outer, planes, s.pitch * 2, (s.plane ? s.plane : s.pitch * s.outer) * 2, 64,
                     mn ? 64 : rows, f32 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
 }
@@ -1370,12 +1379,14 @@ struct Ready {
 };
 
 qsml_status_t prepare(Context* ctx, Workspace& ws, StageJobs* jobs, const Problem& p, bool f32, Ready* r) {
-    // pairs of SMs where the tiles fill them, else 128 x 128 tiles and split sums
+    // pairs of SMs where the tiles fill at least 60 % of them, else 128 x 128 tiles and
+    // split sums (at 64 of 74 pairs, 1024 x 4096 x 4096 takes 27 us against 31; at 32,
+    // 512 x 11008 x 4096 57 against 45)
     if (f32) QSML_TRY_STATUS((p.dual ? max_pairs<true, true>(ctx, &r->pairs) : max_pairs<true, false>(ctx, &r->pairs)));
     else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &r->pairs) : max_pairs<false, false>(ctx, &r->pairs)));
     const int64_t bn = (f32 ? 128 : 256) / (p.dual ? 2 : 1);
     const int64_t tiles = ((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
-    r->pair = r->pairs > 0 && p.M > 128 && tiles >= r->pairs;
+    r->pair = r->pairs > 0 && p.M > 128 && tiles * 10 >= r->pairs * 6;
     for (int i = 0; i < p.segments; ++i) QSML_TRY_STATUS(stage(ctx, ws, jobs, p.a[i], f32, -1, &r->a[i]));
     // a dual product's weights share an order: they meet in one MMA
     for (int i = 0; i < (p.dual ? 2 : p.segments); ++i)
@@ -1389,9 +1400,12 @@ qsml_status_t run_ready(Context* ctx, const Problem& p, bool f32, const Ready& r
     g.M = static_cast<int>(p.M);
     g.N = static_cast<int>(p.N);
     g.kb = static_cast<int>((p.K + 63) / 64);
-    g.segments = p.segments;
-    g.status = ctx->status;
     const int na = p.segments, nb = p.dual ? 2 : p.segments;
+    g.a_halves = !f32 && r.a[0].plane ? 1 : 0;
+    g.b_halves = !f32 && r.b[0].plane ? 1 : 0;
+    g.halves = g.a_halves || g.b_halves ? 2 : 1;
+    g.segments = p.segments * g.halves;
+    g.status = ctx->status;
     // few rows: a K-major tile of A holds no more than them, in whole groups of 8
     int a_rows = !r.pair && p.M <= 64 ? static_cast<int>((p.M + 7) / 8 * 8) : 128;
     for (int i = 0; i < na; ++i)

@@ -9,7 +9,8 @@ Tolerances count roundings, element by element.  With u = 2^-24 and h = half a s
   (binary32) or 2^-18 (1 + |z|) (binary16, fast exponential: 2^-21 and 2^-24 |z| of exp, through
   the slope of the sigmoid and a product), its derivative by at most four times that;
 * outputs are rounded once: h |y|, and half the smallest subnormal.
-The backward passes round dz once to the dtype, which the products' bound carries on."""
+The backward passes round dz once to the dtype (a binary16 dz of up to 2^16 elements to two parts:
+2^-22 and the two roundings' ends), which the products' bound carries on."""
 import numpy as np
 import pytest
 
@@ -119,7 +120,8 @@ def check_backward(c, act, kept, dx, dw, db):
         if o is not None:
             near(o, v.sum(0), e.sum(0) + (c.m + 40) * U * np.abs(v).sum(0), "db")
     if not (c.nw == 1 and act == "none"):
-        ez = [e + STEP[c.dt] * (np.abs(v) + e) + TINY[c.dt] for e, v in zip(ez, dz)]
+        step = 2.0 ** -21 if c.dt == np.float16 and c.m * c.n <= 65536 else STEP[c.dt]
+        ez = [e + step * (np.abs(v) + e) + TINY[c.dt] for e, v in zip(ez, dz)]
     w = [v.astype(F64) for v in c.w]
     if dx is not None:
         ref = sum(v @ m.T for v, m in zip(dz, w))
