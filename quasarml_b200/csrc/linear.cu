@@ -159,11 +159,14 @@ qsml_status_t check_dw(Context* ctx, const char* op, Named v, int32_t dtype, int
 }
 
 void set_vec(Epilogue* e, int es) {
-    bool v = e->N % 8 == 0;
-    const void* p[6] = {e->bias[0], e->bias[1], e->residual, e->pre[0], e->pre[1], e->y};
-    for (const void* q : p) v = v && (!q || aligned16(q));
-    if (e->residual) v = v && (e->res_ld * es) % 16 == 0;
-    e->vec = v ? 1 : 0;
+    // the biases are read as single elements where not all is whole
+    const void* p[6] = {e->residual, e->pre[0], e->pre[1], e->y, e->bias[0], e->bias[1]};
+    auto aligned = [&](int n, int64_t elements) {
+        bool v = e->N % elements == 0;
+        for (int i = 0; i < n; ++i) v = v && reinterpret_cast<uintptr_t>(p[i]) % (n == 6 ? 16 : elements * es) == 0;
+        return v && (!e->residual || e->res_ld % elements == 0);
+    };
+    e->vec = aligned(6, 8) ? 1 : aligned(4, 2) ? 2 : 0;
 }
 
 bool on_tensor_cores(int32_t precision, const Problem& p) { return precision != QSML_MM_FP32_FFMA && p.K > 0; }

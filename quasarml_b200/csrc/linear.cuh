@@ -37,7 +37,8 @@ struct Epilogue {
     void* pre[2] = {nullptr, nullptr};
     void* y = nullptr;             // y and pre: rows of N elements
     int64_t N = 0;
-    int vec = 0;                   // groups of 8 columns are whole and 16-byte aligned everywhere
+    int vec = 0;                   // 1: groups of 8 columns are whole and 16-byte aligned everywhere; 2: pairs are
+                                   // whole and aligned; 0: neither
 };
 
 struct Problem {
@@ -152,10 +153,18 @@ template <typename T> __device__ __forceinline__ float act_grad(int act, float z
     return 1.0f;
 }
 
+// Two neighbours, aligned together.
+__device__ __forceinline__ float2 ld2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 ld2(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+__device__ __forceinline__ void st2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void st2(__half* p, float a, float b) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+}
+
 // 8 consecutive elements of a row to binary32 and back; n of them are inside
-// (vec: all 8, 16-byte aligned).
-template <typename T> __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
-    if (vec) {
+// (vec as in Epilogue).
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, int vec, float (&v)[8]) {
+    if (vec == 1) {
         if constexpr (sizeof(T) == 2) {
             const uint4 u = *reinterpret_cast<const uint4*>(p);
             const __half2* h = reinterpret_cast<const __half2*>(&u);
@@ -169,6 +178,13 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int n, b
             const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
             v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+    } else if (vec == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float2 f = i < n ? ld2(p + i) : make_float2(0.0f, 0.0f);
+            v[i] = f.x;
+            v[i + 1] = f.y;
         }
     } else {
 #pragma unroll
@@ -196,7 +212,13 @@ template <typename T> __device__ __forceinline__ void ldg8(const T* p, int n, bo
         load8(p, n, false, v);
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+template <typename T> __device__ __forceinline__ void store8(T* p, int n, int vec, const float (&v)[8]) {
+    if (vec == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if (i < n) st2(p + i, v[i], v[i + 1]);
+        return;
+    }
     if constexpr (sizeof(T) == 2) {
         if (vec) {
             uint4 u;
@@ -277,9 +299,9 @@ __device__ __forceinline__ void bias8(const Epilogue& e, int64_t col, float (&b)
 #pragma unroll
             for (int i = 0; i < 8; ++i) b[w][i] = 0.0f;
         } else if (e.bias_f32) {
-            load8(static_cast<const float*>(e.bias[w]) + col, n, e.vec, b[w]);
+            load8(static_cast<const float*>(e.bias[w]) + col, n, e.vec == 1, b[w]);
         } else {
-            load8(static_cast<const T*>(e.bias[w]) + col, n, e.vec, b[w]);
+            load8(static_cast<const T*>(e.bias[w]) + col, n, e.vec == 1, b[w]);
         }
     }
 }

@@ -101,8 +101,8 @@ __device__ __forceinline__ void add_bias32(const Epilogue& e, int which, int64_t
         if (c >= e.N) break;
         const int n = e.N - c < 8 ? static_cast<int>(e.N - c) : 8;
         float b[8];
-        if (e.bias_f32) ldg8(static_cast<const float*>(e.bias[which]) + c, n, e.vec, b);
-        else ldg8(static_cast<const __half*>(e.bias[which]) + c, n, e.vec, b);
+        if (e.bias_f32) ldg8(static_cast<const float*>(e.bias[which]) + c, n, e.vec == 1, b);
+        else ldg8(static_cast<const __half*>(e.bias[which]) + c, n, e.vec == 1, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[8 * j + i] = __fadd_rn(z[8 * j + i], b[i]);
     }
@@ -149,42 +149,63 @@ template <int COLS> struct HalfRows {
         }
     }
     // The buffer's rows to or from a matrix of N columns, rows of `ld`, whose element
-    // (0, 0) lies at p; a row's units by neighbouring lanes.  `rows` of the 32 exist.
+    // (0, 0) lies at p; `rows` of the 32 exist.  Neighbouring lanes take neighbouring
+    // units of a row (vec 1), pairs (2) or elements (0).
     template <bool LOAD>
-    __device__ void copy(__half* p, int64_t ld, int64_t col, int64_t N, int64_t row0, int rows, bool vec) const {
-        const int lane = threadIdx.x & 31, unit = lane % UNITS;
-        const int64_t c = col + unit * 8;
-        if (c >= N) return;
-        const int n = N - c < 8 ? static_cast<int>(N - c) : 8;
+    __device__ void copy(__half* p, int64_t ld, int64_t col, int64_t N, int64_t row0, int rows, int vec) const {
+        if (vec == 1) move<LOAD, 8>(p + row0 * ld + col, ld, N - col, rows);
+        else if (vec == 2) move<LOAD, 2>(p + row0 * ld + col, ld, N - col, rows);
+        else move<LOAD, 1>(p + row0 * ld + col, ld, N - col, rows);
+    }
+
+private:
+    // E elements a lane; the first `left` columns exist, a multiple of E
+    template <bool LOAD, int E> __device__ void move(__half* p, int64_t ld, int64_t left, int rows) const {
+        constexpr int LANES = COLS / E;  // of a row
+        constexpr int STEPS = LANES > 32 ? LANES / 32 : 1, ROWS = LANES > 32 ? 1 : 32 / LANES;
+        const int lane = threadIdx.x & 31, c0 = lane % LANES * E;
 #pragma unroll 4
-        for (int r = lane / UNITS; r < rows; r += 32 / UNITS) {
-            __half* q = p + (row0 + r) * ld + c;
-            uint4 u;
-            __half* h = reinterpret_cast<__half*>(&u);
-            if constexpr (LOAD) {
-                if (vec) {
-                    u = *reinterpret_cast<const uint4*>(q);
-                } else {
+        for (int r = LANES > 32 ? 0 : lane / LANES; r < rows; r += ROWS)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = i < n ? q[i] : __float2half_rn(0.0f);
-                }
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(r, unit)), "r"(u.x), "r"(u.y), "r"(u.z),
-                             "r"(u.w)
-                             : "memory");
-            } else {
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                             : "r"(at(r, unit))
-                             : "memory");
-                if (vec) {
-                    *reinterpret_cast<uint4*>(q) = u;
+            for (int j = 0; j < STEPS; ++j) {
+                const int c = c0 + j * 32 * E;
+                if (c >= left) continue;
+                __half* q = p + r * ld + c;
+                const uint32_t s = at(r, c / 8) + c % 8 * 2;
+                if constexpr (E == 8) {
+                    uint4 u;
+                    if (LOAD) {
+                        u = *reinterpret_cast<const uint4*>(q);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s), "r"(u.x), "r"(u.y), "r"(u.z),
+                                     "r"(u.w)
+                                     : "memory");
+                    } else {
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                     : "r"(s)
+                                     : "memory");
+                        *reinterpret_cast<uint4*>(q) = u;
+                    }
+                } else if constexpr (E == 2) {
+                    uint32_t u;
+                    if (LOAD) {
+                        u = *reinterpret_cast<const uint32_t*>(q);
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(s), "r"(u) : "memory");
+                    } else {
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(s) : "memory");
+                        *reinterpret_cast<uint32_t*>(q) = u;
+                    }
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i < n) q[i] = h[i];
+                    uint16_t u;
+                    if (LOAD) {
+                        u = *reinterpret_cast<const uint16_t*>(q);
+                        asm volatile("st.shared.b16 [%0], %1;" ::"r"(s), "h"(u) : "memory");
+                    } else {
+                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(u) : "r"(s) : "memory");
+                        *reinterpret_cast<uint16_t*>(q) = u;
+                    }
                 }
             }
-        }
     }
 };
 
@@ -559,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 }
             return t;
         };
-        if (g.e.vec) {
+        if (g.e.vec == 1) {
             // 8 columns a thread, always the same ones
             constexpr int UNITS = BN / 8;
             static_assert(THREADS % UNITS == 0, "a thread keeps its columns");
@@ -582,68 +603,91 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 }
             }
         } else {
-            // rows off 16 bytes: a warp a row, every 32nd column a lane, ROWS rows together
-            constexpr int STEPS = BN / 32, ROWS = 4, WARPS = THREADS / 32;
-            auto sum1 = [&](int r, int c) { return lds1(base + r * 512 + (((c / 4) ^ (r & 31)) << 4) + (c & 3) * 4); };
+            // rows off 16 bytes: a warp a row, every 32nd column (or pair of them) a lane,
+            // ROWS rows together
+            constexpr int STEPS = BN / 32, ROWS = 4, WARPS = THREADS / 32, ALL = ROWS * STEPS;
             const Epilogue& e = g.e;
-            float b0[STEPS], b1[STEPS];
-            bool in[STEPS];
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) {
-                const int64_t col = col0 + j * 32 + lane;
-                in[j] = col < g.N;
-                b0[j] = in[j] ? bias1<T>(e, 0, col) : 0.0f;
-                b1[j] = DUAL && in[j] ? bias1<T>(e, 1, col) : 0.0f;
-            }
             const int step = g.splits * WARPS;
-            for (int r0 = rank * WARPS + warp; r0 < rows; r0 += ROWS * step) {
-                if (g.splits > 1) {  // the cluster's sums of these rows, in place of this CTA's part
+            auto rows_of = [&](auto pairs) {
+                constexpr bool P = pairs.value;
+                // element k of the ROWS rows: its column, its row, whether it exists, where it is
+                auto col = [&](int k) { return P ? k % STEPS / 2 * 64 + lane * 2 + (k & 1) : k % STEPS * 32 + lane; };
+                float b0[STEPS], b1[STEPS];
 #pragma unroll
-                    for (int i = 0; i < ROWS; ++i) {
-                        const int r = r0 + i * step;
-                        if (r >= rows) break;
-                        const float4 t = sum4(r, lane);
-                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(base + r * 512 + ((lane ^ (r & 31)) << 4)),
-                                     "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w)
-                                     : "memory");
+                for (int j = 0; j < STEPS; ++j) {
+                    const bool in = col0 + col(j) < g.N;
+                    b0[j] = in ? bias1<T>(e, 0, col0 + col(j)) : 0.0f;
+                    b1[j] = DUAL && in ? bias1<T>(e, 1, col0 + col(j)) : 0.0f;
+                }
+                for (int r0 = rank * WARPS + warp; r0 < rows; r0 += ROWS * step) {
+                    auto row = [&](int k) { return r0 + k / STEPS * step; };
+                    auto here = [&](int k) { return row(k) < rows && col0 + col(k) < g.N; };
+                    auto at = [&](int k, int64_t ld) { return (row0 + row(k)) * ld + col0 + col(k); };
+                    if (g.splits > 1) {  // the cluster's sums of these rows, in place of this CTA's part
+#pragma unroll
+                        for (int i = 0; i < ROWS; ++i) {
+                            const int r = r0 + i * step;
+                            if (r >= rows) break;
+                            const float4 t = sum4(r, lane);
+                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             base + r * 512 + ((lane ^ (r & 31)) << 4)),
+                                         "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w)
+                                         : "memory");
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    float z[ALL], u[DUAL ? ALL : 1];
+                    [[maybe_unused]] float res[DUAL ? 1 : ALL];
+                    if constexpr (!DUAL) {
+                        if (e.residual && e.y) {
+                            const T* from = static_cast<const T*>(e.residual);
+#pragma unroll
+                            for (int k = 0; k < ALL; k += P ? 2 : 1)
+                                if (here(k)) {
+                                    if constexpr (P) {
+                                        const float2 f = ld2(from + at(k, e.res_ld));
+                                        res[k] = f.x;
+                                        res[k + 1] = f.y;
+                                    } else {
+                                        res[k] = ld1(from + at(k, e.res_ld));
+                                    }
+                                }
+                        }
+                    }
+                    auto tile = [&](int k, int c) {
+                        const int r = min(row(k), rows - 1);
+                        return lds1(base + r * 512 + (((c / 4) ^ (r & 31)) << 4) + (c & 3) * 4);
+                    };
+#pragma unroll
+                    for (int k = 0; k < ALL; ++k) {
+                        z[k] = __fadd_rn(tile(k, col(k)), b0[k % STEPS]);
+                        if constexpr (DUAL) u[k] = __fadd_rn(tile(k, 64 + col(k)), b1[k % STEPS]);
+                    }
+                    auto store = [&](void* p, const float* v) {
+                        T* to = static_cast<T*>(p);
+#pragma unroll
+                        for (int k = 0; k < ALL; k += P ? 2 : 1)
+                            if (here(k)) {
+                                if constexpr (P) st2(to + at(k, e.N), v[k], v[k + 1]);
+                                else st1(to + at(k, e.N), v[k]);
+                            }
+                    };
+                    if (e.pre[0]) store(e.pre[0], z);
+                    if (DUAL && e.pre[1]) store(e.pre[1], u);
+                    if (!e.y) continue;
+                    act_all<T>(e.act, z);
+                    if constexpr (DUAL) {
+#pragma unroll
+                        for (int k = 0; k < ALL; ++k) z[k] = __fmul_rn(z[k], u[k]);
+                    } else if (e.residual) {
+#pragma unroll
+                        for (int k = 0; k < ALL; ++k) z[k] = __fadd_rn(z[k], res[k]);
+                    }
+                    store(e.y, z);
                 }
-                float z[ROWS * STEPS], u[DUAL ? ROWS * STEPS : 1], res[DUAL ? 1 : ROWS * STEPS];
-                // element k of the ROWS rows: whether it exists, and where
-                auto here = [&](int k) { return in[k % STEPS] && r0 + k / STEPS * step < rows; };
-                auto at = [&](int k, int64_t ld) {
-                    return (row0 + r0 + k / STEPS * step) * ld + col0 + k % STEPS * 32 + lane;
-                };
-                if (!DUAL && e.residual && e.y) {
-#pragma unroll
-                    for (int k = 0; k < ROWS * STEPS; ++k)
-                        if (here(k)) res[DUAL ? 0 : k] = ld1(static_cast<const T*>(e.residual) + at(k, e.res_ld));
-                }
-#pragma unroll
-                for (int k = 0; k < ROWS * STEPS; ++k) {
-                    const int r = min(r0 + k / STEPS * step, rows - 1), c = k % STEPS * 32 + lane;
-                    z[k] = __fadd_rn(sum1(r, c), b0[k % STEPS]);
-                    if constexpr (DUAL) u[k] = __fadd_rn(sum1(r, 64 + c), b1[k % STEPS]);
-                }
-                auto store = [&](void* p, const float* v) {
-#pragma unroll
-                    for (int k = 0; k < ROWS * STEPS; ++k)
-                        if (here(k)) st1(static_cast<T*>(p) + at(k, e.N), v[k]);
-                };
-                if (e.pre[0]) store(e.pre[0], z);
-                if (DUAL && e.pre[1]) store(e.pre[1], u);
-                if (!e.y) continue;
-                act_all<T>(e.act, z);
-                if constexpr (DUAL) {
-#pragma unroll
-                    for (int k = 0; k < ROWS * STEPS; ++k) z[k] = __fmul_rn(z[k], u[k]);
-                } else if (e.residual) {
-#pragma unroll
-                    for (int k = 0; k < ROWS * STEPS; ++k) z[k] = __fadd_rn(z[k], res[k]);
-                }
-                store(e.y, z);
-            }
+            };
+            if (e.vec == 2) rows_of(std::true_type{});
+            else rows_of(std::false_type{});
         }
     } else if (threadIdx.x == 0) {
         atomicExch(g.status, QSML_E_TIMEOUT);
@@ -1034,7 +1078,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 static_assert((DUAL ? 3 : 2) * Rows::BYTES <= S::OUT_WARP, "staging");
                 const int rows = max(0, min(32, g.M - row0));
                 const Epilogue& e = g.e;
-                const bool vec = e.vec;
+                const int vec = e.vec;
                 if (!ready()) break;
                 const uint32_t d = lanes + acc * S::NACC;
                 if (cbegin >= cend) release(tempty_bar(acc));
