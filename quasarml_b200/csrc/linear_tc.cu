@@ -284,6 +284,17 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
+    const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
+    constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
+    // this CTA's share of the k-blocks, and of it the part [lo, hi) in segment seg
+    const int total = g.kb * g.segments;
+    const int u0 = static_cast<int>(static_cast<int64_t>(total) * rank / g.splits);
+    const int u1 = static_cast<int>(static_cast<int64_t>(total) * (rank + 1) / g.splits);
+    auto part = [&](int seg, int& lo, int& hi) {
+        lo = min(max(u0 - seg * g.kb, 0), g.kb);
+        hi = min(max(u1 - seg * g.kb, 0), g.kb);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < g.slots; ++s) {
             mbar_init(full_bar(s), 1);
@@ -311,17 +322,6 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     pdl_begin();  // everything above needed no memory of the kernels before
     const long long limit = wait_limit(g.status);
 
-    const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
-    const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
-    constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
-    // this CTA's share of the k-blocks, and of it the part [lo, hi) in segment seg
-    const int total = g.kb * g.segments;
-    const int u0 = static_cast<int>(static_cast<int64_t>(total) * rank / g.splits);
-    const int u1 = static_cast<int>(static_cast<int64_t>(total) * (rank + 1) / g.splits);
-    auto part = [&](int seg, int& lo, int& hi) {
-        lo = min(max(u0 - seg * g.kb, 0), g.kb);
-        hi = min(max(u1 - seg * g.kb, 0), g.kb);
-    };
     // A's tile comes first: where it has fewer than 128 rows the MMA takes the rest
     // from B's, for rows of the result that are not there
     const uint32_t slot_bytes = g.a_bytes + TILE_BYTES;
@@ -1387,7 +1387,10 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     int splits = 1;
     QSML_TRY_STATUS((best_split<F32, DUAL>(ctx, tiles, g.tiles_m == 1, static_cast<int64_t>(g.kb) * g.segments, &splits)));
     g.splits = splits;
-    g.ring = tiles * splits <= ctx->num_sms ? S::DEEP_RING : S::RING;
+    // few rows: slots are small, and with the small ring the next call's CTAs fit beside
+    // this one's, so that their set-up overlaps its end (gated 5 x 4096 x 11008 35.9 ->
+    // 31.5 us; asking for the weight's first blocks ahead of the wait, into L2, took 36)
+    g.ring = tiles * splits <= ctx->num_sms && g.a_bytes == TILE_BYTES ? S::DEEP_RING : S::RING;
     g.slots = g.ring / (g.a_bytes + TILE_BYTES);
     if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
 
