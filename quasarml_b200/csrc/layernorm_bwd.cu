@@ -475,18 +475,15 @@ __global__ void __launch_bounds__(256)
         work.deviations(__fmul_rn(group_sum(s), inv_n), s3);
 #pragma unroll
         for (int k = 0; k < 3; ++k) s3[k] = group_sum(s3[k]);
-        C out;
-        // a group past the last row must not add to the columns' sums: its dy is 0
-        if (!here) {
+        if (here) {  // a group past the last row adds nothing to the columns' sums
+            C out;
+            work.outputs(s3, inv_n, eps, out);
+            if (dx) {
+                V* dr = reinterpret_cast<V*>(dx + row * cols);
 #pragma unroll
-            for (int j = 0; j < C::H; ++j) work.y[j].v = work.d[j].v = 0;
-        }
-        work.outputs(s3, inv_n, eps, out);
-        if (dx && here) {
-            V* dr = reinterpret_cast<V*>(dx + row * cols);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (work.in(i)) dr[t + i * L] = out.v[i];
+                for (int i = 0; i < NV; ++i)
+                    if (work.in(i)) dr[t + i * L] = out.v[i];
+            }
         }
     }
     if (!partial) return;
@@ -538,13 +535,13 @@ __global__ void __launch_bounds__(512)
     using V = Vec<T, PV>;
     __shared__ float slots[4 * 32];
     const float inv_n = __frcp_rn(static_cast<float>(cols));
-    const int packs = cols / PV;
+    const unsigned packs = cols / PV;  // a step past 2^31 - 1 columns still fits
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const V* xr = reinterpret_cast<const V*>(x + row * cols);
         const V* yr = reinterpret_cast<const V*>(dy + row * cols);
         float s1[1] = {0.0f};
 #pragma unroll 4
-        for (int p = threadIdx.x; p < packs; p += 512) {
+        for (unsigned p = threadIdx.x; p < packs; p += 512) {
             const V v = xr[p];
 #pragma unroll
             for (int e = 0; e < PV; ++e) s1[0] = __fadd_rn(s1[0], to_f(v.v[e]));
@@ -553,7 +550,7 @@ __global__ void __launch_bounds__(512)
         const float mean = __fmul_rn(s1[0], inv_n);
         float s3[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll 2
-        for (int p = threadIdx.x; p < packs; p += 512) {
+        for (unsigned p = threadIdx.x; p < packs; p += 512) {
             const V v = xr[p], y = yr[p];
 #pragma unroll
             for (int e = 0; e < PV; ++e) {
@@ -571,7 +568,7 @@ __global__ void __launch_bounds__(512)
         const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), __fmul_rn(rstd, rstd));
         V* dr = reinterpret_cast<V*>(dx + row * cols);
 #pragma unroll 2
-        for (int p = threadIdx.x; p < packs; p += 512) {
+        for (unsigned p = threadIdx.x; p < packs; p += 512) {
             const V v = xr[p], y = yr[p];
             V o;
 #pragma unroll
@@ -742,7 +739,7 @@ template <typename T, typename GT, int PV, int NV, bool RING> qsml_status_t run_
 // Loads of PV elements.  Rows of up to 512 columns: 4 to 32 lanes with 16 elements
 // each.  Up to 8192: a CTA, whose threads hold 32 elements of binary16 rows (fewer
 // warps meet at the row's two barriers and more rows are on a SM: 16384 x 4096 took
-// 98 us with 16 elements and 124 with 8), 16 of binary32 ones, 8 or 16 single ones.
+// 93 us so, 98 with 16 elements, 124 with 8), 16 of binary32 ones, 8 or 16 single ones.
 template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, const Args& a) {
     const int64_t packs = a.cols / PV;
     if (a.cols <= 512) {

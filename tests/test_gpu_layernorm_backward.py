@@ -13,6 +13,7 @@ dgamma and dbeta sum over rows in at most rows / CTAs + 40 steps:
 |err| <= (60 + rows / 148) u * sum |terms|, plus xh's error, plus half a step."""
 import numpy as np
 import pytest
+import torch
 
 from helpers import d, dev, empty, host
 from quasarml_b200 import abi, datagen
@@ -105,6 +106,28 @@ def test_large_mean_and_constant_rows(ctx):
     x += 1000.0
     x[5] = 3.0
     check(x, g, dy, 1e-3, *run(ctx, x, g, dy, eps=1e-3))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 9, 200])
+@pytest.mark.parametrize("cols", [24, 200, 1024])
+def test_eps_zero(ctx, rows, cols):
+    """Lanes and warps without a row have nothing to add, not 0 times an infinite rstd."""
+    x, g, dy = make((rows, cols), np.float32)
+    check(x, g, dy, 0.0, *run(ctx, x, g, dy, eps=0.0))
+
+
+def test_widest_row(ctx):
+    """2^31 - 1 columns.  x alternates 1, -1 and dy 1, 1, -1, -1: a thread's sums are
+    whole numbers below 2^24, the means 0 to 2^-30, and with eps = 3, rstd = 1/2 and
+    dx = dy / 2 to within 2^-28, which rounds to 1/2."""
+    n = 2**31 - 1
+    fill = lambda *v: torch.tensor(v, dtype=torch.float16, device="cuda").repeat(2**29)[:n]  # noqa: E731
+    x, dy, g = fill(1, -1, 1, -1), fill(1, 1, -1, -1), fill(1, 1, 1, 1)
+    dx = torch.zeros(n, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.layer_norm_backward(d(x), d(g), d(dy), 3.0, d(dx), None, None)
+    ctx.synchronize()
+    assert torch.equal(dx, dy.mul_(0.5))
 
 
 def test_non_finite_rows_stay_in_their_rows(ctx):
