@@ -56,7 +56,8 @@ struct TcArgs {
 // A ring of slots in shared memory, each a tile of A and one of B (of one part, for
 // binary32: a k-block takes three).  Binary16 has two CTAs a SM with 96 KiB each, or
 // one with 192 KiB where there are no more CTAs than SMs (three slots do not cover
-// L2's latency: 512 x 11008 x 4096 took 68 us).
+// L2's latency: 512 x 11008 x 4096 took 70 us, with six 45; 256 x 11008 x 4096 42 and
+// 30).
 template <bool F32> struct Shape {
     static constexpr int PARTS = F32 ? 3 : 1;
     static constexpr int MAX_SLOTS = F32 ? 6 : 10;
@@ -706,8 +707,9 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 // under the products of the next.
 //   binary16: 256 x 256 of the result a pair (dual: 128 columns of each weight, one
 //     from each CTA), six stages of 32 KiB a CTA, two accumulators of 256 columns;
-//   binary32: 256 x 128 (dual: 64 of each), eight slots of one part (24 KiB a CTA), two accumulators for the drains of the main product and two, by tile, for the
-//     lesser ones.
+//   binary32: 256 x 128 (dual: 64 of each), eight slots of one part (24 KiB a CTA), two
+//     accumulators for the drains of the main product and two, by tile, for the lesser
+//     ones.
 // Each CTA loads its own 128 rows of A and half of the tile's columns of B; the
 // leader issues the MMAs of both.  Roles and barriers as in k_linear_tc, the
 // leader's full barrier counting both CTAs' bytes.
@@ -1319,8 +1321,10 @@ template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Pro
 // 5 x 4096 x 11008 took 35 us unsplit in one turn and 41 us in three parts and two).
 // More rows: the tensor pipe of a SM bounds.  A SM works off its CTAs' k-blocks, and
 // each turn has about OVER blocks' time of beginning and end, a joint sum half of it
-// again; the fewest such blocks win, fewer splits on a tie (512 x 11008 x 4096, one
-// tile a SM: 54 us unsplit, 68 us split in two).
+// again; the fewest such blocks win, fewer splits on a tie (512 x 11008 x 4096, 128
+// tiles: 45 us unsplit, 49 in two; 256 x 11008 x 4096, 64 tiles: 41 us unsplit, 29 in
+// two, 37 in three; binary32 128 x 8192 x 1024, 8 tiles of one row: 139 us unsplit, 52 in
+// four, 39 in eight).
 template <bool F32, bool DUAL>
 qsml_status_t best_split(Context* ctx, int64_t tiles, bool one_row, int64_t blocks, int* splits) {
     using S = Shape<F32>;
