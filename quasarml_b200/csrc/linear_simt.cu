@@ -2,8 +2,8 @@
 // alignment, one binary32 fma per k, k ascending.  128 x 64 outputs a CTA (twice
 // that for a dual product), 4 rows x 8 columns a thread, k slices of 16 staged
 // in shared memory with the next slice's loads in flight.  It serves
-// QSML_MM_FP32_FFMA, products with nothing to sum, and those too small for the
-// tensor cores' set-up to pay.  Bound by the FFMA pipe on large products.
+// QSML_MM_FP32_FFMA and products with nothing to sum.  Bound by the FFMA pipe on
+// large products.
 #include "linear.cuh"
 
 namespace qsml {

@@ -418,6 +418,66 @@ def test_large_products(ctx, dt, size):
     assert rel(dw, x.double().t() @ dg) <= 2 * bar(m) and rel(dw2, x.double().t() @ du) <= 2 * bar(m)
 
 
+def whole(tdt, seed, *shape):
+    """Whole numbers from -2 to 2."""
+    import torch
+    return torch.randint(-2, 3, shape, generator=torch.Generator(device="cuda").manual_seed(seed),
+                         device="cuda", dtype=torch.int8).to(tdt)
+
+
+@pytest.mark.parametrize("precision", [abi.MM_AUTO, abi.MM_FP32_FFMA])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_more_than_2_to_the_31_outputs(ctx, dt, precision):
+    """Whole numbers, whose products (at most 8 x 4 + 4) are exact in every type."""
+    import torch
+    if dt == np.float16 and precision == abi.MM_FP32_FFMA:
+        precision = abi.MM_FP16_F32ACC
+    tdt = torch.float32 if dt == np.float32 else torch.float16
+    m, k, n = 2**21 + 77, 8, 1032
+    x, w, b, res = whole(tdt, 1, m, k), whole(tdt, 2, k, n), whole(tdt, 3, n), whole(tdt, 4, m, n)
+    y, pre = torch.empty_like(res), torch.empty_like(res)
+    ctx.linear(d(x), d(w), d(b), abi.ACT_RELU, d(res), d(pre), d(y), precision)
+    for i in range(0, m, 2**18):
+        want = x[i:i + 2**18] @ w + b
+        assert torch.equal(pre[i:i + 2**18], want)
+        assert torch.equal(y[i:i + 2**18], want.relu() + res[i:i + 2**18])
+    # and back: few rows of dy are not 0, so that every sum stays exact
+    del y
+    dy, dx = res.zero_(), torch.full_like(x, float("nan"))
+    rows = torch.tensor([0, 1000, 2**20 + 3, m - 200, m - 1], device="cuda")
+    dy[rows] = whole(tdt, 5, 5, n)
+    dw, db = torch.empty_like(w), torch.empty(n, device="cuda")
+    few = torch.randint(0, 50, (2, 16), generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    w.zero_()[:, few[0] * 20 + few[1] % 20] = 1  # at most 16 columns of 1: dx is at most 32
+    ctx.linear_backward(d(x), d(w), abi.ACT_RELU, d(pre), d(dy), d(dx), d(dw), d(db), precision)
+    dz = dy[rows] * (pre[rows] > 0)
+    want = torch.zeros_like(x)
+    want[rows] = (dz.double() @ w.double().t()).to(tdt)
+    assert torch.equal(dx, want)
+    assert torch.equal(dw, (x[rows].double().t() @ dz.double()).to(tdt))
+    assert torch.equal(db, dz.float().sum(0))
+
+
+@pytest.mark.parametrize("m", [1, 3, 40])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_weight_of_more_than_2_to_the_31_elements(ctx, dt, m):
+    """As above; x is 0 but for its ends."""
+    import torch
+    tdt = torch.float32 if dt == np.float32 else torch.float16
+    k, n = 2**16 + 8, 2**15 + 24
+    w, x = whole(tdt, 1, k, n), torch.zeros(m, k, dtype=tdt, device="cuda")
+    x[:, :4], x[:, -4:] = whole(tdt, 2, m, 4), whole(tdt, 3, m, 4)
+    y, dx = torch.empty(m, n, dtype=tdt, device="cuda"), torch.empty_like(x)
+    ctx.linear(d(x), d(w), None, abi.ACT_NONE, None, None, d(y))
+    ends = torch.tensor([0, 1, 2, 3, k - 4, k - 3, k - 2, k - 1], device="cuda")
+    assert torch.equal(y, (x[:, ends].double() @ w[ends].double()).to(tdt))
+    dy = torch.zeros_like(y)
+    dy[:, :4], dy[:, -4:] = whole(tdt, 4, m, 4), whole(tdt, 5, m, 4)
+    ctx.linear_backward(d(x), d(w), abi.ACT_NONE, None, d(dy), d(dx), None, None)
+    ends = torch.tensor([0, 1, 2, 3, n - 4, n - 3, n - 2, n - 1], device="cuda")
+    assert torch.equal(dx, (dy[:, ends].double() @ w[:, ends].double().t()).to(tdt))
+
+
 @pytest.mark.parametrize("size", [(1, 4096, 1000), (200, 1024, 256), (600, 512, 1024)])
 @pytest.mark.parametrize("dt", DTYPES)
 def test_same_bits_again(ctx, size, dt):
