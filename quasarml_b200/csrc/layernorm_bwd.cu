@@ -21,6 +21,7 @@
 // k_layer_norm_bwd_groups: rows narrower than a CTA's, 4 to 32 lanes a row.
 // k_layer_norm_bwd_rows + k_layer_norm_bwd_cols: rows wider than the registers
 // hold, in two kernels (5 elements of traffic and the row statistics).
+#include "packed.cuh"
 #include "row_pipe.cuh"
 #include "workspace.cuh"
 
@@ -55,40 +56,6 @@ template <int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* 
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_add(lane < nw ? slot[i * 32 + lane] : 0.0f);
-}
-
-// Two binary32 values in one register pair and the packed arithmetic of sm_100.
-struct P2 {
-    uint64_t v;
-};
-__device__ __forceinline__ P2 pack(float a, float b) {
-    P2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack(P2 p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-    return f;
-}
-__device__ __forceinline__ P2 add2(P2 a, P2 b) {
-    P2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ P2 mul2(P2 a, P2 b) {
-    P2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ P2 fma2(P2 a, P2 b, P2 c) {
-    P2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ float sum2(P2 p) {
-    const float2 f = unpack(p);
-    return __fadd_rn(f.x, f.y);
 }
 
 // A thread's columns: NV groups of PV elements, group i at column

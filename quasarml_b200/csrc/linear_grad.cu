@@ -4,8 +4,8 @@
 //   DUAL:   dg = dy u act'(g), du = dy act(g), and the column sums of both
 // dz goes to a workspace that the two products of the backward pass read (in the parts
 // that the tensor cores take, see GradArgs); the sums are taken before it is rounded.
-// Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16,
-// 8192 x 5632: 80 us, 5.8 TB/s).
+// Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16:
+// 16384 x 2048 with gelu 38 us, 5.3 TB/s; DUAL 8192 x 5632 76 us, 6.1 TB/s).
 #include "linear_grad.cuh"
 
 namespace qsml {
@@ -27,7 +27,10 @@ template <typename T> struct alignas(16) Raw8 {
             for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.0f);
         }
     }
-    __device__ float get(int i) const { return ld1(v + i); }
+    __device__ P2 pair(int j) const {  // elements 2 j and 2 j + 1
+        const float2 f = ld2(v + 2 * j);
+        return pack(f.x, f.y);
+    }
 };
 
 // A warp takes 256 columns (8 a lane), a CTA's 8 warps every 8th row of
@@ -42,15 +45,18 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 256 + lane * 8;
     const int n = a.N - col < 8 ? static_cast<int>(a.N - col) : 8;  // may be <= 0
     const int64_t r0 = blockIdx.y * chunk, r1 = r0 + chunk < a.M ? r0 + chunk : a.M;
-    float sum[NO][8];
+    P2 sum[NO][4];
 #pragma unroll
     for (int o = 0; o < NO; ++o)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[o][i] = 0.0f;
+        for (int j = 0; j < 4; ++j) sum[o][j].v = 0;
     if (n > 0) {
-        // two rows in flight under the one at hand
+        // AHEAD rows in flight under the one at hand: as many as leave two CTAs a SM, three
+        // LINEAR ones of binary16 (DUAL binary16 8192 x 5632: 88, 79, 76 us with 1, 2, 3;
+        // binary32 8192 x 4096: 128 us with 1, 171 with 2)
+        constexpr int AHEAD = sizeof(T) == 4 ? 1 : DUAL ? 3 : 2;
         constexpr bool PRE = DUAL || ACT != QSML_ACT_NONE;
-        Raw8<T> ry[3], rz[3], ru[3];
+        Raw8<T> ry[AHEAD + 1], rz[AHEAD + 1], ru[AHEAD + 1];
         auto load = [&](int64_t r, Raw8<T>& y, Raw8<T>& z, Raw8<T>& u) {
             if (r >= r1) return;
             y.load(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec);
@@ -58,49 +64,56 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
             if constexpr (DUAL) u.load(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec);
         };
         auto work = [&](int64_t r, const Raw8<T>& y, const Raw8<T>& z, const Raw8<T>& u) {
-            float d[NO][8];
+            // elements past the row's end were loaded as 0 and so end as 0
+            P2 d[NO][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int j = 0; j < 4; ++j) {
                 if constexpr (!PRE) {
-                    d[0][i] = y.get(i);
+                    d[0][j] = y.pair(j);
                 } else {
-                    float value;
-                    const float g = act_grad<T>(ACT, z.get(i), value);
+                    P2 value;
+                    const P2 g = act_grad2<T>(ACT, z.pair(j), value);
                     if constexpr (DUAL) {
-                        d[0][i] = __fmul_rn(__fmul_rn(y.get(i), u.get(i)), g);
-                        d[1][i] = __fmul_rn(y.get(i), value);
+                        d[0][j] = mul2(mul2(y.pair(j), u.pair(j)), g);
+                        d[1][j] = mul2(y.pair(j), value);
                     } else {
-                        d[0][i] = __fmul_rn(y.get(i), g);
+                        d[0][j] = mul2(y.pair(j), g);
                     }
                 }
             }
 #pragma unroll
             for (int o = 0; o < NO; ++o) {
                 if (a.dz[o]) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 e = unpack(d[o][j]);
+                        f[2 * j] = e.x;
+                        f[2 * j + 1] = e.y;
+                    }
                     if (a.plane) {
                         uint16_t* to = static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) d[o][i] = i < n ? d[o][i] : 0.0f;
-                        if constexpr (sizeof(T) == 4) split8(d[o], to, a.plane);
-                        else halve8(d[o], reinterpret_cast<__half*>(to), a.plane);
+                        if constexpr (sizeof(T) == 4) split8(f, to, a.plane);
+                        else halve8(f, reinterpret_cast<__half*>(to), a.plane);
                     } else {
-                        store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, d[o]);
+                        store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, f);
                     }
                 }
                 if (a.partial) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[o][i] = __fadd_rn(sum[o][i], i < n ? d[o][i] : 0.0f);
+                    for (int j = 0; j < 4; ++j) sum[o][j] = add2(sum[o][j], d[o][j]);
                 }
             }
         };
         int64_t r = r0 + w;
-        load(r, ry[0], rz[0], ru[0]);
-        load(r + 8, ry[1], rz[1], ru[1]);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) load(r + 8 * i, ry[i], rz[i], ru[i]);
         while (r < r1) {
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {
+            for (int i = 0; i <= AHEAD; ++i) {
                 if (r >= r1) break;
-                load(r + 16, ry[(i + 2) % 3], rz[(i + 2) % 3], ru[(i + 2) % 3]);
+                const int to = (i + AHEAD) % (AHEAD + 1);
+                load(r + 8 * AHEAD, ry[to], rz[to], ru[to]);
                 work(r, ry[i], rz[i], ru[i]);
                 r += 8;
             }
@@ -110,7 +123,11 @@ __global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradA
 #pragma unroll
     for (int o = 0; o < NO; ++o)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) fold[o][w][lane * 8 + i] = sum[o][i];
+        for (int j = 0; j < 4; ++j) {
+            const float2 e = unpack(sum[o][j]);
+            fold[o][w][lane * 8 + 2 * j] = e.x;
+            fold[o][w][lane * 8 + 2 * j + 1] = e.y;
+        }
     __syncthreads();
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= a.N) return;
