@@ -52,6 +52,11 @@ struct TcArgs {
     int a_mn[2], b_mn[2];    // MN-major operands, by segment
     int* status;
 };
+// The products of one launch: the grid's first CTAs are those of g[0].
+template <int NP> struct TcBatch {
+    TcArgs g[NP];
+    int first;
+};
 
 // A ring of slots in shared memory, each a tile of A and one of B (of one part, for
 // binary32: a k-block takes three).  Binary16 has two CTAs a SM with 96 KiB each, or
@@ -266,8 +271,11 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
     return v;
 }
 
-template <bool F32, bool DUAL>
-__global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const __grid_constant__ TcArgs g) {
+template <bool F32, bool DUAL, int NP>
+__global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const __grid_constant__ TcBatch<NP> all) {
+    const int second = NP > 1 && static_cast<int>(blockIdx.x) >= all.first ? 1 : 0;
+    const int cta = static_cast<int>(blockIdx.x) - (second ? all.first : 0);
+    const TcArgs& g = all.g[second];
     using T = std::conditional_t<F32, float, __half>;
     using S = Shape<F32>;
     extern __shared__ unsigned char smem_raw[];
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const int tile = static_cast<int>(blockIdx.x) / g.splits, rank = static_cast<int>(blockIdx.x) % g.splits;
+    const int tile = cta / g.splits, rank = cta % g.splits;
     const int mt = tile % g.tiles_m, nt = tile / g.tiles_m;
     constexpr int BN = DUAL ? 64 : 128;  // result columns a tile
     // this CTA's share of the k-blocks, and of it the part [lo, hi) in segment seg
@@ -1315,6 +1323,21 @@ template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Pro
     return after_launch(ctx, name);
 }
 
+// Asks for the kernel's shared memory, once a device.
+template <bool F32, bool DUAL, int NP> qsml_status_t opt_in(Context* ctx) {
+    static std::mutex mu;
+    static uint64_t done = 0;
+    std::lock_guard<std::mutex> lk(mu);
+    const uint64_t bit = uint64_t(1) << (ctx->device & 63);
+    if (done & bit) return QSML_OK;
+    using S = Shape<F32>;
+    QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(k_linear_tc<F32, DUAL, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         static_cast<int>(S::smem(S::DEEP_RING))),
+                               "linear: shared-memory attribute"));
+    done |= bit;
+    return QSML_OK;
+}
+
 // CTAs that share a tile's sum.
 // One row of tiles: every operand of weight is read once, HBM bounds the whole, and
 // as many as the device holds at once pull it fastest (a second turn costs: the gated
@@ -1325,16 +1348,23 @@ template <bool F32, bool DUAL> qsml_status_t launch_pair(Context* ctx, const Pro
 // tiles: 45 us unsplit, 49 in two; 256 x 11008 x 4096, 64 tiles: 41 us unsplit, 29 in
 // two, 37 in three; binary32 128 x 8192 x 1024, 8 tiles of one row: 139 us unsplit, 52 in
 // four, 39 in eight).
-template <bool F32, bool DUAL>
-qsml_status_t best_split(Context* ctx, int64_t tiles, bool one_row, int64_t blocks, int* splits) {
+// The cost of two products in one launch is reckoned as if both had the longer sum.
+struct Split {
+    int64_t tiles, blocks;
+    int64_t most;  // splits at most
+    bool one_row;
+    int splits = 1;
+    int64_t cost = INT64_MAX;
+};
+template <bool F32, bool DUAL> qsml_status_t best_split(Context* ctx, Split* w) {
     using S = Shape<F32>;
+    QSML_TRY_STATUS((opt_in<F32, DUAL, 1>(ctx)));  // the occupancy below counts on it
     static std::mutex mu;
     static int held[64][MAX_SPLIT + 1] = {};  // clusters of each size that the device holds
     std::lock_guard<std::mutex> lk(mu);
     int* n = held[ctx->device & 63];
     constexpr int64_t OVER = F32 ? 2 : 8;
-    int64_t best = INT64_MAX;
-    for (int s = 1; s <= MAX_SPLIT && s <= blocks; ++s) {
+    for (int s = 1; s <= MAX_SPLIT && s <= w->most; ++s) {
         if (n[s] == 0) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute attr[1];
@@ -1347,56 +1377,55 @@ qsml_status_t best_split(Context* ctx, int64_t tiles, bool one_row, int64_t bloc
             cfg.dynamicSmemBytes = S::smem(S::RING);
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n[s], k_linear_tc<F32, DUAL>, &cfg) != cudaSuccess || n[s] <= 0) {
+            if (cudaOccupancyMaxActiveClusters(&n[s], k_linear_tc<F32, DUAL, 1>, &cfg) != cudaSuccess || n[s] <= 0) {
                 cudaGetLastError();
                 n[s] = s == 1 ? ctx->num_sms : -1;
             }
         }
         if (n[s] < 0) continue;
-        const int64_t turns = (tiles + n[s] - 1) / n[s];
-        if (one_row) {
-            if (turns == 1 && blocks >= 2 * s) *splits = s;
+        const int64_t turns = (w->tiles + n[s] - 1) / n[s];
+        if (w->one_row) {
+            if (turns == 1 && w->blocks >= 2 * s) w->splits = s;
             continue;
         }
-        const int64_t on_a_sm = (tiles * s + ctx->num_sms - 1) / ctx->num_sms;
-        const int64_t cost = on_a_sm * ((blocks + s - 1) / s) + OVER * turns + (s > 1 ? OVER / 2 : 0);
-        if (cost < best) {
-            best = cost;
-            *splits = s;
+        const int64_t on_a_sm = (w->tiles * s + ctx->num_sms - 1) / ctx->num_sms;
+        const int64_t cost = on_a_sm * ((w->blocks + s - 1) / s) + OVER * turns + (s > 1 ? OVER / 2 : 0);
+        if (cost < w->cost) {
+            w->cost = cost;
+            w->splits = s;
         }
     }
     return QSML_OK;
 }
 
-template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem& p, TcArgs& g) {
+inline int64_t tiles_of(const TcArgs& g) { return static_cast<int64_t>(g.tiles_m) * g.tiles_n; }
+Split whole_split(const TcArgs& g) {
+    const int64_t blocks = static_cast<int64_t>(g.kb) * g.segments;
+    return Split{tiles_of(g), blocks, blocks, g.tiles_m == 1};
+}
+
+template <bool F32, bool DUAL, int NP> qsml_status_t launch(Context* ctx, TcBatch<NP>& all, int splits) {
     using S = Shape<F32>;
-    constexpr int BN = DUAL ? 64 : 128;
-    auto kernel = k_linear_tc<F32, DUAL>;
-    {
-        static std::mutex mu;
-        static uint64_t done = 0;
-        std::lock_guard<std::mutex> lk(mu);
-        const uint64_t bit = uint64_t(1) << (ctx->device & 63);
-        if (!(done & bit)) {
-            QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                                 static_cast<int>(S::smem(S::DEEP_RING))),
-                                       "linear: shared-memory attribute"));
-            done |= bit;
-        }
+    auto kernel = k_linear_tc<F32, DUAL, NP>;
+    QSML_TRY_STATUS((opt_in<F32, DUAL, NP>(ctx)));
+    int64_t ctas = 0;
+    bool whole = true;
+    for (const TcArgs& g : all.g) {
+        ctas += tiles_of(g) * splits;
+        whole = whole && g.a_bytes == TILE_BYTES;
     }
-    g.tiles_m = static_cast<int>((p.M + 127) / 128);
-    g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
-    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    if (tiles * MAX_SPLIT > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
-    int splits = 1;
-    QSML_TRY_STATUS((best_split<F32, DUAL>(ctx, tiles, g.tiles_m == 1, static_cast<int64_t>(g.kb) * g.segments, &splits)));
-    g.splits = splits;
+    if (ctas > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
+    all.first = static_cast<int>(tiles_of(all.g[0]) * splits);
     // few rows: slots are small, and with the small ring the next call's CTAs fit beside
     // this one's, so that their set-up overlaps its end (gated 5 x 4096 x 11008 35.9 ->
     // 31.5 us; asking for the weight's first blocks ahead of the wait, into L2, took 36)
-    g.ring = tiles * splits <= ctx->num_sms && g.a_bytes == TILE_BYTES ? S::DEEP_RING : S::RING;
-    g.slots = g.ring / (g.a_bytes + TILE_BYTES);
-    if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
+    const int ring = ctas <= ctx->num_sms && whole ? S::DEEP_RING : S::RING;
+    for (TcArgs& g : all.g) {
+        g.splits = splits;
+        g.ring = ring;
+        g.slots = ring / (g.a_bytes + TILE_BYTES);
+        if (g.slots > S::MAX_SLOTS) g.slots = S::MAX_SLOTS;
+    }
 
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -1406,21 +1435,49 @@ template <bool F32, bool DUAL> qsml_status_t launch(Context* ctx, const Problem&
     attr[1].val.clusterDim.x = splits;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::smem(g.ring);
+    cfg.dynamicSmemBytes = S::smem(ring);
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
     cfg.numAttrs = splits > 1 ? 2 : 1;
     const char* name = F32 ? "k_linear_tc<f32>" : "k_linear_tc<f16>";
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, all);
     if (e != cudaSuccess) return check_cuda(ctx, e, name);
     return after_launch(ctx, name);
 }
 
-}  // namespace
+template <bool F32, bool DUAL> qsml_status_t launch_one(Context* ctx, const TcArgs& g) {
+    Split w = whole_split(g);
+    QSML_TRY_STATUS((best_split<F32, DUAL>(ctx, &w)));
+    TcBatch<1> all;
+    all.g[0] = g;
+    return launch<F32, DUAL, 1>(ctx, all, w.splits);
+}
 
-namespace {
+// Two products in one launch where that is reckoned to take less than one after
+// another: each alone splits its sums to fill the GPU, and has a beginning and an end
+// of its own, about 5 us or ALONE blocks' time (backward 512 x 1024 x 1024, binary16:
+// 20 us in two launches, 14 in one; binary32 777 x 1024 x 1000: 45 and 35; but binary16
+// 8192 x 256 x 512, with sums of 8 and of 128 blocks: 27 and 32).
+template <bool F32> qsml_status_t launch_two(Context* ctx, const TcArgs& g0, const TcArgs& g1) {
+    constexpr int64_t ALONE = F32 ? 6 : 40;
+    Split a = whole_split(g0), b = whole_split(g1);
+    if (!a.one_row && !b.one_row) {
+        Split both{a.tiles + b.tiles, std::max(a.blocks, b.blocks), std::min(a.blocks, b.blocks), false};
+        QSML_TRY_STATUS((best_split<F32, false>(ctx, &a)));
+        QSML_TRY_STATUS((best_split<F32, false>(ctx, &b)));
+        QSML_TRY_STATUS((best_split<F32, false>(ctx, &both)));
+        if (both.cost < a.cost + b.cost + ALONE) {
+            TcBatch<2> all;
+            all.g[0] = g0;
+            all.g[1] = g1;
+            return launch<F32, false, 2>(ctx, all, both.splits);
+        }
+    }
+    QSML_TRY_STATUS((launch_one<F32, false>(ctx, g0)));
+    return launch_one<F32, false>(ctx, g1);
+}
 
 // A problem whose operands are known to TMA.
 struct Ready {
@@ -1445,12 +1502,15 @@ qsml_status_t prepare(Context* ctx, Workspace& ws, StageJobs* jobs, const Proble
     return QSML_OK;
 }
 
-qsml_status_t run_ready(Context* ctx, const Problem& p, bool f32, const Ready& r) {
-    TcArgs g;
+// A problem's arguments; the splits and the ring are the launch's.
+qsml_status_t arguments(Context* ctx, const Problem& p, bool f32, const Ready& r, TcArgs* out) {
+    TcArgs& g = *out;
     g.e = p.e;
     g.M = static_cast<int>(p.M);
     g.N = static_cast<int>(p.N);
     g.kb = static_cast<int>((p.K + 63) / 64);
+    g.tiles_m = static_cast<int>((p.M + 127) / 128);
+    g.tiles_n = static_cast<int>((p.N + (p.dual ? 63 : 127)) / (p.dual ? 64 : 128));
     const int na = p.segments, nb = p.dual ? 2 : p.segments;
     g.a_halves = !f32 && r.a[0].plane ? 1 : 0;
     g.b_halves = !f32 && r.b[0].plane ? 1 : 0;
@@ -1473,13 +1533,16 @@ qsml_status_t run_ready(Context* ctx, const Problem& p, bool f32, const Ready& r
         if (i < nb) ok = ok && operand_map(&g.b[i], b, f32, g.b_mn[i], b_rows);
         else g.b[i] = g.b[0];
     }
-    if (!ok) return set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
+    return ok ? QSML_OK : set_error(ctx, QSML_E_CUDA, "linear: tensor map creation failed");
+}
+
+qsml_status_t run_one(Context* ctx, const Problem& p, bool f32, const Ready& r, TcArgs& g) {
     if (r.pair) {
         if (f32) return p.dual ? launch_pair<true, true>(ctx, p, g, r.pairs) : launch_pair<true, false>(ctx, p, g, r.pairs);
         return p.dual ? launch_pair<false, true>(ctx, p, g, r.pairs) : launch_pair<false, false>(ctx, p, g, r.pairs);
     }
-    if (f32) return p.dual ? launch<true, true>(ctx, p, g) : launch<true, false>(ctx, p, g);
-    return p.dual ? launch<false, true>(ctx, p, g) : launch<false, false>(ctx, p, g);
+    if (f32) return p.dual ? launch_one<true, true>(ctx, g) : launch_one<true, false>(ctx, g);
+    return p.dual ? launch_one<false, true>(ctx, g) : launch_one<false, false>(ctx, g);
 }
 
 }  // namespace
@@ -1488,9 +1551,16 @@ qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32) {
     Workspace ws(ctx);
     StageJobs jobs;
     Ready r[2];
-    for (int i = 0; i < n; ++i) QSML_TRY_STATUS(prepare(ctx, ws, &jobs, *p[i], f32, &r[i]));
+    TcArgs g[2];
+    bool together = n == 2;
+    for (int i = 0; i < n; ++i) {
+        QSML_TRY_STATUS(prepare(ctx, ws, &jobs, *p[i], f32, &r[i]));
+        QSML_TRY_STATUS(arguments(ctx, *p[i], f32, r[i], &g[i]));
+        together = together && !r[i].pair && !p[i]->dual;
+    }
     QSML_TRY_STATUS(run_jobs(ctx, jobs, f32));
-    for (int i = 0; i < n; ++i) QSML_TRY_STATUS(run_ready(ctx, *p[i], f32, r[i]));
+    if (together) return f32 ? launch_two<true>(ctx, g[0], g[1]) : launch_two<false>(ctx, g[0], g[1]);
+    for (int i = 0; i < n; ++i) QSML_TRY_STATUS(run_one(ctx, *p[i], f32, r[i], g[i]));
     return QSML_OK;
 }
 

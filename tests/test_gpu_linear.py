@@ -242,6 +242,25 @@ def test_pairs_of_sms(ctx, size, dt, gated):
     check_backward(c, "silu", kept, *backward(ctx, c, "silu", kept))
 
 
+# x's and w's gradients by one launch: tiles and sums of both ragged, shared out over clusters
+# or not, dz in two parts or one, operands that are copied and ones read in place; the last
+# size takes two launches
+@pytest.mark.parametrize("size", [(129, 130, 1), (200, 300, 64), (131, 257, 450), (777, 136, 256), (520, 512, 1030),
+                                  (1100, 260, 130), (8192, 256, 512)])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_both_gradients(ctx, size, dt):
+    c = Case(*size, dt)
+    kept = c.kept()
+    dx, dw, db = backward(ctx, c, "gelu", kept)
+    check_backward(c, "gelu", kept, dx, dw, db)
+    before = [ctx.launch_count()]
+    for want in ("xwb", "xb", "w"):  # dz, its column sums, products; no sums for the last
+        backward(ctx, c, "gelu", kept, want)
+        before.append(ctx.launch_count())
+    if dt == np.float16 and size[1] % 8 == 0 and size[2] % 8 == 0:  # nothing is copied
+        assert list(np.diff(before)) == [4 if size[0] == 8192 else 3, 3, 2]
+
+
 def strided(a, how):
     """A device view with the values of `a`: transposed storage, an odd row pitch, columns of a
     wider matrix, every other column, a start off the 16-byte boundary."""
