@@ -52,10 +52,10 @@ struct TcArgs {
     int a_mn[2], b_mn[2];    // MN-major operands, by segment
     int* status;
 };
-// The products of one launch: the grid's first CTAs are those of g[0].
+// The products of one launch: g[i]'s CTAs begin at CTA first[i].
 template <int NP> struct TcBatch {
     TcArgs g[NP];
-    int first;
+    int first[NP];
 };
 
 // A ring of slots in shared memory, each a tile of A and one of B (of one part, for
@@ -273,9 +273,11 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
 
 template <bool F32, bool DUAL, int NP>
 __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const __grid_constant__ TcBatch<NP> all) {
-    const int second = NP > 1 && static_cast<int>(blockIdx.x) >= all.first ? 1 : 0;
-    const int cta = static_cast<int>(blockIdx.x) - (second ? all.first : 0);
-    const TcArgs& g = all.g[second];
+    int which = 0;
+    for (int i = 1; i < NP; ++i)
+        if (static_cast<int>(blockIdx.x) >= all.first[i]) which = i;
+    const int cta = static_cast<int>(blockIdx.x) - (NP > 1 ? all.first[which] : 0);
+    const TcArgs& g = all.g[which];
     using T = std::conditional_t<F32, float, __half>;
     using S = Shape<F32>;
     extern __shared__ unsigned char smem_raw[];
@@ -1348,7 +1350,7 @@ template <bool F32, bool DUAL, int NP> qsml_status_t opt_in(Context* ctx) {
 // tiles: 45 us unsplit, 49 in two; 256 x 11008 x 4096, 64 tiles: 41 us unsplit, 29 in
 // two, 37 in three; binary32 128 x 8192 x 1024, 8 tiles of one row: 139 us unsplit, 52 in
 // four, 39 in eight).
-// The cost of two products in one launch is reckoned as if both had the longer sum.
+// The cost of products in one launch is reckoned as if all had the longest sum.
 struct Split {
     int64_t tiles, blocks;
     int64_t most;  // splits at most
@@ -1410,12 +1412,12 @@ template <bool F32, bool DUAL, int NP> qsml_status_t launch(Context* ctx, TcBatc
     QSML_TRY_STATUS((opt_in<F32, DUAL, NP>(ctx)));
     int64_t ctas = 0;
     bool whole = true;
-    for (const TcArgs& g : all.g) {
-        ctas += tiles_of(g) * splits;
-        whole = whole && g.a_bytes == TILE_BYTES;
+    for (int i = 0; i < NP; ++i) {
+        all.first[i] = static_cast<int>(ctas);
+        ctas += tiles_of(all.g[i]) * splits;
+        whole = whole && all.g[i].a_bytes == TILE_BYTES;
+        if (ctas > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
     }
-    if (ctas > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
-    all.first = static_cast<int>(tiles_of(all.g[0]) * splits);
     // few rows: slots are small, and with the small ring the next call's CTAs fit beside
     // this one's, so that their set-up overlaps its end (gated 5 x 4096 x 11008 35.9 ->
     // 31.5 us; asking for the weight's first blocks ahead of the wait, into L2, took 36)
@@ -1455,28 +1457,29 @@ template <bool F32, bool DUAL> qsml_status_t launch_one(Context* ctx, const TcAr
     return launch<F32, DUAL, 1>(ctx, all, w.splits);
 }
 
-// Two products in one launch where that is reckoned to take less than one after
-// another: each alone splits its sums to fill the GPU, and has a beginning and an end
-// of its own, about 5 us or ALONE blocks' time (backward 512 x 1024 x 1024, binary16:
-// 20 us in two launches, 14 in one; binary32 777 x 1024 x 1000: 45 and 35; but binary16
-// 8192 x 256 x 512, with sums of 8 and of 128 blocks: 27 and 32).
-template <bool F32> qsml_status_t launch_two(Context* ctx, const TcArgs& g0, const TcArgs& g1) {
-    constexpr int64_t ALONE = F32 ? 6 : 40;
-    Split a = whole_split(g0), b = whole_split(g1);
-    if (!a.one_row && !b.one_row) {
-        Split both{a.tiles + b.tiles, std::max(a.blocks, b.blocks), std::min(a.blocks, b.blocks), false};
-        QSML_TRY_STATUS((best_split<F32, false>(ctx, &a)));
-        QSML_TRY_STATUS((best_split<F32, false>(ctx, &b)));
-        QSML_TRY_STATUS((best_split<F32, false>(ctx, &both)));
-        if (both.cost < a.cost + b.cost + ALONE) {
-            TcBatch<2> all;
-            all.g[0] = g0;
-            all.g[1] = g1;
-            return launch<F32, false, 2>(ctx, all, both.splits);
-        }
+// Products in one launch where that is reckoned to take less than one after another:
+// each alone splits its sums to fill the GPU, and has a beginning and an end of its own,
+// which cost about ALONE blocks' time (backward 512 x 1024 x 1024, binary16: 20 us in
+// two launches, 14 in one; with two weights 2048 x 512 x 512: 27 and 16; binary32 777 x
+// 1024 x 1000: 45 and 35; but binary16 8192 x 256 x 512, with sums of 8 and of 128
+// blocks: 27 and 32; with two weights 1024 x 1024 x 1024, more CTAs than SMs: 27 and 31).
+// `apart`: the cost of the launches it replaces, but for ALONE.
+template <bool F32, int NP>
+qsml_status_t launch_together(Context* ctx, const TcArgs* const (&g)[NP], int64_t apart, bool* launched) {
+    constexpr int64_t ALONE = F32 ? 6 : 24;
+    Split all{0, 0, INT64_MAX, false};
+    for (const TcArgs* one : g) {
+        const Split w = whole_split(*one);
+        all.tiles += w.tiles;
+        all.blocks = std::max(all.blocks, w.blocks);
+        all.most = std::min(all.most, w.blocks);
     }
-    QSML_TRY_STATUS((launch_one<F32, false>(ctx, g0)));
-    return launch_one<F32, false>(ctx, g1);
+    QSML_TRY_STATUS((best_split<F32, false>(ctx, &all)));
+    *launched = all.cost < apart + ALONE;
+    if (!*launched) return QSML_OK;
+    TcBatch<NP> batch;
+    for (int i = 0; i < NP; ++i) batch.g[i] = *g[i];
+    return launch<F32, false, NP>(ctx, batch, all.splits);
 }
 
 // A problem whose operands are known to TMA.
@@ -1545,6 +1548,31 @@ qsml_status_t run_one(Context* ctx, const Problem& p, bool f32, const Ready& r, 
     return p.dual ? launch_one<false, true>(ctx, g) : launch_one<false, false>(ctx, g);
 }
 
+// The two products of a backward pass, neither by pairs of SMs nor of one row of tiles.
+template <bool F32>
+qsml_status_t run_together(Context* ctx, const Problem* const* p, const Ready* r, const TcArgs* g, bool* launched) {
+    Split a = whole_split(g[0]), b = whole_split(g[1]);
+    QSML_TRY_STATUS((best_split<F32, false>(ctx, &a)));
+    if (!p[1]->dual) {
+        QSML_TRY_STATUS((best_split<F32, false>(ctx, &b)));
+        return launch_together<F32, 2>(ctx, {&g[0], &g[1]}, a.cost + b.cost, launched);
+    }
+    // the gradients of two weights, as two products
+    QSML_TRY_STATUS((best_split<F32, true>(ctx, &b)));
+    TcArgs w[2];
+    for (int i = 0; i < 2; ++i) {
+        Problem q = *p[1];
+        Ready rq = r[1];
+        q.dual = false;
+        q.b[0] = p[1]->b[i];
+        rq.b[0] = r[1].b[i];
+        q.e.y = p[1]->e.pre[i];
+        q.e.pre[0] = q.e.pre[1] = nullptr;
+        QSML_TRY_STATUS(arguments(ctx, q, F32, rq, &w[i]));
+    }
+    return launch_together<F32, 3>(ctx, {&g[0], &w[0], &w[1]}, a.cost + b.cost, launched);
+}
+
 }  // namespace
 
 qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32) {
@@ -1556,10 +1584,14 @@ qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32) {
     for (int i = 0; i < n; ++i) {
         QSML_TRY_STATUS(prepare(ctx, ws, &jobs, *p[i], f32, &r[i]));
         QSML_TRY_STATUS(arguments(ctx, *p[i], f32, r[i], &g[i]));
-        together = together && !r[i].pair && !p[i]->dual;
+        together = together && !r[i].pair && g[i].tiles_m > 1;
     }
     QSML_TRY_STATUS(run_jobs(ctx, jobs, f32));
-    if (together) return f32 ? launch_two<true>(ctx, g[0], g[1]) : launch_two<false>(ctx, g[0], g[1]);
+    if (together) {
+        bool launched = false;
+        QSML_TRY_STATUS(f32 ? run_together<true>(ctx, p, r, g, &launched) : run_together<false>(ctx, p, r, g, &launched));
+        if (launched) return QSML_OK;
+    }
     for (int i = 0; i < n; ++i) QSML_TRY_STATUS(run_one(ctx, *p[i], f32, r[i], g[i]));
     return QSML_OK;
 }

@@ -242,14 +242,15 @@ def test_pairs_of_sms(ctx, size, dt, gated):
     check_backward(c, "silu", kept, *backward(ctx, c, "silu", kept))
 
 
-# x's and w's gradients by one launch: tiles and sums of both ragged, shared out over clusters
-# or not, dz in two parts or one, operands that are copied and ones read in place; the last
-# size takes two launches
+# x's and the weights' gradients by one launch: tiles and sums of all ragged, shared out over
+# clusters or not, dz in two parts or one, operands that are copied and ones read in place; the
+# last size takes two launches
 @pytest.mark.parametrize("size", [(129, 130, 1), (200, 300, 64), (131, 257, 450), (777, 136, 256), (520, 512, 1030),
                                   (1100, 260, 130), (8192, 256, 512)])
 @pytest.mark.parametrize("dt", DTYPES)
-def test_both_gradients(ctx, size, dt):
-    c = Case(*size, dt)
+@pytest.mark.parametrize("gated", [False, True])
+def test_both_gradients(ctx, size, dt, gated):
+    c = Case(*size, dt, gated=gated)
     kept = c.kept()
     dx, dw, db = backward(ctx, c, "gelu", kept)
     check_backward(c, "gelu", kept, dx, dw, db)
@@ -258,7 +259,7 @@ def test_both_gradients(ctx, size, dt):
         backward(ctx, c, "gelu", kept, want)
         before.append(ctx.launch_count())
     if dt == np.float16 and size[1] % 8 == 0 and size[2] % 8 == 0:  # nothing is copied
-        assert list(np.diff(before)) == [4 if size[0] == 8192 else 3, 3, 2]
+        assert list(np.diff(before)) == [4 if size[0] == 8192 else 3, 3, 2], before
 
 
 def strided(a, how):
