@@ -20,7 +20,7 @@
 // element, before it was by HBM.
 // k_layer_norm_bwd_groups: rows narrower than a CTA's, 4 to 32 lanes a row.
 // k_layer_norm_bwd_rows + k_layer_norm_bwd_cols: rows wider than the registers
-// hold, in two kernels (5 elements of traffic and the row statistics).
+// hold (8192 columns, 6144 off 16 bytes), in two kernels (5 elements of traffic and the row statistics).
 #include "packed.cuh"
 #include "row_pipe.cuh"
 #include "workspace.cuh"
@@ -706,7 +706,10 @@ template <typename T, typename GT, int PV, int NV, bool RING> qsml_status_t run_
 // Loads of PV elements.  Rows of up to 512 columns: 4 to 32 lanes with 16 elements
 // each.  Up to 8192: a CTA, whose threads hold 32 elements of binary16 rows (fewer
 // warps meet at the row's two barriers and more rows are on a SM: 16384 x 4096 took
-// 93 us so, 98 with 16 elements, 124 with 8), 16 of binary32 ones, 8 or 16 single ones.
+// 93 us so, 98 with 16 elements, 124 with 8), 16 of binary32 ones.  Single elements:
+// 8 a thread, 12 up to 6144 columns (with 16 the compiler runs out of the registers of
+// 512 threads: 6007 x 6001 binary32 took 387 us, with 12 90), then the two kernels
+// (6007 x 8191 binary32: 283 us; with 16 a thread 415).
 template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, const Args& a) {
     const int64_t packs = a.cols / PV;
     if (a.cols <= 512) {
@@ -716,9 +719,11 @@ template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, cons
         if (packs <= 16 * NV) return launch_groups<T, GT, PV, NV, 16>(ctx, a);
         return launch_groups<T, GT, PV, NV, 32>(ctx, a);
     }
-    if (a.cols > 8192) return launch_wide_bwd<T, GT, PV>(ctx, a);
-    if constexpr (PV == 1) return a.cols <= 4096 ? run_cta<T, GT, 1, 8, false>(ctx, a) : run_cta<T, GT, 1, 16, false>(ctx, a);
-    else return run_cta<T, GT, PV, (sizeof(T) == 2 ? 32 : 16) / PV, true>(ctx, a);
+    if (a.cols > (PV == 1 ? 6144 : 8192)) return launch_wide_bwd<T, GT, PV>(ctx, a);
+    if constexpr (PV == 1)
+        return a.cols <= 4096 ? run_cta<T, GT, 1, 8, false>(ctx, a) : run_cta<T, GT, 1, 12, false>(ctx, a);
+    else
+        return run_cta<T, GT, PV, (sizeof(T) == 2 ? 32 : 16) / PV, true>(ctx, a);
 }
 
 template <typename T, typename GT>

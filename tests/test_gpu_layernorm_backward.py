@@ -87,6 +87,14 @@ def test_shapes(ctx, shape, dtype):
     check(x, g, dy, 1e-5, *run(ctx, x, g, dy))
 
 
+@pytest.mark.parametrize("cols", [4095, 4097, 6143, 6145, 8191])
+@pytest.mark.parametrize("rows", [2, 310])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_wide_rows_of_single_elements(ctx, rows, cols, dtype):
+    x, g, dy = make((rows, cols), dtype)
+    check(x, g, dy, 1e-5, *run(ctx, x, g, dy))
+
+
 def test_workload_16384x4096_f16(ctx):
     x, g, dy = make((16384, 4096), np.float16)
     check(x, g, dy, 1e-5, *run(ctx, x, g, dy))
