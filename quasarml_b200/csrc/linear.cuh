@@ -70,63 +70,14 @@ __device__ __forceinline__ float ld1(const __half* p) { return __half2float(*p);
 constexpr float kGeluS = 0.7978845608f, kGeluC = 0.044715f;  // the constants of QSML_UN_GELU
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Activations are computed two values at a time (packed.cuh): one by one they took 29
+// instructions an element in the gradient's pass, which bound it.
+
 // 1 / (1 + exp(-z)); 0 where exp(-z) overflows.  Binary32 results take expf and a
 // correctly rounded reciprocal.  Binary16 ones take 2^t and 1/d of the hardware
 // (2 ulp and 1 ulp; t = -z log2(e) is off by 2^-24 |t|): far below half a step of
 // binary16, and a third of the instructions, which bounded the epilogue and the
 // gradient's pass.
-template <typename T> __device__ __forceinline__ float act_sigmoid(float z) {
-    if constexpr (sizeof(T) == 2) {
-        float e, p;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(-kLog2e, z)));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(__fadd_rn(1.0f, e)));
-        return p;
-    } else {
-        return __frcp_rn(__fadd_rn(1.0f, expf(-z)));
-    }
-}
-
-// act(z).  gelu: 0.5 z (1 + tanh v) = z sigmoid(2 v), v = s (z + c z^3).
-template <typename T> __device__ __forceinline__ float act_value(int act, float z) {
-    switch (act) {
-        case QSML_ACT_RELU: return z != z ? z : (z > 0.0f ? z : 0.0f);
-        case QSML_ACT_GELU: {
-            const float q = __fmul_rn(z, z);
-            const float v2 = __fmul_rn(__fmul_rn(2.0f * kGeluS, z), __fmaf_rn(kGeluC, q, 1.0f));
-            return __fmul_rn(z, act_sigmoid<T>(v2));
-        }
-        case QSML_ACT_SILU: return __fmul_rn(z, act_sigmoid<T>(z));
-        case QSML_ACT_SIGMOID: return act_sigmoid<T>(z);
-    }
-    return z;
-}
-
-// act of N values, one branch for all of them
-template <typename T, int N> __device__ __forceinline__ void act_all(int act, float (&z)[N]) {
-    switch (act) {
-        case QSML_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_RELU, z[i]);
-            break;
-        case QSML_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_GELU, z[i]);
-            break;
-        case QSML_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_SILU, z[i]);
-            break;
-        case QSML_ACT_SIGMOID:
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = act_value<T>(QSML_ACT_SIGMOID, z[i]);
-            break;
-    }
-}
-
-// act(z) and its derivative, two at a time: the scalar form, 29 instructions an element
-// with gelu, bound the gradient's pass.  With p the sigmoid:
-//   silu' = p + z p (1 - p);  sigmoid' = p (1 - p);
-//   gelu' = p + z p (1 - p) 2 v',  2 v' = 2 s (1 + 3 c z^2).
 template <typename T> __device__ __forceinline__ P2 act_sigmoid2(P2 z) {
     if constexpr (sizeof(T) == 2) {
         const float2 t = unpack(mul2(both(-kLog2e), z));
@@ -139,15 +90,54 @@ template <typename T> __device__ __forceinline__ P2 act_sigmoid2(P2 z) {
         return pack(p.x, p.y);
     } else {
         const float2 f = unpack(z);
-        return pack(act_sigmoid<T>(f.x), act_sigmoid<T>(f.y));
+        return pack(__frcp_rn(__fadd_rn(1.0f, expf(-f.x))), __frcp_rn(__fadd_rn(1.0f, expf(-f.y))));
     }
 }
+// act of two values.  gelu: 0.5 z (1 + tanh v) = z sigmoid(2 v), v = s (z + c z^3).
+template <typename T> __device__ __forceinline__ P2 act_value2(int act, P2 z) {
+    switch (act) {
+        case QSML_ACT_RELU: {
+            const float2 f = unpack(z);
+            return pack(f.x != f.x ? f.x : (f.x > 0.0f ? f.x : 0.0f), f.y != f.y ? f.y : (f.y > 0.0f ? f.y : 0.0f));
+        }
+        case QSML_ACT_GELU: {
+            const P2 q = mul2(z, z), s2 = both(2.0f * kGeluS);
+            return mul2(z, act_sigmoid2<T>(mul2(mul2(s2, z), fma2(both(kGeluC), q, both(1.0f)))));
+        }
+        case QSML_ACT_SILU: return mul2(z, act_sigmoid2<T>(z));
+        case QSML_ACT_SIGMOID: return act_sigmoid2<T>(z);
+    }
+    return z;
+}
+
+// act of N values, one branch for all of them
+template <typename T, int N> __device__ __forceinline__ void act_all(int act, float (&z)[N]) {
+    static_assert(N % 2 == 0, "pairs");
+    auto all = [&](auto kind) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 f = unpack(act_value2<T>(kind.value, pack(z[i], z[i + 1])));
+            z[i] = f.x;
+            z[i + 1] = f.y;
+        }
+    };
+    switch (act) {
+        case QSML_ACT_RELU: all(std::integral_constant<int, QSML_ACT_RELU>{}); break;
+        case QSML_ACT_GELU: all(std::integral_constant<int, QSML_ACT_GELU>{}); break;
+        case QSML_ACT_SILU: all(std::integral_constant<int, QSML_ACT_SILU>{}); break;
+        case QSML_ACT_SIGMOID: all(std::integral_constant<int, QSML_ACT_SIGMOID>{}); break;
+    }
+}
+
+// act(z) and its derivative.  With p the sigmoid:
+//   silu' = p + z p (1 - p);  sigmoid' = p (1 - p);
+//   gelu' = p + z p (1 - p) 2 v',  2 v' = 2 s (1 + 3 c z^2).
 template <typename T> __device__ __forceinline__ P2 act_grad2(int act, P2 z, P2& value) {
     const P2 one = both(1.0f);
     switch (act) {
         case QSML_ACT_RELU: {
             const float2 f = unpack(z);
-            value = pack(act_value<T>(QSML_ACT_RELU, f.x), act_value<T>(QSML_ACT_RELU, f.y));
+            value = act_value2<T>(QSML_ACT_RELU, z);
             return pack(f.x != f.x ? f.x : (f.x > 0.0f ? 1.0f : 0.0f), f.y != f.y ? f.y : (f.y > 0.0f ? 1.0f : 0.0f));
         }
         case QSML_ACT_GELU: {
