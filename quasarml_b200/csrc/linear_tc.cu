@@ -1340,6 +1340,13 @@ template <bool F32, bool DUAL, int NP> qsml_status_t opt_in(Context* ctx) {
     return QSML_OK;
 }
 
+// few rows: slots are small, and with the small ring the next call's CTAs fit beside
+// this one's, so that their set-up overlaps its end (gated 5 x 4096 x 11008 35.9 ->
+// 31.5 us; asking for the weight's first blocks ahead of the wait, into L2, took 36)
+template <bool F32> int ring_bytes(Context* ctx, int64_t ctas, bool whole) {
+    return ctas <= ctx->num_sms && whole ? Shape<F32>::DEEP_RING : Shape<F32>::RING;
+}
+
 // CTAs that share a tile's sum.
 // One row of tiles: every operand of weight is read once, HBM bounds the whole, and
 // as many as the device holds at once pull it fastest (a second turn costs: the gated
@@ -1355,6 +1362,7 @@ struct Split {
     int64_t tiles, blocks;
     int64_t most;  // splits at most
     bool one_row;
+    bool whole;    // operand tiles of A of 128 rows
     int splits = 1;
     int64_t cost = INT64_MAX;
 };
@@ -1362,12 +1370,14 @@ template <bool F32, bool DUAL> qsml_status_t best_split(Context* ctx, Split* w) 
     using S = Shape<F32>;
     QSML_TRY_STATUS((opt_in<F32, DUAL, 1>(ctx)));  // the occupancy below counts on it
     static std::mutex mu;
-    static int held[64][MAX_SPLIT + 1] = {};  // clusters of each size that the device holds
+    // clusters of each size that the device holds, with the small ring and the deep one
+    static int held[64][2][MAX_SPLIT + 1] = {};
     std::lock_guard<std::mutex> lk(mu);
-    int* n = held[ctx->device & 63];
     constexpr int64_t OVER = F32 ? 2 : 8;
     for (int s = 1; s <= MAX_SPLIT && s <= w->most; ++s) {
-        if (n[s] == 0) {
+        const int ring = ring_bytes<F32>(ctx, w->tiles * s, w->whole);
+        int& n = held[ctx->device & 63][ring == S::RING ? 0 : 1][s];
+        if (n == 0) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1376,21 +1386,23 @@ template <bool F32, bool DUAL> qsml_status_t best_split(Context* ctx, Split* w) 
             attr[0].val.clusterDim.z = 1;
             cfg.gridDim = dim3(static_cast<unsigned>(s * ctx->num_sms));
             cfg.blockDim = dim3(THREADS);
-            cfg.dynamicSmemBytes = S::smem(S::RING);
+            cfg.dynamicSmemBytes = S::smem(ring);
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n[s], k_linear_tc<F32, DUAL, 1>, &cfg) != cudaSuccess || n[s] <= 0) {
+            if (cudaOccupancyMaxActiveClusters(&n, k_linear_tc<F32, DUAL, 1>, &cfg) != cudaSuccess || n <= 0) {
                 cudaGetLastError();
-                n[s] = s == 1 ? ctx->num_sms : -1;
+                n = s == 1 ? ctx->num_sms : -1;
             }
         }
-        if (n[s] < 0) continue;
-        const int64_t turns = (w->tiles + n[s] - 1) / n[s];
+        if (n < 0) continue;
+        const int64_t turns = (w->tiles + n - 1) / n;
         if (w->one_row) {
             if (turns == 1 && w->blocks >= 2 * s) w->splits = s;
             continue;
         }
-        const int64_t on_a_sm = (w->tiles * s + ctx->num_sms - 1) / ctx->num_sms;
+        // clusters do not fill every SM: 36 of four take two turns (256 x 8192 x 2304, 27 us;
+        // 36 of three 17)
+        const int64_t on_a_sm = std::max((w->tiles * s + ctx->num_sms - 1) / ctx->num_sms, turns);
         const int64_t cost = on_a_sm * ((w->blocks + s - 1) / s) + OVER * turns + (s > 1 ? OVER / 2 : 0);
         if (cost < w->cost) {
             w->cost = cost;
@@ -1403,7 +1415,7 @@ template <bool F32, bool DUAL> qsml_status_t best_split(Context* ctx, Split* w) 
 inline int64_t tiles_of(const TcArgs& g) { return static_cast<int64_t>(g.tiles_m) * g.tiles_n; }
 Split whole_split(const TcArgs& g) {
     const int64_t blocks = static_cast<int64_t>(g.kb) * g.segments;
-    return Split{tiles_of(g), blocks, blocks, g.tiles_m == 1};
+    return Split{tiles_of(g), blocks, blocks, g.tiles_m == 1, g.a_bytes == TILE_BYTES};
 }
 
 template <bool F32, bool DUAL, int NP> qsml_status_t launch(Context* ctx, TcBatch<NP>& all, int splits) {
@@ -1418,10 +1430,7 @@ template <bool F32, bool DUAL, int NP> qsml_status_t launch(Context* ctx, TcBatc
         whole = whole && all.g[i].a_bytes == TILE_BYTES;
         if (ctas > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "linear: too many output tiles");
     }
-    // few rows: slots are small, and with the small ring the next call's CTAs fit beside
-    // this one's, so that their set-up overlaps its end (gated 5 x 4096 x 11008 35.9 ->
-    // 31.5 us; asking for the weight's first blocks ahead of the wait, into L2, took 36)
-    const int ring = ctas <= ctx->num_sms && whole ? S::DEEP_RING : S::RING;
+    const int ring = ring_bytes<F32>(ctx, ctas, whole);
     for (TcArgs& g : all.g) {
         g.splits = splits;
         g.ring = ring;
@@ -1467,12 +1476,13 @@ template <bool F32, bool DUAL> qsml_status_t launch_one(Context* ctx, const TcAr
 template <bool F32, int NP>
 qsml_status_t launch_together(Context* ctx, const TcArgs* const (&g)[NP], int64_t apart, bool* launched) {
     constexpr int64_t ALONE = F32 ? 6 : 24;
-    Split all{0, 0, INT64_MAX, false};
+    Split all{0, 0, INT64_MAX, false, true};
     for (const TcArgs* one : g) {
         const Split w = whole_split(*one);
         all.tiles += w.tiles;
         all.blocks = std::max(all.blocks, w.blocks);
         all.most = std::min(all.most, w.blocks);
+        all.whole = all.whole && w.whole;
     }
     QSML_TRY_STATUS((best_split<F32, false>(ctx, &all)));
     *launched = all.cost < apart + ALONE;
