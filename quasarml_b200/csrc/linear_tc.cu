@@ -1502,12 +1502,15 @@ struct Ready {
 qsml_status_t prepare(Context* ctx, Workspace& ws, StageJobs* jobs, const Problem& p, bool f32, Ready* r) {
     // pairs of SMs where the tiles fill at least 60 % of them, else 128 x 128 tiles and
     // split sums (at 64 of 74 pairs, 1024 x 4096 x 4096 takes 27 us against 31; at 32,
-    // 512 x 11008 x 4096 57 against 45)
+    // 512 x 11008 x 4096 57 against 45), unless there are more of those than SMs (160
+    // against 40 pairs' tiles, 512 x 4096 x 5000: 44 us against 28; gated 256 x 2048 x
+    // 5632: 31 against 18)
     if (f32) QSML_TRY_STATUS((p.dual ? max_pairs<true, true>(ctx, &r->pairs) : max_pairs<true, false>(ctx, &r->pairs)));
     else QSML_TRY_STATUS((p.dual ? max_pairs<false, true>(ctx, &r->pairs) : max_pairs<false, false>(ctx, &r->pairs)));
     const int64_t bn = (f32 ? 128 : 256) / (p.dual ? 2 : 1);
     const int64_t tiles = ((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
-    r->pair = r->pairs > 0 && p.M > 128 && tiles * 10 >= r->pairs * 6;
+    const int64_t small = ((p.M + 127) / 128) * ((p.N + (p.dual ? 63 : 127)) / (p.dual ? 64 : 128));
+    r->pair = r->pairs > 0 && p.M > 128 && (tiles * 10 >= r->pairs * 6 || small > ctx->num_sms);
     for (int i = 0; i < p.segments; ++i) QSML_TRY_STATUS(stage(ctx, ws, jobs, p.a[i], f32, -1, &r->a[i]));
     // a dual product's weights share an order: they meet in one MMA
     for (int i = 0; i < (p.dual ? 2 : p.segments); ++i)

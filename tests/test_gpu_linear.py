@@ -262,6 +262,17 @@ def test_both_gradients(ctx, size, dt, gated):
         assert list(np.diff(before)) == [4 if size[0] == 8192 else 3, 3, 2], before
 
 
+# fewer of the pairs' tiles than 60 % of them, but more of the others than SMs
+@pytest.mark.parametrize("size,gated", [((130, 72, 10100), False), ((200, 40, 5000), True), ((9600, 24, 250), False)])
+def test_few_tiles_for_pairs(ctx, size, gated):
+    c = Case(*size, np.float16, gated=gated)
+    y, pre = forward(ctx, c, "silu", True)
+    assert ctx.last_kernel().startswith("k_linear_pair")
+    check_forward(c, "silu", y, pre, True)
+    kept = c.kept()
+    check_backward(c, "silu", kept, *backward(ctx, c, "silu", kept))
+
+
 def strided(a, how):
     """A device view with the values of `a`: transposed storage, an odd row pitch, columns of a
     wider matrix, every other column, a start off the 16-byte boundary."""
