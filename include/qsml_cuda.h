@@ -435,8 +435,9 @@ QSML_API qsml_status_t qsml_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsm
  * x's dtype; dbias [N] in F32 or x's dtype; each may be NULL when it is not
  * wanted.  Between its computation and the products an F16 dz is rounded to
  * F16, the type of the products' operands, where it has more than 2^16 elements
- * (smaller ones keep 22 bits); dbias is summed before that.  With no rows dw and dbias are 0.  relu' is 0 at
- * 0.  No reference counterpart (it has no gradients). */
+ * (smaller ones keep 22 bits); dbias is summed before that.  With no rows dw and
+ * dbias are 0.  relu' is 0 at 0.  No reference counterpart (it has no
+ * gradients). */
 QSML_API qsml_status_t qsml_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,
                                             const qsml_tdesc* pre, const qsml_tdesc* dy, const qsml_tdesc* dx,
                                             const qsml_tdesc* dw, const qsml_tdesc* dbias, int32_t precision);

@@ -19,8 +19,9 @@
 // rounded as the scalar instruction): the kernel was bound by instructions, 32 an
 // element, before it was by HBM.
 // k_layer_norm_bwd_groups: rows narrower than a CTA's, 4 to 32 lanes a row.
-// k_layer_norm_bwd_rows + k_layer_norm_bwd_cols: rows wider than the registers
-// hold (8192 columns, 6144 off 16 bytes), in two kernels (5 elements of traffic and the row statistics).
+// k_layer_norm_bwd_rows + k_layer_norm_bwd_cols: rows too wide for the registers to
+// hold the columns' sums as well (8192 columns, 6144 off 16 bytes), in two kernels
+// (5 elements of traffic and the row statistics; 4096 x 16384 binary16: 154 us).
 #include "packed.cuh"
 #include "row_pipe.cuh"
 #include "workspace.cuh"
@@ -491,60 +492,98 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Rows of any width, a CTA a row in three sweeps over global memory by loads of PV
-// elements (L2 holds a row between them); leaves the row's mean and rstd for the
-// column kernel.
-template <typename T, typename GT, int PV>
+// PV values of gamma, which lies at a 16-byte boundary for PV > 1 (single loads of
+// neighbouring lanes lie PV apart: 4096 x 16384 of binary16 took 244 us, now 154).
+template <typename GT, int PV> __device__ __forceinline__ void gammas(const GT* g, float (&o)[PV]) {
+    constexpr int W = 16 / sizeof(GT) < PV ? 16 / sizeof(GT) : PV;
+#pragma unroll
+    for (int i = 0; i < PV / W; ++i) {
+        const Vec<GT, W> v = reinterpret_cast<const Vec<GT, W>*>(g)[i];
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[i * W + e] = to_f(v.v[e]);
+    }
+}
+
+// Rows of any width, a CTA a row; leaves the row's mean and rstd for the column kernel.
+// NV > 0: the threads hold the row, NV loads of PV elements each; NV == 0: three sweeps
+// over global memory (L2 holds a row between them).
+template <typename T, typename GT, int PV, int NV>
 __global__ void __launch_bounds__(512)
     k_layer_norm_bwd_rows(const T* __restrict__ x, const GT* __restrict__ gamma, const T* __restrict__ dy,
                           T* __restrict__ dx, float2* __restrict__ stats, int64_t rows, int cols, float eps) {
     pdl_begin();
     using V = Vec<T, PV>;
+    constexpr int HELD = NV > 0 ? NV : 1;
     __shared__ float slots[4 * 32];
     const float inv_n = __frcp_rn(static_cast<float>(cols));
     const unsigned packs = cols / PV;  // a step past 2^31 - 1 columns still fits
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const V* xr = reinterpret_cast<const V*>(x + row * cols);
         const V* yr = reinterpret_cast<const V*>(dy + row * cols);
+        V* dr = dx ? reinterpret_cast<V*>(dx + row * cols) : nullptr;
+        V xh[HELD], yh[HELD];
+        // f(p, x, dy) for this thread's loads p
+        auto sweep = [&](auto&& f) {
+            if constexpr (NV > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (threadIdx.x + i * 512 < packs) f(threadIdx.x + i * 512, xh[i], yh[i]);
+            } else {
+#pragma unroll 2
+                for (unsigned p = threadIdx.x; p < packs; p += 512) {
+                    const V v = xr[p], y = yr[p];
+                    f(p, v, y);
+                }
+            }
+        };
         float s1[1] = {0.0f};
-#pragma unroll 4
-        for (unsigned p = threadIdx.x; p < packs; p += 512) {
-            const V v = xr[p];
+        auto add = [&](const V& v) {
 #pragma unroll
             for (int e = 0; e < PV; ++e) s1[0] = __fadd_rn(s1[0], to_f(v.v[e]));
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (threadIdx.x + i * 512 < packs) {
+                    xh[i] = xr[threadIdx.x + i * 512];
+                    yh[i] = yr[threadIdx.x + i * 512];
+                }
+            sweep([&](unsigned, const V& v, const V&) { add(v); });
+        } else {
+#pragma unroll 4
+            for (unsigned p = threadIdx.x; p < packs; p += 512) add(xr[p]);
         }
         row_sums(s1, slots);
         const float mean = __fmul_rn(s1[0], inv_n);
         float s3[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-        for (unsigned p = threadIdx.x; p < packs; p += 512) {
-            const V v = xr[p], y = yr[p];
+        sweep([&](unsigned p, const V& v, const V& y) {
+            float g[PV];
+            gammas<GT, PV>(gamma + p * PV, g);
 #pragma unroll
             for (int e = 0; e < PV; ++e) {
-                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), to_f(gamma[p * PV + e]));
+                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), g[e]);
                 s3[0] = __fmaf_rn(d, d, s3[0]);
                 s3[1] = __fadd_rn(s3[1], h);
                 s3[2] = __fmaf_rn(h, d, s3[2]);
             }
-        }
+        });
         row_sums(s3, slots + 32);
         const float rstd = rsqrtf(__fmaf_rn(s3[0], inv_n, eps));
         if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
         if (!dx) continue;
         const float a = __fmul_rn(__fmul_rn(s3[1], inv_n), rstd);
         const float b = __fmul_rn(__fmul_rn(__fmul_rn(s3[2], inv_n), rstd), __fmul_rn(rstd, rstd));
-        V* dr = reinterpret_cast<V*>(dx + row * cols);
-#pragma unroll 2
-        for (unsigned p = threadIdx.x; p < packs; p += 512) {
-            const V v = xr[p], y = yr[p];
+        sweep([&](unsigned p, const V& v, const V& y) {
+            float g[PV];
+            gammas<GT, PV>(gamma + p * PV, g);
             V o;
 #pragma unroll
             for (int e = 0; e < PV; ++e) {
-                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), to_f(gamma[p * PV + e]));
+                const float d = __fsub_rn(to_f(v.v[e]), mean), h = __fmul_rn(to_f(y.v[e]), g[e]);
                 from_f(__fmaf_rn(h, rstd, -__fmaf_rn(d, b, a)), o.v[e]);
             }
             dr[p] = o;
-        }
+        });
     }
 }
 
@@ -669,10 +708,12 @@ template <typename T, typename GT, int PV>
 qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
     Workspace ws(ctx);
     void *stats = nullptr, *partial = nullptr;
-    // a chunk of rows for each CTA of the column kernel, about eight CTAs an SM
+    // a chunk of rows for each CTA of the column kernel, about eight CTAs an SM, at least 16
+    // rows (with fewer the partial sums cost more than the rows)
     const int64_t tiles = (a.cols / PV + 127) / 128;
     int64_t parts = (8 * ctx->num_sms + tiles - 1) / tiles;
-    if (parts > a.rows) parts = a.rows;
+    const int64_t most = (a.rows + 15) / 16;
+    if (parts > most) parts = most;
     const int64_t chunk = (a.rows + parts - 1) / parts;
     parts = (a.rows + chunk - 1) / chunk;
     if (a.sums()) {
@@ -680,8 +721,18 @@ qsml_status_t launch_wide_bwd(Context* ctx, const Args& a) {
         QSML_TRY_STATUS(ws.get(static_cast<size_t>(parts) * a.cols * 2 * sizeof(float), &partial));
     }
     const int64_t grid = a.rows < 4 * ctx->num_sms ? a.rows : 4 * ctx->num_sms;
-    cudaError_t e = launch_pdl(k_layer_norm_bwd_rows<T, GT, PV>, dim3(static_cast<unsigned>(grid)), dim3(512), 0,
-                               ctx->stream, static_cast<const T*>(a.x), static_cast<const GT*>(a.gamma),
+    // the row in registers where 512 threads hold it, unless that costs resident CTAs that
+    // many binary32 rows need (148 x 16384: 35 us in sweeps, 28 held; 4096 x 10000: 161 and
+    // 190; binary16 4096 x 10000: 177 and 113)
+    const int64_t packs = a.cols / PV;
+    constexpr int FEW = PV == 8 ? 4 : 0, MANY = PV == 1 ? 16 : 8;
+    auto kernel = k_layer_norm_bwd_rows<T, GT, PV, 0>;
+    if (sizeof(T) == 2 || a.rows <= 4 * ctx->num_sms) {
+        if (packs <= FEW * 512) kernel = k_layer_norm_bwd_rows<T, GT, PV, FEW>;
+        else if (packs <= MANY * 512) kernel = k_layer_norm_bwd_rows<T, GT, PV, MANY>;
+    }
+    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(512), 0, ctx->stream,
+                               static_cast<const T*>(a.x), static_cast<const GT*>(a.gamma),
                                static_cast<const T*>(a.dy), static_cast<T*>(a.dx), static_cast<float2*>(stats), a.rows,
                                static_cast<int>(a.cols), a.eps);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_layer_norm_bwd_rows");
@@ -729,7 +780,8 @@ template <typename T, typename GT, int PV> qsml_status_t pick(Context* ctx, cons
 template <typename T, typename GT>
 qsml_status_t run_bwd(Context* ctx, const Args& a) {
     constexpr int PV = 16 / sizeof(T);
-    if (a.cols % PV == 0 && aligned16(a.x) && aligned16(a.dy) && (!a.dx || aligned16(a.dx)))
+    if (a.cols % PV == 0 && aligned16(a.x) && aligned16(a.dy) && (!a.dx || aligned16(a.dx)) &&
+        (a.cols <= 8192 || aligned16(a.gamma)))
         return pick<T, GT, PV>(ctx, a);
     return pick<T, GT, 1>(ctx, a);
 }

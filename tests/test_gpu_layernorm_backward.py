@@ -95,6 +95,17 @@ def test_wide_rows_of_single_elements(ctx, rows, cols, dtype):
     check(x, g, dy, 1e-5, *run(ctx, x, g, dy))
 
 
+@pytest.mark.parametrize("gdt", [np.float32, np.float16])
+@pytest.mark.parametrize("cols", [64, 4096, 8200, 16384])
+def test_gamma_off_16_bytes(ctx, cols, gdt):
+    x, g, dy = make((5, cols), np.float16, gdt=gdt)
+    wide = dev(np.concatenate([g[:1], g]))
+    out = [empty(x.shape, x.dtype), empty((cols,), np.float32), empty((cols,), np.float32)]
+    tx, tdy = dev(x), dev(dy)
+    ctx.layer_norm_backward(d(tx), d(wide[1:]), d(tdy), 1e-5, *[d(t) for t in out])
+    check(x, g, dy, 1e-5, *[host(t) for t in out])
+
+
 def test_workload_16384x4096_f16(ctx):
     x, g, dy = make((16384, 4096), np.float16)
     check(x, g, dy, 1e-5, *run(ctx, x, g, dy))
