@@ -1561,10 +1561,12 @@ qsml_status_t run_one(Context* ctx, const Problem& p, bool f32, const Ready& r, 
     return p.dual ? launch_one<false, true>(ctx, g) : launch_one<false, false>(ctx, g);
 }
 
-// The two products of a backward pass, neither by pairs of SMs nor of one row of tiles.
+// The two products of a backward pass, neither by pairs of SMs.  So the weights are small
+// (44 of the pairs' tiles), and HBM does not bound one row of tiles.
 template <bool F32>
 qsml_status_t run_together(Context* ctx, const Problem* const* p, const Ready* r, const TcArgs* g, bool* launched) {
     Split a = whole_split(g[0]), b = whole_split(g[1]);
+    a.one_row = b.one_row = false;
     QSML_TRY_STATUS((best_split<F32, false>(ctx, &a)));
     if (!p[1]->dual) {
         QSML_TRY_STATUS((best_split<F32, false>(ctx, &b)));
@@ -1597,7 +1599,7 @@ qsml_status_t run_tc(Context* ctx, const Problem* const* p, int n, bool f32) {
     for (int i = 0; i < n; ++i) {
         QSML_TRY_STATUS(prepare(ctx, ws, &jobs, *p[i], f32, &r[i]));
         QSML_TRY_STATUS(arguments(ctx, *p[i], f32, r[i], &g[i]));
-        together = together && !r[i].pair && g[i].tiles_m > 1;
+        together = together && !r[i].pair;
     }
     QSML_TRY_STATUS(run_jobs(ctx, jobs, f32));
     if (together) {

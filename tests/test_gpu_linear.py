@@ -245,7 +245,7 @@ def test_pairs_of_sms(ctx, size, dt, gated):
 # x's and the weights' gradients by one launch: tiles and sums of all ragged, shared out over
 # clusters or not, dz in two parts or one, operands that are copied and ones read in place; the
 # last size takes two launches
-@pytest.mark.parametrize("size", [(129, 130, 1), (200, 300, 64), (131, 257, 450), (777, 136, 256), (520, 512, 1030),
+@pytest.mark.parametrize("size", [(17, 48, 64), (40, 264, 1000), (128, 1024, 256), (129, 130, 1), (200, 300, 64), (131, 257, 450), (777, 136, 256), (520, 512, 1030),
                                   (1100, 260, 130), (8192, 256, 512)])
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("gated", [False, True])
