@@ -793,7 +793,7 @@ using namespace qsml;
 
 extern "C" qsml_status_t qsml_layer_norm_backward(qsml_ctx* handle, const qsml_tdesc* x, const qsml_tdesc* gamma,
                                                   const qsml_tdesc* dy, float eps, const qsml_tdesc* dx,
-                                                  const qsml_tdesc* dgamma, const qsml_tdesc* dbeta) {
+                                                  const qsml_tdesc* dgamma, const qsml_tdesc* dbeta) try {
     QSML_CTX(handle);
     QSML_TRY_STATUS(check_desc(C_, x, "x"));
     QSML_TRY_STATUS(check_desc(C_, gamma, "gamma"));
@@ -864,4 +864,4 @@ extern "C" qsml_status_t qsml_layer_norm_backward(qsml_ctx* handle, const qsml_t
     if (x->dtype == QSML_F32) return run_bwd<float, float>(C_, a);
     if (gamma->dtype == QSML_F32) return run_bwd<__half, float>(C_, a);
     return run_bwd<__half, __half>(C_, a);
-}
+} QSML_NO_THROW

@@ -304,7 +304,7 @@ using namespace qsml::linear;
 
 extern "C" qsml_status_t qsml_linear(qsml_ctx* handle, const qsml_tdesc* x, const qsml_tdesc* w, const qsml_tdesc* bias,
                                      int32_t act, const qsml_tdesc* residual, const qsml_tdesc* pre,
-                                     const qsml_tdesc* y, int32_t precision) {
+                                     const qsml_tdesc* y, int32_t precision) try {
     QSML_CTX(handle);
     const char* op = "qsml_linear";
     const Named all[6] = {{x, "x"}, {w, "w"}, {y, "y"}, {bias, "bias"}, {residual, "residual"}, {pre, "pre"}};
@@ -331,11 +331,11 @@ extern "C" qsml_status_t qsml_linear(qsml_ctx* handle, const qsml_tdesc* x, cons
     p.e.pre[0] = pre ? pre->data : nullptr;
     p.e.y = y->data;
     return run(C_, x->dtype, precision, p);
-}
+} QSML_NO_THROW
 
 extern "C" qsml_status_t qsml_linear_backward(qsml_ctx* handle, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,
                                               const qsml_tdesc* pre, const qsml_tdesc* dy, const qsml_tdesc* dx,
-                                              const qsml_tdesc* dw, const qsml_tdesc* dbias, int32_t precision) {
+                                              const qsml_tdesc* dw, const qsml_tdesc* dbias, int32_t precision) try {
     QSML_CTX(handle);
     const char* op = "qsml_linear_backward";
     const Named all[7] = {{x, "x"}, {w, "w"}, {dy, "dy"}, {pre, "pre"}, {dx, "dx"}, {dw, "dw"}, {dbias, "dbias"}};
@@ -358,12 +358,12 @@ extern "C" qsml_status_t qsml_linear_backward(qsml_ctx* handle, const qsml_tdesc
     const Named out[3] = {{dx, "dx"}, {dw, "dw"}, {dbias, "dbias"}};
     QSML_TRY_STATUS(check_overlap(C_, op, in, 4, out, 3, nullptr));
     return backward(C_, op, x->dtype, precision, act, mx, &mw, 1, dy, dy_ld, &pre, dx, &dw, &dbias);
-}
+} QSML_NO_THROW
 
 extern "C" qsml_status_t qsml_gated_linear(qsml_ctx* handle, const qsml_tdesc* x, const qsml_tdesc* w_gate,
                                            const qsml_tdesc* w_up, const qsml_tdesc* b_gate, const qsml_tdesc* b_up,
                                            int32_t act, const qsml_tdesc* gate, const qsml_tdesc* up,
-                                           const qsml_tdesc* y, int32_t precision) {
+                                           const qsml_tdesc* y, int32_t precision) try {
     QSML_CTX(handle);
     const char* op = "qsml_gated_linear";
     const Named all[8] = {{x, "x"}, {w_gate, "w_gate"}, {w_up, "w_up"}, {y, "y"}, {b_gate, "b_gate"}, {b_up, "b_up"},
@@ -397,14 +397,14 @@ extern "C" qsml_status_t qsml_gated_linear(qsml_ctx* handle, const qsml_tdesc* x
     p.e.pre[1] = up ? up->data : nullptr;
     p.e.y = y->data;
     return run(C_, x->dtype, precision, p);
-}
+} QSML_NO_THROW
 
 extern "C" qsml_status_t qsml_gated_linear_backward(qsml_ctx* handle, const qsml_tdesc* x, const qsml_tdesc* w_gate,
                                                     const qsml_tdesc* w_up, int32_t act, const qsml_tdesc* gate,
                                                     const qsml_tdesc* up, const qsml_tdesc* dy, const qsml_tdesc* dx,
                                                     const qsml_tdesc* dw_gate, const qsml_tdesc* dw_up,
                                                     const qsml_tdesc* db_gate, const qsml_tdesc* db_up,
-                                                    int32_t precision) {
+                                                    int32_t precision) try {
     QSML_CTX(handle);
     const char* op = "qsml_gated_linear_backward";
     const Named all[11] = {{x, "x"}, {w_gate, "w_gate"}, {w_up, "w_up"}, {gate, "gate"}, {up, "up"}, {dy, "dy"},
@@ -433,4 +433,4 @@ extern "C" qsml_status_t qsml_gated_linear_backward(qsml_ctx* handle, const qsml
     const qsml_tdesc* dw[2] = {dw_gate, dw_up};
     const qsml_tdesc* db[2] = {db_gate, db_up};
     return backward(C_, op, x->dtype, precision, act, mx, mw, 2, dy, dy_ld, pre, dx, dw, db);
-}
+} QSML_NO_THROW

@@ -2,7 +2,15 @@
 // operators with a backward pass share.
 #pragma once
 
+#include <new>
+
 #include "qsml_internal.cuh"
+
+// The end of an entry point (extern "C" ... f(...) try { ... } QSML_NO_THROW): the
+// standard library's exceptions, thrown where host memory runs out, become a status.
+#define QSML_NO_THROW                                  \
+    catch (const std::bad_alloc&) { return QSML_E_OOM; } \
+    catch (...) { return QSML_E_INVALID; }
 
 namespace qsml {
 

@@ -5,6 +5,10 @@ A wait limit of one cycle makes the first wait for a copy still in flight run ou
 qsml_synchronize then reports QSML_E_TIMEOUT once, and with the default limit the next call of the
 same context gives the right result.  Every wait stays bounded, and the waits that drain a kernel's
 own copies and MMAs keep the full limit."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -12,6 +16,7 @@ from helpers import d, dev, empty, host
 from quasarml_b200 import abi, datagen
 
 pytestmark = pytest.mark.gpu
+HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 @pytest.fixture
@@ -54,6 +59,56 @@ def test_linear_wait_expires_then_recovers(fresh, m, k, n, dt):
     # sums of k terms in binary32 and one rounding, over the largest result
     bar = 2.0 ** -11 + (k + 100) * 2.0 ** -24 if dt == np.float16 else (k + 100) * 2.0 ** -24
     assert np.max(np.abs(host(y) - ref)) <= bar * np.max(np.abs(ref))
+
+
+@pytest.mark.parametrize("dt", [np.float16, np.float32])
+def test_backward_wait_expires_then_recovers(fresh, dt):
+    """Both gradients in one launch."""
+    m, k, n = 512, 1024, 1024
+    x, w, dy = normal(1, m, k, dt=dt), normal(2, k, n, s=k ** -0.5, dt=dt), normal(3, m, n, dt=dt)
+    tx, tw, tdy, dx, dw = dev(x), dev(w), dev(dy), empty((m, k), dt), empty((k, n), dt)
+
+    def call():
+        fresh.linear_backward(d(tx), d(tw), abi.ACT_NONE, None, d(tdy), d(dx), d(dw))
+    fresh.set_wait_limit(1)
+    call()
+    expect_timeout(fresh)
+    fresh.set_wait_limit(0)
+    call()
+    fresh.synchronize()
+    x, w, dy = (v.astype(np.float64) for v in (x, w, dy))
+    step = 2.0 ** -11 if dt == np.float16 else 2.0 ** -24
+    for out, a, b, terms in ((dx, dy, w.T, n), (dw, x.T, dy, m)):
+        # as many roundings of a binary32 sum as terms, 100 for the operands' parts, one of the result
+        ref, bar = a @ b, (terms + 100) * 2.0 ** -24 * (np.abs(a) @ np.abs(b))
+        assert np.all(np.abs(host(out) - ref) <= bar + step * (np.abs(ref) + bar))
+
+
+def test_no_memory_for_a_workspace():
+    """The first driver allocation reports out-of-memory (on the host): the call returns it, the
+    next one works."""
+    code = """
+import sys
+sys.path.insert(0, %r)
+sys.path.insert(0, %r)
+import torch
+from helpers import d
+from quasarml_b200 import abi
+c = abi.Context(0)
+x, w, dy = (torch.ones(s, device="cuda") for s in ((40, 64), (64, 72), (40, 72)))
+dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(72, device="cuda")
+for _ in range(2):
+    try:
+        c.linear_backward(d(x), d(w), abi.ACT_NONE, None, d(dy), d(dx), d(dw), d(db))
+        c.synchronize()
+        print("SUMS", dx.unique().tolist(), dw.unique().tolist(), db.unique().tolist())
+    except abi.QsmlError as e:
+        print("STATUS", e.status)
+""" % (os.path.dirname(HERE), HERE)
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, QSML_FAULT_ALLOC_N="1"),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.splitlines() == [f"STATUS {abi.E_OOM}", "SUMS [72.0] [40.0] [40.0]"], r.stdout
 
 
 # larger than L2 and bound by HBM, so that among the rows of ten calls some are waited for
