@@ -216,9 +216,9 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
     // it is where the CUDA cores take it (FFMA, few rows).
     // binary16: rounding dz adds to dx and dw an error of the size of their own rounding
     // (1.4 times the error in all).  A dz of up to 2^16 elements is kept in two parts, 22
-    // bits: its products are short (256 x 256 x 256: 21 us either way), and so few roundings
-    // do not even out.  Beyond, two parts cost (512 x 1024 x 1024: 20 us to 28; 16384 x
-    // 1024 x 2048: 155 to 270).
+    // bits: its products are short (256 x 256 x 256: 12 us, in one part 10), and so few
+    // roundings do not even out.  Beyond, two parts cost more (512 x 1024 x 1024: 16 us for
+    // 13; 16384 x 1024 x 2048: 262 for 152).
     // Without an activation dz = dy and needs no copy, binary32's split apart.
     const bool exact = act == QSML_ACT_NONE && nw == 1;
     const bool split = (dx || want_dw) && (dtype == QSML_F32 ? precision != QSML_MM_FP32_FFMA && M > 16
