@@ -434,8 +434,11 @@ QSML_API qsml_status_t qsml_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsm
  * last dim and rows of one stride; dx [.., K] and dw [K, N] are contiguous, in
  * x's dtype; dbias [N] in F32 or x's dtype; each may be NULL when it is not
  * wanted.  Between its computation and the products an F16 dz is rounded to
- * F16, the type of the products' operands, where it has more than 2^16 elements
- * (smaller ones keep 22 bits); dbias is summed before that.  With no rows dw and
+ * the 11 bits of F16, the type of the products' operands, where it has more than
+ * 2^16 elements (smaller ones keep 22 bits), which makes the error of dx and dw
+ * about 1.4 times that of their own rounding.  It is scaled by a power of two for
+ * that, so dz may lie far beyond F16's range: an element keeps those bits or is off
+ * by 2^-33 of the largest one (of dg and du together).  dbias is summed before.  With no rows dw and
  * dbias are 0.  relu' is 0 at 0.  No reference counterpart (it has no
  * gradients). */
 QSML_API qsml_status_t qsml_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,

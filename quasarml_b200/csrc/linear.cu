@@ -214,12 +214,13 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
     // How dz lies between its computation and the products.
     // binary32: in the three parts of the tensor cores, split once for both products; as
     // it is where the CUDA cores take it (FFMA, few rows).
-    // binary16: rounding dz adds to dx and dw an error of the size of their own rounding
-    // (1.4 times the error in all).  A dz of up to 2^16 elements is kept in two parts, 22
-    // bits: its products are short (256 x 256 x 256: 12 us, in one part 10), and so few
-    // roundings do not even out.  Beyond, two parts cost more (512 x 1024 x 1024: 16 us for
-    // 13; 16384 x 1024 x 2048: 262 for 152).
+    // binary16: rounding dz to 11 bits adds to dx and dw an error of the size of their own
+    // rounding (1.4 times the error in all, however long the sums).  A dz of up to 2^16
+    // elements is kept in two parts, 22 bits, which costs little there (256 x 256 x 256:
+    // 12 us, in one part 10).  Beyond, it costs more than the bits are worth (512 x 1024 x
+    // 1024: 16 us for 13; 16384 x 1024 x 2048: 262 for 152).
     // Without an activation dz = dy and needs no copy, binary32's split apart.
+    // What binary16's dz lacks in range a power of two makes good (linear_grad.cu).
     const bool exact = act == QSML_ACT_NONE && nw == 1;
     const bool split = (dx || want_dw) && (dtype == QSML_F32 ? precision != QSML_MM_FP32_FFMA && M > 16
                                                              : !exact && M * N <= 65536);
@@ -239,7 +240,11 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
         if (!plain) {
             if (act != QSML_ACT_NONE || nw == 2) g.pre[i] = pre[i]->data;
             if ((dx || want_dw) && M * N > 0) {
-                QSML_TRY_STATUS(ws.get(static_cast<size_t>(M) * g.pitch * dz_bytes, &g.dz[i]));
+                // behind the first of binary16's: the scale of both
+                const size_t bytes = static_cast<size_t>(M) * g.pitch * dz_bytes;
+                const bool scaled = dtype == QSML_F16 && i == 0;
+                QSML_TRY_STATUS(ws.get(bytes + (scaled ? sizeof(float) : 0), &g.dz[i]));
+                if (scaled) g.unscale = reinterpret_cast<float*>(static_cast<char*>(g.dz[i]) + bytes);
                 dz[i] = Mat{g.dz[i], M, N, g.pitch, 1, g.plane};
             }
         } else {
@@ -272,6 +277,7 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
             p.b[i] = w[i].t();
         }
         p.e.y = dx->data;
+        p.e.scale = g.unscale;
     }
     if (want_dw) {  // x^T dz
         Problem& p = *(wanted[n] = &products[n]);
@@ -280,6 +286,7 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
         p.N = N;
         p.K = M;
         p.dual = nw == 2 && dw[0] && dw[1];
+        p.e.scale = g.unscale;
         p.a[0] = x.t();
         if (p.dual) {
             p.b[0] = dz[0];

@@ -30,6 +30,7 @@ struct Mat {
 inline int64_t line_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }
 
 struct Epilogue {
+    const float* scale = nullptr;  // binary16: the products are multiplied by it, a power of two; null: by 1
     const void* bias[2] = {nullptr, nullptr};
     int bias_f32 = 1;              // else the dtype of the outputs
     int act = QSML_ACT_NONE;
@@ -315,16 +316,30 @@ __device__ __forceinline__ void bias8(const Epilogue& e, int64_t col, float (&b)
     }
 }
 
-// Columns col .. col + 7 of `row` from their products (u: DUAL only) to the
-// outputs.  col is a multiple of 8; columns from N on are not written.
+// What Epilogue::scale points to.
+template <typename T> __device__ __forceinline__ float scale_of(const Epilogue& e) {
+    if constexpr (sizeof(T) == 4) return 1.0f;
+    return e.scale ? *e.scale : 1.0f;
+}
+
+// Columns col .. col + 7 of `row` from their products (u: DUAL only), which are
+// multiplied by `scale`, to the outputs.  col is a multiple of 8; columns from N on are
+// not written.
 template <typename T, bool DUAL>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int64_t col, const float (&b)[DUAL ? 2 : 1][8],
-                                        float (&z)[8], float (&u)[8]) {
+                                        float (&z)[8], float (&u)[8], float scale = 1.0f) {
     const int n = e.N - col < 8 ? static_cast<int>(e.N - col) : 8;
     const int64_t at = row * e.N + col;
     float r[8];
     if constexpr (!DUAL) {  // first, so that it is in flight under the rest
         if (e.residual) load8(static_cast<const T*>(e.residual) + row * e.res_ld + col, n, e.vec, r);
+    }
+    if (scale != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            z[i] = __fmul_rn(z[i], scale);
+            if constexpr (DUAL) u[i] = __fmul_rn(u[i], scale);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

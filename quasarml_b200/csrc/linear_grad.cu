@@ -4,8 +4,22 @@
 //   DUAL:   dg = dy u act'(g), du = dy act(g), and the column sums of both
 // dz goes to a workspace that the two products of the backward pass read (in the parts
 // that the tensor cores take, see GradArgs); the sums are taken before it is rounded.
+//
+// binary16's dz is stored times a power of two s, which the products' epilogue undoes:
+// dy u can be far beyond binary16 where dx and dw are not, and a small dz is held in few
+// bits where a sum of many is an ordinary number.  s is one number for the whole of dz
+// (dg and du), since dx sums over its columns and dw over its rows.  It is 2^8 where the
+// largest finite |dz| is in [1, 255]: which that is is known at the end, behind a barrier
+// of the grid (with its cooperative launch 7 us of the 165 of a backward pass of 16384 x
+// 1024 x 2048, 2.5 of small ones).  Where it is not, the grid goes over its inputs again, with the s that
+// brings the largest into [2^14, 2^15) (37 us more there, 1.5 at 512 x 1024 x 1024).  Either way an element keeps binary16's 11 bits,
+// or is off by 2^-25 of the scaled numbers' unit, 2^-33 of the largest.
 // Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16:
 // 16384 x 2048 with gelu 38 us, 5.3 TB/s; DUAL 8192 x 5632 76 us, 6.1 TB/s).
+#include <cfloat>
+
+#include <cooperative_groups.h>
+
 #include "linear_grad.cuh"
 
 namespace qsml {
@@ -33,138 +47,242 @@ template <typename T> struct alignas(16) Raw8 {
     }
 };
 
-// A warp takes 256 columns (8 a lane), a CTA's 8 warps every 8th row of
-// [blockIdx.y * chunk, + chunk).  A thread keeps its columns and sums them in
+// The largest of the block's values, in every thread.
+__device__ __forceinline__ float block_max(float v) {
+    __shared__ float by_warp[8];
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    if ((threadIdx.x & 31) == 0) by_warp[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = by_warp[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v = fmaxf(v, by_warp[k]);
+    __syncthreads();
+    return v;
+}
+
+// The largest finite magnitude among eight values (0 if there is none).
+__device__ __forceinline__ float largest(const P2 (&d)[4]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 e = unpack(d[j]);
+        m = fmaxf(m, fmaxf(fabsf(e.x), fabsf(e.y)));  // passes over NaN
+    }
+    if (m <= FLT_MAX) return m;
+    m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 e = unpack(d[j]);
+        if (fabsf(e.x) <= FLT_MAX) m = fmaxf(m, fabsf(e.x));
+        if (fabsf(e.y) <= FLT_MAX) m = fmaxf(m, fabsf(e.y));
+    }
+    return m;
+}
+
+constexpr int kDzExponent = 8;
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// An item is 256 columns (8 a lane) by `chunk` rows, a CTA's 8 warps taking every 8th row;
+// items go round the grid, columns first.  A thread keeps its columns and sums them in
 // registers; the warps' sums are added in warp order in shared memory.
-template <typename T, bool DUAL, int ACT>
-__global__ void __launch_bounds__(256) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, bool vec) {
+// SCALED: dz times a power of two (above); the grid is cooperative.
+template <typename T, bool DUAL, int ACT, bool SCALED>
+__global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, int tiles, int items,
+                                                   bool vec) {
     pdl_begin();
     constexpr int NO = DUAL ? 2 : 1;
     __shared__ float fold[NO][8][256 + 8];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 256 + lane * 8;
-    const int n = a.N - col < 8 ? static_cast<int>(a.N - col) : 8;  // may be <= 0
-    const int64_t r0 = blockIdx.y * chunk, r1 = r0 + chunk < a.M ? r0 + chunk : a.M;
-    P2 sum[NO][4];
+    float scale = power_of_two(kDzExponent), most = 0.0f;
+    bool again = false;  // the second time: neither sums nor the largest
+    for (int item = blockIdx.x;; item += gridDim.x) {
+        if (item >= items) {
+            if (!SCALED || again) return;
+            most = block_max(most);
+            if (threadIdx.x == 0) a.most[blockIdx.x] = most;
+            cooperative_groups::this_grid().sync();
+            most = 0.0f;
+            for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) most = fmaxf(most, a.most[i]);
+            most = block_max(most);
+            const bool fits = most == 0.0f || (most >= 1.0f && most <= 255.0f);
+            const int e = fits ? kDzExponent : min(14 - ilogbf(most), 100);
+            if (blockIdx.x == 0 && threadIdx.x == 0) *a.unscale = power_of_two(-e);
+            if (fits) return;
+            scale = power_of_two(e);
+            again = true;
+            item = blockIdx.x;
+        }
+        const int64_t col = static_cast<int64_t>(item % tiles) * 256 + lane * 8;
+        const int n = a.N - col < 8 ? static_cast<int>(a.N - col) : 8;  // may be <= 0
+        const int64_t r0 = item / tiles * chunk, r1 = r0 + chunk < a.M ? r0 + chunk : a.M;
+        const bool sums = a.partial && !again;
+        P2 sum[NO][4];
 #pragma unroll
-    for (int o = 0; o < NO; ++o)
+        for (int o = 0; o < NO; ++o)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[o][j].v = 0;
-    if (n > 0) {
-        // AHEAD rows in flight under the one at hand: as many as leave two CTAs a SM, three
-        // LINEAR ones of binary16 (DUAL binary16 8192 x 5632: 88, 79, 76 us with 1, 2, 3;
-        // binary32 8192 x 4096: 128 us with 1, 171 with 2)
-        constexpr int AHEAD = sizeof(T) == 4 ? 1 : DUAL ? 3 : 2;
-        constexpr bool PRE = DUAL || ACT != QSML_ACT_NONE;
-        Raw8<T> ry[AHEAD + 1], rz[AHEAD + 1], ru[AHEAD + 1];
-        auto load = [&](int64_t r, Raw8<T>& y, Raw8<T>& z, Raw8<T>& u) {
-            if (r >= r1) return;
-            y.load(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec);
-            if constexpr (PRE) z.load(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec);
-            if constexpr (DUAL) u.load(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec);
-        };
-        auto work = [&](int64_t r, const Raw8<T>& y, const Raw8<T>& z, const Raw8<T>& u) {
-            // elements past the row's end were loaded as 0 and so end as 0
-            P2 d[NO][4];
+            for (int j = 0; j < 4; ++j) sum[o][j].v = 0;
+        if (n > 0) {
+            // AHEAD rows in flight under the one at hand: as many as leave two CTAs a SM, three
+            // LINEAR ones of binary16 (DUAL binary16 8192 x 5632: 88, 79, 76 us with 1, 2, 3;
+            // binary32 8192 x 4096: 128 us with 1, 171 with 2)
+            constexpr int AHEAD = sizeof(T) == 4 ? 1 : DUAL ? 3 : 2;
+            constexpr bool PRE = DUAL || ACT != QSML_ACT_NONE;
+            Raw8<T> ry[AHEAD + 1], rz[AHEAD + 1], ru[AHEAD + 1];
+            auto load = [&](int64_t r, Raw8<T>& y, Raw8<T>& z, Raw8<T>& u) {
+                if (r >= r1) return;
+                y.load(static_cast<const T*>(a.dy) + r * a.dy_ld + col, n, vec);
+                if constexpr (PRE) z.load(static_cast<const T*>(a.pre[0]) + r * a.N + col, n, vec);
+                if constexpr (DUAL) u.load(static_cast<const T*>(a.pre[1]) + r * a.N + col, n, vec);
+            };
+            auto work = [&](int64_t r, const Raw8<T>& y, const Raw8<T>& z, const Raw8<T>& u) {
+                // elements past the row's end were loaded as 0 and so end as 0
+                P2 d[NO][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (!PRE) {
+                        d[0][j] = y.pair(j);
+                    } else {
+                        P2 value;
+                        const P2 g = act_grad2<T>(ACT, z.pair(j), value);
+                        if constexpr (DUAL) {
+                            d[0][j] = mul2(mul2(y.pair(j), u.pair(j)), g);
+                            d[1][j] = mul2(y.pair(j), value);
+                        } else {
+                            d[0][j] = mul2(y.pair(j), g);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int o = 0; o < NO; ++o) {
+                    if (sums) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[o][j] = add2(sum[o][j], d[o][j]);
+                    }
+                    if (a.dz[o]) {
+                        float f[8];
+                        if constexpr (SCALED) {
+                            if (!again) most = fmaxf(most, largest(d[o]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 e = unpack(SCALED ? mul2(d[o][j], both(scale)) : d[o][j]);
+                            f[2 * j] = e.x;
+                            f[2 * j + 1] = e.y;
+                        }
+                        if (a.plane) {
+                            uint16_t* to = static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col;
+                            if constexpr (sizeof(T) == 4) split8(f, to, a.plane);
+                            else halve8(f, reinterpret_cast<__half*>(to), a.plane);
+                        } else {
+                            store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, f);
+                        }
+                    }
+                }
+            };
+            int64_t r = r0 + w;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) load(r + 8 * i, ry[i], rz[i], ru[i]);
+            while (r < r1) {
+#pragma unroll
+                for (int i = 0; i <= AHEAD; ++i) {
+                    if (r >= r1) break;
+                    const int to = (i + AHEAD) % (AHEAD + 1);
+                    load(r + 8 * AHEAD, ry[to], rz[to], ru[to]);
+                    work(r, ry[i], rz[i], ru[i]);
+                    r += 8;
+                }
+            }
+        }
+        if (!sums) continue;
+#pragma unroll
+        for (int o = 0; o < NO; ++o)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (!PRE) {
-                    d[0][j] = y.pair(j);
-                } else {
-                    P2 value;
-                    const P2 g = act_grad2<T>(ACT, z.pair(j), value);
-                    if constexpr (DUAL) {
-                        d[0][j] = mul2(mul2(y.pair(j), u.pair(j)), g);
-                        d[1][j] = mul2(y.pair(j), value);
-                    } else {
-                        d[0][j] = mul2(y.pair(j), g);
-                    }
-                }
+                const float2 e = unpack(sum[o][j]);
+                fold[o][w][lane * 8 + 2 * j] = e.x;
+                fold[o][w][lane * 8 + 2 * j + 1] = e.y;
             }
+        __syncthreads();
+        const int64_t c = static_cast<int64_t>(item % tiles) * 256 + threadIdx.x;
+        if (c < a.N) {
 #pragma unroll
             for (int o = 0; o < NO; ++o) {
-                if (a.dz[o]) {
-                    float f[8];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 e = unpack(d[o][j]);
-                        f[2 * j] = e.x;
-                        f[2 * j + 1] = e.y;
-                    }
-                    if (a.plane) {
-                        uint16_t* to = static_cast<uint16_t*>(a.dz[o]) + r * a.pitch + col;
-                        if constexpr (sizeof(T) == 4) split8(f, to, a.plane);
-                        else halve8(f, reinterpret_cast<__half*>(to), a.plane);
-                    } else {
-                        store8(static_cast<T*>(a.dz[o]) + r * a.pitch + col, n, n == 8, f);
-                    }
-                }
-                if (a.partial) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[o][j] = add2(sum[o][j], d[o][j]);
-                }
-            }
-        };
-        int64_t r = r0 + w;
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) load(r + 8 * i, ry[i], rz[i], ru[i]);
-        while (r < r1) {
-#pragma unroll
-            for (int i = 0; i <= AHEAD; ++i) {
-                if (r >= r1) break;
-                const int to = (i + AHEAD) % (AHEAD + 1);
-                load(r + 8 * AHEAD, ry[to], rz[to], ru[to]);
-                work(r, ry[i], rz[i], ru[i]);
-                r += 8;
+                float s = fold[o][0][threadIdx.x];
+                for (int k = 1; k < 8; ++k) s = __fadd_rn(s, fold[o][k][threadIdx.x]);
+                a.partial[(static_cast<int64_t>(o) * (items / tiles) + item / tiles) * a.N + c] = s;
             }
         }
-    }
-    if (!a.partial) return;
-#pragma unroll
-    for (int o = 0; o < NO; ++o)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 e = unpack(sum[o][j]);
-            fold[o][w][lane * 8 + 2 * j] = e.x;
-            fold[o][w][lane * 8 + 2 * j + 1] = e.y;
-        }
-    __syncthreads();
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= a.N) return;
-#pragma unroll
-    for (int o = 0; o < NO; ++o) {
-        float s = fold[o][0][threadIdx.x];
-        for (int k = 1; k < 8; ++k) s = __fadd_rn(s, fold[o][k][threadIdx.x]);
-        a.partial[(static_cast<int64_t>(o) * gridDim.y + blockIdx.y) * a.N + c] = s;
+        __syncthreads();  // the sums have been read
     }
 }
 
-template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradArgs& given) {
+// CTAs of a cooperative launch that the device holds at once, once a device and kernel.
+template <typename T, bool DUAL, int ACT> qsml_status_t resident(Context* ctx, int64_t* ctas) {
+    static std::mutex mu;
+    static int known[64] = {};
+    std::lock_guard<std::mutex> lk(mu);
+    int& n = known[ctx->device & 63];
+    if (n == 0) {
+        int per_sm = 0;
+        QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_linear_dz<T, DUAL, ACT, true>,
+                                                                                      256, 0),
+                                   "linear: occupancy"));
+        if (per_sm < 1) return set_error(ctx, QSML_E_CUDA, "linear: k_linear_dz does not fit a SM");
+        n = per_sm * ctx->num_sms;
+    }
+    *ctas = n;
+    return QSML_OK;
+}
+
+template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx, const GradArgs& given) {
     GradArgs a = given;
     const int64_t tiles = (a.N + 255) / 256;
-    // about eight CTAs an SM, at least 2 rows a warp (8 left most SMs without a CTA at
-    // 515 x 1366: 23 us)
-    int64_t parts = (8 * ctx->num_sms + tiles - 1) / tiles;
+    // binary32's parts have its range, and binary16's dy without an activation is dz itself
+    constexpr bool CAN_SCALE = sizeof(T) == 2 && (DUAL || ACT != QSML_ACT_NONE);
+    const bool scaled = CAN_SCALE && a.unscale;
+    // about eight items an SM, at least 2 rows a warp (8 left most SMs without a CTA at
+    // 515 x 1366: 23 us); a cooperative grid takes whole turns of what the device holds
+    // (16384 x 2048, 1184 items on 444 CTAs: 1.5 us more than 1328)
+    int64_t held = 0, parts = (8 * ctx->num_sms + tiles - 1) / tiles;
+    if constexpr (CAN_SCALE) {
+        if (scaled) {
+            QSML_TRY_STATUS((resident<T, DUAL, ACT>(ctx, &held)));
+            const int64_t turns = (8 * ctx->num_sms + held - 1) / held;
+            parts = std::max<int64_t>(1, turns * held / tiles);
+        }
+    }
     const int64_t most = (a.M + 15) / 16;
     if (parts > most) parts = most;
     const int64_t chunk = (a.M + parts - 1) / parts;
     parts = (a.M + chunk - 1) / chunk;
+    const int64_t items = tiles * parts, grid = scaled && items > held ? held : items;
     Workspace ws(ctx);
     const bool sums = a.db[0].out || a.db[1].out;
-    void* partial = nullptr;
-    if (sums) QSML_TRY_STATUS(ws.get(static_cast<size_t>(DUAL ? 2 : 1) * parts * a.N * sizeof(float), &partial));
-    a.partial = static_cast<float*>(partial);
+    const size_t partial = sums ? static_cast<size_t>(DUAL ? 2 : 1) * parts * a.N : 0;
+    void* memory = nullptr;
+    const size_t floats = partial + (scaled ? grid : 0);
+    if (floats) QSML_TRY_STATUS(ws.get(floats * sizeof(float), &memory));
+    if (sums) a.partial = static_cast<float*>(memory);
+    if (scaled) a.most = static_cast<float*>(memory) + partial;
     bool vec = a.N % 8 == 0 && a.dy_ld % 8 == 0 && aligned16(a.dy);
     for (int i = 0; i < 2; ++i) vec = vec && (!a.pre[i] || aligned16(a.pre[i]));
-    auto kernel = k_linear_dz<T, DUAL, QSML_ACT_NONE>;
-    switch (a.act) {
-        case QSML_ACT_RELU: kernel = k_linear_dz<T, DUAL, QSML_ACT_RELU>; break;
-        case QSML_ACT_GELU: kernel = k_linear_dz<T, DUAL, QSML_ACT_GELU>; break;
-        case QSML_ACT_SILU: kernel = k_linear_dz<T, DUAL, QSML_ACT_SILU>; break;
-        case QSML_ACT_SIGMOID: kernel = k_linear_dz<T, DUAL, QSML_ACT_SIGMOID>; break;
-    }
-    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)),
-                                     dim3(256), 0, ctx->stream, a, chunk, vec);
+    // A grid with a barrier has to be on the device whole, whatever else runs there: a cooperative
+    // launch, which does not begin before the kernel ahead of it has ended.
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = scaled ? cudaLaunchAttributeCooperative : cudaLaunchAttributeProgrammaticStreamSerialization;
+    if (scaled) attr[0].val.cooperative = 1;
+    else attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(256);
+    cfg.stream = ctx->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto kernel = k_linear_dz<T, DUAL, ACT, false>;
+    if constexpr (CAN_SCALE)
+        if (scaled) kernel = k_linear_dz<T, DUAL, ACT, true>;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, chunk, static_cast<int>(tiles), static_cast<int>(items), vec);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_dz");
     QSML_TRY_STATUS(after_launch(ctx, "k_linear_dz"));
     if (!sums) return QSML_OK;
@@ -172,6 +290,16 @@ template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradAr
     s0.partial = a.partial;
     s1.partial = a.partial + parts * a.N;
     return finish_column_sums(ctx, s0, s1, parts, a.N);
+}
+
+template <typename T, bool DUAL> qsml_status_t launch(Context* ctx, const GradArgs& a) {
+    switch (a.act) {
+        case QSML_ACT_RELU: return launch_act<T, DUAL, QSML_ACT_RELU>(ctx, a);
+        case QSML_ACT_GELU: return launch_act<T, DUAL, QSML_ACT_GELU>(ctx, a);
+        case QSML_ACT_SILU: return launch_act<T, DUAL, QSML_ACT_SILU>(ctx, a);
+        case QSML_ACT_SIGMOID: return launch_act<T, DUAL, QSML_ACT_SIGMOID>(ctx, a);
+    }
+    return launch_act<T, DUAL, QSML_ACT_NONE>(ctx, a);
 }
 
 }  // namespace

@@ -15,8 +15,9 @@ struct GradArgs {
     void* dz[2] = {nullptr, nullptr};         // rows of `pitch` (a multiple of 8), 16-byte aligned; null: not wanted
     int64_t pitch = 0;
     int64_t plane = 0;                        // > 0: dz in parts `plane` elements apart (Mat::plane)
+    float* unscale = nullptr;                 // not null: a binary16 dz is stored times a power of two; 1 / it goes here
     ColumnSum db[2];
-    float* partial = nullptr;
+    float *partial = nullptr, *most = nullptr;  // workspace of the launch: column sums by part, the CTAs' largest |dz|
 };
 
 template <typename T> qsml_status_t run_grad(Context* ctx, const GradArgs& a, bool dual);

@@ -572,6 +572,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     if (!*abort_flag) {
         const int rows = min(128, g.M - mt * 128);
         const int64_t row0 = static_cast<int64_t>(mt) * 128, col0 = static_cast<int64_t>(nt) * BN;
+        const float scale = scale_of<T>(g.e);
         // 16-byte unit `unit` of row r of the tiles, added over the cluster in rank order, all loads under way together
         auto sum4 = [&](int r, int unit) {
             const uint32_t at = r * 512 + ((unit ^ (r & 31)) << 4);
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                     };
                     sum(c / 4, z);
                     if constexpr (DUAL) sum(16 + c / 4, u);
-                    finish8<T, DUAL>(g.e, row0 + r, col0 + c, bias, z, u);
+                    finish8<T, DUAL>(g.e, row0 + r, col0 + c, bias, z, u, scale);
                 }
             }
         } else {
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                     }
                     auto tile = [&](int k, int c) {
                         const int r = min(row(k), rows - 1);
-                        return lds1(base + r * 512 + (((c / 4) ^ (r & 31)) << 4) + (c & 3) * 4);
+                        return __fmul_rn(lds1(base + r * 512 + (((c / 4) ^ (r & 31)) << 4) + (c & 3) * 4), scale);
                     };
 #pragma unroll
                     for (int k = 0; k < ALL; ++k) {
@@ -1093,6 +1094,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 const int vec = e.vec;
                 if (!ready()) break;
                 const uint32_t d = lanes + acc * S::NACC;
+                const float scale = scale_of<T>(e);
                 if (cbegin >= cend) release(tempty_bar(acc));
                 for (int c0 = cbegin; c0 < cend; c0 += COLS) {
                     const int64_t col = col0 + c0;
@@ -1110,6 +1112,10 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             tmem_ld32(from, r);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                            if (scale != 1.0f) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], scale);
+                            }
                         };
                         load(d + c0 + h * 32, z);
                         if constexpr (DUAL) load(d + 128 + c0, u);

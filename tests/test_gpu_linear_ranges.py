@@ -1,0 +1,128 @@
+"""Linear layers at the ends of their types' ranges, against binary64: gradients far above and far
+below 1, activations far out, sums of a million terms of one sign, binary32 operands far from 1.
+
+The bounds are those of test_gpu_linear.py's docstring, with U = 2^-24, unless a test says more."""
+import numpy as np
+import pytest
+
+from helpers import dev, empty, host
+from quasarml_b200 import abi, datagen
+from test_gpu_linear import ACT, DTYPES, F64, STEP, TINY, U, Case, act64, act_error, backward, d, near
+
+pytestmark = pytest.mark.gpu
+
+
+def check_scaled(c, act, kept, dx, dw, db):
+    """test_gpu_linear.py's check of a binary16 backward pass, but for dz's rounding between its
+    computation and the products: 2^-11 of each element (in two parts 2^-21), or 2^-33 of the
+    largest element of all (dg and du together), whichever is more."""
+    x, dy = c.x.astype(F64), c.dy.astype(F64)
+    z = kept[0].astype(F64)
+    a, g = act64(z, act)
+    ea = act_error(z, act, c.dt)
+    if c.nw == 2:
+        u = kept[1].astype(F64)
+        dz, ez = [dy * u * g, dy * a], [np.abs(dy * u) * 4 * ea, np.abs(dy) * ea]
+    else:
+        dz, ez = [dy * g], [np.abs(dy) * 4 * ea]
+    ez = [e + 4 * U * np.abs(v) for e, v in zip(ez, dz)]
+    for v, e, o in zip(dz, ez, db):
+        near(o, v.sum(0), e.sum(0) + (c.m + 40) * U * np.abs(v).sum(0), "db")
+    floor = 2.0 ** -33 * max(np.abs(v).max() for v in dz)
+    step = 2.0 ** -21 if c.m * c.n <= 65536 else STEP[c.dt]
+    ez = [e + step * (np.abs(v) + e) + floor for e, v in zip(ez, dz)]
+    w = [v.astype(F64) for v in c.w]
+    ref = sum(v @ m.T for v, m in zip(dz, w))
+    mag = sum((np.abs(v) + e) @ np.abs(m).T for v, e, m in zip(dz, ez, w))
+    near(dx, ref, sum(e @ np.abs(m).T for e, m in zip(ez, w)) + (c.nw * c.n + 100) * U * mag, "dx")
+    ax = np.abs(x).T
+    for v, e, o in zip(dz, ez, dw):
+        near(o, x.T @ v, ax @ e + (c.m + 100) * U * (ax @ (np.abs(v) + e)), "dw")
+
+
+def times(a, p):
+    return (a.astype(np.float32) * 2.0 ** p).astype(a.dtype)
+
+
+# dy far above 1 (with x and w small, so that dx and dw are numbers of binary16), far below 1 (with
+# x and w large); dz in two parts, in one, products by pairs of SMs
+@pytest.mark.parametrize("size", [(100, 72, 200), (700, 264, 520), (2200, 136, 2500)])
+@pytest.mark.parametrize("act", ["gelu", "silu", "relu"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("up", [12, 0, -14, -20])
+def test_gradients_far_from_1(ctx, size, act, gated, up):
+    c = Case(*size, np.float16, gated=gated)
+    kept = c.kept()
+    c.dy = times(c.dy, up)
+    if gated and up > 0:
+        kept[1] = times(kept[1], 5)
+    shift = {12: -12, 0: 0, -14: 5, -20: 8}[up]
+    c.x, c.w = times(c.x, shift), [times(w, shift + (3 if up < 0 else 0)) for w in c.w]
+    check_scaled(c, act, kept, *backward(ctx, c, act, kept))
+
+
+@pytest.mark.parametrize("size", [(60, 64, 96), (700, 264, 520)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradients_of_zeros_and_of_one_large_row(ctx, size, gated):
+    """dy 0 but for one row: of ordinary size, or far above the others."""
+    for rest, row in ((0.0, 1.0), (2.0 ** -10, 2.0 ** 11), (0.0, 0.0)):
+        c = Case(*size, np.float16, gated=gated)
+        kept = c.kept()
+        c.dy = (c.dy * np.float16(rest)).astype(np.float16)
+        c.dy[size[0] // 2] = datagen.normal(9, (size[2],), 0, row).astype(np.float16) if row else 0
+        c.x, c.w = times(c.x, -6), [times(w, -6) for w in c.w]
+        check_scaled(c, "silu", kept, *backward(ctx, c, "silu", kept))
+
+
+@pytest.mark.parametrize("size", [(60, 64, 96), (700, 264, 520)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_a_gradient_that_is_no_number_stays_in_its_row(ctx, size, bad):
+    """dx's other rows and dw's other columns are those of the rest, which lies far above 1 or below."""
+    for up in (0, 12, -14):
+        c = Case(*size, np.float16, gated=True)
+        kept = c.kept()
+        c.dy = times(c.dy, up)
+        if up > 0:
+            kept[1] = times(kept[1], 5)
+        c.x, c.w = times(c.x, -up // 2 - 4), [times(w, -up // 2 - 4) for w in c.w]
+        dx, dw, db = backward(ctx, c, "silu", kept)
+        c.dy[7, 11] = bad
+        bx, bw, bb = backward(ctx, c, "silu", kept)
+        rows, cols = np.arange(size[0]) != 7, np.arange(size[2]) != 11
+        assert not np.isfinite(bx[7]).any()
+        assert np.array_equal(bx[rows], dx[rows])
+        for p, q in zip(bw, dw):
+            assert not np.isfinite(p[:, 11]).any()
+            assert np.array_equal(p[:, cols], q[:, cols])
+        for p, q in zip(bb, db):
+            assert not np.isfinite(p[11]) and np.array_equal(p[cols], q[cols])
+
+
+def test_scale_of_a_captured_gradient(ctx):
+    """A captured backward pass finds the scale of each replay's dz, not the capture's."""
+    import torch
+    c = Case(700, 264, 520, np.float16, gated=True)
+    kept = c.kept()
+    c.x, c.w = times(c.x, -12), [times(w, -12) for w in c.w]  # 2^-4 left dw of dz near 2^17 beyond 65504
+    t = [dev(v) for v in (c.x, c.w[0], c.w[1], kept[0], kept[1], c.dy)]
+    out = [empty(s, np.float16) for s in ((c.m, c.k), (c.k, c.n), (c.k, c.n))]
+    db = [empty((c.n,), np.float32) for _ in range(2)]
+    stream, before, graph = torch.cuda.Stream(), ctx.stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    try:
+        ctx.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            ctx.gated_linear_backward(*(d(v) for v in t[:3]), abi.ACT_SILU, *(d(v) for v in t[3:]),
+                                      *(d(v) for v in out), *(d(v) for v in db))
+    finally:
+        torch.cuda.synchronize()
+        ctx.set_stream(before)
+    dy, u = c.dy, kept[1]
+    for up, more in ((0, 0), (12, 5), (-10, 0), (0, 0)):
+        c.dy, kept[1] = times(dy, up), times(u, more)
+        t[5].copy_(torch.from_numpy(c.dy))
+        t[4].copy_(torch.from_numpy(kept[1]))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_scaled(c, "silu", kept, host(out[0]), [host(v) for v in out[1:]], [host(v) for v in db])
