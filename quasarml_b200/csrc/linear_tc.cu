@@ -9,12 +9,15 @@
 // both dims) are copied once to a workspace.
 //
 // binary16: one product, kind::f16, binary32 accumulators; an operand that comes in
-// two parts (its value their sum) is two segments of the sum.
+// two parts (its value their sum) is two segments of the sum.  A tensor-core accumulator
+// is truncated at each step, so one stands for no more than 8192 k: sums of one sign lose
+// 5e-5 of theirs so (measured; with 16384 k 1.0e-4, with 131072 8.4e-4, more than
+// binary16's rounding).  The accumulators of a longer sum are added, to the nearest, in a
+// second one.
 // binary32: x = x0 + x1 + x2 exactly, three bf16 parts of 8 bits each (the upper
 // bits by truncation, so no part overflows and all have x's sign); the six
 // products x_i w_j with i + j <= 2 are formed on the bf16 pipe, the dropped ones
-// being below 3 * 2^-24 |x w|.  A tensor-core accumulator is truncated at each
-// step, so the main product x0 w0 is drained every 256 k into binary32 registers
+// being below 3 * 2^-24 |x w|.  Truncation again: the main product x0 w0 is drained every 256 k into binary32 registers
 // (rounded to nearest there); the other five, 2^-8 of it and less, have an
 // accumulator of their own for the whole sum.  Cost: six times binary16's.
 //
@@ -34,6 +37,7 @@ using namespace tc;
 
 constexpr int TILE_BYTES = 128 * 128;     // one operand tile: 128 rows x 64 k
 constexpr int CHUNK = 4;                  // binary32: k-blocks between drains
+constexpr int LONG = 128;                 // binary16: k-blocks that one accumulator stands for
 constexpr int THREADS = 192;              // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int MAX_SPLIT = 8;              // portable cluster size
 
@@ -66,7 +70,7 @@ template <int NP> struct TcBatch {
 template <bool F32> struct Shape {
     static constexpr int PARTS = F32 ? 3 : 1;
     static constexpr int MAX_SLOTS = F32 ? 6 : 10;
-    static constexpr int TMEM = F32 ? 512 : 128;
+    static constexpr int TMEM = F32 ? 256 : 128;  // columns; twice that for binary32 and long sums
     static constexpr int RING = F32 ? 6 * 32768 : 3 * 32768;
     static constexpr int DEEP_RING = 6 * 32768;
     static constexpr int BARS = 8 * (2 * MAX_SLOTS + 5) + 8;
@@ -88,6 +92,20 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
         : "memory");
+}
+
+// total (or nothing, for the first) + the 32 columns at `from`, each in this thread's lane, to
+// `total`: binary32 additions to the nearest.
+__device__ __forceinline__ void tmem_add32(uint32_t total, uint32_t from, bool first) {
+    uint32_t v[32];
+    tmem_ld32(from, v);
+    if (!first) {
+        uint32_t t[32];
+        tmem_ld32(total, t);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(t[i]), __uint_as_float(v[i])));
+    }
+    tmem_st32(total, v);
 }
 
 // The k16 slice k of a tile: K-major rows of 128 bytes (32 bytes a slice), or
@@ -306,6 +324,9 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         lo = min(max(u0 - seg * g.kb, 0), g.kb);
         hi = min(max(u1 - seg * g.kb, 0), g.kb);
     };
+    // binary16: the accumulators of the CTA's sum, added up behind the first 128 columns
+    const int sums = (u1 - u0 + LONG - 1) / LONG;
+    const uint32_t tmem_cols = F32 || sums > 1 ? 2 * S::TMEM : S::TMEM;
     if (threadIdx.x == 0) {
         for (int s = 0; s < g.slots; ++s) {
             mbar_init(full_bar(s), 1);
@@ -322,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(S::TMEM)
+                     "r"(tmem_cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -404,6 +425,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         bool ok = true;
         const uint32_t small = tmem + 256;  // binary32: the five lesser products
         bool begun = false;
+        int blocks = 0;  // binary16: in the accumulator
         for (int sp = 0; sp < g.segments && ok; ++sp) {
             const int seg = sp / g.halves;
             int lo, hi;
@@ -423,6 +445,17 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                     }
                     const uint32_t d = F32 ? tmem + acc * 128 : tmem;
                     for (int kb = k0; kb < k1 && ok; ++kb) {
+                        if (!F32 && blocks++ == LONG) {
+                            if (issue) mma_commit(tfull_bar(0));
+                            if (!warp_wait(tempty_bar(0), acc_phase, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            acc_phase ^= 1u;
+                            blocks = 1;
+                            begun = false;
+                        }
                         int at[S::PARTS] = {};  // the parts' slots
                         auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
                             const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (slot_bytes >> 4));
@@ -549,13 +582,23 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 }
             }
         } else {
-            done = ready(0, 0);
+            for (int u = 0; u < sums; ++u) {
+                done = ready(0, u & 1);
+                if (!done) break;
+                if (sums > 1) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_add32(lanes + 128 + c * 32, lanes + c * 32, u == 0);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar(0));
+                }
+            }
             if (done && rows_here) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t r[32];
                     float v[32];
-                    tmem_ld32(lanes + c * 32, r);
+                    tmem_ld32(lanes + (sums > 1 ? 128 : 0) + c * 32, r);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                     put(c * 32, v);
@@ -709,7 +752,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
     }
 }
 
@@ -815,6 +858,8 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
     };
     // binary32: drains a tile (the CHUNK k-blocks between them counted by segment)
     const int drains = (g.kb + CHUNK - 1) / CHUNK * g.segments;
+    // binary16: accumulators a tile; where there are several, the second one's columns hold their sum
+    const int sums = (g.kb * g.segments + LONG - 1) / LONG;
     if (warp == 0) {
         const bool issue = elect_one();
         int slot = 0;
@@ -870,6 +915,14 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
             int slot = 0, acc = 0, par = 0;
             uint32_t phase = 0, acc_phase = 0, par_phase = 0;
             bool ok = true;
+            auto next_acc = [&]() {
+                if (!F32 && sums > 1) {
+                    acc_phase ^= 1u;
+                } else if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            };
             for (int t = pair; t < total && ok; t += pairs) {
                 if (F32) {
                     if (!warp_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) break;
@@ -881,6 +934,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     tc_fence_after();
                 }
                 bool begun = false;
+                int blocks = 0;  // binary16: in the accumulator
                 for (int sp = 0; sp < g.segments && ok; ++sp) {
                     const int seg = sp / g.halves;
                     by_order(g.a_mn[seg], g.b_mn[DUAL ? 0 : seg], [&](auto a_mn, auto b_mn) {
@@ -897,6 +951,17 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             }
                             const uint32_t d = tmem + acc * S::NACC;
                             for (int kb = k0; kb < k1 && ok; ++kb) {
+                                if (!F32 && blocks++ == LONG) {
+                                    if (issue) mma_commit_pair(tfull_bar(acc));
+                                    next_acc();
+                                    if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) {
+                                        ok = false;
+                                        break;
+                                    }
+                                    tc_fence_after();
+                                    blocks = 1;
+                                    begun = false;
+                                }
                                 int at[S::PARTS] = {};  // the parts' slots
                                 auto product = [&](int pa, int pb, uint32_t dst, bool fresh) {
                                     const uint64_t as = wa + static_cast<uint32_t>(at[pa] * (S::SLOT >> 4));
@@ -942,10 +1007,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             }
                             if (F32 && ok) {
                                 if (issue) mma_commit_pair(tfull_bar(acc));
-                                if (++acc == 2) {
-                                    acc = 0;
-                                    acc_phase ^= 1u;
-                                }
+                                next_acc();
                             }
                         }
                     });
@@ -953,10 +1015,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 if (!ok) break;
                 if (!F32) {
                     if (issue) mma_commit_pair(tfull_bar(acc));
-                    if (++acc == 2) {
-                        acc = 0;
-                        acc_phase ^= 1u;
-                    }
+                    next_acc();
                 }
                 if (++par == 2) {
                     par = 0;
@@ -986,7 +1045,9 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
             if (lane == 0) mbar_arrive_remote(map_to_rank(bar, 0));
         };
         auto next_acc = [&]() {
-            if (++acc == 2) {
+            if (!F32 && sums > 1) {
+                phase ^= 1u;
+            } else if (++acc == 2) {
                 acc = 0;
                 phase ^= 1u;
             }
@@ -1092,7 +1153,17 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 const int rows = max(0, min(32, g.M - row0));
                 const Epilogue& e = g.e;
                 const int vec = e.vec;
-                if (!ready()) break;
+                for (int u = 0; u + 1 < sums && ok; ++u) {
+                    ok = ready();
+                    if (!ok) break;
+                    for (int c0 = cbegin; c0 < cend; c0 += 32) {
+                        tmem_add32(lanes + S::NACC + c0, lanes + c0, u == 0);
+                        if constexpr (DUAL) tmem_add32(lanes + S::NACC + 128 + c0, lanes + 128 + c0, u == 0);
+                    }
+                    release(tempty_bar(0));
+                    next_acc();
+                }
+                if (!ok || !ready()) break;
                 const uint32_t d = lanes + acc * S::NACC;
                 const float scale = scale_of<T>(e);
                 if (cbegin >= cend) release(tempty_bar(acc));
@@ -1112,6 +1183,11 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             tmem_ld32(from, r);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                            if (sums > 1) {
+                                tmem_ld32(from + S::NACC, r);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(__uint_as_float(r[i]), v[i]);
+                            }
                             if (scale != 1.0f) {
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], scale);

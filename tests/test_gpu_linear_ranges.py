@@ -126,3 +126,69 @@ def test_scale_of_a_captured_gradient(ctx):
         graph.replay()
         torch.cuda.synchronize()
         check_scaled(c, "silu", kept, host(out[0]), [host(v) for v in out[1:]], [host(v) for v in db])
+
+
+def uniform(seed, *shape, dt, scale=1.0):
+    """Numbers in [1/2, 1] times scale."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return ((torch.rand(shape, generator=g, device="cuda") * 0.5 + 0.5) * scale).to(dt)
+
+
+def one_sign(out, ref, dt):
+    """The mean relative error of sums of one sign, where roundings to nearest cancel.  A tensor-core
+    accumulator is cut at each step of 8 terms, by less than 2^-23 of it, and stands for at most
+    8192 terms of binary16: 1024 steps, the accumulator half its last value in the mean, 2^-14.
+    binary32's main accumulator stands for 256 terms: 32 steps, 2^-19 at the most, 2^-20 in the mean;
+    that of the lesser products (2^-7 of each operand, so 2^-6 of the sum) for 2048 terms of five products,
+    1280 steps: 2^-6 2^-23 640 = 2^-19.7.  2^-18.8 in all.  A thousandth of 2^-11 for binary16's own roundings,
+    of which there are thousands."""
+    import torch
+    e = float((out.double() / ref - 1).mean())
+    assert abs(e) <= (2.0 ** -14 + 2.0 ** -11 / 64 if dt == torch.float16 else 2.0 ** -18.8), e
+
+
+# few tiles, whose sums are shared out over clusters, and pairs of SMs
+@pytest.mark.parametrize("m,k,n", [(2**20, 64, 72), (2**17, 2048, 2048)])
+@pytest.mark.parametrize("half", [True])
+def test_long_sums_of_one_sign(ctx, m, k, n, half):
+    import torch
+    dt = torch.float16 if half else torch.float32
+    x, dy = uniform(1, m, k, dt=dt), uniform(2, m, n, dt=dt, scale=2.0 ** -5)
+    x *= 2.0 ** -5
+    dw = torch.empty(k, n, dtype=dt, device="cuda")
+    w = torch.zeros(k, n, dtype=dt, device="cuda")
+    ctx.linear_backward(d(x), d(w), abi.ACT_NONE, None, d(dy), None, d(dw))
+    ref = torch.zeros(k, n, dtype=torch.float64, device="cuda")
+    for i in range(0, m, 2**16):
+        ref += x[i:i + 2**16].double().t() @ dy[i:i + 2**16].double()
+    one_sign(dw, ref, dt)
+    # the forward product, of the transposes
+    y = torch.empty(k, n, dtype=dt, device="cuda")
+    ctx.linear(d(x.t()), d(dy), None, abi.ACT_NONE, None, None, d(y))
+    assert torch.equal(y, dw)
+    # two weights
+    gate, up = torch.empty_like(y), torch.empty_like(y)
+    ctx.gated_linear(d(x.t()), d(dy), d(dy), None, None, abi.ACT_RELU, d(gate), d(up), d(y))
+    one_sign(gate, ref, dt)
+    assert torch.equal(gate, up)
+    # more terms than one accumulator takes by one block, and by a part of one
+    for terms in (16384 + 64, 16384 + 3, 3 * 16384 + 100, 2048 + 1, 8192 + 8):
+        ref = x[:terms].double().t() @ dy[:terms].double()
+        ctx.linear_backward(d(x[:terms]), d(w), abi.ACT_NONE, None, d(dy[:terms]), None, d(dw))
+        one_sign(dw, ref, dt)
+
+
+def test_long_sums_of_a_gradient_in_two_parts(ctx):
+    """dz of 40000 rows of one column, kept in two parts: both are in the sum."""
+    import torch
+    m, k, n = 40000, 16, 1
+    x, dy = uniform(1, m, k, dt=torch.float16), uniform(2, m, n, dt=torch.float16)
+    pre = uniform(3, m, n, dt=torch.float16)
+    w, dw, db = torch.ones(k, n, dtype=torch.float16, device="cuda"), empty((k, n), np.float16), empty((n,), np.float32)
+    ctx.linear_backward(d(x), d(w), abi.ACT_SIGMOID, d(pre), d(dy), None, d(dw), d(db))
+    p = torch.sigmoid(pre.double())
+    dz = dy.double() * p * (1 - p)
+    ref = x.double().t() @ dz
+    assert torch.all((dw.double() / ref - 1).abs() <= 2.0 ** -11 + 2.0 ** -13)
+    assert torch.all((db.double() / dz.sum(0) - 1).abs() <= 2.0 ** -18)
