@@ -19,7 +19,8 @@
 // products x_i w_j with i + j <= 2 are formed on the bf16 pipe, the dropped ones
 // being below 3 * 2^-24 |x w|.  Truncation again: the main product x0 w0 is drained every 256 k into binary32 registers
 // (rounded to nearest there); the other five, 2^-8 of it and less, have an
-// accumulator of their own for the whole sum.  Cost: six times binary16's.
+// accumulator of their own, drained every 2048 k: sums of one sign lose 3e-7 of theirs
+// (measured at 131072 k, where one accumulator for the whole sum lost 1.9e-5).  Cost: six times binary16's.
 //
 // k_linear_tc: 128 x 128 of the result a CTA (64 columns of each weight for a dual
 // product).  Where the tiles do not fill the GPU, a cluster of up to 8 CTAs splits
@@ -37,6 +38,8 @@ using namespace tc;
 
 constexpr int TILE_BYTES = 128 * 128;     // one operand tile: 128 rows x 64 k
 constexpr int CHUNK = 4;                  // binary32: k-blocks between drains
+constexpr int LESSER = 8;                 // binary32: drains of the main product to one of the lesser ones
+static_assert(LESSER >= 2, "two columns of lesser products in turn");
 constexpr int LONG = 128;                 // binary16: k-blocks that one accumulator stands for
 constexpr int THREADS = 192;              // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int MAX_SPLIT = 8;              // portable cluster size
@@ -423,7 +426,8 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
         int slot = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        const uint32_t small = tmem + 256;  // binary32: the five lesser products
+        uint32_t small = tmem + 256;  // binary32: the five lesser products, here or 128 columns on
+        int drains = 0;               // of the main product, since the lesser ones' last
         bool begun = false;
         int blocks = 0;  // binary16: in the accumulator
         for (int sp = 0; sp < g.segments && ok; ++sp) {
@@ -442,6 +446,13 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                             break;
                         }
                         tc_fence_after();
+                        // the lesser products' other columns have been read: the wait above was for a
+                        // later drain than theirs
+                        if (drains++ == LESSER) {
+                            small ^= (tmem + 256) ^ (tmem + 384);
+                            drains = 1;
+                            begun = false;
+                        }
                     }
                     const uint32_t d = F32 ? tmem + acc * 128 : tmem;
                     for (int kb = k0; kb < k1 && ok; ++kb) {
@@ -543,8 +554,17 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
             for (int c = 0; c < 4; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
-            int acc = 0;
+            int acc = 0, lesser = 0, since = 0;
             uint32_t phase = 0;
+            auto add = [&](uint32_t from) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(from + c * 32, r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
+                }
+            };
             int drains = 0;  // as the MMA warp's loops make them
             for (int seg = 0; seg < g.segments; ++seg) {
                 int lo, hi;
@@ -552,17 +572,16 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 drains += (hi - lo + CHUNK - 1) / CHUNK;
             }
             for (int u = 0; u < drains; ++u) {
+                if (since++ == LESSER) {
+                    add(lanes + 256 + lesser * 128);
+                    lesser ^= 1;
+                    since = 1;
+                }
                 if (!ready(acc, phase)) {
                     done = false;
                     break;
                 }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(lanes + acc * 128 + c * 32, r);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
-                }
+                add(lanes + acc * 128);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty_bar(acc));
@@ -572,14 +591,9 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
                 }
             }
             if (done && rows_here) {
+                add(lanes + 256 + lesser * 128);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(lanes + 256 + c * 32, r);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
-                    put(c * 32, sum[c]);
-                }
+                for (int c = 0; c < 4; ++c) put(c * 32, sum[c]);
             }
         } else {
             for (int u = 0; u < sums; ++u) {
@@ -762,7 +776,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 //   binary16: 256 x 256 of the result a pair (dual: 128 columns of each weight, one
 //     from each CTA), six stages of 32 KiB a CTA, two accumulators of 256 columns;
 //   binary32: 256 x 128 (dual: 64 of each), eight slots of one part (24 KiB a CTA), two
-//     accumulators for the drains of the main product and two, by tile, for the lesser
+//     accumulators for the drains of the main product and two, in turn, for the lesser
 //     ones.
 // Each CTA loads its own 128 rows of A and half of the tile's columns of B; the
 // leader issues the MMAs of both.  Roles and barriers as in k_linear_tc, the
@@ -923,12 +937,19 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     acc_phase ^= 1u;
                 }
             };
+            auto next_par = [&]() {
+                if (++par == 2) {
+                    par = 0;
+                    par_phase ^= 1u;
+                }
+            };
             for (int t = pair; t < total && ok; t += pairs) {
                 if (F32) {
                     if (!warp_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) break;
                     tc_fence_after();
                 }
-                const uint32_t small = tmem + 256 + par * 128;
+                uint32_t small = tmem + 256 + par * 128;
+                int since = 0;  // binary32: drains of the main product since the lesser ones' last
                 if (!F32) {
                     if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, limit)) break;
                     tc_fence_after();
@@ -948,6 +969,17 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                                     break;
                                 }
                                 tc_fence_after();
+                                if (since++ == LESSER) {  // as at a tile's end
+                                    next_par();
+                                    if (!warp_wait(sempty_bar(par), par_phase ^ 1u, abort_flag, limit)) {
+                                        ok = false;
+                                        break;
+                                    }
+                                    tc_fence_after();
+                                    small = tmem + 256 + par * 128;
+                                    since = 1;
+                                    begun = false;
+                                }
                             }
                             const uint32_t d = tmem + acc * S::NACC;
                             for (int kb = k0; kb < k1 && ok; ++kb) {
@@ -1017,10 +1049,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     if (issue) mma_commit_pair(tfull_bar(acc));
                     next_acc();
                 }
-                if (++par == 2) {
-                    par = 0;
-                    par_phase ^= 1u;
-                }
+                next_par();
             }
             if (issue) mma_commit_pair_local(drain_bar);
             const long long t0 = clock64();
@@ -1119,7 +1148,13 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                         for (int i = 0; i < 32; ++i) sum[c][i] = __fadd_rn(sum[c][i], __uint_as_float(r[i]));
                     }
                 };
+                auto drain_lesser = [&]() {
+                    drain(lanes + 256 + par * 128);
+                    release(sempty_bar(par));
+                    par ^= 1;
+                };
                 for (int u = 0; u < drains; ++u) {
+                    if (u > 0 && u % LESSER == 0) drain_lesser();
                     if (!ready()) {
                         ok = false;
                         break;
@@ -1129,9 +1164,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     next_acc();
                 }
                 if (!ok) break;
-                drain(lanes + 256 + par * 128);
-                release(sempty_bar(par));
-                par ^= 1;
+                drain_lesser();
 #pragma unroll
                 for (int round = 0; round < 2; ++round) {
                     if (cbegin + round * STEP >= cend) break;

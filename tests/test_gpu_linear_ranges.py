@@ -150,7 +150,7 @@ def one_sign(out, ref, dt):
 
 # few tiles, whose sums are shared out over clusters, and pairs of SMs
 @pytest.mark.parametrize("m,k,n", [(2**20, 64, 72), (2**17, 2048, 2048)])
-@pytest.mark.parametrize("half", [True])
+@pytest.mark.parametrize("half", [False, True])
 def test_long_sums_of_one_sign(ctx, m, k, n, half):
     import torch
     dt = torch.float16 if half else torch.float32
