@@ -278,6 +278,12 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ int ld_cluster1(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float lds1(uint32_t addr) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -626,7 +632,13 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
     if (g.splits > 1) cluster_arrive_wait();
     else __syncthreads();
     tc_fence_after();
-    if (!*abort_flag) {
+    // a tile is whole if no CTA of the cluster gave up: the others' sums lack its part
+    bool gave_up = *abort_flag != 0;
+    if (g.splits > 1) {
+        const uint32_t flag = bars + 8u * (2 * S::MAX_SLOTS + 5) + 4;
+        gave_up = __any_sync(0xffffffffu, ld_cluster1(map_to_rank(flag, lane < g.splits ? lane : 0)));
+    }
+    if (!gave_up) {
         const int rows = min(128, g.M - mt * 128);
         const int64_t row0 = static_cast<int64_t>(mt) * 128, col0 = static_cast<int64_t>(nt) * BN;
         const float scale = scale_of<T>(g.e);
