@@ -133,6 +133,8 @@ template <typename T, int N> __device__ __forceinline__ void act_all(int act, fl
 // act(z) and its derivative.  With p the sigmoid:
 //   silu' = p + z p (1 - p);  sigmoid' = p (1 - p);
 //   gelu' = p + z p (1 - p) 2 v',  2 v' = 2 s (1 + 3 c z^2).
+// sigmoid' is even: taken at -|z|, where p is the small factor and 1 - p loses nothing (at
+// z = 12 1 - p has 7 bits left).  In the others p itself is beside the product there.
 template <typename T> __device__ __forceinline__ P2 act_grad2(int act, P2 z, P2& value) {
     const P2 one = both(1.0f);
     switch (act) {
@@ -154,9 +156,11 @@ template <typename T> __device__ __forceinline__ P2 act_grad2(int act, P2 z, P2&
             return fma2(value, fma2(p, both(-1.0f), one), p);
         }
         case QSML_ACT_SIGMOID: {
-            const P2 p = act_sigmoid2<T>(z);
-            value = p;
-            return mul2(p, fma2(p, both(-1.0f), one));
+            const float2 f = unpack(z);
+            const P2 p = act_sigmoid2<T>(pack(-fabsf(f.x), -fabsf(f.y))), q = fma2(p, both(-1.0f), one);
+            const float2 pf = unpack(p), qf = unpack(q);
+            value = pack(f.x > 0.0f ? qf.x : pf.x, f.y > 0.0f ? qf.y : pf.y);
+            return mul2(p, q);
         }
     }
     value = z;

@@ -128,6 +128,33 @@ def test_scale_of_a_captured_gradient(ctx):
         check_scaled(c, "silu", kept, host(out[0]), [host(v) for v in out[1:]], [host(v) for v in db])
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+def test_sigmoid_gradient_far_out(ctx, dt, gated):
+    """sigmoid'(z) = p (1 - p) to a relative error, on both sides: exp carries a few u, binary16's fast
+    one 2^-21 and 2^-24 |z| of its argument, and the sum and products 4 u more.  One row, so that the
+    binary32 bias gradient is dz itself."""
+    z = np.concatenate([np.linspace(-16, 16, 201), [-30.0, 30.0, -80.0, 80.0]])[None, :].astype(dt)
+    n = z.shape[1]
+    up = np.full((1, n), 3.0, dt)
+    dy = np.full((1, n), 0.5, dt)
+    x, w = np.ones((1, 8), dt), np.ones((8, n), dt)
+    t = [dev(v) for v in (x, w, w, z, up, dy)]
+    db = [empty((n,), np.float32) for _ in range(2)]
+    if gated:
+        ctx.gated_linear_backward(*(d(v) for v in t[:3]), abi.ACT_SIGMOID, *(d(v) for v in t[3:]), None, None, None,
+                                  d(db[0]), d(db[1]))
+    else:
+        ctx.linear_backward(d(t[0]), d(t[1]), abi.ACT_SIGMOID, d(t[3]), d(t[5]), None, None, d(db[0]))
+    z = z[0].astype(F64)
+    p, q = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))
+    rel = 12 * U if dt == np.float32 else 2.0 ** -20 + 2.0 ** -23 * np.abs(z)
+    want = p * q * (1.5 if gated else 0.5)
+    assert np.all(np.abs(host(db[0]) - want) <= rel * want + 2.0 ** -126)
+    if gated:
+        assert np.all(np.abs(host(db[1]) - 0.5 * p) <= rel * p + 2.0 ** -126)
+
+
 def uniform(seed, *shape, dt, scale=1.0):
     """Numbers in [1/2, 1] times scale."""
     import torch
