@@ -144,7 +144,12 @@ template <typename T> __device__ __forceinline__ P2 act_grad2(int act, P2 z, P2&
             return pack(f.x != f.x ? f.x : (f.x > 0.0f ? 1.0f : 0.0f), f.y != f.y ? f.y : (f.y > 0.0f ? 1.0f : 0.0f));
         }
         case QSML_ACT_GELU: {
-            const P2 q = mul2(z, z), s2 = both(2.0f * kGeluS);
+            P2 q = mul2(z, z);
+            const P2 s2 = both(2.0f * kGeluS);
+            if constexpr (sizeof(T) == 4) {  // from 1e19 on z z is infinite, and 0 times that no number
+                const float2 f = unpack(q);
+                q = pack(fminf(f.x, 0x1p96f), fminf(f.y, 0x1p96f));
+            }
             const P2 p = act_sigmoid2<T>(mul2(mul2(s2, z), fma2(both(kGeluC), q, one)));
             value = mul2(z, p);
             const P2 dv = mul2(s2, fma2(both(3.0f * kGeluC), q, one));

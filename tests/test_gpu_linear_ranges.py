@@ -155,6 +155,16 @@ def test_sigmoid_gradient_far_out(ctx, dt, gated):
         assert np.all(np.abs(host(db[1]) - 0.5 * p) <= rel * p + 2.0 ** -126)
 
 
+def test_gelu_gradient_far_out(ctx):
+    """gelu' of a binary32 number whose square is beyond binary32 is 1 or 0."""
+    z = np.array([[1e18, 2e19, 1e30, 3e38, -1e18, -2e19, -1e30, -3e38, 1e10, -1e10]], np.float32)
+    n = z.shape[1]
+    t = [dev(v) for v in (np.ones((1, 4), np.float32), np.ones((4, n), np.float32), z, np.full((1, n), 2, np.float32))]
+    db = empty((n,), np.float32)
+    ctx.linear_backward(d(t[0]), d(t[1]), abi.ACT_GELU, d(t[2]), d(t[3]), None, None, d(db))
+    assert np.array_equal(host(db), np.where(z[0] > 0, 2, 0))
+
+
 def uniform(seed, *shape, dt, scale=1.0):
     """Numbers in [1/2, 1] times scale."""
     import torch
