@@ -413,9 +413,10 @@ QSML_API qsml_status_t qsml_matmul(qsml_ctx* ctx, const qsml_tdesc* a, const qsm
  * F16 and QSML_MM_FP32_FFMA for F32 (CUDA-core fma).  F32 under QSML_MM_AUTO runs
  * on the tensor cores as three bf16 parts of each operand (exact) and six of
  * their nine products, the others being below 2^-22 of |x| |w|: binary32
- * accuracy for finite operands, but an infinite operand gives NaN where the
- * CUDA cores give an infinity; a few rows (16, or 8 of a gated layer) run on
- * the CUDA cores.
+ * accuracy for finite operands (below 2^-110 they lose bits), but an infinite
+ * operand gives NaN, where the CUDA cores give an infinity, beside one whose
+ * lower parts are 0 (a whole number, say); a few rows (16, or 8 of a gated
+ * layer) run on the CUDA cores.
  * With no rows nothing is written; with K = 0 the products are 0.  Operands that
  * TMA cannot read (F32, a row pitch or start off 16 bytes, strides in both dims)
  * are copied once a call to a workspace, taken as qsml_layer_norm_backward takes

@@ -16,8 +16,10 @@
 // second one.
 // binary32: x = x0 + x1 + x2 exactly, three bf16 parts of 8 bits each (the upper
 // bits by truncation, so no part overflows and all have x's sign); the six
-// products x_i w_j with i + j <= 2 are formed on the bf16 pipe, the dropped ones
-// being below 3 * 2^-24 |x w|.  Truncation again: the main product x0 w0 is drained every 256 k into binary32 registers
+// products x_i w_j with i + j <= 2 are formed on the bf16 pipe.  x1 is below 2^-7 |x| and
+// x2 below 2^-15 |x|, so the dropped ones are below 2^-21 |x w| together (7.83 * 2^-24 at
+// x = w = 1 + 2^-7 - 2^-23); they have the product's sign, so that sums of one sign lose
+// 0.7 * 2^-24 of theirs in the mean.  The accumulators are truncated here too: the main product x0 w0 is drained every 256 k into binary32 registers
 // (rounded to nearest there); the other five, 2^-8 of it and less, have an
 // accumulator of their own, drained every 2048 k: sums of one sign lose 3e-7 of theirs
 // (measured at 131072 k, where one accumulator for the whole sum lost 1.9e-5).  Cost: six times binary16's.

@@ -229,3 +229,55 @@ def test_long_sums_of_a_gradient_in_two_parts(ctx):
     ref = x.double().t() @ dz
     assert torch.all((dw.double() / ref - 1).abs() <= 2.0 ** -11 + 2.0 ** -13)
     assert torch.all((db.double() / dz.sum(0) - 1).abs() <= 2.0 ** -18)
+
+
+# binary32 products of 17 rows and more run as three bf16 parts of each operand, cut: the parts are below
+# |x|, 2^-7 |x| and 2^-15 |x|.  The dropped x1 w2, x2 w1 and x2 w2 are below 2^-21 |x w| together.
+@pytest.mark.parametrize("rows", [17, 300])
+def test_the_largest_dropped_products(ctx, rows):
+    x = np.full((rows, 1), 1 + 2.0 ** -7 - 2.0 ** -23, np.float32)
+    w = np.full((1, 40), 1 + 2.0 ** -7 - 2.0 ** -23, np.float32)
+    y = empty((rows, 40), np.float32)
+    tx, tw = dev(x), dev(w)
+    ctx.linear(d(tx), d(tw), None, abi.ACT_NONE, None, None, d(y))
+    want = float(x[0, 0]) * float(w[0, 0])
+    assert np.all(np.abs(host(y) - want) <= (2.0 ** -21 + 2 * U) * want)
+
+
+@pytest.mark.parametrize("size", [(1, 300, 40), (100, 300, 200), (300, 520, 136), (2200, 136, 2500)])
+@pytest.mark.parametrize("px,pw", [(-60, 0), (-60, -40), (100, -90), (60, 60), (-100, 90), (-100, 10)])
+def test_binary32_far_from_1(ctx, size, px, pw):
+    """Operands of 2^px and 2^pw, none below 2^-110, so that all three parts are whole."""
+    m, k, n = size
+    x = datagen.normal(1, (m, k), 0, 1).astype(np.float32)
+    w = datagen.normal(2, (k, n), 0, 1).astype(np.float32)
+    x, w = (np.where(np.abs(v) < 2.0 ** -9, 0, v).astype(np.float32) for v in (x, w))
+    x, w = np.ldexp(x, px), np.ldexp(w, pw)
+    tx, tw, y = dev(x), dev(w), empty((m, n), np.float32)
+    ctx.linear(d(tx), d(tw), None, abi.ACT_NONE, None, None, d(y))
+    x, w = x.astype(F64), w.astype(F64)
+    near(host(y), x @ w, (k + 100) * U * (np.abs(x) @ np.abs(w)) + 2.0 ** -126, "y")
+
+
+@pytest.mark.parametrize("rows", [3, 17, 300])
+def test_infinite_binary32_operands(ctx, rows):
+    """An infinite x is an infinity or, beside a w that fewer than three parts hold, no number; it
+    stays in its row.  The CUDA cores give the infinity."""
+    k, n = 24, 40
+    x = datagen.normal(1, (rows, k), 0, 1).astype(np.float32)
+    w = datagen.normal(2, (k, n), 0, 1).astype(np.float32)
+    w[5, ::2] = 1.5
+    want = x.astype(F64) @ w.astype(F64)
+    x[1, 5] = np.inf
+    tx, tw = dev(x), dev(w)
+    for precision in (abi.MM_AUTO, abi.MM_FP32_FFMA):
+        y = empty((rows, n), np.float32)
+        ctx.linear(d(tx), d(tw), None, abi.ACT_NONE, None, None, d(y), precision)
+        y = host(y)
+        rest = np.arange(rows) != 1
+        near(y[rest], want[rest], (k + 100) * U * (np.abs(np.where(np.isinf(x), 0, x)) @ np.abs(w))[rest], "y")
+        inf = np.sign(w[5]) * np.inf
+        if rows == 3 or precision == abi.MM_FP32_FFMA:
+            assert np.array_equal(y[1], inf)
+        else:
+            assert np.all(np.isnan(y[1]) | (y[1] == inf)) and not np.isfinite(y[1]).any()
