@@ -274,3 +274,19 @@ def test_refusals(ctx):
     refused(ctx, abi.E_INVALID, d(x), d(g), d(dy), 1e-5, d(dy))
     refused(ctx, abi.E_INVALID, d(x), d(g), d(dy), 1e-5, d(dx), d(dg), d(dg))
     refused(ctx, abi.E_SHAPE, abi.make_desc(g.data_ptr(), abi.F32, ()), d(g), d(dy), 1e-5, None)
+
+
+@pytest.mark.parametrize("shape", [(6, 256), (6, 1001), (6, 4096), (6, 9000)])
+def test_column_sums_of_non_finite_rows(ctx, shape):
+    """A row with an infinite x has no xh, so dgamma is no number anywhere; dbeta is dy's sum and has
+    none only where dy has none."""
+    x, g, dy = make(shape, np.float32)
+    want = run(ctx, x, g, dy)
+    dy[4, 9] = np.nan
+    _, dg, db = run(ctx, x, g, dy)
+    others = np.arange(shape[1]) != 9
+    assert np.isnan(db[9]) and np.array_equal(db[others], want[2][others])
+    x[2, 7] = np.inf
+    _, dg, db = run(ctx, x, g, dy)
+    assert np.isnan(dg).all()
+    assert np.isnan(db[9]) and np.array_equal(db[others], want[2][others])
