@@ -18,8 +18,6 @@
 // 16384 x 2048 with gelu 38 us, 5.3 TB/s; DUAL 8192 x 5632 76 us, 6.1 TB/s).
 #include <cfloat>
 
-#include <cooperative_groups.h>
-
 #include "linear_grad.cuh"
 
 namespace qsml {
@@ -80,6 +78,26 @@ __device__ __forceinline__ float largest(const P2 (&d)[4]) {
     return m;
 }
 
+// The block's writes are seen by all blocks that pass, once all of the grid have come and *arrived
+// is `all`.  False if they do not come within the default limit (the device holds the whole grid,
+// so only where something is wrong).
+__device__ __forceinline__ bool grid_barrier(unsigned* arrived, unsigned all) {
+    int here = 1;
+    if (threadIdx.x == 0) {
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+        const long long t0 = clock64();
+        for (unsigned n = 0;;) {
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(arrived) : "memory");
+            if (static_cast<int>(n - all) >= 0) break;
+            if (clock64() - t0 > kDefaultWaitCycles) {
+                here = 0;
+                break;
+            }
+        }
+    }
+    return __syncthreads_and(here) != 0;
+}
+
 constexpr int kDzExponent = 8;
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -101,7 +119,10 @@ __global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_co
             if (!SCALED || again) return;
             most = block_max(most);
             if (threadIdx.x == 0) a.most[blockIdx.x] = most;
-            cooperative_groups::this_grid().sync();
+            if (!grid_barrier(a.arrived, a.all)) {
+                if (threadIdx.x == 0) atomicExch(a.status, QSML_E_TIMEOUT);
+                return;
+            }
             most = 0.0f;
             for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) most = fmaxf(most, a.most[i]);
             most = block_max(most);
@@ -261,10 +282,23 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
     const bool sums = a.db[0].out || a.db[1].out;
     const size_t partial = sums ? static_cast<size_t>(DUAL ? 2 : 1) * parts * a.N : 0;
     void* memory = nullptr;
-    const size_t floats = partial + (scaled ? grid : 0);
+    const size_t floats = partial + (scaled ? grid + 1 : 0);  // 1: a captured call's barrier
     if (floats) QSML_TRY_STATUS(ws.get(floats * sizeof(float), &memory));
     if (sums) a.partial = static_cast<float*>(memory);
-    if (scaled) a.most = static_cast<float*>(memory) + partial;
+    if (scaled) {
+        a.most = static_cast<float*>(memory) + partial;
+        a.status = ctx->status;
+        // The context's count of arrivals goes on from call to call, which are in stream order; a
+        // captured call may be replayed beside them and counts on its own, from 0.
+        if (ws.captured()) {
+            a.arrived = reinterpret_cast<unsigned*>(a.most + grid);
+            a.all = static_cast<unsigned>(grid);
+            QSML_TRY_STATUS(check_cuda(ctx, cudaMemsetAsync(a.arrived, 0, sizeof(unsigned), ctx->stream), "linear: barrier"));
+        } else {
+            a.arrived = reinterpret_cast<unsigned*>(ctx->status + 4);
+            a.all = ctx->arrivals + static_cast<unsigned>(grid);
+        }
+    }
     bool vec = a.N % 8 == 0 && a.dy_ld % 8 == 0 && aligned16(a.dy);
     for (int i = 0; i < 2; ++i) vec = vec && (!a.pre[i] || aligned16(a.pre[i]));
     // A grid with a barrier has to be on the device whole, whatever else runs there: a cooperative
@@ -284,6 +318,7 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
         if (scaled) kernel = k_linear_dz<T, DUAL, ACT, true>;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, chunk, static_cast<int>(tiles), static_cast<int>(items), vec);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_dz");
+    if (scaled && !ws.captured()) ctx->arrivals = a.all;
     QSML_TRY_STATUS(after_launch(ctx, "k_linear_dz"));
     if (!sums) return QSML_OK;
     ColumnSum s0 = a.db[0], s1 = a.db[1];

@@ -17,7 +17,9 @@ struct GradArgs {
     int64_t plane = 0;                        // > 0: dz in parts `plane` elements apart (Mat::plane)
     float* unscale = nullptr;                 // not null: a binary16 dz is stored times a power of two; 1 / it goes here
     ColumnSum db[2];
-    float *partial = nullptr, *most = nullptr;  // workspace of the launch: column sums by part, the CTAs' largest |dz|
+    float *partial = nullptr, *most = nullptr;  // workspace of the launch: column sums by part, the CTAs' largest |dz|,
+    unsigned *arrived = nullptr, all = 0;       // the count of CTAs at the barrier, and what it is when all are
+    int* status = nullptr;
 };
 
 template <typename T> qsml_status_t run_grad(Context* ctx, const GradArgs& a, bool dual);

@@ -59,8 +59,11 @@ struct Context {
     // Device word where kernels with bounded waits report QSML_E_TIMEOUT;
     // qsml_synchronize reads and clears it.  Layout of the 256-byte block:
     // int at [0] the status code; int64 at byte 8 the wait limit in SM
-    // cycles (0 = kDefaultWaitCycles), set with qsml_set_wait_limit.
+    // cycles (0 = kDefaultWaitCycles), set with qsml_set_wait_limit; unsigned
+    // at byte 16 the CTAs that have come to a grid barrier since the context
+    // was made (modulo 2^32), of which `arrivals` are enqueued.
     int* status = nullptr;
+    unsigned arrivals = 0;
     // Overlap of independent reductions on the stream (qsml_set_overlap) and
     // the launch count the last plan_launch was made for.
     bool overlap = false;

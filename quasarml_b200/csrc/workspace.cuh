@@ -29,6 +29,8 @@ public:
     Workspace& operator=(const Workspace&) = delete;
     // `bytes` bytes at *ptr, 256-byte aligned; at most kMax blocks a call.
     qsml_status_t get(size_t bytes, void** ptr);
+    // Whether the last block belongs to a graph.
+    bool captured() const { return n_ > 0 && captured_[n_ - 1]; }
 
 private:
     static constexpr int kMax = 12;
