@@ -219,7 +219,7 @@ __device__ __forceinline__ float warp_sum3(const float (&v)[3]) {
     return r;
 }
 
-constexpr int kMaxSlots = 4;
+constexpr int kSlots = 2;  // two rows in flight a CTA (about four CTAs a SM)
 
 // PV elements a load, NV loads a thread; FULL: the threads' groups are exactly the
 // row's.  slots > 0: rows come through a ring of that many slots of x and dy.
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(PV * NV > 16 ? 256 : 512)
     using C = Cols<T, PV, NV>;
     using V = typename C::V;
     extern __shared__ __align__(16) unsigned char ring[];  // slots x (a row of x, a row of dy), then gamma (WIDE)
-    __shared__ uint64_t bars[kMaxSlots];
+    __shared__ uint64_t bars[kSlots];
     __shared__ float sum1[32], sum3[3][32];  // by warp; those past the last one stay 0
     const int t = threadIdx.x, th = blockDim.x, lane = t & 31, w = t >> 5;
     const int packs = cols / PV;
@@ -664,9 +664,8 @@ qsml_status_t resident(Context* ctx, const void* kernel, int block, size_t smem,
 template <typename T, typename GT, int PV, int NV, bool RING, bool FULL>
 qsml_status_t launch_cta(Context* ctx, const Args& a, int th) {
     auto kernel = k_layer_norm_bwd<T, GT, PV, NV, RING, FULL>;
-    // two rows in flight a CTA (about four CTAs a SM)
     const size_t slot = 2 * static_cast<size_t>(a.cols) * sizeof(T);
-    const int slots = RING ? 2 : 0;
+    const int slots = RING ? kSlots : 0;
     const size_t smem = slots * slot + (PV * NV > 16 ? a.cols * sizeof(float) : 0);
     int per_sm = 0;
     QSML_TRY_STATUS(resident(ctx, reinterpret_cast<const void*>(kernel), th, smem, &per_sm));

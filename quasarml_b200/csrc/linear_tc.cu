@@ -74,7 +74,7 @@ template <int NP> struct TcBatch {
 // 30).
 template <bool F32> struct Shape {
     static constexpr int PARTS = F32 ? 3 : 1;
-    static constexpr int MAX_SLOTS = F32 ? 6 : 10;
+    static constexpr int MAX_SLOTS = 6;
     static constexpr int TMEM = F32 ? 256 : 128;  // columns; twice that for binary32 and long sums
     static constexpr int RING = F32 ? 6 * 32768 : 3 * 32768;
     static constexpr int DEEP_RING = 6 * 32768;
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(THREADS, Shape<F32>::CTAS) k_linear_tc(const _
 // Large products: persistent pairs of SMs (cta_group::2), the epilogue of a tile
 // under the products of the next.
 //   binary16: 256 x 256 of the result a pair (dual: 128 columns of each weight, one
-//     from each CTA), six stages of 32 KiB a CTA, two accumulators of 256 columns;
+//     from each CTA), five slots of 32 KiB a CTA, two accumulators of 256 columns;
 //   binary32: 256 x 128 (dual: 64 of each), eight slots of one part (24 KiB a CTA), two
 //     accumulators for the drains of the main product and two, in turn, for the lesser
 //     ones.
