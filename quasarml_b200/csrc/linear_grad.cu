@@ -12,7 +12,7 @@
 // largest finite |dz| is in [1, 255]: which that is is known at the end, behind a barrier
 // of the grid (with its cooperative launch 7 us of the 165 of a backward pass of 16384 x
 // 1024 x 2048, 2.5 of small ones).  Where it is not, the grid goes over its inputs again, with the s that
-// brings the largest into [2^14, 2^15) (37 us more there, 1.5 at 512 x 1024 x 1024).  Either way an element keeps binary16's 11 bits,
+// brings the largest into [2^14, 2^15) (37 us more there).  Either way an element keeps binary16's 11 bits,
 // or is off by 2^-25 of the scaled numbers' unit, 2^-33 of the largest.
 // Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16:
 // 16384 x 2048 with gelu 38 us, 5.3 TB/s; DUAL 8192 x 5632 76 us, 6.1 TB/s).
@@ -263,14 +263,13 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
     constexpr bool CAN_SCALE = sizeof(T) == 2 && (DUAL || ACT != QSML_ACT_NONE);
     const bool scaled = CAN_SCALE && a.unscale;
     // about eight items an SM, at least 2 rows a warp (8 left most SMs without a CTA at
-    // 515 x 1366: 23 us); a cooperative grid takes whole turns of what the device holds
-    // (16384 x 2048, 1184 items on 444 CTAs: 1.5 us more than 1328)
+    // 515 x 1366: 23 us); as many as the device holds where the grid is cooperative
+    // (16384 x 2048, 440 items: three a CTA took 3 us more)
     int64_t held = 0, parts = (8 * ctx->num_sms + tiles - 1) / tiles;
     if constexpr (CAN_SCALE) {
         if (scaled) {
             QSML_TRY_STATUS((resident<T, DUAL, ACT>(ctx, &held)));
-            const int64_t turns = (8 * ctx->num_sms + held - 1) / held;
-            parts = std::max<int64_t>(1, turns * held / tiles);
+            parts = std::max<int64_t>(1, held / tiles);
         }
     }
     const int64_t most = (a.M + 15) / 16;

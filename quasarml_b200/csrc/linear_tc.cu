@@ -1200,7 +1200,10 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                 const int rows = max(0, min(32, g.M - row0));
                 const Epilogue& e = g.e;
                 const int vec = e.vec;
-                for (int u = 0; u + 1 < sums && ok; ++u) {
+                // several accumulators: each is added to the second's columns, so that the next
+                // tile's products begin under this one's outputs
+                const bool joined = sums > 1;
+                for (int u = 0; joined && u < sums; ++u) {
                     ok = ready();
                     if (!ok) break;
                     for (int c0 = cbegin; c0 < cend; c0 += 32) {
@@ -1210,10 +1213,13 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                     release(tempty_bar(0));
                     next_acc();
                 }
-                if (!ok || !ready()) break;
-                const uint32_t d = lanes + acc * S::NACC;
+                if (!ok || (!joined && !ready())) break;
+                const uint32_t d = lanes + (joined ? 1 : acc) * S::NACC;
+                auto read = [&]() {
+                    if (!joined) release(tempty_bar(acc));
+                };
                 const float scale = scale_of<T>(e);
-                if (cbegin >= cend) release(tempty_bar(acc));
+                if (cbegin >= cend) read();
                 for (int c0 = cbegin; c0 < cend; c0 += COLS) {
                     const int64_t col = col0 + c0;
                     if (!DUAL && e.residual && e.y) {
@@ -1230,11 +1236,6 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                             tmem_ld32(from, r);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                            if (sums > 1) {
-                                tmem_ld32(from + S::NACC, r);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(__uint_as_float(r[i]), v[i]);
-                            }
                             if (scale != 1.0f) {
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], scale);
@@ -1242,7 +1243,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                         };
                         load(d + c0 + h * 32, z);
                         if constexpr (DUAL) load(d + 128 + c0, u);
-                        if (c0 + h * 32 + 32 >= cend) release(tempty_bar(acc));
+                        if (c0 + h * 32 + 32 >= cend) read();
                         add_bias32(e, 0, col + h * 32, z);
                         if constexpr (DUAL) add_bias32(e, 1, col, u);
                         if (e.pre[0]) kept0.put(lane, h, z);
@@ -1267,7 +1268,7 @@ __global__ void __launch_bounds__(PairShape<F32>::THREADS, 1) k_linear_pair(cons
                         kept1.template copy<false>(static_cast<__half*>(e.pre[1]), g.N, col, g.N, row0, rows, vec);
                     __syncwarp();
                 }
-                next_acc();
+                if (!joined) next_acc();
             }
         }
     }
