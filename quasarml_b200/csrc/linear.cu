@@ -217,8 +217,8 @@ qsml_status_t backward(Context* ctx, const char* op, int32_t dtype, int32_t prec
     // binary16: rounding dz to 11 bits adds to dx and dw an error of the size of their own
     // rounding (1.4 times the error in all, however long the sums).  A dz of up to 2^16
     // elements is kept in two parts, 22 bits, which costs little there (256 x 256 x 256:
-    // 12 us, in one part 10).  Beyond, it costs more than the bits are worth (512 x 1024 x
-    // 1024: 16 us for 13; 16384 x 1024 x 2048: 262 for 152).
+    // 16 us, in one part 13).  Beyond, it costs more than the bits are worth (512 x 1024 x
+    // 1024: 20 us for 17; 16384 x 1024 x 2048: 271 for 157).
     // Without an activation dz = dy and needs no copy, binary32's split apart.
     // What binary16's dz lacks in range a power of two makes good (linear_grad.cu).
     const bool exact = act == QSML_ACT_NONE && nw == 1;

@@ -10,12 +10,13 @@
 // bits where a sum of many is an ordinary number.  s is one number for the whole of dz
 // (dg and du), since dx sums over its columns and dw over its rows.  It is 2^8 where the
 // largest finite |dz| is in [1, 255]: which that is is known at the end, behind a barrier
-// of the grid (with its cooperative launch 7 us of the 165 of a backward pass of 16384 x
-// 1024 x 2048, 2.5 of small ones).  Where it is not, the grid goes over its inputs again, with the s that
-// brings the largest into [2^14, 2^15) (37 us more there).  Either way an element keeps binary16's 11 bits,
-// or is off by 2^-25 of the scaled numbers' unit, 2^-33 of the largest.
+// of the grid or, where few CTAs do, of a cluster (7 us of the 164 of a backward pass of
+// 16384 x 1024 x 2048; of small ones, back to back, 4 with the grid's cooperative launch and
+// 2 with a cluster).  Where it is not, the CTAs go over their inputs again, with the s that
+// brings the largest into [2^14, 2^15) (37 us more there).  Either way an element keeps
+// binary16's 11 bits, or is off by 2^-25 of the scaled numbers' unit, 2^-33 of the largest.
 // Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16:
-// 16384 x 2048 with gelu 38 us, 5.3 TB/s; DUAL 8192 x 5632 76 us, 6.1 TB/s).
+// 16384 x 2048 with gelu 45 us, 4.5 TB/s; DUAL 8192 x 5632 79 us, 5.8 TB/s).
 #include <cfloat>
 
 #include "linear_grad.cuh"
@@ -104,7 +105,7 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // An item is 256 columns (8 a lane) by `chunk` rows, a CTA's 8 warps taking every 8th row;
 // items go round the grid, columns first.  A thread keeps its columns and sums them in
 // registers; the warps' sums are added in warp order in shared memory.
-// SCALED: dz times a power of two (above); the grid is cooperative.
+// SCALED: dz times a power of two (above); the grid is cooperative, or one cluster (no `arrived`).
 template <typename T, bool DUAL, int ACT, bool SCALED>
 __global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, int tiles, int items,
                                                    bool vec) {
@@ -119,7 +120,10 @@ __global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_co
             if (!SCALED || again) return;
             most = block_max(most);
             if (threadIdx.x == 0) a.most[blockIdx.x] = most;
-            if (!grid_barrier(a.arrived, a.all)) {
+            bool met = true;
+            if (a.arrived) met = grid_barrier(a.arrived, a.all);
+            else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+            if (!met) {
                 if (threadIdx.x == 0) atomicExch(a.status, QSML_E_TIMEOUT);
                 return;
             }
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_co
             for (int j = 0; j < 4; ++j) sum[o][j].v = 0;
         if (n > 0) {
             // AHEAD rows in flight under the one at hand: as many as leave two CTAs a SM, three
-            // LINEAR ones of binary16 (DUAL binary16 8192 x 5632: 88, 79, 76 us with 1, 2, 3;
+            // LINEAR ones of binary16 (DUAL binary16 8192 x 5632, not scaled: 88, 79, 76 us with 1, 2, 3;
             // binary32 8192 x 4096: 128 us with 1, 171 with 2)
             constexpr int AHEAD = sizeof(T) == 4 ? 1 : DUAL ? 3 : 2;
             constexpr bool PRE = DUAL || ACT != QSML_ACT_NONE;
@@ -256,6 +260,8 @@ template <typename T, bool DUAL, int ACT> qsml_status_t resident(Context* ctx, i
     return QSML_OK;
 }
 
+constexpr int64_t MAX_CLUSTER = 8;  // portable
+
 template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx, const GradArgs& given) {
     GradArgs a = given;
     const int64_t tiles = (a.N + 255) / 256;
@@ -266,13 +272,18 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
     // 515 x 1366: 23 us); as many as the device holds where the grid is cooperative
     // (16384 x 2048, 440 items: three a CTA took 3 us more)
     int64_t held = 0, parts = (8 * ctx->num_sms + tiles - 1) / tiles;
-    if constexpr (CAN_SCALE) {
-        if (scaled) {
-            QSML_TRY_STATUS((resident<T, DUAL, ACT>(ctx, &held)));
-            parts = std::max<int64_t>(1, held / tiles);
-        }
-    }
     const int64_t most = (a.M + 15) / 16;
+    // few items: one cluster, whose barrier needs no cooperative launch and none of its 2 us
+    // (64 x 256 x 1024, 16 items, the whole pass: 15.5 us for 17.0; 32 items: 17.5 for 17.0)
+    const bool cluster = scaled && tiles * most <= 16;
+    if constexpr (CAN_SCALE) {
+        if (cluster) {
+            held = MAX_CLUSTER;
+        } else if (scaled) {
+            QSML_TRY_STATUS((resident<T, DUAL, ACT>(ctx, &held)));
+        }
+        if (scaled) parts = std::max<int64_t>(1, held / tiles);
+    }
     if (parts > most) parts = most;
     const int64_t chunk = (a.M + parts - 1) / parts;
     parts = (a.M + chunk - 1) / chunk;
@@ -281,7 +292,7 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
     const bool sums = a.db[0].out || a.db[1].out;
     const size_t partial = sums ? static_cast<size_t>(DUAL ? 2 : 1) * parts * a.N : 0;
     void* memory = nullptr;
-    const size_t floats = partial + (scaled ? grid + 1 : 0);  // 1: a captured call's barrier
+    const size_t floats = partial + (scaled ? grid + 1 : 0);  // 1: a captured cooperative call's barrier
     if (floats) QSML_TRY_STATUS(ws.get(floats * sizeof(float), &memory));
     if (sums) a.partial = static_cast<float*>(memory);
     if (scaled) {
@@ -289,11 +300,11 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
         a.status = ctx->status;
         // The context's count of arrivals goes on from call to call, which are in stream order; a
         // captured call may be replayed beside them and counts on its own, from 0.
-        if (ws.captured()) {
+        if (!cluster && ws.captured()) {
             a.arrived = reinterpret_cast<unsigned*>(a.most + grid);
             a.all = static_cast<unsigned>(grid);
             QSML_TRY_STATUS(check_cuda(ctx, cudaMemsetAsync(a.arrived, 0, sizeof(unsigned), ctx->stream), "linear: barrier"));
-        } else {
+        } else if (!cluster) {
             a.arrived = reinterpret_cast<unsigned*>(ctx->status + 4);
             a.all = ctx->arrivals + static_cast<unsigned>(grid);
         }
@@ -303,21 +314,25 @@ template <typename T, bool DUAL, int ACT> qsml_status_t launch_act(Context* ctx,
     // A grid with a barrier has to be on the device whole, whatever else runs there: a cooperative
     // launch, which does not begin before the kernel ahead of it has ended.
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = scaled ? cudaLaunchAttributeCooperative : cudaLaunchAttributeProgrammaticStreamSerialization;
-    if (scaled) attr[0].val.cooperative = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = a.arrived ? cudaLaunchAttributeCooperative : cudaLaunchAttributeProgrammaticStreamSerialization;
+    if (a.arrived) attr[0].val.cooperative = 1;
     else attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(grid);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(256);
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster && grid > 1 ? 2 : 1;
     auto kernel = k_linear_dz<T, DUAL, ACT, false>;
     if constexpr (CAN_SCALE)
         if (scaled) kernel = k_linear_dz<T, DUAL, ACT, true>;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, chunk, static_cast<int>(tiles), static_cast<int>(items), vec);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_linear_dz");
-    if (scaled && !ws.captured()) ctx->arrivals = a.all;
+    if (a.arrived && !ws.captured()) ctx->arrivals = a.all;
     QSML_TRY_STATUS(after_launch(ctx, "k_linear_dz"));
     if (!sums) return QSML_OK;
     ColumnSum s0 = a.db[0], s1 = a.db[1];

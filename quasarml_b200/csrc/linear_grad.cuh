@@ -18,7 +18,7 @@ struct GradArgs {
     float* unscale = nullptr;                 // not null: a binary16 dz is stored times a power of two; 1 / it goes here
     ColumnSum db[2];
     float *partial = nullptr, *most = nullptr;  // workspace of the launch: column sums by part, the CTAs' largest |dz|,
-    unsigned *arrived = nullptr, all = 0;       // the count of CTAs at the barrier, and what it is when all are
+    unsigned *arrived = nullptr, all = 0;       // the count of CTAs at the grid's barrier, and what it is when all are
     int* status = nullptr;
 };
 

@@ -1598,10 +1598,10 @@ template <bool F32, bool DUAL> qsml_status_t launch_one(Context* ctx, const TcAr
 
 // Products in one launch where that is reckoned to take less than one after another:
 // each alone splits its sums to fill the GPU, and has a beginning and an end of its own,
-// which cost about ALONE blocks' time (backward 512 x 1024 x 1024, binary16: 20 us in
-// two launches, 14 in one; with two weights 2048 x 512 x 512: 27 and 16; binary32 777 x
+// which cost about ALONE blocks' time (backward 512 x 1024 x 1024, binary16, gelu: 25 us
+// in two launches, 17 in one; with two weights 2048 x 512 x 512: 33 and 21; binary32 777 x
 // 1024 x 1000: 45 and 35; but binary16 8192 x 256 x 512, with sums of 8 and of 128
-// blocks: 27 and 32; with two weights 1024 x 1024 x 1024, more CTAs than SMs: 27 and 31).
+// blocks: 33 and 37; with two weights 1024 x 1024 x 1024, more CTAs than SMs: 33 and 35).
 // `apart`: the cost of the launches it replaces, but for ALONE.
 template <bool F32, int NP>
 qsml_status_t launch_together(Context* ctx, const TcArgs* const (&g)[NP], int64_t apart, bool* launched) {
