@@ -439,9 +439,9 @@ QSML_API qsml_status_t qsml_linear(qsml_ctx* ctx, const qsml_tdesc* x, const qsm
  * 2^16 elements (smaller ones keep 22 bits), which makes the error of dx and dw
  * about 1.4 times that of their own rounding.  It is scaled by a power of two for
  * that, so dz may lie far beyond F16's range: an element keeps those bits or is off
- * by 2^-33 of the largest one (of dg and du together).  dbias is summed before.  With no rows dw and
- * dbias are 0.  relu' is 0 at 0.  No reference counterpart (it has no
- * gradients). */
+ * by 2^-33 of the largest one (of dg and du together).  dbias is summed before.
+ * With no rows dw and dbias are 0.  relu' is 0 at 0.  No reference counterpart (it
+ * has no gradients). */
 QSML_API qsml_status_t qsml_linear_backward(qsml_ctx* ctx, const qsml_tdesc* x, const qsml_tdesc* w, int32_t act,
                                             const qsml_tdesc* pre, const qsml_tdesc* dy, const qsml_tdesc* dx,
                                             const qsml_tdesc* dw, const qsml_tdesc* dbias, int32_t precision);

@@ -8,11 +8,11 @@
 // binary16's dz is stored times a power of two s, which the products' epilogue undoes:
 // dy u can be far beyond binary16 where dx and dw are not, and a small dz is held in few
 // bits where a sum of many is an ordinary number.  s is one number for the whole of dz
-// (dg and du), since dx sums over its columns and dw over its rows.  It is 2^8 where the
-// largest finite |dz| is in [1, 255]: which that is is known at the end, behind a barrier
-// of the grid or, where few CTAs do, of a cluster (7 us of the 164 of a backward pass of
+// (dg and du), since dx sums over its columns and dw over its rows.  It is 2^8 if
+// the largest finite |dz| turns out to be in [1, 255], which is known behind a barrier of
+// the grid or, where few CTAs do, of a cluster (7 us of the 164 of a backward pass of
 // 16384 x 1024 x 2048; of small ones, back to back, 4 with the grid's cooperative launch and
-// 2 with a cluster).  Where it is not, the CTAs go over their inputs again, with the s that
+// 2 with a cluster).  If not, the CTAs go over their inputs again, with the s that
 // brings the largest into [2^14, 2^15) (37 us more there).  Either way an element keeps
 // binary16's 11 bits, or is off by 2^-25 of the scaled numbers' unit, 2^-33 of the largest.
 // Bound by HBM: LINEAR reads 2 and writes 1 element, DUAL reads 3 and writes 2 (binary16:
@@ -107,8 +107,8 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // registers; the warps' sums are added in warp order in shared memory.
 // SCALED: dz times a power of two (above); the grid is cooperative, or one cluster (no `arrived`).
 template <typename T, bool DUAL, int ACT, bool SCALED>
-__global__ void __launch_bounds__(256, DUAL ? 2 : 3) k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, int tiles, int items,
-                                                   bool vec) {
+__global__ void __launch_bounds__(256, DUAL ? 2 : 3)
+    k_linear_dz(const __grid_constant__ GradArgs a, int64_t chunk, int tiles, int items, bool vec) {
     pdl_begin();
     constexpr int NO = DUAL ? 2 : 1;
     __shared__ float fold[NO][8][256 + 8];

@@ -19,10 +19,11 @@
 // products x_i w_j with i + j <= 2 are formed on the bf16 pipe.  x1 is below 2^-7 |x| and
 // x2 below 2^-15 |x|, so the dropped ones are below 2^-21 |x w| together (7.83 * 2^-24 at
 // x = w = 1 + 2^-7 - 2^-23); they have the product's sign, so that sums of one sign lose
-// 0.7 * 2^-24 of theirs in the mean.  The accumulators are truncated here too: the main product x0 w0 is drained every 256 k into binary32 registers
-// (rounded to nearest there); the other five, 2^-8 of it and less, have an
-// accumulator of their own, drained every 2048 k: sums of one sign lose 3e-7 of theirs
-// (measured at 131072 k, where one accumulator for the whole sum lost 1.9e-5).  Cost: six times binary16's.
+// 0.7 * 2^-24 of theirs in the mean.  The accumulators are truncated here too: the main
+// product x0 w0 is drained every 256 k into binary32 registers (rounded to nearest
+// there); the other five, 2^-7 of it and less, have an accumulator of their own, drained
+// every 2048 k: sums of one sign lose 3e-7 of theirs (measured at 131072 k, where one
+// accumulator for the whole sum lost 1.9e-5).  Cost: six times binary16's.
 //
 // k_linear_tc: 128 x 128 of the result a CTA (64 columns of each weight for a dual
 // product).  Where the tiles do not fill the GPU, a cluster of up to 8 CTAs splits
