@@ -467,6 +467,95 @@ QSML_API qsml_status_t qsml_gated_linear_backward(qsml_ctx* ctx, const qsml_tdes
                                                   const qsml_tdesc* db_gate, const qsml_tdesc* db_up,
                                                   int32_t precision);
 
+/* ---- attention ----------------------------------------------------------- */
+
+/* Which columns of a head the rotation pairs (qsml_norm_rotary): the first
+ * 2n of them for n frequencies, as (i, n + i) or as (2i, 2i + 1). */
+#define QSML_ROTARY_HALVES 0
+#define QSML_ROTARY_PAIRS 1
+
+/* Norms of queries and keys for each head and the rotation by positions, in one
+ * pass:  y = x / sqrt(mean(x^2) + eps) * w  over a head's columns, then for pair
+ * i of y, with t = position * frequencies[i],
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t);
+ * columns beyond the pairs stay as they are.  q [tokens, heads, D] or
+ * [sequences, tokens, heads, D] and k, with the same tokens and D but heads of
+ * its own (NULL: no keys), F32 or F16, unit stride in the last dim, any others:
+ * slices of one projection are read in place.  wq, wk [D] in F32 or q's dtype
+ * (NULL: those heads are only rotated).  positions I32 [tokens] or [sequences,
+ * tokens], any value; frequencies F32, 1 to D / 2 of them.  sections (host
+ * memory; NULL and 0: one axis): with n_sections (at most 4) counts that add up
+ * to the frequencies, the first sections[0] pairs go by axis 0, the next
+ * sections[1] by axis 1 and so on, and positions has a last dim of n_sections
+ * (time, height and width of an image's or a video's patches).  D is even, at
+ * most 512.  q_out and k_out have q's and k's shapes, unit stride in the last
+ * dim and any other strides that address no element twice (a slice of a cache);
+ * they may be q and k themselves, and may lie between them as heads of one
+ * buffer.  Other overlaps return QSML_E_INVALID.  Angles are computed in
+ * binary64, the rest in binary32, rounded once.  No reference counterpart. */
+QSML_API qsml_status_t qsml_norm_rotary(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k, const qsml_tdesc* wq,
+                                        const qsml_tdesc* wk, float eps, const qsml_tdesc* positions,
+                                        const qsml_tdesc* frequencies, const int32_t* sections, int32_t n_sections,
+                                        int32_t pairing, const qsml_tdesc* q_out, const qsml_tdesc* k_out);
+
+/* Gradients of qsml_norm_rotary, from its inputs and dq_out, dk_out, the
+ * gradients of its outputs (any strides but the last's):  with g the outputs'
+ * gradient turned back, h = g w and xh = x rstd,
+ *   dx = rstd (h - xh mean(h xh)),   dw = sum over tokens and heads of g xh.
+ * dq and dk as q_out and k_out above; they may be dq_out and dk_out themselves.
+ * dwq and dwk [D] in F32 or q's dtype.  Each may be NULL when it is not wanted.
+ * The sums run in an order fixed by the shapes; with no rows they are 0.
+ * Workspace as for qsml_layer_norm_backward. */
+QSML_API qsml_status_t qsml_norm_rotary_backward(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k,
+                                                 const qsml_tdesc* wq, const qsml_tdesc* wk, float eps,
+                                                 const qsml_tdesc* positions, const qsml_tdesc* frequencies,
+                                                 const int32_t* sections, int32_t n_sections, int32_t pairing,
+                                                 const qsml_tdesc* dq_out, const qsml_tdesc* dk_out,
+                                                 const qsml_tdesc* dq, const qsml_tdesc* dk, const qsml_tdesc* dwq,
+                                                 const qsml_tdesc* dwk);
+
+/* Causal attention with a sliding window and first tokens that stay visible:
+ *   o = softmax(scale * q k^T) v   for each head, over the keys that a query sees.
+ * q [sequences, queries, heads, D], k and v [sequences, keys, kv heads, D], with
+ * heads a multiple of kv heads (head h reads kv head h / (heads / kv heads)); F32
+ * or F16, unit stride in the last dim, any others (a permuted [sequences, heads,
+ * ..] view, a slice of a projection or of a cache).  D is at most 256.
+ * q_lengths, k_lengths I32 [sequences] (NULL: all): the queries and keys that a
+ * sequence has, its first ones; taken as 0 below 0 and as all above that.  With
+ * nq queries and nk keys, query i stands at position p = nk - nq + i, so the last
+ * query at the last key: a prompt has nq = nk, the next token of a cache nq = 1.
+ * It sees key j if j <= p and, where window > 0, p - j < window or j < sinks;
+ * window 0 hides no earlier key.  scale > 0.
+ * o has q's shape, unit stride in the last dim and other strides that address no
+ * element twice.  lse (F32 [sequences, heads, queries], contiguous; NULL: not
+ * wanted) takes each row's logarithm of the sum of exponentials, for
+ * qsml_attention_backward.  A query that sees nothing, and those behind a
+ * sequence's last, give 0 and -inf.  What lies behind a sequence's last key is not
+ * used, whatever its bits; a key that a row does not see, but rows next to it do
+ * (by window or position), has to be finite in v.
+ * Scores, sums and norms are binary32; F16 weights of the values (the
+ * exponentials) are rounded to F16 between the two products.  Outputs may not
+ * overlap inputs or each other.  Workspace as for qsml_layer_norm_backward.
+ * No reference counterpart. */
+QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k, const qsml_tdesc* v,
+                                      const qsml_tdesc* q_lengths, const qsml_tdesc* k_lengths, float scale,
+                                      int64_t window, int64_t sinks, const qsml_tdesc* lse, const qsml_tdesc* o);
+
+/* Gradients of qsml_attention, from its inputs, its o and lse, and dout, the gradient
+ * of o (o and dout: any strides but the last's):  P = exp(scale q k^T - lse) where
+ * visible, dP = dout v^T, dS = scale P (dP - sum(dout o)),
+ *   dq = dS k,  dk = dS^T q,  dv = P^T dout,  summed over the heads of a kv head.
+ * dq has q's shape, dk and dv k's, strides as o's above.  Each may be NULL when it
+ * is not wanted; rows and keys behind a sequence's last get 0.  What lies behind a
+ * sequence's last query or key is not used.  F16: P and dS are rounded to F16
+ * between the products, dS times a power of two that keeps it in range.  No
+ * atomics: the same bits at every call. */
+QSML_API qsml_status_t qsml_attention_backward(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k,
+                                               const qsml_tdesc* v, const qsml_tdesc* o, const qsml_tdesc* lse,
+                                               const qsml_tdesc* dout, const qsml_tdesc* q_lengths,
+                                               const qsml_tdesc* k_lengths, float scale, int64_t window, int64_t sinks,
+                                               const qsml_tdesc* dq, const qsml_tdesc* dk, const qsml_tdesc* dv);
+
 /* ---- Multi-GPU groups (NCCL) ------------------------------------------------
  * The reference is single-GPU; sharded execution combines per-GPU partial
  * results with an in-place all-reduce.  Two ways to form a group:

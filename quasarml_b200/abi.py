@@ -30,6 +30,7 @@ RED_SUM, RED_MEAN, RED_MAX, RED_MIN, RED_PROD = range(5)
 AXIS_ALL = -1000
 ARG_MAX, ARG_MIN = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU, ACT_SIGMOID = range(5)
+ROTARY_HALVES, ROTARY_PAIRS = range(2)
 MM_AUTO, MM_FP32_FFMA, MM_FP32_3XTF32, MM_FP16_F32ACC = range(4)
 
 DTYPE_SIZE = {F32: 4, F16: 2, I32: 4, I16: 2, I8: 1, U32: 4, U16: 2, U8: 1}
@@ -155,6 +156,14 @@ _SIGS = {
                           + [_c.c_int32]),
     "qsml_gated_linear_backward": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 3 + [_c.c_int32] + [_P(TDesc)] * 8
                                    + [_c.c_int32]),
+    "qsml_norm_rotary": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 4 + [_c.c_float] + [_P(TDesc)] * 2
+                         + [_P(_c.c_int32), _c.c_int32, _c.c_int32] + [_P(TDesc)] * 2),
+    "qsml_norm_rotary_backward": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 4 + [_c.c_float] + [_P(TDesc)] * 2
+                                  + [_P(_c.c_int32), _c.c_int32, _c.c_int32] + [_P(TDesc)] * 6),
+    "qsml_attention": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 5 + [_c.c_float, _c.c_int64, _c.c_int64]
+                       + [_P(TDesc)] * 2),
+    "qsml_attention_backward": (_c.c_int32, [_c.c_void_p] + [_P(TDesc)] * 8 + [_c.c_float, _c.c_int64, _c.c_int64]
+                                + [_P(TDesc)] * 3),
     "qsml_reduce_noalloc": (_c.c_int32, [_c.c_void_p, _c.c_int32, _P(TDesc), _c.c_int32, _c.c_int32, _P(TDesc)]),
     "qsml_allreduce_partials": (_c.c_int32, [_c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int64]),
     "qsml_finish_partial": (_c.c_int32, [_c.c_void_p, _c.c_int32, _P(TDesc), _c.c_int64, _P(TDesc)]),
@@ -315,6 +324,13 @@ def desc_of(t) -> TDesc:
 def _opt(d: Optional[TDesc]):
     """An optional descriptor argument: None is NULL."""
     return None if d is None else ctypes.byref(d)
+
+
+def _sections(sections: Optional[Sequence[int]]):
+    """Counts of pairs by axis as a C array and its length."""
+    if sections is None:
+        return None, 0
+    return (ctypes.c_int32 * max(len(sections), 1))(*sections), len(sections)
 
 
 class Context:
@@ -516,6 +532,47 @@ class Context:
             self.h, ctypes.byref(x), ctypes.byref(w_gate), ctypes.byref(w_up), int(act), ctypes.byref(gate),
             ctypes.byref(up), ctypes.byref(dy), _opt(dx), _opt(dw_gate), _opt(dw_up), _opt(db_gate), _opt(db_up),
             precision))
+
+    def norm_rotary(self, q: TDesc, k: Optional[TDesc], wq: Optional[TDesc], wk: Optional[TDesc], positions: TDesc,
+                    frequencies: TDesc, q_out: TDesc, k_out: Optional[TDesc], eps: float = 1e-6,
+                    sections: Optional[Sequence[int]] = None, pairing: int = ROTARY_HALVES) -> None:
+        """Norm of each head of q and k, then the rotation of its pairs by position * frequency
+        (sections: how many pairs go by each axis of positions)."""
+        arr, n = _sections(sections)
+        self.check(self.lib.qsml_norm_rotary(self.h, ctypes.byref(q), _opt(k), _opt(wq), _opt(wk),
+                                             ctypes.c_float(eps), ctypes.byref(positions), ctypes.byref(frequencies),
+                                             arr, n, int(pairing), ctypes.byref(q_out), _opt(k_out)))
+
+    def norm_rotary_backward(self, q: TDesc, k: Optional[TDesc], wq: Optional[TDesc], wk: Optional[TDesc],
+                             positions: TDesc, frequencies: TDesc, dq_out: TDesc, dk_out: Optional[TDesc],
+                             dq: Optional[TDesc], dk: Optional[TDesc], dwq: Optional[TDesc] = None,
+                             dwk: Optional[TDesc] = None, eps: float = 1e-6,
+                             sections: Optional[Sequence[int]] = None, pairing: int = ROTARY_HALVES) -> None:
+        """Gradients of norm_rotary for q, k and the weights (None: not wanted)."""
+        arr, n = _sections(sections)
+        self.check(self.lib.qsml_norm_rotary_backward(
+            self.h, ctypes.byref(q), _opt(k), _opt(wq), _opt(wk), ctypes.c_float(eps), ctypes.byref(positions),
+            ctypes.byref(frequencies), arr, n, int(pairing), ctypes.byref(dq_out), _opt(dk_out), _opt(dq), _opt(dk),
+            _opt(dwq), _opt(dwk)))
+
+    def attention(self, q: TDesc, k: TDesc, v: TDesc, o: TDesc, scale: float, window: int = 0, sinks: int = 0,
+                  q_lengths: Optional[TDesc] = None, k_lengths: Optional[TDesc] = None,
+                  lse: Optional[TDesc] = None) -> None:
+        """o = softmax(scale q k^T) v over the keys that each query sees; lse is what
+        attention_backward reads."""
+        self.check(self.lib.qsml_attention(self.h, ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), _opt(q_lengths),
+                                           _opt(k_lengths), ctypes.c_float(scale), int(window), int(sinks), _opt(lse),
+                                           ctypes.byref(o)))
+
+    def attention_backward(self, q: TDesc, k: TDesc, v: TDesc, o: TDesc, lse: TDesc, dout: TDesc,
+                           dq: Optional[TDesc], dk: Optional[TDesc], dv: Optional[TDesc], scale: float,
+                           window: int = 0, sinks: int = 0, q_lengths: Optional[TDesc] = None,
+                           k_lengths: Optional[TDesc] = None) -> None:
+        """Gradients of attention for q, k and v (None: not wanted)."""
+        self.check(self.lib.qsml_attention_backward(
+            self.h, ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(o), ctypes.byref(lse),
+            ctypes.byref(dout), _opt(q_lengths), _opt(k_lengths), ctypes.c_float(scale), int(window), int(sinks),
+            _opt(dq), _opt(dk), _opt(dv)))
 
 
 def broadcast_shape(a: Iterable[int], b: Iterable[int]) -> tuple:

@@ -1,0 +1,320 @@
+// Attention of few queries over many keys: the next tokens of sequences over their caches.
+//
+// Bound by HBM: the visible keys and values are read once, for all heads of a group and all
+// queries together (RT rows a CTA).  A sequence's visible keys are split over CTAs so that
+// the device is full however few sequences there are; each CTA goes over its part in tiles
+// of keys that cp.async brings in while the tile before is used, with the rows' running
+// maximum and sum, and leaves its sums and statistics in a workspace that k_attention_join
+// adds up in the order of the parts.  With one part there is nothing to join.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention.cuh"
+#include "packed.cuh"
+
+namespace qsml {
+namespace attn {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Row r of a kv head's Sq * G: query r / G, head r % G of the group.
+struct Parts {
+    float* sum;    // [rows][parts][D], not divided by l
+    float* stat;   // [rows][parts][2]: m (base 2, scaled), l
+    int parts;
+};
+
+template <typename T, int DP, int RT> struct Shape {
+    static constexpr int V = 16 / sizeof(T);
+    static constexpr int KT = sizeof(T) * DP >= 512 ? 32 : 64;  // keys a tile: two stages and three CTAs a SM
+    static constexpr int LD = DP + V;  // elements between rows: lanes' 16-byte loads 8 by 8 in no bank
+    static constexpr int TILE = KT * LD * sizeof(T);
+    static constexpr size_t SMEM = 4 * TILE + sizeof(float) * (RT * DP + RT * KT + 3 * RT);
+};
+
+// The n-th visible keys [n0, n0 + KT) below end of a head into a tile; zeros elsewhere.
+template <typename T, int DP, int RT>
+__device__ __forceinline__ void load_keys(unsigned char* dst, const View& v, int64_t at, const Keys& keys, int n0, int end, int D, bool vec) {
+    using S = Shape<T, DP, RT>;
+    const T* p = reinterpret_cast<const T*>(v.p) + at;
+    if (vec) {
+        constexpr int C = DP / S::V;
+        for (int i = threadIdx.x; i < S::KT * C; i += kThreads) {
+            const int r = i / C, c = i % C * S::V, n = n0 + r;
+            const bool in = n < end && c < D;
+            const T* src = in ? p + keys.key(n) * v.s + c : reinterpret_cast<const T*>(v.p);
+            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst + (r * S::LD + c) * sizeof(T)));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+        }
+    } else {
+        for (int i = threadIdx.x; i < S::KT * DP; i += kThreads) {
+            const int r = i / DP, c = i % DP, n = n0 + r;
+            T x;
+            heads::from_f(0.0f, x);
+            if (n < end && c < D) x = p[keys.key(n) * v.s + c];
+            reinterpret_cast<T*>(dst)[r * S::LD + c] = x;
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <typename T, int DP, int RT>
+__global__ void __launch_bounds__(kThreads) k_attention_few(const __grid_constant__ Problem p, Parts parts, int row_tiles, bool vec) {
+    using S = Shape<T, DP, RT>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    unsigned char *sk = smem, *sv = smem + 2 * S::TILE;
+    constexpr int KT = S::KT;
+    float *sq = reinterpret_cast<float*>(smem + 4 * S::TILE), *sp = sq + RT * DP, *sm = sp + RT * KT, *sl = sm + RT, *sf = sl + RT;
+    pdl_begin();
+    const int part = blockIdx.x % parts.parts, group = blockIdx.x / parts.parts;
+    const int rt = group % row_tiles, hk = group / row_tiles % p.Hk, b = group / row_tiles / p.Hk;
+    const Seq seq(p, b);
+    const int off = seq.nk - seq.nq, R = p.Sq * p.G, r0 = rt * RT;
+    const int first = r0 / p.G, last = (min(r0 + RT, R) - 1) / p.G;  // queries of the rows
+    const Keys keys(p, seq.nk, first + off, min(last, seq.nq - 1) + off);
+    const int all = first < seq.nq ? keys.count() : 0;
+    const int share = (all + parts.parts - 1) / parts.parts;
+    const int n0 = min(part * share, all), n1 = min(n0 + share, all);
+    const int64_t ak = b * p.k.b + hk * p.k.h, av = b * p.v.b + hk * p.v.h;
+    if (n0 < n1) {
+        load_keys<T, DP, RT>(sk, p.k, ak, keys, n0, n1, p.D, vec);
+        load_keys<T, DP, RT>(sv, p.v, av, keys, n0, n1, p.D, vec);
+    }
+    const float c = p.scale * kLog2e;
+    for (int i = threadIdx.x; i < RT * DP; i += kThreads) {
+        const int r = r0 + i / DP, col = i % DP;
+        const bool in = r < R && r / p.G < seq.nq && col < p.D;
+        sq[i] = in ? heads::to_f(reinterpret_cast<const T*>(p.q.p)[b * p.q.b + r / p.G * p.q.s + (hk * p.G + r % p.G) * p.q.h + col]) : 0.0f;
+    }
+    if (threadIdx.x < RT) sm[threadIdx.x] = -INFINITY, sl[threadIdx.x] = 0.0f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // scores: a key and RH of the rows a thread
+    constexpr int RH = RT * KT / kThreads;
+    const int key = threadIdx.x % KT, half = threadIdx.x / KT;
+    // sums: four columns (and those DP / 2 on, with 256) and a quarter of the rows
+    constexpr int RQ = (RT + 3) / 4, NC = DP / 4 > 32 ? DP / 128 : 1, LANES = DP / 4 < 32 ? DP / 4 : 32;
+    P2 acc[RQ][NC][2];
+#pragma unroll
+    for (auto& x : acc)
+#pragma unroll
+        for (auto& y : x) y[0] = y[1] = pack(0.0f, 0.0f);
+    int stage = 0;
+    for (int n = n0; n < n1; n += KT, stage ^= 1) {
+        if (n + KT < n1) {
+            load_keys<T, DP, RT>(sk + (stage ^ 1) * S::TILE, p.k, ak, keys, n + KT, n1, p.D, vec);
+            load_keys<T, DP, RT>(sv + (stage ^ 1) * S::TILE, p.v, av, keys, n + KT, n1, p.D, vec);
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();
+        {
+            const T* k = reinterpret_cast<const T*>(sk + stage * S::TILE) + key * S::LD;
+            P2 s[RH];
+#pragma unroll
+            for (int i = 0; i < RH; ++i) s[i] = pack(0.0f, 0.0f);
+#pragma unroll 2
+            for (int d = 0; d < DP; d += S::V) {
+                const heads::Pack<T, S::V> x = *reinterpret_cast<const heads::Pack<T, S::V>*>(k + d);
+                P2 y[S::V / 2];
+#pragma unroll
+                for (int e = 0; e < S::V / 2; ++e) y[e] = pack(heads::to_f(x.v[2 * e]), heads::to_f(x.v[2 * e + 1]));
+#pragma unroll
+                for (int i = 0; i < RH; ++i)
+#pragma unroll
+                    for (int e = 0; e < S::V / 4; ++e) {
+                        const float4 q = *reinterpret_cast<const float4*>(sq + (half * RH + i) * DP + d + 4 * e);
+                        s[i] = fma2(pack(q.x, q.y), y[2 * e], s[i]);
+                        s[i] = fma2(pack(q.z, q.w), y[2 * e + 1], s[i]);
+                    }
+            }
+            const int j = n + key < n1 ? keys.key(n + key) : INT32_MAX;
+#pragma unroll
+            for (int i = 0; i < RH; ++i) {
+                const int r = half * RH + i, q = (r0 + r) / p.G;
+                const bool seen = q < seq.nq && r0 + r < R && q + off < seq.nk && sees(p, q + off, j);
+                sp[r * KT + key] = seen ? sum2(s[i]) * c : -INFINITY;
+            }
+        }
+        __syncthreads();
+        // a warp takes every fourth row's maximum and sum
+        for (int r = warp; r < RT; r += 4) {
+            constexpr int N = KT / 32;
+            float x[N], most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) most = fmaxf(most, x[i] = sp[r * KT + lane + 32 * i]);
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+            const float old = sm[r], now = fmaxf(old, most), ref = now == -INFINITY ? 0.0f : now;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = exp2f(x[i] - ref);
+                sp[r * KT + lane + 32 * i] = x[i];
+                sum += x[i];
+            }
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+            __syncwarp();
+            if (lane == 0) {
+                const float f = exp2f(old - ref);
+                sf[r] = f;
+                sm[r] = now;
+                sl[r] = fmaf(sl[r], f, sum);
+            }
+        }
+        __syncthreads();
+        if (lane < LANES) {
+            const T* v = reinterpret_cast<const T*>(sv + stage * S::TILE);
+#pragma unroll
+            for (int i = 0; i < RQ; ++i) {
+                const int r = warp * RQ + i;
+                const P2 f = both(r < RT ? sf[r] : 0.0f);
+#pragma unroll
+                for (auto& y : acc[i]) y[0] = mul2(y[0], f), y[1] = mul2(y[1], f);
+            }
+#pragma unroll 2
+            for (int k = 0; k < KT; k += 4) {
+                float w[RQ][4];
+#pragma unroll
+                for (int i = 0; i < RQ; ++i)
+                    *reinterpret_cast<float4*>(w[i]) =
+                        warp * RQ + i < RT ? *reinterpret_cast<const float4*>(sp + (warp * RQ + i) * KT + k) : make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int m = 0; m < NC; ++m) {
+                        const heads::Pack<T, 4> x = *reinterpret_cast<const heads::Pack<T, 4>*>(v + (k + e) * S::LD + 4 * lane + 128 * m);
+                        const P2 y0 = pack(heads::to_f(x.v[0]), heads::to_f(x.v[1])), y1 = pack(heads::to_f(x.v[2]), heads::to_f(x.v[3]));
+#pragma unroll
+                        for (int i = 0; i < RQ; ++i) {
+                            const P2 ww = both(w[i][e]);
+                            acc[i][m][0] = fma2(ww, y0, acc[i][m][0]);
+                            acc[i][m][1] = fma2(ww, y1, acc[i][m][1]);
+                        }
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (lane >= LANES) return;
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        const int r = warp * RQ + i;
+        if (r >= RT || r0 + r >= R) continue;
+        const int q = (r0 + r) / p.G, h = hk * p.G + (r0 + r) % p.G;
+        const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + q;
+        const float l = sl[r];
+        const bool any = l > 0.0f || isnan(l), whole = parts.parts == 1;
+        const float f = whole ? (any ? 1.0f / l : 0.0f) : 1.0f;
+#pragma unroll
+        for (int m = 0; m < NC; ++m) {
+            const float2 a = unpack(acc[i][m][0]), d = unpack(acc[i][m][1]);
+            const float y[4] = {a.x * f, a.y * f, d.x * f, d.y * f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int col = 4 * lane + 128 * m + e;
+                if (col >= p.D) continue;
+                if (whole)
+                    heads::from_f(y[e], reinterpret_cast<T*>(p.o.p)[b * p.o.b + q * p.o.s + h * p.o.h + col]);
+                else
+                    parts.sum[(row * parts.parts + part) * p.D + col] = y[e];
+            }
+        }
+        if (lane == 0) {
+            if (!whole) {
+                parts.stat[(row * parts.parts + part) * 2] = sm[r];
+                parts.stat[(row * parts.parts + part) * 2 + 1] = l;
+            } else if (p.lse) {
+                p.lse[row] = any ? (sm[r] + log2f(l)) * kLn2 : -INFINITY;
+            }
+        }
+    }
+}
+
+// The parts of a row joined in their order: a warp a row.
+template <typename T> __global__ void __launch_bounds__(128) k_attention_join(const __grid_constant__ Problem p, Parts parts, int64_t rows) {
+    pdl_begin();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int q = static_cast<int>(row % p.Sq), h = static_cast<int>(row / p.Sq % p.Hq), b = static_cast<int>(row / p.Sq / p.Hq);
+    const float* stat = parts.stat + row * parts.parts * 2;
+    float m = -INFINITY;
+    for (int i = lane; i < parts.parts; i += 32) m = fmaxf(m, stat[2 * i]);
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    for (int i = 0; i < parts.parts; ++i) l = fmaf(stat[2 * i + 1], exp2f(stat[2 * i] - ref), l);
+    const bool any = l > 0.0f || isnan(l);
+    const float f = any ? 1.0f / l : 0.0f;
+    T* o = reinterpret_cast<T*>(p.o.p) + b * p.o.b + q * p.o.s + h * p.o.h;
+    for (int c = lane; c < p.D; c += 32) {
+        float s = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < parts.parts; ++i) s = fmaf(parts.sum[(row * parts.parts + i) * p.D + c], exp2f(stat[2 * i] - ref), s);
+        heads::from_f(s * f, o[c]);
+    }
+    if (p.lse && lane == 0) p.lse[row] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Problem& p, bool vec) {
+    using S = Shape<T, DP, RT>;
+    const auto kernel = k_attention_few<T, DP, RT>;
+    const char* name = "k_attention_few";
+    QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::SMEM)), name));
+    int resident = 1;
+    QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, S::SMEM), name));
+    const int R = p.Sq * p.G, row_tiles = (R + RT - 1) / RT;
+    const int64_t groups = static_cast<int64_t>(row_tiles) * p.Hk * p.B;
+    // as many parts as fill the device, each of at least two tiles
+    const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
+    const int64_t want = (static_cast<int64_t>(ctx->num_sms) * std::max(resident, 1) + groups - 1) / groups;
+    const int64_t most = std::min<int64_t>(128, (visible + 2 * S::KT - 1) / (2 * S::KT));
+    Parts parts{nullptr, nullptr, static_cast<int>(std::max<int64_t>(1, std::min(want, most)))};
+    if (groups * parts.parts > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+    Workspace ws(ctx);
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
+    if (parts.parts > 1) {
+        void* m = nullptr;
+        QSML_TRY_STATUS(ws.get(sizeof(float) * rows * parts.parts * (p.D + 2), &m));
+        parts.sum = static_cast<float*>(m);
+        parts.stat = parts.sum + rows * parts.parts * p.D;
+    }
+    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(groups * parts.parts)), dim3(kThreads), S::SMEM, ctx->stream, p, parts, row_tiles, vec);
+    if (e != cudaSuccess) return check_cuda(ctx, e, name);
+    QSML_TRY_STATUS(after_launch(ctx, name));
+    if (parts.parts == 1) return QSML_OK;
+    e = launch_pdl(k_attention_join<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, ctx->stream, p, parts, rows);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
+    return after_launch(ctx, "k_attention_join");
+}
+
+template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
+    const int64_t es = sizeof(T);
+    const bool vec = p.D * es % 16 == 0 && heads::rows_on(p.k, es, 16) && heads::rows_on(p.v, es, 16);
+    const int R = p.Sq * p.G;
+    return by_width(p.D, [&](auto width) {
+        constexpr int DP = decltype(width)::value;
+        if (R <= 4) return run<T, DP, 4>(ctx, p, vec);
+        if (R <= 8 || (sizeof(T) == 4 && DP == 256)) return run<T, DP, 8>(ctx, p, vec);
+        if constexpr (sizeof(T) == 4 && DP == 256)
+            return static_cast<qsml_status_t>(QSML_E_UNSUPPORTED);
+        else
+            return run<T, DP, 16>(ctx, p, vec);
+    });
+}
+
+}  // namespace
+
+// Up to 64 rows a kv head.
+bool few_queries(const Problem& p) { return static_cast<int64_t>(p.Sq) * p.G <= 64; }
+
+qsml_status_t forward_few(Context* ctx, const Problem& p) { return p.f16 ? forward<__half>(ctx, p) : forward<float>(ctx, p); }
+
+}  // namespace attn
+}  // namespace qsml

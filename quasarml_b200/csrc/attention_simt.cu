@@ -1,0 +1,387 @@
+// Attention and its gradients on the CUDA cores, for binary32 and for what the tensor
+// cores' kernels do not take (heads of more than 128 columns, rows off 16 bytes).
+//
+// A tile of BT queries meets a tile of BT keys, both in shared memory as binary32; 16 x 16
+// threads hold RT x RT of its scores (RT = BT / 16) and RT rows x DP / 16 columns of each
+// sum.  Products are packed pairs (fma.rn.f32x2).  Forward: one pass over the visible keys
+// with each row's running maximum and sum (exp(s - m), the sum and what was summed before
+// multiplied by exp(m_old - m) where m grows); nothing of the scores leaves the SM.
+// Backward: P = exp(s - lse) again from the kept lse.  dk and dv of a tile of keys are
+// summed by one CTA over all queries that see it and all heads of its group, dq of a tile
+// of queries by another over its keys: seven products instead of five, no atomics.
+// Bound by the FFMA pipe and by shared memory, a 16-byte load for 8 multiply-adds.
+#include <type_traits>
+
+#include "attention.cuh"
+#include "packed.cuh"
+
+namespace qsml {
+namespace attn {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int DP> struct Shape {
+    static constexpr int BT = DP <= 128 ? 64 : 32;
+    static constexpr int RT = BT / 16;   // rows and columns of scores a thread
+    static constexpr int CT = DP / 16;   // columns of a sum a thread
+    static constexpr int LD = DP + 4;    // floats between rows: 16 lanes' 16-byte loads meet 8 by 8 in no bank
+    static constexpr int LP = BT + 4;
+    static constexpr int TILE = BT * LD, PROBS = BT * LP;
+};
+
+// Rows [r0, r0 + BT) of a head, those in [lo, hi) or below sink, as floats; 0 elsewhere.
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at, int r0, int sink, int lo, int hi, int D, bool vec) {
+    using S = Shape<DP>;
+    constexpr int V = 16 / sizeof(T);
+    const T* p = reinterpret_cast<const T*>(v.p) + at;
+    if (vec) {
+        for (int i = threadIdx.x; i < S::BT * (DP / V); i += kThreads) {
+            const int r = i / (DP / V), c = i % (DP / V) * V, row = r0 + r;
+            heads::Pack<T, V> x;
+            const bool in = (row >= lo || row < sink) && row < hi && c < D;
+            if (in) x = *reinterpret_cast<const heads::Pack<T, V>*>(p + row * v.s + c);
+#pragma unroll
+            for (int e = 0; e < V; e += 4)
+                *reinterpret_cast<float4*>(dst + r * S::LD + c + e) =
+                    in ? make_float4(heads::to_f(x.v[e]), heads::to_f(x.v[e + 1]), heads::to_f(x.v[e + 2]), heads::to_f(x.v[e + 3]))
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    } else {
+        for (int i = threadIdx.x; i < S::BT * DP; i += kThreads) {
+            const int r = i / DP, c = i % DP, row = r0 + r;
+            dst[r * S::LD + c] = (row >= lo || row < sink) && row < hi && c < D ? heads::to_f(p[row * v.s + c]) : 0.0f;
+        }
+    }
+}
+
+// acc[i][j] = sum over columns of a[ty RT + i] b[tx + 16 j].
+template <int DP> __device__ __forceinline__ void dots(const float* a, const float* b, float (&acc)[Shape<DP>::RT][Shape<DP>::RT]) {
+    using S = Shape<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    P2 s[S::RT][S::RT];
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+        for (int j = 0; j < S::RT; ++j) s[i][j] = pack(0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = 0; c < DP; c += 4) {
+        float4 x[S::RT], y[S::RT];
+#pragma unroll
+        for (int i = 0; i < S::RT; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty * S::RT + i) * S::LD + c);
+#pragma unroll
+        for (int j = 0; j < S::RT; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * S::LD + c);
+#pragma unroll
+        for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::RT; ++j) {
+                s[i][j] = fma2(pack(x[i].x, x[i].y), pack(y[j].x, y[j].y), s[i][j]);
+                s[i][j] = fma2(pack(x[i].z, x[i].w), pack(y[j].z, y[j].w), s[i][j]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+        for (int j = 0; j < S::RT; ++j) acc[i][j] = sum2(s[i][j]);
+}
+
+// Columns of a thread's sums: 4 tx + 64 n + e.
+template <int DP> struct Sum {
+    P2 v[Shape<DP>::RT][Shape<DP>::CT / 2];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (auto& r : v)
+#pragma unroll
+            for (auto& x : r) x = pack(0.0f, 0.0f);
+    }
+    // += p (rows ty RT + i of [BT][LP]) times x ([BT][LD])
+    __device__ __forceinline__ void add(const float* p, const float* x) {
+        using S = Shape<DP>;
+        const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll 2
+        for (int k = 0; k < S::BT; k += 4) {
+            float w[S::RT][4];
+#pragma unroll
+            for (int i = 0; i < S::RT; ++i) *reinterpret_cast<float4*>(w[i]) = *reinterpret_cast<const float4*>(p + (ty * S::RT + i) * S::LP + k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < DP / 64; ++n) {
+                    const float4 y = *reinterpret_cast<const float4*>(x + (k + e) * S::LD + 4 * tx + 64 * n);
+#pragma unroll
+                    for (int i = 0; i < S::RT; ++i) {
+                        v[i][2 * n] = fma2(both(w[i][e]), pack(y.x, y.y), v[i][2 * n]);
+                        v[i][2 * n + 1] = fma2(both(w[i][e]), pack(y.z, y.w), v[i][2 * n + 1]);
+                    }
+                }
+        }
+    }
+    template <typename T> __device__ __forceinline__ void store(int i, T* row, float f, int D) const {
+        const int tx = threadIdx.x & 15;
+#pragma unroll
+        for (int n = 0; n < DP / 64; ++n) {
+            const float2 a = unpack(v[i][2 * n]), b = unpack(v[i][2 * n + 1]);
+            const float y[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * tx + 64 * n + e < D) heads::from_f(y[e], row[4 * tx + 64 * n + e]);
+        }
+    }
+};
+
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
+}
+
+// A CTA's tile (the last first: with the most keys), head and sequence.
+struct Where {
+    int tile, h, b;
+    __device__ __forceinline__ Where(int tiles, int H) {
+        const int i = blockIdx.x / H / tiles, r = blockIdx.x - i * H * tiles;
+        b = i;
+        tile = tiles - 1 - r / H;
+        h = r % H;
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_constant__ Problem p, int tiles, bool vec) {
+    using S = Shape<DP>;
+    extern __shared__ float4 smem[];
+    float *sq = reinterpret_cast<float*>(smem), *skv = sq + S::TILE, *sp = skv + S::TILE;
+    pdl_begin();
+    const Where w(tiles, p.Hq);
+    const Seq seq(p, w.b);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
+    const Keys keys(p, seq.nk, q0 + off, min(q0 + S::BT, seq.nq) - 1 + off);
+    const Tiles t(keys, S::BT);
+    load_tile<T, DP>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+    Sum<DP> o;
+    o.zero();
+    float m[S::RT], l[S::RT];
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i) m[i] = -INFINITY, l[i] = 0.0f;
+    const float c = p.scale * kLog2e;
+    for (int n = 0; n < (q0 < seq.nq ? t.n : 0); ++n) {
+        const int k0 = t.tile(n) * S::BT;
+        __syncthreads();
+        load_tile<T, DP>(skv, p.k, w.b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
+        __syncthreads();
+        float s[S::RT][S::RT];
+        dots<DP>(sq, skv, s);
+#pragma unroll
+        for (int i = 0; i < S::RT; ++i) {
+            const int pos = q0 + ty * S::RT + i + off;
+            float most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < S::RT; ++j) {
+                s[i][j] = pos < seq.nk && sees(p, pos, k0 + tx + 16 * j) ? s[i][j] * c : -INFINITY;
+                most = fmaxf(most, s[i][j]);
+            }
+            const float now = fmaxf(m[i], row_max(most)), ref = now == -INFINITY ? 0.0f : now;
+            const float f = exp2f(m[i] - ref);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < S::RT; ++j) {
+                const float e = exp2f(s[i][j] - ref);
+                sum += e;
+                sp[(ty * S::RT + i) * S::LP + tx + 16 * j] = e;
+            }
+            l[i] = fmaf(l[i], f, row_sum(sum));
+            m[i] = now;
+#pragma unroll
+            for (auto& x : o.v[i]) x = mul2(x, both(f));
+        }
+        __syncthreads();
+        // values that no row of the tile sees count for nothing, whatever they are
+        load_tile<T, DP>(skv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        __syncthreads();
+        o.add(sp, skv);
+    }
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i) {
+        const int q = q0 + ty * S::RT + i;
+        if (q >= p.Sq) continue;
+        const bool any = l[i] > 0.0f || isnan(l[i]);
+        o.store(i, reinterpret_cast<T*>(p.o.p) + w.b * p.o.b + q * p.o.s + w.h * p.o.h, any ? 1.0f / l[i] : 0.0f, p.D);
+        if (p.lse && tx == 0) p.lse[(static_cast<int64_t>(w.b) * p.Hq + w.h) * p.Sq + q] = any ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+    }
+}
+
+// Shared memory of the gradients' kernels: two fixed tiles, two that come and go, P and dS.
+template <int DP> constexpr size_t grad_smem() { return sizeof(float) * (4 * Shape<DP>::TILE + 2 * Shape<DP>::PROBS + 2 * Shape<DP>::BT); }
+
+// dk and dv of a tile of keys.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_constant__ Problem p, const float* delta, int tiles, bool vec) {
+    using S = Shape<DP>;
+    extern __shared__ float4 smem[];
+    float *sk = reinterpret_cast<float*>(smem), *sv = sk + S::TILE, *sq = sv + S::TILE, *sg = sq + S::TILE, *sp = sg + S::TILE,
+          *sd = sp + S::PROBS, *sl = sd + S::PROBS, *sdel = sl + S::BT;
+    pdl_begin();
+    const int hk = blockIdx.x % p.Hk, tile = blockIdx.x / p.Hk % tiles, b = blockIdx.x / p.Hk / tiles;
+    const Seq seq(p, b);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int k0 = tile * S::BT, off = seq.nk - seq.nq;
+    load_tile<T, DP>(sk, p.k, b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
+    load_tile<T, DP>(sv, p.v, b * p.v.b + hk * p.v.h, k0, 0, 0, seq.nk, p.D, vec);
+    Sum<DP> dk, dv;
+    dk.zero();
+    dv.zero();
+    const Queries qs(p, seq, k0, k0 + S::BT);
+    for (int g = 0; g < p.G; ++g) {
+        const int h = hk * p.G + g;
+        const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
+        for (int q0 = qs.lo / S::BT * S::BT; q0 < qs.hi; q0 += S::BT) {
+            __syncthreads();
+            load_tile<T, DP>(sq, p.q, b * p.q.b + h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+            load_tile<T, DP>(sg, p.dout, b * p.dout.b + h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
+            if (threadIdx.x < S::BT) {
+                const int q = q0 + threadIdx.x;
+                sl[threadIdx.x] = q < seq.nq ? p.lse[stat + q] : 0.0f;
+                sdel[threadIdx.x] = q < seq.nq ? delta[stat + q] : 0.0f;
+            }
+            __syncthreads();
+            float s[S::RT][S::RT], d[S::RT][S::RT];
+            dots<DP>(sk, sq, s);
+            dots<DP>(sv, sg, d);
+#pragma unroll
+            for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+                for (int j = 0; j < S::RT; ++j) {
+                    const int key = k0 + ty * S::RT + i, q = tx + 16 * j;
+                    const bool seen = q0 + q < seq.nq && sees(p, q0 + q + off, key);
+                    const float e = seen ? exp2f((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
+                    sp[(ty * S::RT + i) * S::LP + q] = e;
+                    sd[(ty * S::RT + i) * S::LP + q] = seen ? e * (d[i][j] - sdel[q]) : 0.0f;
+                }
+            __syncthreads();
+            dv.add(sp, sg);
+            dk.add(sd, sq);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i) {
+        const int k = k0 + ty * S::RT + i;
+        if (k >= p.Sk) continue;
+        if (p.dk.p) dk.store(i, reinterpret_cast<T*>(p.dk.p) + b * p.dk.b + k * p.dk.s + hk * p.dk.h, p.scale, p.D);
+        if (p.dv.p) dv.store(i, reinterpret_cast<T*>(p.dv.p) + b * p.dv.b + k * p.dv.s + hk * p.dv.h, 1.0f, p.D);
+    }
+}
+
+// dq of a tile of queries.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_constant__ Problem p, const float* delta, int tiles, bool vec) {
+    using S = Shape<DP>;
+    extern __shared__ float4 smem[];
+    float *sq = reinterpret_cast<float*>(smem), *sg = sq + S::TILE, *sk = sg + S::TILE, *sv = sk + S::TILE, *sd = sv + S::TILE;
+    pdl_begin();
+    const Where w(tiles, p.Hq);
+    const Seq seq(p, w.b);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
+    const Keys keys(p, seq.nk, q0 + off, min(q0 + S::BT, seq.nq) - 1 + off);
+    const Tiles t(keys, S::BT);
+    load_tile<T, DP>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+    load_tile<T, DP>(sg, p.dout, w.b * p.dout.b + w.h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
+    Sum<DP> dq;
+    dq.zero();
+    const int64_t stat = (static_cast<int64_t>(w.b) * p.Hq + w.h) * p.Sq;
+    float lse[S::RT], del[S::RT];
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i) {
+        const int q = q0 + ty * S::RT + i;
+        lse[i] = q < seq.nq ? p.lse[stat + q] : 0.0f;
+        del[i] = q < seq.nq ? delta[stat + q] : 0.0f;
+    }
+    for (int n = 0; n < (q0 < seq.nq ? t.n : 0); ++n) {
+        const int k0 = t.tile(n) * S::BT;
+        __syncthreads();
+        load_tile<T, DP>(sk, p.k, w.b * p.k.b + hk * p.k.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        load_tile<T, DP>(sv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        __syncthreads();
+        float s[S::RT][S::RT], d[S::RT][S::RT];
+        dots<DP>(sq, sk, s);
+        dots<DP>(sg, sv, d);
+#pragma unroll
+        for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::RT; ++j) {
+                const int q = q0 + ty * S::RT + i;
+                const bool seen = q < seq.nq && sees(p, q + off, k0 + tx + 16 * j);
+                const float e = seen ? exp2f((s[i][j] * p.scale - lse[i]) * kLog2e) : 0.0f;
+                sd[(ty * S::RT + i) * S::LP + tx + 16 * j] = seen ? e * (d[i][j] - del[i]) : 0.0f;
+            }
+        __syncthreads();
+        dq.add(sd, sk);
+    }
+#pragma unroll
+    for (int i = 0; i < S::RT; ++i) {
+        const int q = q0 + ty * S::RT + i;
+        if (q < p.Sq) dq.store(i, reinterpret_cast<T*>(p.dq.p) + w.b * p.dq.b + q * p.dq.s + w.h * p.dq.h, p.scale, p.D);
+    }
+}
+
+// Whether all rows read can be read in 16 bytes.
+bool whole(const Problem& p, bool backward) {
+    const int64_t es = p.f16 ? 2 : 4;
+    bool ok = p.D * es % 16 == 0 && heads::rows_on(p.q, es, 16) && heads::rows_on(p.k, es, 16) && heads::rows_on(p.v, es, 16);
+    return ok && (!backward || heads::rows_on(p.dout, es, 16));
+}
+
+// One CTA for each of tiles x heads x sequences.
+template <typename K, typename... A>
+qsml_status_t launch(Context* ctx, K kernel, const char* name, size_t smem, int64_t tiles, int heads, int B, A... args) {
+    if (tiles * heads * B > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+    QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), name));
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * heads * B)), dim3(kThreads), smem, ctx->stream, args...);
+    if (e != cudaSuccess) return check_cuda(ctx, e, name);
+    return after_launch(ctx, name);
+}
+
+template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
+    return by_width(p.D, [&](auto width) {
+        constexpr int DP = decltype(width)::value;
+        using S = Shape<DP>;
+        const int tiles = (p.Sq + S::BT - 1) / S::BT;
+        return launch(ctx, k_attention_simt<T, DP>, "k_attention_simt", sizeof(float) * (2 * S::TILE + S::PROBS), tiles, p.Hq, p.B, p, tiles,
+                      whole(p, false));
+    });
+}
+
+template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, const float* delta) {
+    return by_width(p.D, [&](auto width) {
+        constexpr int DP = decltype(width)::value;
+        using S = Shape<DP>;
+        const bool vec = whole(p, true);
+        if (p.dk.p || p.dv.p) {
+            const int tiles = (p.Sk + S::BT - 1) / S::BT;
+            QSML_TRY_STATUS(launch(ctx, k_attention_dkv_simt<T, DP>, "k_attention_dkv_simt", grad_smem<DP>(), tiles, p.Hk, p.B, p, delta, tiles, vec));
+        }
+        if (p.dq.p) {
+            const int tiles = (p.Sq + S::BT - 1) / S::BT;
+            QSML_TRY_STATUS(launch(ctx, k_attention_dq_simt<T, DP>, "k_attention_dq_simt", grad_smem<DP>(), tiles, p.Hq, p.B, p, delta, tiles, vec));
+        }
+        return static_cast<qsml_status_t>(QSML_OK);
+    });
+}
+
+}  // namespace
+
+qsml_status_t forward_simt(Context* ctx, const Problem& p) { return p.f16 ? forward<__half>(ctx, p) : forward<float>(ctx, p); }
+qsml_status_t backward_simt(Context* ctx, const Problem& p, const float* delta) {
+    return p.f16 ? backward<__half>(ctx, p, delta) : backward<float>(ctx, p, delta);
+}
+
+}  // namespace attn
+}  // namespace qsml
