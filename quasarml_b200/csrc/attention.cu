@@ -135,7 +135,7 @@ extern "C" qsml_status_t qsml_attention(qsml_ctx* handle, const qsml_tdesc* q, c
     QSML_TRY_STATUS(heads::check_overlap(C_, op, in, 5, out, 2));
     if (numel(q) == 0) return QSML_OK;
     if (few_queries(p)) return forward_few(C_, p);
-    return forward_simt(C_, p);
+    return tc_takes(p) ? forward_tc(C_, p) : forward_simt(C_, p);
 } QSML_NO_THROW
 
 extern "C" qsml_status_t qsml_attention_backward(qsml_ctx* handle, const qsml_tdesc* q, const qsml_tdesc* k, const qsml_tdesc* v,

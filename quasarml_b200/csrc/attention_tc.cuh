@@ -1,0 +1,187 @@
+// What the tensor cores' attention kernels share: tiles of 128 tokens of a head by TMA, and
+// products of them.
+//
+// A tile is DP / 64 boxes of 128 rows x 64 columns (128 bytes a row, 128-byte swizzle, columns
+// past D zero).  The same tile serves as a K-major operand (its columns summed over: scores) and
+// as an MN-major one (its tokens summed over: what is multiplied by P or dS), which come as the
+// A operand from TMEM, where the threads that compute them leave them as pairs of binary16.
+#pragma once
+
+#include "attention.cuh"
+#include "packed.cuh"
+#include "tcgen05.cuh"
+
+namespace qsml {
+namespace attn {
+
+using namespace tc;
+
+constexpr int TILE = 128;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int DP> struct TileOf {
+    static constexpr int BOX = TILE * 128, BOXES = DP / 64, BYTES = BOX * BOXES;
+};
+
+// A view's tensor map {columns, tokens, heads, sequences} and which of the last two it moves along.
+struct HeadMap {
+    CUtensorMap map;
+    int sh, sb;
+};
+
+inline bool mappable(const View& v, int D, int S, int H, int B) {
+    const int64_t most = int64_t(1) << 39;
+    auto ok = [&](int64_t s, int64_t n) { return n == 1 || (s >= 0 && s * 2 < most); };
+    return D % 8 == 0 && D <= 128 && heads::rows_on(v, 2, 16) && ok(v.s, S) && ok(v.h, H) && ok(v.b, B) && (S == 1 || v.s > 0);
+}
+
+inline bool make_head_map(HeadMap* m, const View& v, int D, int S, int H, int B) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    // a dim that is not moved along has extent 1
+    m->sh = H > 1 && v.h > 0;
+    m->sb = B > 1 && v.b > 0;
+    const cuuint64_t row = static_cast<cuuint64_t>(D) * 2;
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), m->sh ? static_cast<cuuint64_t>(H) : 1,
+                          m->sb ? static_cast<cuuint64_t>(B) : 1};
+    cuuint64_t strides[3] = {S > 1 ? static_cast<cuuint64_t>(v.s) * 2 : row, m->sh ? static_cast<cuuint64_t>(v.h) * 2 : row,
+                             m->sb ? static_cast<cuuint64_t>(v.b) * 2 : row};
+    cuuint32_t box[4] = {64, TILE, 1, 1}, step[4] = {1, 1, 1, 1};
+    return fn(&m->map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows [row, row + 128) of head h of sequence b.
+template <int DP> __device__ __forceinline__ void load_tile(uint32_t dst, const HeadMap& m, uint32_t bar, int row, int h, int b) {
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+            ::"r"(dst + i * TileOf<DP>::BOX), "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(i * 64), "r"(row), "r"(m.sh ? h : 0), "r"(m.sb ? b : 0),
+            "r"(bar)
+            : "memory");
+}
+
+// Rows of a landed tile that are not tokens of [0, sink) or [lo, hi) become zeros (a row's 128
+// bytes lie together whatever the swizzle); by one warp.
+template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, int row0, int sink, int lo, int hi) {
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < TILE; ++r) {
+        const int row = row0 + r;
+        if (row < hi && (row >= lo || row < sink)) continue;
+        if (lane < 8 * (DP / 64)) {
+            const uint32_t a = tile + (lane >> 3) * TileOf<DP>::BOX + r * 128 + (lane & 7) * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// binary16 x binary16 -> binary32, M = 128: both operands K-major with N = 128 (scores), or B
+// MN-major with N = DP (sums over tokens).
+constexpr uint32_t IDESC_SCORES = (1u << 4) | (uint32_t(TILE >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
+template <int DP> constexpr uint32_t IDESC_SUMS = (1u << 4) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
+
+// d = a b^T over the columns of two tiles.
+template <int DP> __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t at = (k / 4) * TileOf<DP>::BOX + (k % 4) * 32;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d), "l"(smem_desc(a + at, 16, 1024)), "l"(smem_desc(b + at, 16, 1024)), "r"(IDESC_SCORES), "r"(k ? 1 : 0)
+            : "memory");
+    }
+}
+
+// d (+)= p x: p [128, 128] binary16 in TMEM, x a tile summed over its tokens.
+template <int DP> __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t p, uint32_t x, bool add) {
+#pragma unroll
+    for (int k = 0; k < TILE / 16; ++k)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+            ::"r"(d), "r"(p + k * 8), "l"(smem_desc(x + k * 16 * 128, TileOf<DP>::BOX, 1024)), "r"(IDESC_SUMS<DP>), "r"(add || k ? 1 : 0)
+            : "memory");
+}
+
+// 32 columns of this thread's TMEM lane, to be used after tmem_wait on them.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// Waits for this thread's loads; ties the registers so that no use is moved before it.
+__device__ __forceinline__ void tmem_wait(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+// 16 columns from registers; visible to the tensor core after tmem_st_wait and the fences.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One lane waits, the warp follows its result.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, limit) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// A row of binary32 sums in TMEM, times f, as binary16 to `to` (null: nowhere), D columns.
+template <int DP> __device__ __forceinline__ void store_row(uint32_t taddr, float f, __half* to, int D) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+        if (c >= D) break;
+        uint32_t r[32];
+        tmem_ld32_start(taddr + c, r);
+        tmem_wait(r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (to && c + 8 * j < D) {
+                uint4 w;
+                uint32_t* h = &w.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    h[e] = half2_of(__uint_as_float(r[8 * j + 2 * e]) * f, __uint_as_float(r[8 * j + 2 * e + 1]) * f);
+                *reinterpret_cast<uint4*>(to + c + 8 * j) = w;
+            }
+    }
+}
+__device__ __forceinline__ void zero_row(__half* to, int D) {
+    for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace attn
+}  // namespace qsml

@@ -107,6 +107,7 @@ SIZES = [  # sq, sk, hq, hk, D, window, sinks
     (513, 513, 2, 1, 96, 130, 130), (100, 400, 2, 2, 80, 0, 0), (90, 700, 4, 1, 128, 64, 7), (150, 90, 2, 1, 64, 0, 0),
     (200, 130, 1, 1, 128, 33, 2), (640, 640, 1, 1, 128, 0, 0), (333, 333, 2, 1, 40, 77, 1), (65, 65, 3, 3, 8, 0, 0),
     (130, 130, 2, 1, 200, 60, 5), (140, 140, 1, 1, 256, 0, 0), (75, 75, 2, 1, 33, 20, 2), (385, 1000, 1, 1, 128, 500, 0),
+    (1000, 1000, 1, 1, 64, 0, 0), (700, 1500, 2, 1, 64, 600, 300), (900, 900, 1, 1, 128, 0, 0), (777, 777, 2, 1, 104, 300, 140),
 ]
 
 
