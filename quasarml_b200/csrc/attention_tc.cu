@@ -227,10 +227,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool partial = k0 + TILE - 1 > first_pos || qt + TILE > seq.nq ||
                                  (p.window && last_pos - k0 >= p.window && k0 + TILE > p.sinks);
             if (partial) {
-                const int hi = row_hi - k0, lo = row_lo - k0, sink = p.sinks - k0;
+                const int hi = row_hi - k0 + 1, lo = row_lo - k0, sink = min(p.sinks - k0, hi);
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (i > hi || (i < lo && i >= sink)) r[i] = 0xff800000u;
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t seen = (below(hi - 32 * g) & ~below(lo - 32 * g)) | below(sink - 32 * g);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[32 * g + i] = seen & (1u << i) ? r[32 * g + i] : 0xff800000u;
+                }
             }
             float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

@@ -65,12 +65,12 @@ template <int DP> __device__ __forceinline__ void load_tile(uint32_t dst, const 
 // Rows of a landed tile that are not tokens of [0, sink) or [lo, hi) become zeros (a row's 128
 // bytes lie together whatever the swizzle); by one warp.
 template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, int row0, int sink, int lo, int hi) {
-    const int lane = threadIdx.x & 31;
-    for (int r = 0; r < TILE; ++r) {
+    for (int r = threadIdx.x & 31; r < TILE; r += 32) {
         const int row = row0 + r;
         if (row < hi && (row >= lo || row < sink)) continue;
-        if (lane < 8 * (DP / 64)) {
-            const uint32_t a = tile + (lane >> 3) * TileOf<DP>::BOX + r * 128 + (lane & 7) * 16;
+#pragma unroll
+        for (int i = 0; i < 8 * (DP / 64); ++i) {
+            const uint32_t a = tile + (i >> 3) * TileOf<DP>::BOX + r * 128 + ((i + r) & 7) * 16;  // lanes in different banks
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
         }
     }
@@ -147,6 +147,8 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 below 2^-126
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The bits below n (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
