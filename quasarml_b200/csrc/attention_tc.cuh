@@ -78,34 +78,42 @@ template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, int 
     __syncwarp();
 }
 
-// binary16 x binary16 -> binary32, M = 128: both operands K-major with N = 128 (scores), or B
+// binary16 x binary16 -> binary32, M = 128: both operands K-major (scores), or B
 // MN-major with N = DP (sums over tokens).
-constexpr uint32_t IDESC_SCORES = (1u << 4) | (uint32_t(TILE >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
+template <int N> constexpr uint32_t IDESC_SCORES = (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
 template <int DP> constexpr uint32_t IDESC_SUMS = (1u << 4) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
 
-// d = a b^T over the columns of two tiles.
-template <int DP> __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+// A descriptor moved on by `bytes`: its address field stays below 2^14 in 16 bytes.
+__device__ __forceinline__ uint64_t desc_on(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
+// A tile as operand of scores (columns summed over) and of sums (tokens summed over).
+__device__ __forceinline__ uint64_t score_desc(uint32_t tile) { return smem_desc(tile, 16, 1024); }
+template <int DP> __device__ __forceinline__ uint64_t sum_desc(uint32_t tile) { return smem_desc(tile, TileOf<DP>::BOX, 1024); }
+
+// d = a b^T over the columns of a tile and N rows of another.
+template <int DP, int N> __device__ __forceinline__ void mma_scores(bool issue, uint32_t d, uint64_t a, uint64_t b) {
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
         const uint32_t at = (k / 4) * TileOf<DP>::BOX + (k % 4) * 32;
+        if (issue)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "setp.ne.b32 p, %4, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d), "l"(smem_desc(a + at, 16, 1024)), "l"(smem_desc(b + at, 16, 1024)), "r"(IDESC_SCORES), "r"(k ? 1 : 0)
+            ::"r"(d), "l"(desc_on(a, at)), "l"(desc_on(b, at)), "r"(IDESC_SCORES<N>), "r"(k ? 1 : 0)
             : "memory");
     }
 }
 
-// d (+)= p x: p [128, 128] binary16 in TMEM, x a tile summed over its tokens.
-template <int DP> __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t p, uint32_t x, bool add) {
+// d (+)= p x: p [128, N] binary16 in TMEM, x N rows of a tile, summed over.
+template <int DP, int N> __device__ __forceinline__ void mma_sums(bool issue, uint32_t d, uint32_t p, uint64_t x, bool add) {
 #pragma unroll
-    for (int k = 0; k < TILE / 16; ++k)
+    for (int k = 0; k < N / 16; ++k)
+        if (issue)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "setp.ne.b32 p, %4, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-            ::"r"(d), "r"(p + k * 8), "l"(smem_desc(x + k * 16 * 128, TileOf<DP>::BOX, 1024)), "r"(IDESC_SUMS<DP>), "r"(add || k ? 1 : 0)
+            ::"r"(d), "r"(p + k * 8), "l"(desc_on(x, k * 16 * 128)), "r"(IDESC_SUMS<DP>), "r"(add || k ? 1 : 0)
             : "memory");
 }
 
@@ -142,6 +150,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over NaN
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 below 2^-126
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,11 +167,15 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One lane waits, the warp follows its result.
+// The producer and MMA warps run their loops with all lanes, so that addresses and
+// descriptors stay in uniform registers; one lane of them issues.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
-    int ok = 0;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, limit) ? 1 : 0;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)) != 0;
 }
 
 // A row of binary32 sums in TMEM, times f, as binary16 to `to` (null: nowhere), D columns.
