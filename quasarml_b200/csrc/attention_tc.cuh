@@ -157,14 +157,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
 }
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 below 2^-126
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 // The bits below n (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t half2_of(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {  // in the order written, as exp2_fast
+    uint32_t h;
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
+    return h;
 }
 
 // The producer and MMA warps run their loops with all lanes, so that addresses and
