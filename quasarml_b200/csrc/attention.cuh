@@ -38,7 +38,6 @@ __device__ __forceinline__ bool sees(const Problem& a, int p, int j) {
 // with sink <= lo.
 struct Keys {
     int sink, lo, hi;
-    Keys() = default;
     __device__ __forceinline__ Keys(const Problem& a, int nk, int p0, int p1) {
         hi = max(min(nk, p1 + 1), 0);
         lo = a.window && p0 >= a.window ? p0 - a.window + 1 : 0;

@@ -1,67 +1,58 @@
 // Attention on the tensor cores (binary16, heads of up to 128 columns).
 //
-// A CTA takes NT tiles of 128 queries of a head and goes once over the keys that they see, in
-// tiles of 128.  For each tile of queries S = Q K^T goes to TMEM; 128 threads, a row each, turn it
-// into P = 2^(S c - m c + 6) with the row's running maximum m and leave P as binary16 where S was;
-// O += P V stays in TMEM.  P is multiplied in two parts, the first while the second's exponentials
-// are computed.  A row's O and sum are multiplied by 2^((m_old - m) c) only where m has grown by
-// more than 2^8 since they were last: P then stays below 2^14, and the factor 2^6 keeps weights
-// down to 2^-20 of the largest in binary16's normal range; both cancel in the end.
-// Bound by the way from S over P and P V to the next S, which two tiles of queries walk in turn:
-// up to 64 columns as two CTAs a SM, with 128, which fill shared memory and TMEM (two S and two O
-// of 128 columns), in one CTA, whose tiles share the loads.  Two buffers of S of 64 keys each
-// instead take the products of 64 columns beyond their time (512 -> 609 us at 8192 tokens of 32
-// heads); a part of the exponentials on the FMA pipe gains nothing.
-// Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, a warpgroup a tile has the rows and the
-// registers that the first warpgroup gives up.  Values that no row of the CTA sees are cleared in
-// shared memory, since a weight of 0 does not cancel what is not finite.
+// A CTA takes 128 queries of a head and goes once over the keys that they see, in tiles of 128.
+// S = Q K^T goes to TMEM; 128 threads, a row each, turn it into P = 2^(S c - m c + 6) with the row's
+// running maximum m and leave P as binary16 where S was; O += P V stays in TMEM.  P is multiplied
+// in two parts, the first while the second's exponentials are computed.  A row's O and sum are
+// multiplied by 2^((m_old - m) c) only where m has grown by more than 2^8 since they were last: P
+// then stays below 2^14, and the factor 2^6 keeps weights down to 2^-20 of the largest in
+// binary16's normal range; both cancel in the end.
+// Bound by the way from S over P and P V to the next S (2400 cycles, of which the exponentials
+// take 1024 and the products of 128 columns as many), which two CTAs on a SM walk in turn: each
+// has half of TMEM and of shared memory, with 128 columns one tile of K and one of V, the next
+// loaded while the other is in use.  Measured at 8192 tokens of 32 heads over 8, 128 columns:
+// 500 us, 1100 TFLOP/s.  One CTA with two tiles of queries that share the loads: 495, but 67 us
+// instead of 53 for one head of 4096 tokens; two buffers of S with 64 keys each: 609; a quarter
+// of the exponentials on the FMA pipe: no gain.
+// Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, the second warpgroup has the rows and
+// the registers that the first gives up.  Values that no row of the CTA sees are cleared in shared
+// memory, since a weight of 0 does not cancel what is not finite.
 #include "attention_tc.cuh"
 
 namespace qsml {
 namespace attn {
 namespace {
 
-template <int DP, int NT> struct Fwd {
-    static constexpr int THREADS = 128 * (1 + NT);
-    static constexpr int STAGES = DP == 128 ? 4 : NT == 1 ? 5 : 8;
+constexpr int kThreads = 256;
+
+template <int DP> struct Fwd {
+    static constexpr int STAGES = DP == 128 ? 2 : 5;
     static constexpr int PARTS = 2;
-    static constexpr int BARS = 2 * STAGES + 5 + NT * (1 + PARTS);
-    static constexpr uint32_t TMEM = 256 * NT;  // 128 columns of S a tile, then DP of O
-    // registers a thread: 3 x 168 or 2 x 128 warpgroups' worth in all
-    static constexpr int FEW = NT == 2 ? 56 : 40, MANY = NT == 2 ? 224 : 216;
-    static constexpr size_t SMEM = (NT + STAGES) * size_t(TileOf<DP>::BYTES) + 1024 + 8 * BARS + 16;
-    static_assert(SMEM <= (NT == 1 ? 116224 : 232448), "shared memory");
+    static constexpr int BARS = 2 * STAGES + 5 + PARTS;
+    static constexpr uint32_t TMEM = 256;  // 128 columns of S, then DP of O
+    static constexpr int FEW = 40, MANY = 216;  // registers a thread of the warpgroups, of 2 x 128
+    static constexpr size_t SMEM = (1 + STAGES) * size_t(TileOf<DP>::BYTES) + 1024 + 8 * BARS + 16;
+    static_assert(2 * (SMEM + 1024) <= 233472, "shared memory of two CTAs");
 };
 
 struct FwdMaps {
     HeadMap q, k, v;
 };
 
-// The keys of one tile of 128 queries that starts at q0, none where no query is there.
-__device__ __forceinline__ Keys keys_of(const Problem& p, const Seq& s, int q0) {
-    const int off = s.nk - s.nq, last = min(q0 + TILE, s.nq) - 1;
-    Keys k(p, s.nk, q0 + off, q0 < s.nq ? last + off : -1);
-    if (q0 >= s.nq) k.sink = k.lo = k.hi = 0;
-    return k;
-}
-// Whether any key of the tile at k0 is among them.
-__device__ __forceinline__ bool meets(const Keys& k, int k0) { return k0 < k.hi && (k0 + TILE > k.lo || k0 < k.sink); }
-
-template <int DP, int NT>
-__global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 2)
     k_attention_tc(const __grid_constant__ Problem p, const __grid_constant__ FwdMaps maps, int tiles, int* status) {
-    using L = Fwd<DP, NT>;
+    using L = Fwd<DP>;
     constexpr int BYTES = TileOf<DP>::BYTES, STAGES = L::STAGES, PARTS = L::PARTS;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    auto q_tile = [&](int t) { return base + t * BYTES; };
-    auto ring = [&](int s) { return base + (NT + s) * BYTES; };
-    const uint32_t bars = base + (NT + STAGES) * BYTES;
+    const uint32_t q_tile = base;
+    auto ring = [&](int s) { return base + (1 + s) * BYTES; };
+    const uint32_t bars = base + (1 + STAGES) * BYTES;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (STAGES + s); };
-    const uint32_t q_full = bars + 8u * (2 * STAGES), land = q_full + 8, drain = q_full + 16, o_full = q_full + 24;
-    auto s_full = [&](int t) { return q_full + 32 + 8u * t; };
-    auto p_full = [&](int t, int part) { return q_full + 32 + 8u * (NT + PARTS * t + part); };
+    const uint32_t q_full = bars + 8u * (2 * STAGES), land = q_full + 8, drain = q_full + 16, o_full = q_full + 24, s_full = q_full + 32;
+    auto p_full = [&](int part) { return q_full + 40 + 8u * part; };
     unsigned char* misc = smem_raw + (bars - raw) + 8 * L::BARS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
@@ -76,10 +67,8 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
         mbar_init(land, 1);
         mbar_init(drain, 1);
         mbar_init(o_full, 1);
-        for (int t = 0; t < NT; ++t) {
-            mbar_init(s_full(t), 1);
-            for (int i = 0; i < PARTS; ++i) mbar_init(p_full(t, i), 4);  // one arrival a warp
-        }
+        mbar_init(s_full, 1);
+        for (int i = 0; i < PARTS; ++i) mbar_init(p_full(i), 4);  // one arrival a warp
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -97,13 +86,11 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
 
     // the last queries, with the most keys, first
     const int b = blockIdx.x / p.Hq / tiles, rest = blockIdx.x - b * p.Hq * tiles;
-    const int q0 = (tiles - 1 - rest / p.Hq) * NT * TILE, h = rest % p.Hq, hk = h / p.G;
+    const int q0 = (tiles - 1 - rest / p.Hq) * TILE, h = rest % p.Hq, hk = h / p.G;
     const Seq seq(p, b);
     const int off = seq.nk - seq.nq;
-    Keys keys[NT] = {keys_of(p, seq, q0)};
-    if constexpr (NT == 2) keys[1] = keys_of(p, seq, q0 + TILE);
-    const Keys all(p, seq.nk, q0 + off, min(q0 + NT * TILE, seq.nq) - 1 + off);
-    const Tiles list(all, TILE);
+    const Keys keys(p, seq.nk, q0 + off, min(q0 + TILE, seq.nq) - 1 + off);
+    const Tiles list(keys, TILE);
     const int steps = q0 < seq.nq ? list.n : 0;
 
     if (warp < 4) {
@@ -113,16 +100,15 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
             uint32_t land_phase = 0;
             bool ok = true, land_open = false;
             if (issue) {
-                const int n = NT == 2 && q0 + TILE < seq.nq ? 2 : 1;
-                mbar_expect_tx(q_full, n * BYTES);
-                for (int t = 0; t < n; ++t) load_tile<DP>(q_tile(t), maps.q, q_full, q0 + t * TILE, h, b);
+                mbar_expect_tx(q_full, BYTES);
+                load_tile<DP>(q_tile, maps.q, q_full, q0, h, b);
             }
             int stage = 0;
             uint32_t phase = 0, flying = 0;  // slots whose last load has no other wait
             for (int n = 0; n < steps && ok; ++n) {
                 const int k0 = list.tile(n) * TILE;
                 // rows of V that nobody sees
-                const bool ragged = k0 + TILE > all.hi || (k0 < all.lo && k0 + TILE > all.sink);
+                const bool ragged = k0 + TILE > keys.hi || (k0 < keys.lo && k0 + TILE > keys.sink);
                 for (int i = 0; i < 2; ++i) {
                     ok = warp_wait(empty(stage), phase ^ 1u, abort_flag, limit);
                     if (!ok) break;
@@ -135,7 +121,7 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
                         land_open = !ok;
                         if (!ok) break;
                         land_phase ^= 1u;
-                        clear_rows<DP>(ring(stage), k0, all.sink, all.lo, all.hi);
+                        clear_rows<DP>(ring(stage), k0, keys.sink, keys.lo, keys.hi);
                         if (issue) mbar_arrive(full(stage));
                         flying &= ~(1u << stage);
                     } else {
@@ -161,47 +147,38 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
         } else if (warp == 1 && steps > 0) {
             const bool issue = elect_one();
             bool ok = warp_wait(q_full, 0, abort_flag, limit);
-            int waiting[NT], count[NT];  // the step whose P is still to be multiplied, or -1; steps begun
-#pragma unroll
-            for (int t = 0; t < NT; ++t) waiting[t] = -1, count[t] = 0;
             auto slot = [&](int i) { return i % STAGES; };
             auto turn = [&](int i) { return static_cast<uint32_t>(i / STAGES) & 1u; };
-            // O += P V of the step before, then S = Q K^T: MMAs are executed in the order of their
-            // issue, so P has been read when S is written over it.
-            auto sums = [&](int t) {
-                const int v = 2 * waiting[t] + 1, i = count[t] - 1;
-                if (!warp_wait(full(slot(v)), turn(v), abort_flag, limit)) return false;
-                const uint64_t x = sum_desc<DP>(ring(slot(v)));
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    constexpr int N = TILE / PARTS;
-                    if (!warp_wait(p_full(t, part), i & 1, abort_flag, limit)) return false;
-                    tc_fence_after();
-                    mma_sums<DP, N>(issue, tmem + NT * TILE + t * DP, tmem + t * TILE + part * N / 2, desc_on(x, part * N * 128), i > 0 || part > 0);
+            // S = Q K^T of step n, after O += P V of the one before: MMAs are executed in the order of
+            // their issue, so P has been read when S is written over it.
+            for (int n = 0; n <= steps && ok; ++n) {
+                if (n < steps) {
+                    ok = warp_wait(full(slot(2 * n)), turn(2 * n), abort_flag, limit);
+                    if (!ok) break;
                 }
-                return true;
-            };
-            for (int n = 0; n < steps && ok; ++n) {
-                const int k0 = list.tile(n) * TILE;
-                ok = warp_wait(full(slot(2 * n)), turn(2 * n), abort_flag, limit);
+                if (n > 0) {
+                    const int v = 2 * n - 1;
+                    ok = warp_wait(full(slot(v)), turn(v), abort_flag, limit);
+                    const uint64_t x = sum_desc<DP>(ring(slot(v)));
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        constexpr int N = TILE / PARTS;
+                        ok = ok && warp_wait(p_full(part), (n - 1) & 1, abort_flag, limit);
+                        if (!ok) break;
+                        tc_fence_after();
+                        mma_sums<DP, N>(issue, tmem + TILE, tmem + part * N / 2, desc_on(x, part * N * 128), n > 1 || part > 0);
+                    }
+                    if (!ok) break;
+                    if (issue) mma_commit(empty(slot(v)));
+                }
+                if (n == steps) break;
                 tc_fence_after();
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (ok && waiting[t] >= 0) ok = sums(t);
-                    waiting[t] = -1;
-                    if (!ok || !meets(keys[t], k0)) continue;
-                    mma_scores<DP, TILE>(issue, tmem + t * TILE, score_desc(q_tile(t)), score_desc(ring(slot(2 * n))));
-                    if (issue) mma_commit(s_full(t));
-                    waiting[t] = n;
-                    ++count[t];
+                mma_scores<DP, TILE>(issue, tmem, score_desc(q_tile), score_desc(ring(slot(2 * n))));
+                if (issue) {
+                    mma_commit(s_full);
+                    mma_commit(empty(slot(2 * n)));
                 }
-                if (!ok || !issue) continue;
-                mma_commit(empty(slot(2 * n)));
-                if (n > 0) mma_commit(empty(slot(2 * n - 1)));
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-                if (ok && waiting[t] >= 0) ok = sums(t);
             if (ok && issue) mma_commit(o_full);
             if (issue) mma_commit(drain);
             const long long t0 = clock64();
@@ -210,23 +187,18 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::MANY));
-        const int t = NT == 2 ? (warp - 4) >> 2 : 0, quarter = warp & 3, row = quarter * 32 + lane;
-        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_at = tmem + lanes + t * TILE, o_at = tmem + lanes + NT * TILE + t * DP;
-        const int qt = q0 + t * TILE, q = qt + row;
+        const int quarter = warp & 3, q = q0 + quarter * 32 + lane;
+        const uint32_t s_at = tmem + (static_cast<uint32_t>(quarter * 32) << 16), o_at = s_at + TILE;
         const float c = p.scale * kLog2e;
         // the row's keys: [row_lo, row_hi] and those below p.sinks
         const int pos = q + off;
         const int row_hi = q < seq.nq ? pos : -1, row_lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
-        const int first_pos = qt + off, last_pos = min(qt + TILE, seq.nq) - 1 + off;
-        const Keys mine = keys[t];
+        const int first_pos = q0 + off, last_pos = min(q0 + TILE, seq.nq) - 1 + off;
         float m = -INFINITY, l = 0.0f;
-        uint32_t i = 0;  // steps done
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
             const int k0 = list.tile(n) * TILE;
-            if (!meets(mine, k0)) continue;
-            ok = warp_wait(s_full(t), i & 1u, abort_flag, limit);
+            ok = warp_wait(s_full, n & 1, abort_flag, limit);
             if (!ok) break;
             tc_fence_after();
             uint32_t r[TILE];
@@ -234,7 +206,7 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
             for (int g = 0; g < TILE; g += 32) tmem_ld32_start(s_at + g, r + g);
 #pragma unroll
             for (int g = 0; g < TILE; g += 32) tmem_wait(r + g);
-            const bool partial = k0 + TILE - 1 > first_pos || qt + TILE > seq.nq ||
+            const bool partial = k0 + TILE - 1 > first_pos || q0 + TILE > seq.nq ||
                                  (p.window && last_pos - k0 >= p.window && k0 + TILE > p.sinks);
             if (partial) {  // as bits: compares of every element became branches, 5 us a tile
                 const int hi = row_hi - k0 + 1, lo = row_lo - k0, sink = min(p.sinks - k0, hi);
@@ -256,7 +228,7 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
                 const float f = grow ? exp2_fast((m - top) * c) : 1.0f;
                 if (grow) m = top;
                 l *= f;
-                if (i > 0) {  // the P V before had been added when S came
+                if (n > 0) {  // the P V before had been added when S came
 #pragma unroll
                     for (int d = 0; d < DP; d += 32) {
                         uint32_t o[32];
@@ -296,17 +268,16 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(p_full(t, (k + 1) / (PAIRS / PARTS) - 1));
+                        if (lane == 0) mbar_arrive(p_full((k + 1) / (PAIRS / PARTS) - 1));
                     }
                 }
             }
             l += sum2(add2(sum[0], sum[1]));
-            ++i;
         }
-        const bool begun = i > 0;
+        const bool begun = steps > 0;
         if (ok && begun) ok = warp_wait(o_full, 0, abort_flag, limit);
         tc_fence_after();
-        if (ok && qt < p.Sq) {
+        if (ok) {
             __half* to = q < p.Sq ? reinterpret_cast<__half*>(p.o.p) + b * p.o.b + q * p.o.s + h * p.o.h : nullptr;
             const bool any = l > 0.0f || isnan(l);
             if (begun)
@@ -326,18 +297,18 @@ __global__ void __launch_bounds__(Fwd<DP, NT>::THREADS, NT == 1 ? 2 : 1)
     }
 }
 
-template <int DP, int NT> qsml_status_t forward(Context* ctx, const Problem& p) {
-    using L = Fwd<DP, NT>;
+template <int DP> qsml_status_t forward(Context* ctx, const Problem& p) {
+    using L = Fwd<DP>;
     FwdMaps maps;
     if (!make_head_map(&maps.q, p.q, p.D, p.Sq, p.Hq, p.B) || !make_head_map(&maps.k, p.k, p.D, p.Sk, p.Hk, p.B) ||
         !make_head_map(&maps.v, p.v, p.D, p.Sk, p.Hk, p.B))
         return set_error(ctx, QSML_E_CUDA, "qsml_attention: cuTensorMapEncodeTiled failed");
     const char* name = "k_attention_tc";
-    const auto kernel = k_attention_tc<DP, NT>;
-    const int tiles = (p.Sq + NT * TILE - 1) / (NT * TILE);
+    const auto kernel = k_attention_tc<DP>;
+    const int tiles = (p.Sq + TILE - 1) / TILE;
     if (static_cast<int64_t>(tiles) * p.Hq * p.B > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::SMEM)), name));
-    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * p.Hq * p.B)), dim3(L::THREADS), L::SMEM, ctx->stream, p, maps, tiles,
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * p.Hq * p.B)), dim3(kThreads), L::SMEM, ctx->stream, p, maps, tiles,
                                      ctx->status);
     if (e != cudaSuccess) return check_cuda(ctx, e, name);
     return after_launch(ctx, name);
@@ -350,7 +321,7 @@ bool tc_takes(const Problem& p) {
            mappable(p.v, p.D, p.Sk, p.Hk, p.B) && heads::rows_on(p.o, 2, 16);
 }
 
-qsml_status_t forward_tc(Context* ctx, const Problem& p) { return p.D <= 64 ? forward<64, 1>(ctx, p) : forward<128, 2>(ctx, p); }
+qsml_status_t forward_tc(Context* ctx, const Problem& p) { return p.D <= 64 ? forward<64>(ctx, p) : forward<128>(ctx, p); }
 
 }  // namespace attn
 }  // namespace qsml
