@@ -165,6 +165,7 @@ extern "C" qsml_status_t qsml_attention_backward(qsml_ctx* handle, const qsml_td
     if (numel(q) == 0) p.dq.p = nullptr;
     if (numel(k) == 0) p.dk.p = p.dv.p = nullptr;
     if (!p.dq.p && !p.dk.p && !p.dv.p) return QSML_OK;
+    if (tc_takes_backward(p)) return backward_tc(C_, p);
     Workspace ws(C_);
     void* delta = nullptr;
     QSML_TRY_STATUS(ws.get(sizeof(float) * p.B * p.Hq * static_cast<size_t>(p.Sq), &delta));

@@ -83,6 +83,9 @@ qsml_status_t backward_simt(Context* ctx, const Problem& p, const float* delta);
 // o and lse by the tensor cores (attention_tc.cu), where tc_takes: F16, rows on 16 bytes, up to 128 columns.
 bool tc_takes(const Problem& p);
 qsml_status_t forward_tc(Context* ctx, const Problem& p);
+// dq, dk, dv by the tensor cores (attention_tc_bwd.cu).
+bool tc_takes_backward(const Problem& p);
+qsml_status_t backward_tc(Context* ctx, const Problem& p);
 // Few queries over many keys (attention_few.cu).
 bool few_queries(const Problem& p);
 qsml_status_t forward_few(Context* ctx, const Problem& p);

@@ -138,18 +138,23 @@ class Attention:
 
     def backward(self, o, lse, do):
         """(dq, dk, dv) and their bounds, from the o and lse given.  P as in forward (lse is an input);
-        dP and delta are off by (D + 100) u of their terms; F16 rounds P (2^-11, 2^-25 at least) and dS
-        (2^-11; below 2^-39 of a bound on the largest, 2 |dout| |v|, bits go: the power of two brings that
-        bound to 2^14 at least and a step of the smallest numbers is 2^-25)."""
+        dP and delta are off by (D + 100) u of their terms.  delta is sum(P dP) = sum(dout o), which the
+        operator may take either way: o is rounded by half a step of its type, so the second differs from the
+        first by at most that of sum|dout||o| (2^-11; binary32's 2^-24 is within the 100 u).  F16 rounds P
+        (2^-11, 2^-25 at least) and dS (2^-11; below 2^-39 of a bound on the largest, 2 |dout| |v|, bits go:
+        the power of two brings that bound to 2^14 at least and a step of the smallest numbers is 2^-25)."""
         live = self.seen.any(1)[:, None]
         do, o = np.where(live, do.astype(F64), 0.0), np.where(live, o.astype(F64), 0.0)
         lse = np.where(live, lse.astype(F64)[:, None], 0.0)
         D = self.q.shape[1]
         p = np.where(self.seen, np.exp(np.where(self.seen, self.z, 0.0) - lse), 0.0)
-        dp, delta = do @ self.v.T, (do * o).sum(1, keepdims=True)
+        dp = do @ self.v.T
+        delta = (p * dp).sum(1, keepdims=True)
         ds = p * (dp - delta)
         ep = self.es + 6 * U * np.abs(lse) + 8 * U
         ed = (D + 100) * U * (np.abs(do) @ np.abs(self.v).T + (np.abs(do) * np.abs(o)).sum(1, keepdims=True))
+        if self.half:
+            ed = ed + 2.0 ** -11 * (np.abs(do) * np.abs(o)).sum(1, keepdims=True)
         eds = p * ((ep + 4 * U) * np.abs(dp - delta) + ed)
         epp = p * ep
         if self.half:
