@@ -8,10 +8,16 @@
 // Bound by HBM: each element is read and written once (backward: two read, one written).
 // A group of lanes holds a row, each lane 16 bytes of both halves of its pairs (or of
 // neighbouring pairs), so a pair never leaves its lane and the row's sums are a few
-// shuffles.  All heads of a token share its angles: the CTA computes them once, in binary64
-// (at position 10^6 a binary32 angle is off by 0.03), reduced to a turn before the binary32
-// sine and cosine.  The reference has neither.
+// shuffles.  A CTA has lanes for all heads of a token and goes from token to token, so that a
+// lane keeps its columns of the weight (and sums their gradient) in registers; the next row is
+// loaded, and the next token's angles are computed, under the present one.  Angles are shared by
+// the heads and taken in binary64 (at position 10^6 a binary32 angle is off by 0.03), less whole
+// turns, before the binary32 sine and cosine.  The reference has neither.
+#include <algorithm>
+#include <type_traits>
+
 #include "heads.cuh"
+#include "packed.cuh"
 
 namespace qsml {
 namespace {
@@ -21,10 +27,10 @@ using heads::Pack;
 using heads::to_f;
 using heads::View;
 
-constexpr int kThreads = 256;
+// Threads of a CTA, at most; two CTAs a SM keep enough rows on their way.
+constexpr int most_threads(bool backward) { return backward ? 320 : 384; }
 constexpr int kMaxAxes = 4;
 constexpr int kMaxD = 512;
-constexpr int kMaxTokens = 8;  // of one pass of a CTA
 
 struct RotaryArgs {
     View x[2], g[2], out[2];  // queries, keys; g: the outputs' gradients (backward)
@@ -36,17 +42,22 @@ struct RotaryArgs {
     const float* freq;
     int ends[kMaxAxes];  // the pairs before ends[a] go by axis a or an earlier one
     int axes;
-    int64_t T, S;  // tokens in all, and of one sequence
+    int T, S;  // tokens in all, and of one sequence
     int D, rot, pairs, w_f32;
     float eps;
 };
 
-template <typename T> __device__ __forceinline__ float weight(const void* w, int f32, int c) {
-    return f32 ? static_cast<const float*>(w)[c] : to_f(static_cast<const T*>(w)[c]);
-}
+// Sequence and place of token t.
+struct Token {
+    int b, s;
+    __device__ __forceinline__ Token(const RotaryArgs& a, int t) {
+        b = t < a.S ? 0 : static_cast<int>(static_cast<unsigned>(t) / static_cast<unsigned>(a.S));
+        s = t - b * a.S;
+    }
+};
 
-// (cos, sin) of pair i at token t.
-__device__ __forceinline__ float2 turn(const RotaryArgs& a, int64_t b, int64_t s, int i) {
+// (cos, sin) of pair i of a token.
+__device__ __forceinline__ float2 turn(const RotaryArgs& a, int b, int s, int i) {
     int axis = 0;
     while (axis + 1 < a.axes && i >= a.ends[axis]) ++axis;
     const int64_t at = b * a.pos_b + s * a.pos_s + axis * a.pos_a;
@@ -60,221 +71,326 @@ __device__ __forceinline__ float2 turn(const RotaryArgs& a, int64_t b, int64_t s
 
 // A lane's chunk pair c of a row: where its two chunks of V columns start, the first pair it
 // turns by, and whether it is turned.
-template <int V> struct Chunk {
+template <int V, bool PAIRS> struct Chunk {
     int c0, c1, pair;
     bool turned;
     __device__ __forceinline__ Chunk(const RotaryArgs& a, int c) {
         const int half = a.rot / (2 * V);
         turned = c < half;
-        if (V > 1 && a.pairs) {
-            c0 = c * 2 * V;
-            c1 = c0 + V;
-            pair = c * V;
-        } else if (V == 1 && a.pairs) {
-            c0 = 2 * c;
-            c1 = c0 + 1;
-            pair = c;
-        } else {
-            c0 = turned ? c * V : a.rot + (c - half) * 2 * V;
-            c1 = turned ? a.rot / 2 + c * V : c0 + V;
-            pair = c * V;
-        }
+        c0 = PAIRS || !turned ? (PAIRS ? c * 2 * V : a.rot + (c - half) * 2 * V) : c * V;
+        c1 = PAIRS || !turned ? c0 + V : a.rot / 2 + c * V;
+        pair = c * V;
     }
 };
 
-// Turns a chunk pair by its V angles (sign -1: back).
-template <int V> __device__ __forceinline__ void rotate(float (&p)[V], float (&q)[V], const float2 (&cs)[V], bool neighbours, float sign) {
-    auto one = [&](float& a, float& b, float2 t) {
-        const float s = sign * t.y, x = a, y = b;
-        a = fmaf(x, t.x, -(y * s));
-        b = fmaf(y, t.x, x * s);
-    };
-    if (V > 1 && neighbours) {
+// Arithmetic on V columns: packed pairs, or one number.
+__device__ __forceinline__ float mul2(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float sum2(float a) { return a; }
+template <int V> struct Cols {
+    using E = typename std::conditional<V == 1, float, P2>::type;
+    static constexpr int N = V == 1 ? 1 : V / 2;
+    E v[N];
+    static __device__ __forceinline__ E all(float a) {
+        if constexpr (V == 1)
+            return a;
+        else
+            return both(a);
+    }
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int e = 0; e + 1 < V; e += 2) {
-            one(p[e], p[e + 1], cs[e / 2]);
-            one(q[e], q[e + 1], cs[V / 2 + e / 2]);
+        for (E& x : v) x = all(0.0f);
+    }
+    template <typename T> __device__ __forceinline__ void from(const Pack<T, V>& p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if constexpr (V == 1) {
+                v[i] = to_f(p.v[i]);
+            } else if constexpr (sizeof(T) == 2) {
+                const float2 f = __half22float2(reinterpret_cast<const __half2*>(&p)[i]);
+                v[i] = pack(f.x, f.y);
+            } else
+                v[i] = pack(to_f(p.v[2 * i]), to_f(p.v[2 * i + 1]));
+    }
+    template <typename T> __device__ __forceinline__ void store(T* to) const {
+        Pack<T, V> p;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if constexpr (V == 1) {
+                from_f(v[i], p.v[i]);
+            } else {
+                const float2 f = unpack(v[i]);
+                if constexpr (sizeof(T) == 2) {
+                    reinterpret_cast<__half2*>(&p)[i] = __floats2half2_rn(f.x, f.y);
+                } else {
+                    p.v[2 * i] = f.x;
+                    p.v[2 * i + 1] = f.y;
+                }
+            }
+        *reinterpret_cast<Pack<T, V>*>(to) = p;
+    }
+};
+
+// Turns a chunk pair by V angles, their cosines and sines (BACK: by their opposites).
+template <int V, bool PAIRS, bool BACK>
+__device__ __forceinline__ void rotate(Cols<V>& p, Cols<V>& q, const float* cosine, const float* sine) {
+    const Pack<float, V> c = *reinterpret_cast<const Pack<float, V>*>(cosine), s = *reinterpret_cast<const Pack<float, V>*>(sine);
+    if constexpr (V > 1 && PAIRS) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            P2& x = e < V / 2 ? p.v[e] : q.v[e - V / 2];
+            const float2 f = unpack(x);
+            const float t = BACK ? -s.v[e] : s.v[e];
+            x = fma2(pack(f.y, f.x), pack(-t, t), mul2(x, both(c.v[e])));
         }
     } else {
+        Cols<V> cc, ss, ns;
+        cc.from(c);
 #pragma unroll
-        for (int e = 0; e < V; ++e) one(p[e], q[e], cs[e]);
+        for (int i = 0; i < Cols<V>::N; ++i) {
+            if constexpr (V == 1) {
+                ss.v[i] = s.v[i];
+                ns.v[i] = -s.v[i];
+            } else {
+                ss.v[i] = pack(s.v[2 * i], s.v[2 * i + 1]);
+                ns.v[i] = pack(-s.v[2 * i], -s.v[2 * i + 1]);
+            }
+            const auto x = p.v[i], y = q.v[i];
+            p.v[i] = fma2(y, BACK ? ss.v[i] : ns.v[i], mul2(x, cc.v[i]));
+            q.v[i] = fma2(x, BACK ? ns.v[i] : ss.v[i], mul2(y, cc.v[i]));
+        }
     }
 }
 
-template <typename T, int V> __device__ __forceinline__ void load(float (&r)[V], const T* p) {
-    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-    for (int e = 0; e < V; ++e) r[e] = to_f(v.v[e]);
-}
-template <typename T, int V> __device__ __forceinline__ void store(const float (&r)[V], T* p) {
-    Pack<T, V> v;
-#pragma unroll
-    for (int e = 0; e < V; ++e) from_f(r[e], v.v[e]);
-    *reinterpret_cast<Pack<T, V>*>(p) = v;
-}
+// How a CTA's lanes are laid over a token's rows: groups of `lanes` (a power of two), the first
+// slots[0] of them for queries, the next slots[1] for keys, each for `rounds` rows; tokens in batches, whose angles are computed together.
+struct Shape {
+    int vec, lanes, slots[2], rounds, threads, batch;
+    size_t smem;
+};
 
-// Row r of a token: head r of the queries, or r - H[0] of the keys.
-__device__ __forceinline__ int64_t row_at(const View& v, int64_t b, int64_t s, int h) { return b * v.b + s * v.s + h * v.h; }
-
-// NC chunk pairs of V columns a lane; `lanes` (a power of two) lanes a row; `tokens` tokens a
-// pass of the CTA.
-template <typename T, int V, int NC, bool BWD>
-__global__ void __launch_bounds__(kThreads) k_norm_rotary(const __grid_constant__ RotaryArgs a, int lanes, int tokens) {
-    __shared__ float2 angle[kMaxTokens * kMaxD / 2];
+// NC chunk pairs of V columns a lane.
+template <typename T, int V, int NC, bool PAIRS, bool BWD>
+__global__ void __launch_bounds__(most_threads(BWD), 2) k_norm_rotary(const __grid_constant__ RotaryArgs a, Shape sh) {
+    extern __shared__ float4 shared[];  // cosines and sines [2][batch][2][pairs]; backward: then [slots][D] partial sums
+    float* angle = reinterpret_cast<float*>(shared);
     pdl_begin();
-    const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes;
-    const int slots = kThreads / lanes / tokens;  // rows of one token in flight
-    const int sub = slot / slots, row0 = slot % slots;
-    const int pairs = a.rot / 2, rows = a.H[0] + a.H[1], chunks = a.D / (2 * V);
+    const int lane = threadIdx.x & (sh.lanes - 1), slot = threadIdx.x / sh.lanes;
+    const int which = slot < sh.slots[0] ? 0 : 1, row0 = which ? slot - sh.slots[0] : slot, step = sh.slots[which];
+    const int rows = which && row0 >= step ? 0 : a.H[which];  // lanes that fill the last warp have none
+    const int pairs = a.rot / 2, chunks = a.D / (2 * V);
     const float inv_d = 1.0f / static_cast<float>(a.D);
-    float dw[2][BWD ? NC : 1][BWD ? 2 * V : 1] = {};
-    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens; t0 < a.T; t0 += static_cast<int64_t>(gridDim.x) * tokens) {
-        const int64_t t = t0 + sub;
-        const bool here = t < a.T;
-        const int64_t b = here ? t / a.S : 0, s = here ? t - b * a.S : 0;
-        for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-            const int64_t ti = t0 + i / pairs;
-            if (ti < a.T) angle[i] = turn(a, ti / a.S, ti % a.S, i % pairs);
-        }
-        __syncthreads();
-        float2 cs[NC][V];
+    const bool normed = a.w[which] != nullptr;
+    using Chunks = Chunk<V, PAIRS>;
+    constexpr int N = Cols<V>::N;
+    Cols<V> wt[NC][2], dw[BWD ? NC : 1][2];
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const Chunk<V> c(a, lane + n * lanes);
-#pragma unroll
-            for (int e = 0; e < V; ++e) cs[n][e] = c.turned && here ? angle[sub * pairs + c.pair + e] : make_float2(1.0f, 0.0f);
-        }
-        // the group's lanes stay together: every lane of a warp goes through as many rows
-        for (int r = row0; r - row0 < rows; r += slots) {
-            const int which = r < a.H[0] ? 0 : 1;
-            const bool live = here && r < rows;
-            const int h = which ? r - a.H[0] : r;
-            const void* w = a.w[which];
-            const T* x = reinterpret_cast<const T*>(a.x[which].p) + (live ? row_at(a.x[which], b, s, h) : 0);
-            float p[NC][2][V], sq = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const Chunk<V> c(a, lane + n * lanes);
-#pragma unroll
-                for (int e = 0; e < V; ++e) p[n][0][e] = p[n][1][e] = 0.0f;
-                if (live && lane + n * lanes < chunks) {
-                    load<T, V>(p[n][0], x + c.c0);
-                    load<T, V>(p[n][1], x + c.c1);
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e) sq = fmaf(p[n][0][e], p[n][0][e], fmaf(p[n][1][e], p[n][1][e], sq));
-            }
-            float g[BWD ? NC : 1][2][V];
-            float hx = 0.0f;
-            if constexpr (BWD) {
-                const T* y = reinterpret_cast<const T*>(a.g[which].p) + (live ? row_at(a.g[which], b, s, h) : 0);
-#pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    const Chunk<V> c(a, lane + n * lanes);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) g[n][0][e] = g[n][1][e] = 0.0f;
-                    if (live && lane + n * lanes < chunks) {
-                        load<T, V>(g[n][0], y + c.c0);
-                        load<T, V>(g[n][1], y + c.c1);
-                        if (c.turned) rotate<V>(g[n][0], g[n][1], cs[n], a.pairs, -1.0f);
-                        if (w) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int e = 0; e < V; ++e)
-                                    hx = fmaf(g[n][i][e] * weight<T>(w, a.w_f32, (i ? c.c1 : c.c0) + e), p[n][i][e], hx);
-                        }
-                    }
-                }
-            }
-            for (int m = lanes >> 1; m >= 1; m >>= 1) {
-                sq += __shfl_xor_sync(0xffffffffu, sq, m);
-                if (BWD) hx += __shfl_xor_sync(0xffffffffu, hx, m);
-            }
-            const float rstd = w ? 1.0f / sqrtf(fmaf(sq, inv_d, a.eps)) : 1.0f;
-            if (!live) continue;
-            T* out = a.out[which].p ? reinterpret_cast<T*>(a.out[which].p) + row_at(a.out[which], b, s, h) : nullptr;
-            const float along = hx * rstd * rstd * inv_d;  // mean(h xh) rstd, that x takes
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                if (lane + n * lanes >= chunks) continue;
-                const Chunk<V> c(a, lane + n * lanes);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const int col = (i ? c.c1 : c.c0) + e;
-                        if constexpr (BWD) {
-                            if (w) {
-                                const float xv = p[n][i][e];
-                                if (which == 0)
-                                    dw[0][n][i * V + e] = fmaf(g[n][i][e], xv * rstd, dw[0][n][i * V + e]);
-                                else
-                                    dw[1][n][i * V + e] = fmaf(g[n][i][e], xv * rstd, dw[1][n][i * V + e]);
-                                g[n][i][e] = rstd * fmaf(-xv, along, g[n][i][e] * weight<T>(w, a.w_f32, col));
-                            }
-                        } else if (w) {
-                            p[n][i][e] = p[n][i][e] * rstd * weight<T>(w, a.w_f32, col);
-                        }
-                    }
-                if constexpr (BWD) {
-                    if (out) {
-                        store<T, V>(g[n][0], out + c.c0);
-                        store<T, V>(g[n][1], out + c.c1);
-                    }
-                } else {
-                    if (c.turned) rotate<V>(p[n][0], p[n][1], cs[n], a.pairs, 1.0f);
-                    store<T, V>(p[n][0], out + c.c0);
-                    store<T, V>(p[n][1], out + c.c1);
-                }
-            }
-        }
-        __syncthreads();
-    }
-    if constexpr (BWD) {
-        // the CTA's rows joined in the order of their slots
-        __shared__ float part[kThreads * 2 * V * NC];  // [slots of the CTA][D at most]
-        const int all = kThreads / lanes;
+    for (int n = 0; n < NC; ++n) {
+        const Chunks c(a, lane + n * sh.lanes);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            if (!a.sums[k]) continue;
-            __syncthreads();
+            if constexpr (BWD) dw[n][k].zero();
+            Pack<float, V> w;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                if (lane + n * lanes >= chunks) continue;
-                const Chunk<V> c(a, lane + n * lanes);
+            for (int e = 0; e < V; ++e) {
+                const int col = (k ? c.c1 : c.c0) + e;
+                w.v[e] = 1.0f;
+                if (normed && lane + n * sh.lanes < chunks)
+                    w.v[e] = a.w_f32 ? static_cast<const float*>(a.w[which])[col] : to_f(static_cast<const T*>(a.w[which])[col]);
+            }
+            wt[n][k].from(w);
+        }
+    }
+    // a lane's rows of the CTA's tokens come one after the other
+    Pack<T, V> nx[NC][2], ng[BWD ? NC : 1][2];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    part[slot * a.D + c.c0 + e] = dw[k][n][e];
-                    part[slot * a.D + c.c1 + e] = dw[k][n][V + e];
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                from_f(0.0f, nx[n][k].v[e]);  // what no row is read into stays 0
+                if constexpr (BWD) from_f(0.0f, ng[n][k].v[e]);
+            }
+    // the lane's first row of token 0 and the step to the next token; sequences and further rounds, which
+    // are rare, by the arguments
+    struct Base {
+        T* p;
+        int64_t s;
+        __device__ __forceinline__ Base(const View& v, int row) : p(reinterpret_cast<T*>(v.p) + row * v.h), s(v.s) {}
+        __device__ __forceinline__ T* at(const View& v, const Token& k, int more) const {
+            T* q = p + k.s * s;
+            if (k.b) q += k.b * v.b;
+            if (more) q += more * v.h;
+            return q;
+        }
+    };
+    const Base bx(a.x[which], row0), bg(a.g[which], row0), bo(a.out[which], row0);
+    const bool wanted = a.out[which].p != nullptr;
+    auto fetch = [&](int t, int r) {
+        if (t >= a.T || r >= rows) return;
+        const Token k(a, t);
+        const T* x = bx.at(a.x[which], k, r - row0);
+        const T* g = BWD ? bg.at(a.g[which], k, r - row0) : nullptr;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            if (lane + n * sh.lanes >= chunks) continue;
+            const Chunks c(a, lane + n * sh.lanes);
+            nx[n][0] = *reinterpret_cast<const Pack<T, V>*>(x + c.c0);
+            nx[n][1] = *reinterpret_cast<const Pack<T, V>*>(x + c.c1);
+            if constexpr (BWD) {
+                ng[n][0] = *reinterpret_cast<const Pack<T, V>*>(g + c.c0);
+                ng[n][1] = *reinterpret_cast<const Pack<T, V>*>(g + c.c1);
+            }
+        }
+    };
+    auto angles = [&](int t0, float* to) {
+        for (int i = threadIdx.x; i < sh.batch * pairs; i += blockDim.x) {
+            const int j = i / pairs;
+            if (j < a.T - t0) {
+                const Token k(a, t0 + j);
+                const float2 cs = turn(a, k.b, k.s, i - j * pairs);
+                to[i + j * pairs] = cs.x;
+                to[i + (j + 1) * pairs] = cs.y;
+            }
+        }
+    };
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * sh.batch;
+    int t = blockIdx.x * sh.batch;
+    fetch(t, row0);
+    angles(t, angle);
+    int buffer = 0, at = 0;  // of the angles; in the batch
+    while (t < a.T) {
+        if (at == 0) __syncthreads();
+        const bool more = at + 1 < sh.batch && t + 1 < a.T;
+        const int first = t - at, then = stride < a.T - first ? first + static_cast<int>(stride) : a.T;
+        const int after = more ? t + 1 : then;
+        const Token tk(a, t);
+        const float* cs_at = angle + 2 * (buffer * sh.batch + at) * pairs;
+        // every lane of a warp goes through as many rows
+        for (int i = 0; i < sh.rounds; ++i) {
+            const int r = row0 + i * step;
+            const bool live = r < rows;
+            Cols<V> p[NC][2], g[BWD ? NC : 1][2];
+            auto sq = Cols<V>::all(0.0f), hx = sq;
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    p[n][k].from(nx[n][k]);
+                    if constexpr (BWD) g[n][k].from(ng[n][k]);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sq = fma2(p[n][k].v[e], p[n][k].v[e], sq);
+                }
+            if (i + 1 < sh.rounds)
+                fetch(t, r + step);
+            else
+                fetch(after, row0);
+            if (i == 0 && at == 0) angles(then, angle + 2 * (buffer ^ 1) * sh.batch * pairs);
+            if constexpr (BWD) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    const Chunks c(a, lane + n * sh.lanes);
+                    if (c.turned) rotate<V, PAIRS, true>(g[n][0], g[n][1], cs_at + c.pair, cs_at + pairs + c.pair);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) hx = fma2(mul2(g[n][k].v[e], wt[n][k].v[e]), p[n][k].v[e], hx);
                 }
             }
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.D; c += kThreads) {
-                float v = 0.0f;
-                for (int i = 0; i < all; ++i) v += part[i * a.D + c];
-                a.sums[k][static_cast<int64_t>(blockIdx.x) * a.D + c] = v;
+            float square = sum2(sq), dot = sum2(hx);
+            for (int m = sh.lanes >> 1; m >= 1; m >>= 1) {
+                square += __shfl_xor_sync(0xffffffffu, square, m);
+                if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, m);
             }
+            if (!live) continue;
+            // the reciprocal root by one step of Newton's from the approximate one
+            const float var = fmaf(square, inv_d, a.eps), y0 = rsqrtf(var);
+            const float step1 = y0 * fmaf(-0.5f * (var * y0), y0, 1.5f);
+            const float rstd = !normed ? 1.0f : step1 == step1 ? step1 : y0;  // y0 is 0 or infinite
+            const float along = normed ? -dot * rstd * rstd * inv_d : 0.0f;  // -mean(h xh) rstd, that x takes
+            const auto r2 = Cols<V>::all(rstd), along2 = Cols<V>::all(along);
+            T* out = wanted ? bo.at(a.out[which], tk, r - row0) : nullptr;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                if (lane + n * sh.lanes >= chunks) continue;
+                const Chunks c(a, lane + n * sh.lanes);
+                if (normed) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            auto& x = p[n][k].v[e];
+                            const auto w = wt[n][k].v[e];
+                            if constexpr (BWD) {
+                                auto& y = g[n][k].v[e];
+                                dw[n][k].v[e] = fma2(y, mul2(x, r2), dw[n][k].v[e]);
+                                y = mul2(r2, fma2(x, along2, mul2(y, w)));
+                            } else {
+                                x = mul2(mul2(x, r2), w);
+                            }
+                        }
+                }
+                if constexpr (BWD) {
+                    if (out) {
+                        g[n][0].store(out + c.c0);
+                        g[n][1].store(out + c.c1);
+                    }
+                } else {
+                    if (c.turned) rotate<V, PAIRS, false>(p[n][0], p[n][1], cs_at + c.pair, cs_at + pairs + c.pair);
+                    p[n][0].store(out + c.c0);
+                    p[n][1].store(out + c.c1);
+                }
+            }
+        }
+        at = more ? at + 1 : 0;
+        buffer ^= !more;
+        t = after;
+    }
+    if constexpr (BWD) {
+        // the CTA's rows joined in the order of their groups
+        float* part = angle + 4 * sh.batch * pairs;
+        const int all = sh.slots[0] + sh.slots[1];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            if (lane + n * sh.lanes >= chunks || slot >= all) continue;
+            const Chunks c(a, lane + n * sh.lanes);
+            dw[n][0].store(part + slot * a.D + c.c0);
+            dw[n][1].store(part + slot * a.D + c.c1);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * a.D; i += blockDim.x) {
+            const int k = i / a.D, c = i % a.D;
+            if (!a.sums[k]) continue;
+            float v = 0.0f;
+            for (int r = k ? sh.slots[0] : 0; r < (k ? all : sh.slots[0]); ++r) v += part[r * a.D + c];
+            a.sums[k][static_cast<int64_t>(blockIdx.x) * a.D + c] = v;
         }
     }
 }
 
-template <typename T, bool BWD> qsml_status_t launch(Context* ctx, const RotaryArgs& a, int vec, unsigned grid, int lanes, int tokens) {
+template <typename T, bool BWD> qsml_status_t launch(Context* ctx, const RotaryArgs& a, const Shape& h, unsigned grid) {
     cudaError_t e = cudaSuccess;
-    const int chunks = a.D / (2 * vec);
-    const bool one = chunks <= 32;
-    auto go = [&](auto kernel) { e = launch_pdl(kernel, dim3(grid), dim3(kThreads), 0, ctx->stream, a, lanes, tokens); };
-    constexpr int FULL = 16 / sizeof(T);
-    if (vec == FULL) {
-        if constexpr (sizeof(T) == 2)
-            go(k_norm_rotary<T, FULL, 1, BWD>);
-        else
-            one ? go(k_norm_rotary<T, FULL, 1, BWD>) : go(k_norm_rotary<T, FULL, 2, BWD>);
-    } else if (vec == 2) {
-        one ? go(k_norm_rotary<T, 2, 1, BWD>) : go(k_norm_rotary<T, 2, 4, BWD>);
-    } else {
-        one ? go(k_norm_rotary<T, 1, 1, BWD>) : go(k_norm_rotary<T, 1, 8, BWD>);
-    }
+    const bool one = a.D / (2 * h.vec) <= 32;
+    auto go = [&](auto kernel) {
+        e = launch_pdl(kernel, dim3(grid), dim3(h.threads), h.smem, ctx->stream, a, h);
+    };
+    auto pairing = [&](auto pairs) {
+        constexpr bool P = decltype(pairs)::value;
+        constexpr int FULL = 16 / sizeof(T);
+        if (h.vec == FULL) {
+            if constexpr (sizeof(T) == 2)
+                go(k_norm_rotary<T, FULL, 1, P, BWD>);
+            else
+                one ? go(k_norm_rotary<T, FULL, 1, P, BWD>) : go(k_norm_rotary<T, FULL, 2, P, BWD>);
+        } else if (h.vec == 2) {
+            one ? go(k_norm_rotary<T, 2, 1, P, BWD>) : go(k_norm_rotary<T, 2, 4, P, BWD>);
+        } else {
+            one ? go(k_norm_rotary<T, 1, 1, P, BWD>) : go(k_norm_rotary<T, 1, 8, P, BWD>);
+        }
+    };
+    a.pairs ? pairing(std::true_type()) : pairing(std::false_type());
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_norm_rotary");
     return after_launch(ctx, BWD ? "k_norm_rotary_bwd" : "k_norm_rotary");
 }
@@ -352,8 +468,9 @@ qsml_status_t check_inputs(Context* ctx, const char* op, const Inputs& in, Rotar
     a->freq = static_cast<const float*>(in.freq->data);
     a->H[0] = static_cast<int>(dq->H);
     a->H[1] = static_cast<int>(dk->H);
-    a->S = dq->S;
-    a->T = dq->B * dq->S;
+    if (dq->B && dq->S > INT32_MAX / dq->B) return fail(ctx, QSML_E_UNSUPPORTED, op, "too many tokens");
+    a->S = static_cast<int>(dq->S);
+    a->T = static_cast<int>(dq->B * dq->S);
     a->D = static_cast<int>(dq->D);
     a->rot = static_cast<int>(2 * pairs);
     a->pairs = in.pairing == QSML_ROTARY_PAIRS;
@@ -387,13 +504,33 @@ int chunk_of(const RotaryArgs& a, int es, bool backward) {
     return 1;
 }
 
-// Lanes a row (a power of two), and tokens a pass: as many as keep every lane at a row.
-void shape_of(const RotaryArgs& a, int vec, int* lanes, int* tokens) {
-    const int chunks = a.D / (2 * vec);
-    *lanes = 1;
-    while (*lanes < chunks && *lanes < 32) *lanes *= 2;
-    *tokens = 1;
-    while (*tokens < kMaxTokens && kThreads / *lanes / (*tokens * 2) >= a.H[0] + a.H[1]) *tokens *= 2;
+int64_t most_ctas(Context* ctx, const Shape& h) { return static_cast<int64_t>(ctx->num_sms) * (h.threads <= 256 ? 8 : 4); }
+
+// All of a token's rows at once, or even shares of them.
+Shape shape_of(Context* ctx, const RotaryArgs& a, int es, bool backward) {
+    Shape h;
+    h.vec = chunk_of(a, es, backward);
+    const int chunks = a.D / (2 * h.vec);
+    h.lanes = 1;
+    while (h.lanes < chunks && h.lanes < 32) h.lanes *= 2;
+    h.rounds = 1;
+    for (;; ++h.rounds) {
+        for (int k = 0; k < 2; ++k) h.slots[k] = (a.H[k] + h.rounds - 1) / h.rounds;
+        if (static_cast<int64_t>(h.slots[0] + h.slots[1]) * h.lanes <= most_threads(backward)) break;
+    }
+    const int all = h.slots[0] + h.slots[1];
+    h.threads = (all * h.lanes + 31) / 32 * 32;
+    // a batch has an angle for every lane, where there are that many tokens for every CTA: the angles
+    // of a token at a time, by two of ten warps, keep the others waiting
+    const int64_t tokens = a.T / std::max<int64_t>(1, most_ctas(ctx, h));
+    h.batch = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(8, h.threads / (a.rot / 2)), tokens)));
+    h.smem = 2 * sizeof(float) * a.rot * h.batch + (backward ? sizeof(float) * all * a.D : 0);
+    return h;
+}
+
+// A batch a CTA, or as many CTAs as fill the device.
+unsigned grid_of(Context* ctx, const RotaryArgs& a, const Shape& h) {
+    return static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(a.T) + h.batch - 1) / h.batch, most_ctas(ctx, h)));
 }
 
 }  // namespace
@@ -420,13 +557,9 @@ extern "C" qsml_status_t qsml_norm_rotary(qsml_ctx* handle, const qsml_tdesc* q,
     const heads::Named out[2] = {{q_out, "q_out"}, {k_out, "k_out"}};
     QSML_TRY_STATUS(heads::check_overlap(C_, op, in, 6, out, 2, 2));
     if (a.T == 0 || a.D == 0 || a.H[0] + a.H[1] == 0) return QSML_OK;
-    const int es = dtype_size(q->dtype), vec = chunk_of(a, es, false);
-    int lanes, tokens;
-    shape_of(a, vec, &lanes, &tokens);
-    const int64_t passes = (a.T + tokens - 1) / tokens;
-    const unsigned grid = static_cast<unsigned>(passes < 1 << 20 ? passes : 1 << 20);
-    return q->dtype == QSML_F16 ? launch<__half, false>(C_, a, vec, grid, lanes, tokens)
-                                : launch<float, false>(C_, a, vec, grid, lanes, tokens);
+    const Shape h = shape_of(C_, a, dtype_size(q->dtype), false);
+    const unsigned grid = grid_of(C_, a, h);
+    return q->dtype == QSML_F16 ? launch<__half, false>(C_, a, h, grid) : launch<float, false>(C_, a, h, grid);
 } QSML_NO_THROW
 
 extern "C" qsml_status_t qsml_norm_rotary_backward(qsml_ctx* handle, const qsml_tdesc* q, const qsml_tdesc* k,
@@ -476,12 +609,8 @@ extern "C" qsml_status_t qsml_norm_rotary_backward(qsml_ctx* handle, const qsml_
     if (!dq && !dwq) a.H[0] = 0;
     if (!dk && !dwk) a.H[1] = 0;
     if (a.H[0] + a.H[1] == 0) return QSML_OK;
-    const int es = dtype_size(q->dtype), vec = chunk_of(a, es, true);
-    int lanes, tokens;
-    shape_of(a, vec, &lanes, &tokens);
-    const int64_t passes = (a.T + tokens - 1) / tokens;
-    const int64_t most = 4 * static_cast<int64_t>(C_->num_sms);
-    const unsigned grid = static_cast<unsigned>(passes < most ? passes : most);
+    const Shape h = shape_of(C_, a, dtype_size(q->dtype), true);
+    const unsigned grid = grid_of(C_, a, h);
     Workspace ws(C_);
     ColumnSum sums[2];
     for (int i = 0; i < 2; ++i) {
@@ -491,7 +620,6 @@ extern "C" qsml_status_t qsml_norm_rotary_backward(qsml_ctx* handle, const qsml_
         a.sums[i] = static_cast<float*>(p);
         sums[i] = ColumnSum{a.sums[i], dw[i]->data, dw[i]->dtype};
     }
-    QSML_TRY_STATUS((q->dtype == QSML_F16 ? launch<__half, true>(C_, a, vec, grid, lanes, tokens)
-                                          : launch<float, true>(C_, a, vec, grid, lanes, tokens)));
+    QSML_TRY_STATUS((q->dtype == QSML_F16 ? launch<__half, true>(C_, a, h, grid) : launch<float, true>(C_, a, h, grid)));
     return finish_column_sums(C_, sums[0], sums[1], grid, a.D);
 } QSML_NO_THROW
