@@ -86,6 +86,16 @@ qsml_status_t forward_tc(Context* ctx, const Problem& p);
 // dq, dk, dv by the tensor cores (attention_tc_bwd.cu).
 bool tc_takes_backward(const Problem& p);
 qsml_status_t backward_tc(Context* ctx, const Problem& p);
+// A row's keys in parts, row = (b Hq + h) Sq + query: each part's sum, maximum (base 2, scaled) and norm.
+struct Parts {
+    float* sum = nullptr;   // [rows][parts][D], not divided by l
+    float* stat = nullptr;  // [rows][parts][2]: m, l
+    int parts = 1;
+};
+// Room for them in ws, where there is more than one.
+qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t parts, Parts* out);
+// o and lse from the parts, in their order (attention_few.cu).
+qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts);
 // Few queries over many keys (attention_few.cu).
 bool few_queries(const Problem& p);
 qsml_status_t forward_few(Context* ctx, const Problem& p);

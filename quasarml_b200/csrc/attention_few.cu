@@ -19,13 +19,6 @@ namespace {
 constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Row r of a kv head's Sq * G: query r / G, head r % G of the group.
-struct Parts {
-    float* sum;    // [rows][parts][D], not divided by l
-    float* stat;   // [rows][parts][2]: m (base 2, scaled), l
-    int parts;
-};
-
 template <typename T, int DP, int RT> struct Shape {
     static constexpr int V = 16 / sizeof(T);
     static constexpr int KT = sizeof(T) * DP >= 512 ? 32 : 64;  // keys a tile: two stages and three CTAs a SM
@@ -60,6 +53,7 @@ __device__ __forceinline__ void load_keys(unsigned char* dst, const View& v, int
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+// Row r of a kv head's Sq * G: query r / G, head r % G of the group.
 template <typename T, int DP, int RT>
 __global__ void __launch_bounds__(kThreads) k_attention_few(const __grid_constant__ Problem p, Parts parts, int row_tiles, bool vec) {
     using S = Shape<T, DP, RT>;
@@ -275,23 +269,15 @@ template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Prob
     const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
     const int64_t want = (static_cast<int64_t>(ctx->num_sms) * std::max(resident, 1) + groups - 1) / groups;
     const int64_t most = std::min<int64_t>(128, (visible + 2 * S::KT - 1) / (2 * S::KT));
-    Parts parts{nullptr, nullptr, static_cast<int>(std::max<int64_t>(1, std::min(want, most)))};
-    if (groups * parts.parts > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+    const int64_t n = std::max<int64_t>(1, std::min(want, most));
+    if (groups * n > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     Workspace ws(ctx);
-    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
-    if (parts.parts > 1) {
-        void* m = nullptr;
-        QSML_TRY_STATUS(ws.get(sizeof(float) * rows * parts.parts * (p.D + 2), &m));
-        parts.sum = static_cast<float*>(m);
-        parts.stat = parts.sum + rows * parts.parts * p.D;
-    }
-    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(groups * parts.parts)), dim3(kThreads), S::SMEM, ctx->stream, p, parts, row_tiles, vec);
+    Parts parts;
+    QSML_TRY_STATUS(get_parts(ctx, &ws, p, n, &parts));
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(groups * parts.parts)), dim3(kThreads), S::SMEM, ctx->stream, p, parts, row_tiles, vec);
     if (e != cudaSuccess) return check_cuda(ctx, e, name);
     QSML_TRY_STATUS(after_launch(ctx, name));
-    if (parts.parts == 1) return QSML_OK;
-    e = launch_pdl(k_attention_join<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, ctx->stream, p, parts, rows);
-    if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
-    return after_launch(ctx, "k_attention_join");
+    return join_parts(ctx, p, parts);
 }
 
 template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
@@ -313,6 +299,26 @@ template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
 
 // Up to 64 rows a kv head.
 bool few_queries(const Problem& p) { return static_cast<int64_t>(p.Sq) * p.G <= 64; }
+
+qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t n, Parts* out) {
+    out->parts = static_cast<int>(n);
+    if (n == 1) return QSML_OK;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
+    void* m = nullptr;
+    QSML_TRY_STATUS(ws->get(sizeof(float) * rows * n * (p.D + 2), &m));
+    out->sum = static_cast<float*>(m);
+    out->stat = out->sum + rows * n * p.D;
+    return QSML_OK;
+}
+
+qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts) {
+    if (parts.parts == 1) return QSML_OK;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
+    const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>((rows + 3) / 4)),
+                                     dim3(128), 0, ctx->stream, p, parts, rows);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
+    return after_launch(ctx, "k_attention_join");
+}
 
 qsml_status_t forward_few(Context* ctx, const Problem& p) { return p.f16 ? forward<__half>(ctx, p) : forward<float>(ctx, p); }
 

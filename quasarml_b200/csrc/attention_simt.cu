@@ -8,8 +8,10 @@
 // multiplied by exp(m_old - m) where m grows); nothing of the scores leaves the SM.
 // Backward: P = exp(s - lse) again from the kept lse.  dk and dv of a tile of keys are
 // summed by one CTA over all queries that see it and all heads of its group, dq of a tile
-// of queries by another over its keys: seven products instead of five, no atomics.
+// of queries by another over its keys: seven products instead of five, no atomics.  Where the tiles
+// do not fill the device, each one's steps are split over CTAs whose sums are joined in order.
 // Bound by the FFMA pipe and by shared memory, a 16-byte load for 8 multiply-adds.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.cuh"
@@ -38,16 +40,24 @@ __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at,
     constexpr int V = 16 / sizeof(T);
     const T* p = reinterpret_cast<const T*>(v.p) + at;
     if (vec) {
-        for (int i = threadIdx.x; i < S::BT * (DP / V); i += kThreads) {
-            const int r = i / (DP / V), c = i % (DP / V) * V, row = r0 + r;
-            heads::Pack<T, V> x;
+        // a thread's loads are all on their way before the first is stored
+        constexpr int COLS = DP / V, N = S::BT * COLS / kThreads;
+        heads::Pack<T, V> x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = threadIdx.x + i * kThreads, c = at % COLS * V, row = r0 + at / COLS;
             const bool in = (row >= lo || row < sink) && row < hi && c < D;
-            if (in) x = *reinterpret_cast<const heads::Pack<T, V>*>(p + row * v.s + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) heads::from_f(0.0f, x[i].v[e]);
+            if (in) x[i] = *reinterpret_cast<const heads::Pack<T, V>*>(p + row * v.s + c);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = threadIdx.x + i * kThreads, c = at % COLS * V, r = at / COLS;
 #pragma unroll
             for (int e = 0; e < V; e += 4)
                 *reinterpret_cast<float4*>(dst + r * S::LD + c + e) =
-                    in ? make_float4(heads::to_f(x.v[e]), heads::to_f(x.v[e + 1]), heads::to_f(x.v[e + 2]), heads::to_f(x.v[e + 3]))
-                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    make_float4(heads::to_f(x[i].v[e]), heads::to_f(x[i].v[e + 1]), heads::to_f(x[i].v[e + 2]), heads::to_f(x[i].v[e + 3]));
         }
     } else {
         for (int i = threadIdx.x; i < S::BT * DP; i += kThreads) {
@@ -58,7 +68,7 @@ __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at,
 }
 
 // acc[i][j] = sum over columns of a[ty RT + i] b[tx + 16 j].
-template <int DP> __device__ __forceinline__ void dots(const float* a, const float* b, float (&acc)[Shape<DP>::RT][Shape<DP>::RT]) {
+template <int DP> __device__ __forceinline__ void dots(int D, const float* a, const float* b, float (&acc)[Shape<DP>::RT][Shape<DP>::RT]) {
     using S = Shape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     P2 s[S::RT][S::RT];
@@ -67,7 +77,7 @@ template <int DP> __device__ __forceinline__ void dots(const float* a, const flo
 #pragma unroll
         for (int j = 0; j < S::RT; ++j) s[i][j] = pack(0.0f, 0.0f);
 #pragma unroll 4
-    for (int c = 0; c < DP; c += 4) {
+    for (int c = 0; c < D; c += 4) {
         float4 x[S::RT], y[S::RT];
 #pragma unroll
         for (int i = 0; i < S::RT; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty * S::RT + i) * S::LD + c);
@@ -142,24 +152,37 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// A CTA's tile (the last first: with the most keys), head and sequence.
+// A CTA's part of a tile's steps, the tile (of queries the last first: with the most keys), head and
+// sequence.
 struct Where {
-    int tile, h, b;
-    __device__ __forceinline__ Where(int tiles, int H) {
-        const int i = blockIdx.x / H / tiles, r = blockIdx.x - i * H * tiles;
-        b = i;
-        tile = tiles - 1 - r / H;
-        h = r % H;
+    int part, tile, h, b;
+    __device__ __forceinline__ Where(int parts, int tiles, int H, bool backwards) {
+        int i = blockIdx.x;
+        part = i % parts;
+        i /= parts;
+        h = i % H;
+        i /= H;
+        tile = backwards ? tiles - 1 - i % tiles : i % tiles;
+        b = i / tiles;
+    }
+};
+// The steps of a part.
+struct Share {
+    int lo, hi;
+    __device__ __forceinline__ Share(int steps, int parts, int part) {
+        const int n = (steps + parts - 1) / parts;
+        lo = min(part * n, steps);
+        hi = min(lo + n, steps);
     }
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_constant__ Problem p, int tiles, bool vec) {
+__global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_constant__ Problem p, Parts parts, int tiles, bool vec) {
     using S = Shape<DP>;
     extern __shared__ float4 smem[];
     float *sq = reinterpret_cast<float*>(smem), *skv = sq + S::TILE, *sp = skv + S::TILE;
     pdl_begin();
-    const Where w(tiles, p.Hq);
+    const Where w(parts.parts, tiles, p.Hq, true);
     const Seq seq(p, w.b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
@@ -172,13 +195,14 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
 #pragma unroll
     for (int i = 0; i < S::RT; ++i) m[i] = -INFINITY, l[i] = 0.0f;
     const float c = p.scale * kLog2e;
-    for (int n = 0; n < (q0 < seq.nq ? t.n : 0); ++n) {
+    const Share steps(q0 < seq.nq ? t.n : 0, parts.parts, w.part);
+    for (int n = steps.lo; n < steps.hi; ++n) {
         const int k0 = t.tile(n) * S::BT;
         __syncthreads();
         load_tile<T, DP>(skv, p.k, w.b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
         __syncthreads();
         float s[S::RT][S::RT];
-        dots<DP>(sq, skv, s);
+        dots<DP>(p.D, sq, skv, s);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i) {
             const int pos = q0 + ty * S::RT + i + off;
@@ -212,6 +236,12 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
     for (int i = 0; i < S::RT; ++i) {
         const int q = q0 + ty * S::RT + i;
         if (q >= p.Sq) continue;
+        if (parts.parts > 1) {
+            const int64_t at = ((static_cast<int64_t>(w.b) * p.Hq + w.h) * p.Sq + q) * parts.parts + w.part;
+            o.store(i, parts.sum + at * p.D, 1.0f, p.D);
+            if (tx == 0) parts.stat[2 * at] = m[i], parts.stat[2 * at + 1] = l[i];
+            continue;
+        }
         const bool any = l[i] > 0.0f || isnan(l[i]);
         o.store(i, reinterpret_cast<T*>(p.o.p) + w.b * p.o.b + q * p.o.s + w.h * p.o.h, any ? 1.0f / l[i] : 0.0f, p.D);
         if (p.lse && tx == 0) p.lse[(static_cast<int64_t>(w.b) * p.Hq + w.h) * p.Sq + q] = any ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
@@ -221,59 +251,74 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
 // Shared memory of the gradients' kernels: two fixed tiles, two that come and go, P and dS.
 template <int DP> constexpr size_t grad_smem() { return sizeof(float) * (4 * Shape<DP>::TILE + 2 * Shape<DP>::PROBS + 2 * Shape<DP>::BT); }
 
+// Sums of a gradient in parts: [parts][B][H][S][D] binary32.
+struct Sums {
+    float* p = nullptr;
+    int parts = 1;
+    __device__ __forceinline__ float* row(const Problem& a, int part, int b, int h, int H, int i, int S) const {
+        return p + (((static_cast<int64_t>(part) * a.B + b) * H + h) * S + i) * a.D;
+    }
+};
+
 // dk and dv of a tile of keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_constant__ Problem p, const float* delta, int tiles, bool vec) {
+__global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_constant__ Problem p, const float* delta, Sums to_k, Sums to_v, int tiles, bool vec) {
     using S = Shape<DP>;
     extern __shared__ float4 smem[];
     float *sk = reinterpret_cast<float*>(smem), *sv = sk + S::TILE, *sq = sv + S::TILE, *sg = sq + S::TILE, *sp = sg + S::TILE,
           *sd = sp + S::PROBS, *sl = sd + S::PROBS, *sdel = sl + S::BT;
     pdl_begin();
-    const int hk = blockIdx.x % p.Hk, tile = blockIdx.x / p.Hk % tiles, b = blockIdx.x / p.Hk / tiles;
+    const Where w(to_k.parts, tiles, p.Hk, false);
+    const int hk = w.h, b = w.b;
     const Seq seq(p, b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int k0 = tile * S::BT, off = seq.nk - seq.nq;
+    const int k0 = w.tile * S::BT, off = seq.nk - seq.nq;
     load_tile<T, DP>(sk, p.k, b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
     load_tile<T, DP>(sv, p.v, b * p.v.b + hk * p.v.h, k0, 0, 0, seq.nk, p.D, vec);
     Sum<DP> dk, dv;
     dk.zero();
     dv.zero();
     const Queries qs(p, seq, k0, k0 + S::BT);
-    for (int g = 0; g < p.G; ++g) {
-        const int h = hk * p.G + g;
+    const int t0 = qs.lo / S::BT, per = qs.hi > qs.lo ? (qs.hi + S::BT - 1) / S::BT - t0 : 0;  // tiles of queries a head
+    const Share steps(per * p.G, to_k.parts, w.part);
+    for (int n = steps.lo; n < steps.hi; ++n) {
+        const int h = hk * p.G + n / per, q0 = (t0 + n % per) * S::BT;
         const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
-        for (int q0 = qs.lo / S::BT * S::BT; q0 < qs.hi; q0 += S::BT) {
-            __syncthreads();
-            load_tile<T, DP>(sq, p.q, b * p.q.b + h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
-            load_tile<T, DP>(sg, p.dout, b * p.dout.b + h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
-            if (threadIdx.x < S::BT) {
-                const int q = q0 + threadIdx.x;
-                sl[threadIdx.x] = q < seq.nq ? p.lse[stat + q] : 0.0f;
-                sdel[threadIdx.x] = q < seq.nq ? delta[stat + q] : 0.0f;
-            }
-            __syncthreads();
-            float s[S::RT][S::RT], d[S::RT][S::RT];
-            dots<DP>(sk, sq, s);
-            dots<DP>(sv, sg, d);
-#pragma unroll
-            for (int i = 0; i < S::RT; ++i)
-#pragma unroll
-                for (int j = 0; j < S::RT; ++j) {
-                    const int key = k0 + ty * S::RT + i, q = tx + 16 * j;
-                    const bool seen = q0 + q < seq.nq && sees(p, q0 + q + off, key);
-                    const float e = seen ? exp2f((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
-                    sp[(ty * S::RT + i) * S::LP + q] = e;
-                    sd[(ty * S::RT + i) * S::LP + q] = seen ? e * (d[i][j] - sdel[q]) : 0.0f;
-                }
-            __syncthreads();
-            dv.add(sp, sg);
-            dk.add(sd, sq);
+        __syncthreads();
+        load_tile<T, DP>(sq, p.q, b * p.q.b + h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+        load_tile<T, DP>(sg, p.dout, b * p.dout.b + h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
+        if (threadIdx.x < S::BT) {
+            const int q = q0 + threadIdx.x;
+            sl[threadIdx.x] = q < seq.nq ? p.lse[stat + q] : 0.0f;
+            sdel[threadIdx.x] = q < seq.nq ? delta[stat + q] : 0.0f;
         }
+        __syncthreads();
+        float s[S::RT][S::RT], d[S::RT][S::RT];
+        dots<DP>(p.D, sk, sq, s);
+        dots<DP>(p.D, sv, sg, d);
+#pragma unroll
+        for (int i = 0; i < S::RT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::RT; ++j) {
+                const int key = k0 + ty * S::RT + i, q = tx + 16 * j;
+                const bool seen = q0 + q < seq.nq && sees(p, q0 + q + off, key);
+                const float e = seen ? exp2f((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
+                sp[(ty * S::RT + i) * S::LP + q] = e;
+                sd[(ty * S::RT + i) * S::LP + q] = seen ? e * (d[i][j] - sdel[q]) : 0.0f;
+            }
+        __syncthreads();
+        dv.add(sp, sg);
+        dk.add(sd, sq);
     }
 #pragma unroll
     for (int i = 0; i < S::RT; ++i) {
         const int k = k0 + ty * S::RT + i;
         if (k >= p.Sk) continue;
+        if (to_k.parts > 1) {
+            if (p.dk.p) dk.store(i, to_k.row(p, w.part, b, hk, p.Hk, k, p.Sk), p.scale, p.D);
+            if (p.dv.p) dv.store(i, to_v.row(p, w.part, b, hk, p.Hk, k, p.Sk), 1.0f, p.D);
+            continue;
+        }
         if (p.dk.p) dk.store(i, reinterpret_cast<T*>(p.dk.p) + b * p.dk.b + k * p.dk.s + hk * p.dk.h, p.scale, p.D);
         if (p.dv.p) dv.store(i, reinterpret_cast<T*>(p.dv.p) + b * p.dv.b + k * p.dv.s + hk * p.dv.h, 1.0f, p.D);
     }
@@ -281,12 +326,12 @@ __global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_co
 
 // dq of a tile of queries.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_constant__ Problem p, const float* delta, int tiles, bool vec) {
+__global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_constant__ Problem p, const float* delta, Sums to, int tiles, bool vec) {
     using S = Shape<DP>;
     extern __shared__ float4 smem[];
     float *sq = reinterpret_cast<float*>(smem), *sg = sq + S::TILE, *sk = sg + S::TILE, *sv = sk + S::TILE, *sd = sv + S::TILE;
     pdl_begin();
-    const Where w(tiles, p.Hq);
+    const Where w(to.parts, tiles, p.Hq, true);
     const Seq seq(p, w.b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
@@ -304,15 +349,16 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
         lse[i] = q < seq.nq ? p.lse[stat + q] : 0.0f;
         del[i] = q < seq.nq ? delta[stat + q] : 0.0f;
     }
-    for (int n = 0; n < (q0 < seq.nq ? t.n : 0); ++n) {
+    const Share steps(q0 < seq.nq ? t.n : 0, to.parts, w.part);
+    for (int n = steps.lo; n < steps.hi; ++n) {
         const int k0 = t.tile(n) * S::BT;
         __syncthreads();
         load_tile<T, DP>(sk, p.k, w.b * p.k.b + hk * p.k.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
         load_tile<T, DP>(sv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
         __syncthreads();
         float s[S::RT][S::RT], d[S::RT][S::RT];
-        dots<DP>(sq, sk, s);
-        dots<DP>(sg, sv, d);
+        dots<DP>(p.D, sq, sk, s);
+        dots<DP>(p.D, sg, sv, d);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i)
 #pragma unroll
@@ -328,7 +374,26 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
 #pragma unroll
     for (int i = 0; i < S::RT; ++i) {
         const int q = q0 + ty * S::RT + i;
-        if (q < p.Sq) dq.store(i, reinterpret_cast<T*>(p.dq.p) + w.b * p.dq.b + q * p.dq.s + w.h * p.dq.h, p.scale, p.D);
+        if (q >= p.Sq) continue;
+        if (to.parts > 1)
+            dq.store(i, to.row(p, w.part, w.b, w.h, p.Hq, q, p.Sq), p.scale, p.D);
+        else
+            dq.store(i, reinterpret_cast<T*>(p.dq.p) + w.b * p.dq.b + q * p.dq.s + w.h * p.dq.h, p.scale, p.D);
+    }
+}
+
+// out = the parts' sums, added in their order.
+template <typename T> __global__ void __launch_bounds__(256) k_attention_sum(const __grid_constant__ Problem p, Sums from, View out, int H, int S) {
+    pdl_begin();
+    const int64_t n = static_cast<int64_t>(p.B) * H * S * p.D;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < from.parts; ++k) v += from.p[k * n + i];
+        const int c = static_cast<int>(i % p.D);
+        const int64_t row = i / p.D;
+        const int s = static_cast<int>(row % S), h = static_cast<int>(row / S % H), b = static_cast<int>(row / S / H);
+        heads::from_f(v, reinterpret_cast<T*>(out.p)[b * out.b + s * out.s + h * out.h + c]);
     }
 }
 
@@ -339,12 +404,18 @@ bool whole(const Problem& p, bool backward) {
     return ok && (!backward || heads::rows_on(p.dout, es, 16));
 }
 
-// One CTA for each of tiles x heads x sequences.
+// Parts of each of `ctas` tiles of at most `steps` steps: enough for two CTAs a SM.  2048 tokens of 8
+// heads over 2 with 128 columns, binary32: gradients 2535 -> 1130 us, 3 x 200 of 6 over 3: 193 -> 77.
+int64_t parts_of(Context* ctx, int64_t ctas, int64_t steps) {
+    const int64_t want = (2 * static_cast<int64_t>(ctx->num_sms) + ctas - 1) / std::max<int64_t>(ctas, 1);
+    return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps));
+}
+
 template <typename K, typename... A>
-qsml_status_t launch(Context* ctx, K kernel, const char* name, size_t smem, int64_t tiles, int heads, int B, A... args) {
-    if (tiles * heads * B > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+qsml_status_t launch(Context* ctx, K kernel, const char* name, size_t smem, int64_t ctas, A... args) {
+    if (ctas > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), name));
-    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * heads * B)), dim3(kThreads), smem, ctx->stream, args...);
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, ctx->stream, args...);
     if (e != cudaSuccess) return check_cuda(ctx, e, name);
     return after_launch(ctx, name);
 }
@@ -354,8 +425,13 @@ template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
         constexpr int DP = decltype(width)::value;
         using S = Shape<DP>;
         const int tiles = (p.Sq + S::BT - 1) / S::BT;
-        return launch(ctx, k_attention_simt<T, DP>, "k_attention_simt", sizeof(float) * (2 * S::TILE + S::PROBS), tiles, p.Hq, p.B, p, tiles,
-                      whole(p, false));
+        const int64_t ctas = static_cast<int64_t>(tiles) * p.Hq * p.B;
+        Workspace ws(ctx);
+        Parts parts;
+        QSML_TRY_STATUS(get_parts(ctx, &ws, p, parts_of(ctx, ctas, (p.Sk + S::BT - 1) / S::BT), &parts));
+        QSML_TRY_STATUS(launch(ctx, k_attention_simt<T, DP>, "k_attention_simt", sizeof(float) * (2 * S::TILE + S::PROBS), ctas * parts.parts, p, parts,
+                               tiles, whole(p, false)));
+        return join_parts(ctx, p, parts);
     });
 }
 
@@ -364,13 +440,38 @@ template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, con
         constexpr int DP = decltype(width)::value;
         using S = Shape<DP>;
         const bool vec = whole(p, true);
+        const int tq = (p.Sq + S::BT - 1) / S::BT, tk = (p.Sk + S::BT - 1) / S::BT;
+        Workspace ws(ctx);
+        auto sums = [&](int64_t parts, int H, int Sn, Sums* out) {
+            out->parts = static_cast<int>(parts);
+            void* m = nullptr;
+            if (parts > 1) QSML_TRY_STATUS(ws.get(sizeof(float) * parts * p.B * H * Sn * p.D, &m));
+            out->p = static_cast<float*>(m);
+            return static_cast<qsml_status_t>(QSML_OK);
+        };
+        auto join = [&](const Sums& from, const View& out, int H, int Sn) {
+            if (from.parts == 1 || !out.p) return static_cast<qsml_status_t>(QSML_OK);
+            const int64_t n = (static_cast<int64_t>(p.B) * H * Sn * p.D + 255) / 256;
+            const cudaError_t e = launch_pdl(k_attention_sum<T>, dim3(static_cast<unsigned>(std::min<int64_t>(n, 8 * ctx->num_sms))), dim3(256), 0,
+                                             ctx->stream, p, from, out, H, Sn);
+            if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_sum");
+            return after_launch(ctx, "k_attention_sum");
+        };
         if (p.dk.p || p.dv.p) {
-            const int tiles = (p.Sk + S::BT - 1) / S::BT;
-            QSML_TRY_STATUS(launch(ctx, k_attention_dkv_simt<T, DP>, "k_attention_dkv_simt", grad_smem<DP>(), tiles, p.Hk, p.B, p, delta, tiles, vec));
+            const int64_t ctas = static_cast<int64_t>(tk) * p.Hk * p.B, parts = parts_of(ctx, ctas, static_cast<int64_t>(tq) * p.G);
+            Sums to_k, to_v;
+            QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_k));
+            QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_v));
+            QSML_TRY_STATUS(launch(ctx, k_attention_dkv_simt<T, DP>, "k_attention_dkv_simt", grad_smem<DP>(), ctas * parts, p, delta, to_k, to_v, tk, vec));
+            QSML_TRY_STATUS(join(to_k, p.dk, p.Hk, p.Sk));
+            QSML_TRY_STATUS(join(to_v, p.dv, p.Hk, p.Sk));
         }
         if (p.dq.p) {
-            const int tiles = (p.Sq + S::BT - 1) / S::BT;
-            QSML_TRY_STATUS(launch(ctx, k_attention_dq_simt<T, DP>, "k_attention_dq_simt", grad_smem<DP>(), tiles, p.Hq, p.B, p, delta, tiles, vec));
+            const int64_t ctas = static_cast<int64_t>(tq) * p.Hq * p.B, parts = parts_of(ctx, ctas, tk);
+            Sums to;
+            QSML_TRY_STATUS(sums(parts, p.Hq, p.Sq, &to));
+            QSML_TRY_STATUS(launch(ctx, k_attention_dq_simt<T, DP>, "k_attention_dq_simt", grad_smem<DP>(), ctas * parts, p, delta, to, tq, vec));
+            QSML_TRY_STATUS(join(to, p.dq, p.Hq, p.Sq));
         }
         return static_cast<qsml_status_t>(QSML_OK);
     });
