@@ -96,7 +96,12 @@ struct Parts {
 qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t parts, Parts* out);
 // o and lse from the parts, in their order (attention_few.cu).
 qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts);
-// Few queries over many keys (attention_few.cu).
+// Parts of a row's keys for `groups` CTAs, of which a SM holds `resident`, each part of `least` keys or more.
+int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least);
+// Few queries over many keys: binary16 on the tensor cores, where few_tc_takes (attention_few_tc.cu).
+bool few_tc_takes(const Problem& p);
+qsml_status_t forward_few_tc(Context* ctx, const Problem& p);
+// And by CUDA cores (attention_few.cu).
 bool few_queries(const Problem& p);
 qsml_status_t forward_few(Context* ctx, const Problem& p);
 

@@ -7,6 +7,7 @@
 // maximum and sum, and leaves its sums and statistics in a workspace that k_attention_join
 // adds up in the order of the parts.  With one part there is nothing to join.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attention.cuh"
@@ -229,31 +230,59 @@ __global__ void __launch_bounds__(kThreads) k_attention_few(const __grid_constan
     }
 }
 
-// The parts of a row joined in their order: a warp a row.
-template <typename T> __global__ void __launch_bounds__(128) k_attention_join(const __grid_constant__ Problem p, Parts parts, int64_t rows) {
+// The parts of a row joined in a fixed order: a CTA a row, its warps every eighth part each.
+constexpr int kMaxParts = 128, kJoinWarps = 8;
+template <typename T> __global__ void __launch_bounds__(32 * kJoinWarps) k_attention_join(const __grid_constant__ Problem p, Parts parts) {
+    __shared__ float weight[kMaxParts], result[2], part[kJoinWarps][256];
     pdl_begin();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    const int64_t row = blockIdx.x;
     const int q = static_cast<int>(row % p.Sq), h = static_cast<int>(row / p.Sq % p.Hq), b = static_cast<int>(row / p.Sq / p.Hq);
-    const float* stat = parts.stat + row * parts.parts * 2;
-    float m = -INFINITY;
-    for (int i = lane; i < parts.parts; i += 32) m = fmaxf(m, stat[2 * i]);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float* sum = parts.sum + row * parts.parts * p.D;
+    if (warp == 0) {
+        float m[kMaxParts / 32], l[kMaxParts / 32], top = -INFINITY, norm = 0.0f;
 #pragma unroll
-    for (int k = 16; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int i = 0; i < parts.parts; ++i) l = fmaf(stat[2 * i + 1], exp2f(stat[2 * i] - ref), l);
-    const bool any = l > 0.0f || isnan(l);
-    const float f = any ? 1.0f / l : 0.0f;
+        for (int i = 0; i < kMaxParts / 32; ++i) {
+            const int k = lane + 32 * i;
+            const float2 st = k < parts.parts ? reinterpret_cast<const float2*>(parts.stat)[row * parts.parts + k] : make_float2(-INFINITY, 0.0f);
+            m[i] = st.x;
+            l[i] = st.y;
+            top = fmaxf(top, st.x);
+        }
+#pragma unroll
+        for (int k = 16; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 32; ++i) {
+            const float f = exp2f(m[i] - ref);
+            weight[lane + 32 * i] = f;
+            norm = fmaf(l[i], f, norm);
+        }
+#pragma unroll
+        for (int k = 16; k >= 1; k >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, k);
+        if (lane == 0) result[0] = top, result[1] = norm;
+    }
+    __syncthreads();
+    const float norm = result[1];
+    const bool any = norm > 0.0f || isnan(norm);
+    const float f = any ? 1.0f / norm : 0.0f;
     T* o = reinterpret_cast<T*>(p.o.p) + b * p.o.b + q * p.o.s + h * p.o.h;
-    for (int c = lane; c < p.D; c += 32) {
-        float s = 0.0f;
+    float acc[8] = {};  // columns lane + 32 j
 #pragma unroll 4
-        for (int i = 0; i < parts.parts; ++i) s = fmaf(parts.sum[(row * parts.parts + i) * p.D + c], exp2f(stat[2 * i] - ref), s);
+    for (int i = warp; i < parts.parts; i += kJoinWarps)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < p.D) acc[j] = fmaf(sum[static_cast<int64_t>(i) * p.D + lane + 32 * j], weight[i], acc[j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][lane + 32 * j] = acc[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.D; c += 32 * kJoinWarps) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) s += part[i][c];
         heads::from_f(s * f, o[c]);
     }
-    if (p.lse && lane == 0) p.lse[row] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (p.lse && threadIdx.x == 0) p.lse[row] = any ? (result[0] + log2f(norm)) * kLn2 : -INFINITY;
 }
 
 template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Problem& p, bool vec) {
@@ -265,11 +294,7 @@ template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Prob
     QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, S::SMEM), name));
     const int R = p.Sq * p.G, row_tiles = (R + RT - 1) / RT;
     const int64_t groups = static_cast<int64_t>(row_tiles) * p.Hk * p.B;
-    // as many parts as fill the device, each of at least two tiles
-    const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
-    const int64_t want = (static_cast<int64_t>(ctx->num_sms) * std::max(resident, 1) + groups - 1) / groups;
-    const int64_t most = std::min<int64_t>(128, (visible + 2 * S::KT - 1) / (2 * S::KT));
-    const int64_t n = std::max<int64_t>(1, std::min(want, most));
+    const int64_t n = few_parts(ctx, p, groups, std::max(resident, 1), 2 * S::KT);
     if (groups * n > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     Workspace ws(ctx);
     Parts parts;
@@ -300,6 +325,24 @@ template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
 // Up to 64 rows a kv head.
 bool few_queries(const Problem& p) { return static_cast<int64_t>(p.Sq) * p.G <= 64; }
 
+int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least) {
+    // no row sees more keys than these
+    const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (visible + least - 1) / least));
+    // The time of n parts: waves of CTAs (whole ones, where all are alike), each of a part's keys and
+    // of what a CTA takes besides, as long as START keys.
+    constexpr double START = 128.0;
+    const double slots = static_cast<double>(ctx->num_sms) * resident;
+    int64_t best = 1;
+    double least_time = 0.0;
+    for (int64_t n = 1; n <= most; ++n) {
+        const double waves = static_cast<double>(groups * n) / slots;
+        const double time = (p.nk ? waves + 1.0 : std::ceil(waves)) * (static_cast<double>(visible) / n + START);
+        if (n == 1 || time < least_time) best = n, least_time = time;
+    }
+    return best;
+}
+
 qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t n, Parts* out) {
     out->parts = static_cast<int>(n);
     if (n == 1) return QSML_OK;
@@ -314,13 +357,17 @@ qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t n
 qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts) {
     if (parts.parts == 1) return QSML_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
-    const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>((rows + 3) / 4)),
-                                     dim3(128), 0, ctx->stream, p, parts, rows);
+    if (rows > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+    const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>(rows)), dim3(32 * kJoinWarps), 0,
+                                     ctx->stream, p, parts);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
     return after_launch(ctx, "k_attention_join");
 }
 
-qsml_status_t forward_few(Context* ctx, const Problem& p) { return p.f16 ? forward<__half>(ctx, p) : forward<float>(ctx, p); }
+qsml_status_t forward_few(Context* ctx, const Problem& p) {
+    if (few_tc_takes(p)) return forward_few_tc(ctx, p);
+    return p.f16 ? forward<__half>(ctx, p) : forward<float>(ctx, p);
+}
 
 }  // namespace attn
 }  // namespace qsml
