@@ -330,8 +330,9 @@ int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, 
     const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (visible + least - 1) / least));
     // The time of n parts: waves of CTAs (whole ones, where all are alike), each of a part's keys and
-    // of what a CTA takes besides, as long as START keys.
-    constexpr double START = 128.0;
+    // of what a CTA takes besides, as long as START keys (128 to 1024 measured: 16 sequences over up to 8192 keys
+    // 81, 79, 76, 85 us; 32 over 1000 43, 38, 38, 30; one over 32768 52, 42, 48, 35).
+    constexpr double START = 512.0;
     const double slots = static_cast<double>(ctx->num_sms) * resident;
     int64_t best = 1;
     double least_time = 0.0;
