@@ -35,74 +35,61 @@ struct Stats {
     int64_t pitch;
 };
 
-// 16 lanes a row.
-__global__ void __launch_bounds__(256) k_attention_prepare(const __grid_constant__ Problem p, Stats st) {
+// A CTA takes 128 rows of a head (blocks below qblocks: of dout and o, then of v), 16 lanes a row.
+__global__ void __launch_bounds__(256) k_attention_prepare(const __grid_constant__ Problem p, Stats st, int qblocks) {
     pdl_begin();
-    const int lane = threadIdx.x & 15;
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4, step = static_cast<int64_t>(gridDim.x) * blockDim.x >> 4;
-    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * st.pitch, vrows = static_cast<int64_t>(p.B) * p.Hk * p.Sk;
-    auto row = [&](const View& v, int b, int i, int h, float (&x)[8]) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (lane * 8 < p.D) w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(v.p) + b * v.b + i * v.s + h * v.h + lane * 8);
-        const __half2* h2 = reinterpret_cast<const __half2*>(&w);
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4;
+    const bool of_q = static_cast<int>(blockIdx.x) < qblocks;
+    const int i = of_q ? blockIdx.x : blockIdx.x - qblocks, H = of_q ? p.Hq : p.Hk;
+    const int bh = i % (p.B * H), first = i / (p.B * H) * TILE, b = bh / H, h = bh - b * H;
+    const Seq seq(p, b);
+    const int n = of_q ? seq.nq : seq.nk;
+    const bool mine = lane * 8 < p.D;
+    auto at = [&](const View& v, int r) { return reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(v.p) + b * v.b + h * v.h + r * v.s + lane * 8); };
+    auto sum = [&](const uint4& x, const uint4& y) {
+        const __half2 *u = reinterpret_cast<const __half2*>(&x), *w = reinterpret_cast<const __half2*>(&y);
+        float s = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float2 f = __half22float2(h2[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-        }
-    };
-    auto total = [&](float v) {
-#pragma unroll
-        for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-        return v;
-    };
-    float most[3] = {0.0f, 0.0f, 0.0f};
-    // both rows of a warp go through the sums
-    for (int64_t n0 = first & ~int64_t(1); n0 < rows; n0 += step) {
-        const int64_t n = n0 + (first & 1);
-        const bool in = n < rows;
-        const int64_t bh = in ? n / st.pitch : 0;
-        const int i = static_cast<int>(n - bh * st.pitch), h = static_cast<int>(bh % p.Hq), b = static_cast<int>(bh / p.Hq);
-        const bool live = in && i < Seq(p, b).nq;
-        float x[8], y[8], s[3] = {0.0f, 0.0f, 0.0f};
-        if (live) {
-            row(p.dout, b, i, h, x);
-            row(p.o, b, i, h, y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                s[0] = fmaf(x[e], x[e], s[0]);
-                s[1] = fmaf(y[e], y[e], s[1]);
-                s[2] = fmaf(x[e], y[e], s[2]);
-            }
+            const float2 f = __half22float2(u[e]), g = __half22float2(w[e]);
+            s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
         }
 #pragma unroll
-        for (float& v : s) v = total(v);
-        most[0] = fmaxf(most[0], s[0]);
-        most[1] = fmaxf(most[1], s[1]);
-        if (in && lane == 0) {
-            const float lse = live ? p.lse[bh * p.Sq + i] : -INFINITY;
-            st.minus[n] = lse == -INFINITY ? -INFINITY : fmaf(lse, -kLog2e, SHIFT);
-            st.delta[n] = s[2];
+        for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        return s;
+    };
+    constexpr int ROWS = TILE / 16;
+    uint4 x[ROWS], y[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const int r = first + row + 16 * k;
+        x[k] = y[k] = make_uint4(0, 0, 0, 0);
+        if (r < n && mine) {
+            x[k] = *at(of_q ? p.dout : p.v, r);
+            if (of_q) y[k] = *at(p.o, r);
         }
     }
-    for (int64_t n0 = first & ~int64_t(1); n0 < vrows; n0 += step) {
-        const int64_t n = n0 + (first & 1);
-        const bool in = n < vrows;
-        const int j = in ? static_cast<int>(n % p.Sk) : 0, h = in ? static_cast<int>(n / p.Sk % p.Hk) : 0, b = in ? static_cast<int>(n / p.Sk / p.Hk) : 0;
-        float x[8], s = 0.0f;
-        if (in && j < Seq(p, b).nk) {
-            row(p.v, b, j, h, x);
+    float most[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf(x[e], x[e], s);
+    for (int k = 0; k < ROWS; ++k) {
+        const int r = first + row + 16 * k;
+        most[0] = fmaxf(most[0], sum(x[k], x[k]));
+        if (!of_q) continue;
+        most[1] = fmaxf(most[1], sum(y[k], y[k]));
+        const float delta = sum(x[k], y[k]);
+        if (lane == 0) {
+            const float lse = r < n ? p.lse[static_cast<int64_t>(bh) * p.Sq + r] : -INFINITY;
+            st.minus[bh * st.pitch + r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -kLog2e, SHIFT);
+            st.delta[bh * st.pitch + r] = delta;
         }
-        most[2] = fmaxf(most[2], total(s));
     }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        const float m = fmaxf(most[k], __shfl_xor_sync(0xffffffffu, most[k], 16));
+    for (int k = 0; k < 2; ++k) {
+        float m = most[k];
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         // bits of numbers that are not negative are in their order; the largest does not depend on it
-        if ((threadIdx.x & 31) == 0 && m > 0.0f) atomicMax(st.largest + k, __float_as_uint(m));
+        if ((threadIdx.x & 31) == 0 && m > 0.0f) atomicMax(st.largest + (of_q ? k : 2), __float_as_uint(m));
     }
 }
 
@@ -157,8 +144,41 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// A row of sums in TMEM (none: zeros), times f, as binary32.
+template <int DP> __device__ __forceinline__ void store_sums(uint32_t at, bool any, float f, float* to, int D) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+        if (c >= D) break;
+        uint32_t r[32];
+        if (any) {
+            tmem_ld32_start(at + c, r);
+            tmem_wait(r);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+            if (c + j < D)
+                *reinterpret_cast<float4*>(to + c + j) =
+                    any ? make_float4(__uint_as_float(r[j]) * f, __uint_as_float(r[j + 1]) * f, __uint_as_float(r[j + 2]) * f, __uint_as_float(r[j + 3]) * f)
+                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+}
+
 struct BwdMaps {
     HeadMap q, k, v, g;
+};
+
+// The steps of a tile of keys (tiles of queries that see it, of all heads of the group) over several
+// CTAs: the tiles with sinks, which all later queries see, in `many` parts, the others in `few`.  A
+// part's dk and dv are binary32 tiles [128][D] each in `sum`, where its tile has more than one.
+struct KeyParts {
+    float* sum;
+    int many, few, sink_tiles, tiles;
+    __host__ __device__ int64_t slots() const { return static_cast<int64_t>(sink_tiles) * many + static_cast<int64_t>(tiles - sink_tiles) * few; }
+    __host__ __device__ int64_t slot(int tile) const {
+        return tile < sink_tiles ? static_cast<int64_t>(tile) * many
+                                 : static_cast<int64_t>(sink_tiles) * many + static_cast<int64_t>(tile - sink_tiles) * few;
+    }
+    __host__ __device__ int parts(int tile) const { return tile < sink_tiles ? many : few; }
 };
 
 template <int DP> struct Dkv {
@@ -168,7 +188,7 @@ template <int DP> struct Dkv {
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attention_dkv(const __grid_constant__ Problem p, const __grid_constant__ BwdMaps maps, Stats st, int* status) {
+    k_attention_dkv(const __grid_constant__ Problem p, const __grid_constant__ BwdMaps maps, Stats st, KeyParts kp, int* status) {
     using L = Dkv<DP>;
     constexpr int BYTES = TileOf<DP>::BYTES;
     extern __shared__ unsigned char smem_raw[];
@@ -213,12 +233,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long limit = wait_limit(status);
 
     // the first keys, which the most queries see, first
-    const int hk = blockIdx.x % p.Hk, b = blockIdx.x / p.Hk % p.B, k0 = blockIdx.x / p.Hk / p.B * TILE;
+    const int hk = blockIdx.x % p.Hk, b = blockIdx.x / p.Hk % p.B, slot = blockIdx.x / p.Hk / p.B;
+    const int rest = slot - kp.sink_tiles * kp.many, tile = rest < 0 ? slot / kp.many : kp.sink_tiles + rest / kp.few;
+    const int k0 = tile * TILE, parts = kp.parts(tile), part = slot - static_cast<int>(kp.slot(tile));
     const Seq seq(p, b);
     const int off = seq.nk - seq.nq;
     const Queries qs(p, seq, k0, k0 + TILE);
     const int t0 = qs.lo / TILE, per = qs.hi > qs.lo ? (qs.hi + TILE - 1) / TILE - t0 : 0;  // tiles of queries a head
-    const int steps = per * p.G;
+    const int share = (per * p.G + parts - 1) / parts, step0 = min(part * share, per * p.G), steps = min(share, per * p.G - step0);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
@@ -233,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 load_tile<DP>(v_tile, maps.v, kv_full, k0, hk, b);
             }
             for (int n = 0; n < steps && ok; ++n) {
-                const int s = n & 1, h = hk * p.G + n / per, q0 = (t0 + n % per) * TILE;
+                const int s = n & 1, h = hk * p.G + (step0 + n) / per, q0 = (t0 + (step0 + n) % per) * TILE;
                 ok = warp_wait(empty(s), (n >> 1 & 1) ^ 1, abort_flag, limit);
                 if (!ok) break;
                 const bool ragged = q0 + TILE > seq.nq;
@@ -313,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int last_key = min(k0 + TILE, seq.nk) - 1;
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
-            const int s = n & 1, q0 = (t0 + n % per) * TILE;
+            const int s = n & 1, q0 = (t0 + (step0 + n) % per) * TILE;
             const float *minus = stats + s * 256 + 64 * w, *delta = minus + 128;
             ok = warp_wait(s_full, n & 1, abort_flag, limit) && warp_wait(full(s), n >> 1 & 1, abort_flag, limit);
             if (!ok) break;
@@ -362,7 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         // a warpgroup each: dV and dK
         const View& to = w ? p.dk : p.dv;
-        if (ok && to.p) {
+        if (ok && parts > 1) {
+            float* row = kp.sum + (((static_cast<int64_t>(slot) * p.B + b) * p.Hk + hk) * 2 + w) * TILE * p.D + static_cast<int64_t>(k - k0) * p.D;
+            store_sums<DP>(lanes + 256 + w * DP, steps > 0, w ? p.scale / gain : exp2f(-SHIFT), row, p.D);
+        } else if (ok && to.p) {
             __half* row = k < p.Sk ? reinterpret_cast<__half*>(to.p) + b * to.b + k * to.s + hk * to.h : nullptr;
             if (steps > 0) {
                 const bool live = k < seq.nk;
@@ -379,6 +404,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// dk and dv of the tiles in several parts: the parts' sums, added in their order; 8 columns a thread.
+__global__ void __launch_bounds__(256) k_attention_dkv_join(const __grid_constant__ Problem p, KeyParts kp, int tiles) {
+    pdl_begin();
+    const int units = p.D / 8, w = blockIdx.y;
+    const View& to = w ? p.dk : p.dv;
+    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int parts = kp.parts(tile), nk = Seq(p, b).nk;
+    const int64_t stride = static_cast<int64_t>(p.B) * p.Hk * 2 * TILE * p.D;
+    const float* from = kp.sum + (kp.slot(tile) * p.B * p.Hk + bh) * 2 * TILE * p.D + static_cast<int64_t>(w) * TILE * p.D;
+    if (!to.p || parts == 1) return;
+    for (int i = threadIdx.x; i < TILE * units; i += 256) {
+        const int r = i / units, c = (i - r * units) * 8, k = tile * TILE + r;
+        if (k >= p.Sk) break;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+        if (k < nk) {
+#pragma unroll 4
+            for (int n = 0; n < parts; ++n) {
+                const float4* a = reinterpret_cast<const float4*>(from + n * stride + static_cast<int64_t>(r) * p.D + c);
+                const float4 u = a[0], v = a[1];
+                x.x += u.x, x.y += u.y, x.z += u.z, x.w += u.w;
+                y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+            }
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(to.p) + b * to.b + k * to.s + hk * to.h + c) =
+            make_uint4(half2_of(x.x, x.y), half2_of(x.z, x.w), half2_of(y.x, y.y), half2_of(y.z, y.w));
     }
 }
 
@@ -621,9 +674,30 @@ template <int DP> qsml_status_t backward(Context* ctx, const Problem& p, const S
     const int tq = (p.Sq + TILE - 1) / TILE, tk = (p.Sk + TILE - 1) / TILE;
     if (p.dq.p || p.dk.p)
         QSML_TRY_STATUS(launch(ctx, k_attention_dq<DP>, "k_attention_dq", Dq<DP>::SMEM, static_cast<int64_t>(tq) * p.Hq * p.B, p, maps, st, tq, ctx->status));
-    if (p.dk.p || p.dv.p)
-        QSML_TRY_STATUS(launch(ctx, k_attention_dkv<DP>, "k_attention_dkv", Dkv<DP>::SMEM, static_cast<int64_t>(tk) * p.Hk * p.B, p, maps, st, ctx->status));
-    return QSML_OK;
+    if (!p.dk.p && !p.dv.p) return QSML_OK;
+    // Parts of about as many steps each, so that the CTAs are three waves: with a tile a CTA the one with
+    // the sinks took as long as all else (2 x 4096 tokens of 16 heads over 2, window 2048: 540 us).
+    KeyParts kp{nullptr, 1, 1, p.window ? std::min((p.sinks + TILE - 1) / TILE, tk) : 0, tk};
+    const int64_t bh = static_cast<int64_t>(p.B) * p.Hk, most = static_cast<int64_t>(p.G) * tq;
+    const int64_t usual = p.window ? std::min(most, static_cast<int64_t>(p.G) * (p.window / TILE + 2)) : most;
+    const int64_t total = bh * (kp.sink_tiles * most + (tk - kp.sink_tiles) * usual);
+    const int64_t chunk = std::max<int64_t>(8, total / (3 * static_cast<int64_t>(ctx->num_sms)));
+    auto parts = [&](int64_t steps) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, steps / chunk))); };
+    kp.many = parts(most);
+    kp.few = parts(usual);
+    Workspace ws(ctx);
+    const bool split = kp.few > 1 || (kp.sink_tiles && kp.many > 1);
+    if (split) {
+        void* m = nullptr;
+        QSML_TRY_STATUS(ws.get(sizeof(float) * kp.slots() * bh * 2 * TILE * p.D, &m));
+        kp.sum = static_cast<float*>(m);
+    }
+    QSML_TRY_STATUS(launch(ctx, k_attention_dkv<DP>, "k_attention_dkv", Dkv<DP>::SMEM, kp.slots() * bh, p, maps, st, kp, ctx->status));
+    if (!split) return QSML_OK;
+    const int tiles = kp.few > 1 ? tk : kp.sink_tiles;
+    const cudaError_t e = launch_pdl(k_attention_dkv_join, dim3(static_cast<unsigned>(tiles * bh), 2), dim3(256), 0, ctx->stream, p, kp, tiles);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_dkv_join");
+    return after_launch(ctx, "k_attention_dkv_join");
 }
 
 }  // namespace
@@ -644,8 +718,10 @@ qsml_status_t backward_tc(Context* ctx, const Problem& p) {
     st.delta = st.minus + rows;
     st.largest = reinterpret_cast<unsigned*>(st.delta + rows);
     QSML_TRY_STATUS(check_cuda(ctx, cudaMemsetAsync(st.largest, 0, 3 * sizeof(unsigned), ctx->stream), "qsml_attention_backward"));
-    const int64_t grid = std::min<int64_t>((rows + 15) / 16, 8 * static_cast<int64_t>(ctx->num_sms));
-    const cudaError_t e = launch_pdl(k_attention_prepare, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, p, st);
+    const int64_t qblocks = rows / TILE, vblocks = static_cast<int64_t>(p.B) * p.Hk * ((p.Sk + TILE - 1) / TILE);
+    if (qblocks + vblocks > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention_backward: dimensions too large");
+    const cudaError_t e = launch_pdl(k_attention_prepare, dim3(static_cast<unsigned>(qblocks + vblocks)), dim3(256), 0, ctx->stream, p, st,
+                                     static_cast<int>(qblocks));
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_prepare");
     QSML_TRY_STATUS(after_launch(ctx, "k_attention_prepare"));
     return p.D <= 64 ? backward<64>(ctx, p, st) : backward<128>(ctx, p, st);
