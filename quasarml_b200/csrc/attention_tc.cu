@@ -84,9 +84,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     pdl_begin();
     const long long limit = wait_limit(status);
 
-    // the last queries, with the most keys, first
-    const int b = blockIdx.x / p.Hq / tiles, rest = blockIdx.x - b * p.Hq * tiles;
-    const int q0 = (tiles - 1 - rest / p.Hq) * TILE, h = rest % p.Hq, hk = h / p.G;
+    // the last queries of all sequences, with the most keys, first
+    const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.G;
+    const int q0 = (tiles - 1 - blockIdx.x / (p.B * p.Hq)) * TILE;
     const Seq seq(p, b);
     const int off = seq.nk - seq.nq;
     const Keys keys(p, seq.nk, q0 + off, min(q0 + TILE, seq.nq) - 1 + off);

@@ -83,13 +83,22 @@ __global__ void __launch_bounds__(256) k_attention_prepare(const __grid_constant
             st.delta[bh * st.pitch + r] = delta;
         }
     }
+    // one atomic a CTA: 18000 on one word took 20 us
+    __shared__ float largest[2][8];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         float m = most[k];
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if ((threadIdx.x & 31) == 0) largest[k][threadIdx.x >> 5] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x < (of_q ? 2 : 1)) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, largest[threadIdx.x][i]);
         // bits of numbers that are not negative are in their order; the largest does not depend on it
-        if ((threadIdx.x & 31) == 0 && m > 0.0f) atomicMax(st.largest + (of_q ? k : 2), __float_as_uint(m));
+        if (m > 0.0f) atomicMax(st.largest + (of_q ? threadIdx.x : 2), __float_as_uint(m));
     }
 }
 
@@ -407,18 +416,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// dk and dv of the tiles in several parts: the parts' sums, added in their order; 8 columns a thread.
+// dk and dv of the tiles in several parts: the parts' sums, added in their order; a quarter of a tile a
+// CTA, 8 columns a thread.
 __global__ void __launch_bounds__(256) k_attention_dkv_join(const __grid_constant__ Problem p, KeyParts kp, int tiles) {
     pdl_begin();
     const int units = p.D / 8, w = blockIdx.y;
     const View& to = w ? p.dk : p.dv;
-    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int quarter = blockIdx.x & 3, tile = (blockIdx.x >> 2) % tiles, bh = (blockIdx.x >> 2) / tiles, b = bh / p.Hk, hk = bh - b * p.Hk;
     const int parts = kp.parts(tile), nk = Seq(p, b).nk;
     const int64_t stride = static_cast<int64_t>(p.B) * p.Hk * 2 * TILE * p.D;
     const float* from = kp.sum + (kp.slot(tile) * p.B * p.Hk + bh) * 2 * TILE * p.D + static_cast<int64_t>(w) * TILE * p.D;
     if (!to.p || parts == 1) return;
-    for (int i = threadIdx.x; i < TILE * units; i += 256) {
-        const int r = i / units, c = (i - r * units) * 8, k = tile * TILE + r;
+    for (int i = threadIdx.x; i < TILE / 4 * units; i += 256) {
+        const int row = i / units, r = quarter * (TILE / 4) + row, c = (i - row * units) * 8, k = tile * TILE + r;
         if (k >= p.Sk) break;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
         if (k < nk) {
@@ -485,8 +495,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_begin();
     const long long limit = wait_limit(status);
 
-    const int b = blockIdx.x / p.Hq / tiles, rest = blockIdx.x - b * p.Hq * tiles;
-    const int q0 = (tiles - 1 - rest / p.Hq) * TILE, h = rest % p.Hq, hk = h / p.G;
+    // the last queries of all sequences, with the most keys, first
+    const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.G;
+    const int q0 = (tiles - 1 - blockIdx.x / (p.B * p.Hq)) * TILE;
     const Seq seq(p, b);
     const int off = seq.nk - seq.nq;
     const Keys keys(p, seq.nk, q0 + off, min(q0 + TILE, seq.nq) - 1 + off);
@@ -582,9 +593,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane, q = q0 + lane_row;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t dp_at = lanes + 2 * TILE + 64 * w;
-        const float c = p.scale * kLog2e, gain = gain_of(st), ds_gain = gain * exp2f(-SHIFT);
+        const float c = p.scale * kLog2e, gain = gain_of(st);
         const int64_t at = (static_cast<int64_t>(b) * p.Hq + h) * st.pitch + q;
-        const float minus = st.minus[at];
+        const float minus = st.minus[at] - SHIFT + log2f(gain);  // P is wanted times the power of two alone
         float delta = st.delta[at];
         const int pos = q + off, first_pos = q0 + off, last_pos = min(q0 + TILE, seq.nq) - 1 + off;
         const int row_hi = q < seq.nq ? pos : -1, row_lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
@@ -616,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(part_full);
                 ok = warp_wait(part_full, 0, abort_flag, limit);
                 if (!ok) break;
-                delta = (part[lane_row] + part[TILE + lane_row]) * exp2f(-SHIFT);
+                delta = (part[lane_row] + part[TILE + lane_row]) / gain;
                 if (w == 0) st.delta[at] = q < seq.nq ? delta : 0.0f;
             }
 #pragma unroll
@@ -626,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 16; ++e) {
                     const int i = 32 * h2 + 2 * e;
                     const P2 x = sub2(pack(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), both(delta));
-                    const float2 y = unpack(mul2(mul2(pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), both(ds_gain)), x));
+                    const float2 y = unpack(mul2(pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), x));
                     f[e] = half2_of(y.x, y.y);
                 }
                 tmem_st16(dp_at + 16 * h2, f);
@@ -694,8 +705,9 @@ template <int DP> qsml_status_t backward(Context* ctx, const Problem& p, const S
     }
     QSML_TRY_STATUS(launch(ctx, k_attention_dkv<DP>, "k_attention_dkv", Dkv<DP>::SMEM, kp.slots() * bh, p, maps, st, kp, ctx->status));
     if (!split) return QSML_OK;
+    if (4 * tk * bh > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention_backward: dimensions too large");
     const int tiles = kp.few > 1 ? tk : kp.sink_tiles;
-    const cudaError_t e = launch_pdl(k_attention_dkv_join, dim3(static_cast<unsigned>(tiles * bh), 2), dim3(256), 0, ctx->stream, p, kp, tiles);
+    const cudaError_t e = launch_pdl(k_attention_dkv_join, dim3(static_cast<unsigned>(4 * tiles * bh), 2), dim3(256), 0, ctx->stream, p, kp, tiles);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_dkv_join");
     return after_launch(ctx, "k_attention_dkv_join");
 }
