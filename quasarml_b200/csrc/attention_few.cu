@@ -230,59 +230,63 @@ __global__ void __launch_bounds__(kThreads) k_attention_few(const __grid_constan
     }
 }
 
-// The parts of a row joined in a fixed order: a CTA a row, its warps every eighth part each.
+// The parts of a row joined in a fixed order: by a warp, or by eight with every eighth part each where
+// there are more than eight.
 constexpr int kMaxParts = 128, kJoinWarps = 8;
-template <typename T> __global__ void __launch_bounds__(32 * kJoinWarps) k_attention_join(const __grid_constant__ Problem p, Parts parts) {
-    __shared__ float weight[kMaxParts], result[2], part[kJoinWarps][256];
+template <typename T> __global__ void __launch_bounds__(32 * kJoinWarps) k_attention_join(const __grid_constant__ Problem p, Parts parts, int64_t rows, int per_row) {
+    __shared__ float weight[kJoinWarps][kMaxParts], part[kJoinWarps][256];
     pdl_begin();
-    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp & (per_row - 1);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinWarps / per_row) + warp / per_row;
+    if (row >= rows) return;  // with eight warps a row, all or none of the CTA
     const int q = static_cast<int>(row % p.Sq), h = static_cast<int>(row / p.Sq % p.Hq), b = static_cast<int>(row / p.Sq / p.Hq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* sum = parts.sum + row * parts.parts * p.D;
-    if (warp == 0) {
-        float m[kMaxParts / 32], l[kMaxParts / 32], top = -INFINITY, norm = 0.0f;
+    float m[kMaxParts / 32], l[kMaxParts / 32], top = -INFINITY, norm = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMaxParts / 32; ++i) {
-            const int k = lane + 32 * i;
-            const float2 st = k < parts.parts ? reinterpret_cast<const float2*>(parts.stat)[row * parts.parts + k] : make_float2(-INFINITY, 0.0f);
-            m[i] = st.x;
-            l[i] = st.y;
-            top = fmaxf(top, st.x);
-        }
-#pragma unroll
-        for (int k = 16; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < kMaxParts / 32; ++i) {
-            const float f = exp2f(m[i] - ref);
-            weight[lane + 32 * i] = f;
-            norm = fmaf(l[i], f, norm);
-        }
-#pragma unroll
-        for (int k = 16; k >= 1; k >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, k);
-        if (lane == 0) result[0] = top, result[1] = norm;
+    for (int i = 0; i < kMaxParts / 32; ++i) {
+        const int k = lane + 32 * i;
+        const float2 st = k < parts.parts ? reinterpret_cast<const float2*>(parts.stat)[row * parts.parts + k] : make_float2(-INFINITY, 0.0f);
+        m[i] = st.x;
+        l[i] = st.y;
+        top = fmaxf(top, st.x);
     }
-    __syncthreads();
-    const float norm = result[1];
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 32; ++i) {
+        const float f = exp2f(m[i] - ref);
+        weight[warp][lane + 32 * i] = f;
+        norm = fmaf(l[i], f, norm);
+    }
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, k);
+    __syncwarp();
     const bool any = norm > 0.0f || isnan(norm);
     const float f = any ? 1.0f / norm : 0.0f;
     T* o = reinterpret_cast<T*>(p.o.p) + b * p.o.b + q * p.o.s + h * p.o.h;
     float acc[8] = {};  // columns lane + 32 j
 #pragma unroll 4
-    for (int i = warp; i < parts.parts; i += kJoinWarps)
+    for (int i = sub; i < parts.parts; i += per_row)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < p.D) acc[j] = fmaf(sum[static_cast<int64_t>(i) * p.D + lane + 32 * j], weight[i], acc[j]);
+            if (lane + 32 * j < p.D) acc[j] = fmaf(sum[static_cast<int64_t>(i) * p.D + lane + 32 * j], weight[warp][i], acc[j]);
+    if (per_row == 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.D; c += 32 * kJoinWarps) {
-        float s = 0.0f;
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < p.D) heads::from_f(acc[j] * f, o[lane + 32 * j]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i) s += part[i][c];
-        heads::from_f(s * f, o[c]);
+        for (int j = 0; j < 8; ++j) part[warp][lane + 32 * j] = acc[j];
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.D; c += 32 * kJoinWarps) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) s += part[i][c];
+            heads::from_f(s * f, o[c]);
+        }
     }
-    if (p.lse && threadIdx.x == 0) p.lse[row] = any ? (result[0] + log2f(norm)) * kLn2 : -INFINITY;
+    if (p.lse && sub == 0 && lane == 0) p.lse[row] = any ? (top + log2f(norm)) * kLn2 : -INFINITY;
 }
 
 template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Problem& p, bool vec) {
@@ -359,8 +363,9 @@ qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts) {
     if (parts.parts == 1) return QSML_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
     if (rows > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
-    const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>(rows)), dim3(32 * kJoinWarps), 0,
-                                     ctx->stream, p, parts);
+    const int per_row = parts.parts > kJoinWarps ? kJoinWarps : 1, at_once = kJoinWarps / per_row;
+    const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>((rows + at_once - 1) / at_once)),
+                                     dim3(32 * kJoinWarps), 0, ctx->stream, p, parts, rows, per_row);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
     return after_launch(ctx, "k_attention_join");
 }

@@ -152,6 +152,17 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Whether every query of [q0, q0 + n), all below nq, sees every key of [k0, k0 + n).
+__device__ __forceinline__ bool all_see(const Problem& a, const Seq& s, int q0, int k0, int n) {
+    const int pos = q0 + s.nk - s.nq;
+    return q0 + n <= s.nq && k0 + n - 1 <= pos && (a.window == 0 || pos + n - 1 - k0 < a.window || k0 + n <= a.sinks);
+}
+
 // A CTA's part of a tile's steps, the tile (of queries the last first: with the most keys), head and
 // sequence.
 struct Where {
@@ -203,21 +214,22 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
         __syncthreads();
         float s[S::RT][S::RT];
         dots<DP>(p.D, sq, skv, s);
+        const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i) {
             const int pos = q0 + ty * S::RT + i + off;
             float most = -INFINITY;
 #pragma unroll
             for (int j = 0; j < S::RT; ++j) {
-                s[i][j] = pos < seq.nk && sees(p, pos, k0 + tx + 16 * j) ? s[i][j] * c : -INFINITY;
+                s[i][j] = whole || (pos < seq.nk && sees(p, pos, k0 + tx + 16 * j)) ? s[i][j] * c : -INFINITY;
                 most = fmaxf(most, s[i][j]);
             }
             const float now = fmaxf(m[i], row_max(most)), ref = now == -INFINITY ? 0.0f : now;
-            const float f = exp2f(m[i] - ref);
+            const float f = exp2_fast(m[i] - ref);
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < S::RT; ++j) {
-                const float e = exp2f(s[i][j] - ref);
+                const float e = exp2_fast(s[i][j] - ref);
                 sum += e;
                 sp[(ty * S::RT + i) * S::LP + tx + 16 * j] = e;
             }
@@ -296,13 +308,14 @@ __global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_co
         float s[S::RT][S::RT], d[S::RT][S::RT];
         dots<DP>(p.D, sk, sq, s);
         dots<DP>(p.D, sv, sg, d);
+        const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i)
 #pragma unroll
             for (int j = 0; j < S::RT; ++j) {
                 const int key = k0 + ty * S::RT + i, q = tx + 16 * j;
-                const bool seen = q0 + q < seq.nq && sees(p, q0 + q + off, key);
-                const float e = seen ? exp2f((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
+                const bool seen = whole || (q0 + q < seq.nq && sees(p, q0 + q + off, key));
+                const float e = seen ? exp2_fast((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
                 sp[(ty * S::RT + i) * S::LP + q] = e;
                 sd[(ty * S::RT + i) * S::LP + q] = seen ? e * (d[i][j] - sdel[q]) : 0.0f;
             }
@@ -359,13 +372,14 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
         float s[S::RT][S::RT], d[S::RT][S::RT];
         dots<DP>(p.D, sq, sk, s);
         dots<DP>(p.D, sg, sv, d);
+        const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i)
 #pragma unroll
             for (int j = 0; j < S::RT; ++j) {
                 const int q = q0 + ty * S::RT + i;
-                const bool seen = q < seq.nq && sees(p, q + off, k0 + tx + 16 * j);
-                const float e = seen ? exp2f((s[i][j] * p.scale - lse[i]) * kLog2e) : 0.0f;
+                const bool seen = whole || (q < seq.nq && sees(p, q + off, k0 + tx + 16 * j));
+                const float e = seen ? exp2_fast((s[i][j] * p.scale - lse[i]) * kLog2e) : 0.0f;
                 sd[(ty * S::RT + i) * S::LP + tx + 16 * j] = seen ? e * (d[i][j] - del[i]) : 0.0f;
             }
         __syncthreads();
@@ -382,9 +396,13 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
     }
 }
 
-// out = the parts' sums, added in their order.
-template <typename T> __global__ void __launch_bounds__(256) k_attention_sum(const __grid_constant__ Problem p, Sums from, View out, int H, int S) {
+// One or two outputs: the parts' sums, added in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attention_sum(const __grid_constant__ Problem p, Sums from0, Sums from1, View out0, View out1, int H, int S) {
     pdl_begin();
+    const Sums& from = blockIdx.y ? from1 : from0;
+    const View& out = blockIdx.y ? out1 : out0;
+    if (!out.p) return;
     const int64_t n = static_cast<int64_t>(p.B) * H * S * p.D;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         float v = 0.0f;
@@ -404,10 +422,10 @@ bool whole(const Problem& p, bool backward) {
     return ok && (!backward || heads::rows_on(p.dout, es, 16));
 }
 
-// Parts of each of `ctas` tiles of at most `steps` steps: enough for two CTAs a SM.  2048 tokens of 8
-// heads over 2 with 128 columns, binary32: gradients 2535 -> 1130 us, 3 x 200 of 6 over 3: 193 -> 77.
+// Parts of each of `ctas` tiles of at most `steps` steps: enough for four CTAs a SM.  2048 tokens of 8
+// heads over 2 with 128 columns, binary32: gradients 2535 -> 918 us, 3 x 200 of 6 over 3: 193 -> 72.
 int64_t parts_of(Context* ctx, int64_t ctas, int64_t steps) {
-    const int64_t want = (2 * static_cast<int64_t>(ctx->num_sms) + ctas - 1) / std::max<int64_t>(ctas, 1);
+    const int64_t want = (4 * static_cast<int64_t>(ctx->num_sms) + ctas - 1) / std::max<int64_t>(ctas, 1);
     return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps));
 }
 
@@ -449,11 +467,11 @@ template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, con
             out->p = static_cast<float*>(m);
             return static_cast<qsml_status_t>(QSML_OK);
         };
-        auto join = [&](const Sums& from, const View& out, int H, int Sn) {
-            if (from.parts == 1 || !out.p) return static_cast<qsml_status_t>(QSML_OK);
+        auto join = [&](const Sums& from0, const Sums& from1, const View& out0, const View& out1, int H, int Sn) {
+            if (from0.parts == 1) return static_cast<qsml_status_t>(QSML_OK);
             const int64_t n = (static_cast<int64_t>(p.B) * H * Sn * p.D + 255) / 256;
-            const cudaError_t e = launch_pdl(k_attention_sum<T>, dim3(static_cast<unsigned>(std::min<int64_t>(n, 8 * ctx->num_sms))), dim3(256), 0,
-                                             ctx->stream, p, from, out, H, Sn);
+            const dim3 grid(static_cast<unsigned>(std::min<int64_t>(n, 8 * ctx->num_sms)), out1.p ? 2 : 1);
+            const cudaError_t e = launch_pdl(k_attention_sum<T>, grid, dim3(256), 0, ctx->stream, p, from0, from1, out0, out1, H, Sn);
             if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_sum");
             return after_launch(ctx, "k_attention_sum");
         };
@@ -463,15 +481,14 @@ template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, con
             QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_k));
             QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_v));
             QSML_TRY_STATUS(launch(ctx, k_attention_dkv_simt<T, DP>, "k_attention_dkv_simt", grad_smem<DP>(), ctas * parts, p, delta, to_k, to_v, tk, vec));
-            QSML_TRY_STATUS(join(to_k, p.dk, p.Hk, p.Sk));
-            QSML_TRY_STATUS(join(to_v, p.dv, p.Hk, p.Sk));
+            QSML_TRY_STATUS(join(to_k, to_v, p.dk, p.dv, p.Hk, p.Sk));
         }
         if (p.dq.p) {
             const int64_t ctas = static_cast<int64_t>(tq) * p.Hq * p.B, parts = parts_of(ctx, ctas, tk);
             Sums to;
             QSML_TRY_STATUS(sums(parts, p.Hq, p.Sq, &to));
             QSML_TRY_STATUS(launch(ctx, k_attention_dq_simt<T, DP>, "k_attention_dq_simt", grad_smem<DP>(), ctas * parts, p, delta, to, tq, vec));
-            QSML_TRY_STATUS(join(to, p.dq, p.Hq, p.Sq));
+            QSML_TRY_STATUS(join(to, to, p.dq, View(), p.Hq, p.Sq));
         }
         return static_cast<qsml_status_t>(QSML_OK);
     });
