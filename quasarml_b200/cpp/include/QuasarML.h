@@ -3,7 +3,8 @@
 // slice with a step, transpose(x, d0, d1) as a view, contiguous, cast,
 // layer_norm, batch_matmul, matmul with an output dtype, cpu_fallback_count,
 // row-sharded reductions over several devices, linear and gated linear layers
-// with their backward passes, layer_norm_backward.
+// with their backward passes, layer_norm_backward, norm_rotary and attention with
+// theirs.
 // The Vulkan-only Kernel type (GLSL pipelines) has no counterpart.
 #pragma once
 
@@ -18,6 +19,7 @@
 #include "Core/Device.h"
 #include "Core/DeviceManager.h"
 #include "Core/Tensor.h"
+#include "Ops/Attention.h"
 #include "Ops/Distributed.h"
 #include "Ops/Elementwise.h"
 #include "Ops/FeedForward.h"
@@ -188,6 +190,31 @@ inline TensorPtr gated_linear(TensorPtr x, TensorPtr w_gate, TensorPtr w_up, Act
 inline GatedLinearGrads gated_linear_backward(TensorPtr x, TensorPtr w_gate, TensorPtr w_up, Activation act, TensorPtr gate,
                                               TensorPtr up, TensorPtr dy, bool want_dbias = false) {
     return QuasarML::Ops::gated_linear_backward(device(), x, w_gate, w_up, act, gate, up, dy, want_dbias);
+}
+
+// The attention sublayer: norms and rotation of queries and keys, attention, and their gradients.
+using QuasarML::AttentionGrads;
+using QuasarML::AttentionOptions;
+using QuasarML::NormRotaryGrads;
+using QuasarML::QueriesKeys;
+using QuasarML::RotaryOptions;
+using QuasarML::RotaryPairing;
+inline QueriesKeys norm_rotary(TensorPtr q, TensorPtr k, TensorPtr wq, TensorPtr wk, TensorPtr positions, TensorPtr frequencies,
+                               const RotaryOptions& options = {}) {
+    return QuasarML::Ops::norm_rotary(device(), q, k, wq, wk, positions, frequencies, options);
+}
+inline NormRotaryGrads norm_rotary_backward(TensorPtr q, TensorPtr k, TensorPtr wq, TensorPtr wk, TensorPtr positions,
+                                            TensorPtr frequencies, TensorPtr dq_out, TensorPtr dk_out,
+                                            const RotaryOptions& options = {}) {
+    return QuasarML::Ops::norm_rotary_backward(device(), q, k, wq, wk, positions, frequencies, dq_out, dk_out, options);
+}
+inline TensorPtr attention(TensorPtr q, TensorPtr k, TensorPtr v, const AttentionOptions& options = {},
+                           TensorPtr* keep_lse = nullptr) {
+    return QuasarML::Ops::attention(device(), q, k, v, options, keep_lse);
+}
+inline AttentionGrads attention_backward(TensorPtr q, TensorPtr k, TensorPtr v, TensorPtr o, TensorPtr lse, TensorPtr dout,
+                                         const AttentionOptions& options = {}) {
+    return QuasarML::Ops::attention_backward(device(), q, k, v, o, lse, dout, options);
 }
 
 inline TensorPtr reshape(TensorPtr x, const std::vector<u32>& new_shape) { return QuasarML::Ops::reshape(device(), x, new_shape); }
