@@ -152,7 +152,7 @@ QSML_API qsml_status_t qsml_synchronize(qsml_ctx* ctx);
 /* Limit, in SM clock cycles, after which a kernel that waits for data on an
  * mbarrier (the one-SM tensor-core GEMM, the one-SM kernel of the linear
  * layers, the layer-norm and softmax row pipelines, the layer norm's backward
- * pass) gives up: it stops, lets every copy and MMA it already issued
+ * pass, the tensor cores' attention kernels) gives up: it stops, lets every copy and MMA it already issued
  * finish, records QSML_E_TIMEOUT for the next qsml_synchronize and returns,
  * so the context stays usable.  0 restores the default (2e9 cycles, about
  * 1 s).  Stream-ordered: applies to kernels enqueued after the call.  Meant
@@ -534,8 +534,9 @@ QSML_API qsml_status_t qsml_norm_rotary_backward(qsml_ctx* ctx, const qsml_tdesc
  * used, whatever its bits; a key that a row does not see, but rows next to it do
  * (by window or position), has to be finite in v.
  * Scores, sums and norms are binary32; F16 weights of the values (the
- * exponentials) are rounded to F16 between the two products.  Outputs may not
- * overlap inputs or each other.  Workspace as for qsml_layer_norm_backward.
+ * exponentials) are rounded to F16 between the two products, and the tensor core's
+ * accumulator truncates: a sum of 8192 values of one sign loses 5e-5 of itself, of
+ * 131072 8e-4.  Outputs may not overlap inputs or each other.  Workspace as for qsml_layer_norm_backward.
  * No reference counterpart. */
 QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k, const qsml_tdesc* v,
                                       const qsml_tdesc* q_lengths, const qsml_tdesc* k_lengths, float scale,
@@ -548,8 +549,10 @@ QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const 
  * dq has q's shape, dk and dv k's, strides as o's above.  Each may be NULL when it
  * is not wanted; rows and keys behind a sequence's last get 0.  What lies behind a
  * sequence's last query or key is not used.  F16: P and dS are rounded to F16
- * between the products, dS times a power of two that keeps it in range.  No
- * atomics: the same bits at every call. */
+ * between the products, dS times a power of two that keeps it in range; where all
+ * the keys that a row sees are close together, sum(P dP) stands for the equal
+ * sum(dout o), whose o has been rounded.  No sum depends on the order in which CTAs
+ * finish: the same bits at every call. */
 QSML_API qsml_status_t qsml_attention_backward(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k,
                                                const qsml_tdesc* v, const qsml_tdesc* o, const qsml_tdesc* lse,
                                                const qsml_tdesc* dout, const qsml_tdesc* q_lengths,
