@@ -326,8 +326,12 @@ template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
 
 }  // namespace
 
-// Up to 64 rows a kv head.
-bool few_queries(const Problem& p) { return static_cast<int64_t>(p.Sq) * p.G <= 64; }
+// Up to 16 rows a kv head, and up to 64 over many keys, which more CTAs then share (64 queries of one head
+// over themselves take 19 us here, 7 by tiles).
+bool few_queries(const Problem& p) {
+    const int64_t rows = static_cast<int64_t>(p.Sq) * p.G;
+    return rows <= 16 || (rows <= 64 && p.Sk >= 4 * rows);
+}
 
 int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least) {
     // no row sees more keys than these

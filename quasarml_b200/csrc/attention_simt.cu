@@ -24,8 +24,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int DP> struct Shape {
-    static constexpr int BT = DP <= 128 ? 64 : 32;
+template <int DP, int B> struct Shape {
+    static constexpr int BT = B;
     static constexpr int RT = BT / 16;   // rows and columns of scores a thread
     static constexpr int CT = DP / 16;   // columns of a sum a thread
     static constexpr int LD = DP + 4;    // floats between rows: 16 lanes' 16-byte loads meet 8 by 8 in no bank
@@ -34,9 +34,9 @@ template <int DP> struct Shape {
 };
 
 // Rows [r0, r0 + BT) of a head, those in [lo, hi) or below sink, as floats; 0 elsewhere.
-template <typename T, int DP>
+template <typename T, int DP, int BT>
 __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at, int r0, int sink, int lo, int hi, int D, bool vec) {
-    using S = Shape<DP>;
+    using S = Shape<DP, BT>;
     constexpr int V = 16 / sizeof(T);
     const T* p = reinterpret_cast<const T*>(v.p) + at;
     if (vec) {
@@ -68,8 +68,8 @@ __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at,
 }
 
 // acc[i][j] = sum over columns of a[ty RT + i] b[tx + 16 j].
-template <int DP> __device__ __forceinline__ void dots(int D, const float* a, const float* b, float (&acc)[Shape<DP>::RT][Shape<DP>::RT]) {
-    using S = Shape<DP>;
+template <int DP, int BT> __device__ __forceinline__ void dots(int D, const float* a, const float* b, float (&acc)[Shape<DP, BT>::RT][Shape<DP, BT>::RT]) {
+    using S = Shape<DP, BT>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     P2 s[S::RT][S::RT];
 #pragma unroll
@@ -98,8 +98,8 @@ template <int DP> __device__ __forceinline__ void dots(int D, const float* a, co
 }
 
 // Columns of a thread's sums: 4 tx + 64 n + e.
-template <int DP> struct Sum {
-    P2 v[Shape<DP>::RT][Shape<DP>::CT / 2];
+template <int DP, int BT> struct Sum {
+    P2 v[Shape<DP, BT>::RT][Shape<DP, BT>::CT / 2];
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (auto& r : v)
@@ -108,7 +108,7 @@ template <int DP> struct Sum {
     }
     // += p (rows ty RT + i of [BT][LP]) times x ([BT][LD])
     __device__ __forceinline__ void add(const float* p, const float* x) {
-        using S = Shape<DP>;
+        using S = Shape<DP, BT>;
         const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll 2
         for (int k = 0; k < S::BT; k += 4) {
@@ -167,8 +167,7 @@ __device__ __forceinline__ bool all_see(const Problem& a, const Seq& s, int q0, 
 // sequence.
 struct Where {
     int part, tile, h, b;
-    __device__ __forceinline__ Where(int parts, int tiles, int H, bool backwards) {
-        int i = blockIdx.x;
+    __device__ __forceinline__ Where(int i, int parts, int tiles, int H, bool backwards) {
         part = i % parts;
         i /= parts;
         h = i % H;
@@ -187,20 +186,20 @@ struct Share {
     }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int BT>
 __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_constant__ Problem p, Parts parts, int tiles, bool vec) {
-    using S = Shape<DP>;
+    using S = Shape<DP, BT>;
     extern __shared__ float4 smem[];
     float *sq = reinterpret_cast<float*>(smem), *skv = sq + S::TILE, *sp = skv + S::TILE;
     pdl_begin();
-    const Where w(parts.parts, tiles, p.Hq, true);
+    const Where w(blockIdx.x, parts.parts, tiles, p.Hq, true);
     const Seq seq(p, w.b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
     const Keys keys(p, seq.nk, q0 + off, min(q0 + S::BT, seq.nq) - 1 + off);
     const Tiles t(keys, S::BT);
-    load_tile<T, DP>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
-    Sum<DP> o;
+    load_tile<T, DP, BT>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+    Sum<DP, BT> o;
     o.zero();
     float m[S::RT], l[S::RT];
 #pragma unroll
@@ -210,10 +209,10 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
     for (int n = steps.lo; n < steps.hi; ++n) {
         const int k0 = t.tile(n) * S::BT;
         __syncthreads();
-        load_tile<T, DP>(skv, p.k, w.b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
+        load_tile<T, DP, BT>(skv, p.k, w.b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
         __syncthreads();
         float s[S::RT][S::RT];
-        dots<DP>(p.D, sq, skv, s);
+        dots<DP, BT>(p.D, sq, skv, s);
         const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i) {
@@ -240,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
         }
         __syncthreads();
         // values that no row of the tile sees count for nothing, whatever they are
-        load_tile<T, DP>(skv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        load_tile<T, DP, BT>(skv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
         __syncthreads();
         o.add(sp, skv);
     }
@@ -261,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) k_attention_simt(const __grid_consta
 }
 
 // Shared memory of the gradients' kernels: two fixed tiles, two that come and go, P and dS.
-template <int DP> constexpr size_t grad_smem() { return sizeof(float) * (4 * Shape<DP>::TILE + 2 * Shape<DP>::PROBS + 2 * Shape<DP>::BT); }
+template <int DP, int BT> constexpr size_t grad_smem() { return sizeof(float) * (4 * Shape<DP, BT>::TILE + 2 * Shape<DP, BT>::PROBS + 2 * Shape<DP, BT>::BT); }
 
 // Sums of a gradient in parts: [parts][B][H][S][D] binary32.
 struct Sums {
@@ -273,21 +272,20 @@ struct Sums {
 };
 
 // dk and dv of a tile of keys.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_constant__ Problem p, const float* delta, Sums to_k, Sums to_v, int tiles, bool vec) {
-    using S = Shape<DP>;
+template <typename T, int DP, int BT>
+__device__ __forceinline__ void gradients_of_keys(const Problem& p, int cta, const float* delta, const Sums& to_k, const Sums& to_v, int tiles, bool vec) {
+    using S = Shape<DP, BT>;
     extern __shared__ float4 smem[];
     float *sk = reinterpret_cast<float*>(smem), *sv = sk + S::TILE, *sq = sv + S::TILE, *sg = sq + S::TILE, *sp = sg + S::TILE,
           *sd = sp + S::PROBS, *sl = sd + S::PROBS, *sdel = sl + S::BT;
-    pdl_begin();
-    const Where w(to_k.parts, tiles, p.Hk, false);
+    const Where w(cta, to_k.parts, tiles, p.Hk, false);
     const int hk = w.h, b = w.b;
     const Seq seq(p, b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int k0 = w.tile * S::BT, off = seq.nk - seq.nq;
-    load_tile<T, DP>(sk, p.k, b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
-    load_tile<T, DP>(sv, p.v, b * p.v.b + hk * p.v.h, k0, 0, 0, seq.nk, p.D, vec);
-    Sum<DP> dk, dv;
+    load_tile<T, DP, BT>(sk, p.k, b * p.k.b + hk * p.k.h, k0, 0, 0, seq.nk, p.D, vec);
+    load_tile<T, DP, BT>(sv, p.v, b * p.v.b + hk * p.v.h, k0, 0, 0, seq.nk, p.D, vec);
+    Sum<DP, BT> dk, dv;
     dk.zero();
     dv.zero();
     const Queries qs(p, seq, k0, k0 + S::BT);
@@ -297,8 +295,8 @@ __global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_co
         const int h = hk * p.G + n / per, q0 = (t0 + n % per) * S::BT;
         const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
         __syncthreads();
-        load_tile<T, DP>(sq, p.q, b * p.q.b + h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
-        load_tile<T, DP>(sg, p.dout, b * p.dout.b + h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
+        load_tile<T, DP, BT>(sq, p.q, b * p.q.b + h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+        load_tile<T, DP, BT>(sg, p.dout, b * p.dout.b + h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
         if (threadIdx.x < S::BT) {
             const int q = q0 + threadIdx.x;
             sl[threadIdx.x] = q < seq.nq ? p.lse[stat + q] : 0.0f;
@@ -306,8 +304,8 @@ __global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_co
         }
         __syncthreads();
         float s[S::RT][S::RT], d[S::RT][S::RT];
-        dots<DP>(p.D, sk, sq, s);
-        dots<DP>(p.D, sv, sg, d);
+        dots<DP, BT>(p.D, sk, sq, s);
+        dots<DP, BT>(p.D, sv, sg, d);
         const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i)
@@ -338,21 +336,20 @@ __global__ void __launch_bounds__(kThreads) k_attention_dkv_simt(const __grid_co
 }
 
 // dq of a tile of queries.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_constant__ Problem p, const float* delta, Sums to, int tiles, bool vec) {
-    using S = Shape<DP>;
+template <typename T, int DP, int BT>
+__device__ __forceinline__ void gradients_of_queries(const Problem& p, int cta, const float* delta, const Sums& to, int tiles, bool vec) {
+    using S = Shape<DP, BT>;
     extern __shared__ float4 smem[];
     float *sq = reinterpret_cast<float*>(smem), *sg = sq + S::TILE, *sk = sg + S::TILE, *sv = sk + S::TILE, *sd = sv + S::TILE;
-    pdl_begin();
-    const Where w(to.parts, tiles, p.Hq, true);
+    const Where w(cta, to.parts, tiles, p.Hq, true);
     const Seq seq(p, w.b);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int q0 = w.tile * S::BT, off = seq.nk - seq.nq, hk = w.h / p.G;
     const Keys keys(p, seq.nk, q0 + off, min(q0 + S::BT, seq.nq) - 1 + off);
     const Tiles t(keys, S::BT);
-    load_tile<T, DP>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
-    load_tile<T, DP>(sg, p.dout, w.b * p.dout.b + w.h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
-    Sum<DP> dq;
+    load_tile<T, DP, BT>(sq, p.q, w.b * p.q.b + w.h * p.q.h, q0, 0, 0, seq.nq, p.D, vec);
+    load_tile<T, DP, BT>(sg, p.dout, w.b * p.dout.b + w.h * p.dout.h, q0, 0, 0, seq.nq, p.D, vec);
+    Sum<DP, BT> dq;
     dq.zero();
     const int64_t stat = (static_cast<int64_t>(w.b) * p.Hq + w.h) * p.Sq;
     float lse[S::RT], del[S::RT];
@@ -366,12 +363,12 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
     for (int n = steps.lo; n < steps.hi; ++n) {
         const int k0 = t.tile(n) * S::BT;
         __syncthreads();
-        load_tile<T, DP>(sk, p.k, w.b * p.k.b + hk * p.k.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
-        load_tile<T, DP>(sv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        load_tile<T, DP, BT>(sk, p.k, w.b * p.k.b + hk * p.k.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
+        load_tile<T, DP, BT>(sv, p.v, w.b * p.v.b + hk * p.v.h, k0, keys.sink, keys.lo, keys.hi, p.D, vec);
         __syncthreads();
         float s[S::RT][S::RT], d[S::RT][S::RT];
-        dots<DP>(p.D, sq, sk, s);
-        dots<DP>(p.D, sg, sv, d);
+        dots<DP, BT>(p.D, sq, sk, s);
+        dots<DP, BT>(p.D, sg, sv, d);
         const bool whole = all_see(p, seq, q0, k0, S::BT);
 #pragma unroll
         for (int i = 0; i < S::RT; ++i)
@@ -396,13 +393,24 @@ __global__ void __launch_bounds__(kThreads) k_attention_dq_simt(const __grid_con
     }
 }
 
-// One or two outputs: the parts' sums, added in their order.
-template <typename T>
-__global__ void __launch_bounds__(256) k_attention_sum(const __grid_constant__ Problem p, Sums from0, Sums from1, View out0, View out1, int H, int S) {
+// The first key_ctas CTAs have keys, the others queries.
+template <typename T, int DP, int BT>
+__global__ void __launch_bounds__(kThreads)
+    k_attention_bwd_simt(const __grid_constant__ Problem p, const float* delta, Sums to_q, Sums to_k, Sums to_v, int key_ctas, int tq, int tk, bool vec) {
     pdl_begin();
-    const Sums& from = blockIdx.y ? from1 : from0;
-    const View& out = blockIdx.y ? out1 : out0;
-    if (!out.p) return;
+    if (static_cast<int>(blockIdx.x) < key_ctas)
+        gradients_of_keys<T, DP, BT>(p, blockIdx.x, delta, to_k, to_v, tk, vec);
+    else
+        gradients_of_queries<T, DP, BT>(p, blockIdx.x - key_ctas, delta, to_q, tq, vec);
+}
+
+// The gradients of which there are parts (dq, dk, dv by blockIdx.y): their sums, added in order.
+template <typename T> __global__ void __launch_bounds__(256) k_attention_sum(const __grid_constant__ Problem p, Sums to_q, Sums to_k, Sums to_v) {
+    pdl_begin();
+    const int which = blockIdx.y, H = which ? p.Hk : p.Hq, S = which ? p.Sk : p.Sq;
+    const Sums& from = which == 0 ? to_q : which == 1 ? to_k : to_v;
+    const View& out = which == 0 ? p.dq : which == 1 ? p.dk : p.dv;
+    if (!out.p || from.parts == 1) return;
     const int64_t n = static_cast<int64_t>(p.B) * H * S * p.D;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         float v = 0.0f;
@@ -438,25 +446,39 @@ qsml_status_t launch(Context* ctx, K kernel, const char* name, size_t smem, int6
     return after_launch(ctx, name);
 }
 
-template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
+// f(width, tile) with constants: tiles of 64, or of 32 for more than 128 columns and where there are few
+// steps of 64, which take four times as long (SMALL a SM: 3 x 200 tokens of 6 heads over 3, binary32,
+// gradients 69 -> 40 us).
+template <typename F> qsml_status_t by_shape(Context* ctx, const Problem& p, int64_t heads, F&& f) {
+    constexpr int64_t SMALL = 8;
+    const int64_t tq = (p.Sq + 63) / 64, tk = std::min<int64_t>((p.Sk + 63) / 64, p.window ? (static_cast<int64_t>(p.window) + p.sinks) / 64 + 2 : p.Sk);
+    const bool small = tq * tk * heads * p.B <= SMALL * ctx->num_sms;
     return by_width(p.D, [&](auto width) {
-        constexpr int DP = decltype(width)::value;
-        using S = Shape<DP>;
+        if constexpr (decltype(width)::value <= 128)
+            if (!small) return f(width, std::integral_constant<int, 64>());
+        return f(width, std::integral_constant<int, 32>());
+    });
+}
+
+template <typename T> qsml_status_t forward(Context* ctx, const Problem& p) {
+    return by_shape(ctx, p, p.Hq, [&](auto width, auto tile) {
+        constexpr int DP = decltype(width)::value, BT = decltype(tile)::value;
+        using S = Shape<DP, BT>;
         const int tiles = (p.Sq + S::BT - 1) / S::BT;
         const int64_t ctas = static_cast<int64_t>(tiles) * p.Hq * p.B;
         Workspace ws(ctx);
         Parts parts;
         QSML_TRY_STATUS(get_parts(ctx, &ws, p, parts_of(ctx, ctas, (p.Sk + S::BT - 1) / S::BT), &parts));
-        QSML_TRY_STATUS(launch(ctx, k_attention_simt<T, DP>, "k_attention_simt", sizeof(float) * (2 * S::TILE + S::PROBS), ctas * parts.parts, p, parts,
+        QSML_TRY_STATUS(launch(ctx, k_attention_simt<T, DP, BT>, "k_attention_simt", sizeof(float) * (2 * S::TILE + S::PROBS), ctas * parts.parts, p, parts,
                                tiles, whole(p, false)));
         return join_parts(ctx, p, parts);
     });
 }
 
 template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, const float* delta) {
-    return by_width(p.D, [&](auto width) {
-        constexpr int DP = decltype(width)::value;
-        using S = Shape<DP>;
+    return by_shape(ctx, p, p.Hq, [&](auto width, auto tile) {
+        constexpr int DP = decltype(width)::value, BT = decltype(tile)::value;
+        using S = Shape<DP, BT>;
         const bool vec = whole(p, true);
         const int tq = (p.Sq + S::BT - 1) / S::BT, tk = (p.Sk + S::BT - 1) / S::BT;
         Workspace ws(ctx);
@@ -467,28 +489,22 @@ template <typename T> qsml_status_t backward(Context* ctx, const Problem& p, con
             out->p = static_cast<float*>(m);
             return static_cast<qsml_status_t>(QSML_OK);
         };
-        auto join = [&](const Sums& from0, const Sums& from1, const View& out0, const View& out1, int H, int Sn) {
-            if (from0.parts == 1) return static_cast<qsml_status_t>(QSML_OK);
-            const int64_t n = (static_cast<int64_t>(p.B) * H * Sn * p.D + 255) / 256;
-            const dim3 grid(static_cast<unsigned>(std::min<int64_t>(n, 8 * ctx->num_sms)), out1.p ? 2 : 1);
-            const cudaError_t e = launch_pdl(k_attention_sum<T>, grid, dim3(256), 0, ctx->stream, p, from0, from1, out0, out1, H, Sn);
+        const bool keys = p.dk.p || p.dv.p, queries = p.dq.p != nullptr;
+        const int64_t kc = keys ? static_cast<int64_t>(tk) * p.Hk * p.B : 0, qc = queries ? static_cast<int64_t>(tq) * p.Hq * p.B : 0;
+        const int64_t kparts = keys ? parts_of(ctx, kc, static_cast<int64_t>(tq) * p.G) : 1, qparts = queries ? parts_of(ctx, qc, tk) : 1;
+        Sums to_q, to_k, to_v;
+        QSML_TRY_STATUS(sums(qparts, p.Hq, p.Sq, &to_q));
+        QSML_TRY_STATUS(sums(kparts, p.Hk, p.Sk, &to_k));
+        QSML_TRY_STATUS(sums(kparts, p.Hk, p.Sk, &to_v));
+        if (kc * kparts > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention_backward: dimensions too large");
+        QSML_TRY_STATUS((launch(ctx, k_attention_bwd_simt<T, DP, BT>, "k_attention_bwd_simt", grad_smem<DP, BT>(), kc * kparts + qc * qparts, p, delta, to_q,
+                                to_k, to_v, static_cast<int>(kc * kparts), tq, tk, vec)));
+        if (kparts > 1 || qparts > 1) {
+            const int64_t most = std::max(static_cast<int64_t>(p.Hq) * p.Sq, static_cast<int64_t>(p.Hk) * p.Sk) * p.B * p.D;
+            const dim3 grid(static_cast<unsigned>(std::min<int64_t>((most + 255) / 256, 8 * ctx->num_sms)), 3);
+            const cudaError_t e = launch_pdl(k_attention_sum<T>, grid, dim3(256), 0, ctx->stream, p, to_q, to_k, to_v);
             if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_sum");
-            return after_launch(ctx, "k_attention_sum");
-        };
-        if (p.dk.p || p.dv.p) {
-            const int64_t ctas = static_cast<int64_t>(tk) * p.Hk * p.B, parts = parts_of(ctx, ctas, static_cast<int64_t>(tq) * p.G);
-            Sums to_k, to_v;
-            QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_k));
-            QSML_TRY_STATUS(sums(parts, p.Hk, p.Sk, &to_v));
-            QSML_TRY_STATUS(launch(ctx, k_attention_dkv_simt<T, DP>, "k_attention_dkv_simt", grad_smem<DP>(), ctas * parts, p, delta, to_k, to_v, tk, vec));
-            QSML_TRY_STATUS(join(to_k, to_v, p.dk, p.dv, p.Hk, p.Sk));
-        }
-        if (p.dq.p) {
-            const int64_t ctas = static_cast<int64_t>(tq) * p.Hq * p.B, parts = parts_of(ctx, ctas, tk);
-            Sums to;
-            QSML_TRY_STATUS(sums(parts, p.Hq, p.Sq, &to));
-            QSML_TRY_STATUS(launch(ctx, k_attention_dq_simt<T, DP>, "k_attention_dq_simt", grad_smem<DP>(), ctas * parts, p, delta, to, tq, vec));
-            QSML_TRY_STATUS(join(to, to, p.dq, View(), p.Hq, p.Sq));
+            QSML_TRY_STATUS(after_launch(ctx, "k_attention_sum"));
         }
         return static_cast<qsml_status_t>(QSML_OK);
     });

@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(most_threads(BWD), 2) k_norm_rotary(const __gr
 
 template <typename T, bool BWD> qsml_status_t launch(Context* ctx, const RotaryArgs& a, const Shape& h, unsigned grid) {
     cudaError_t e = cudaSuccess;
-    const bool one = a.D / (2 * h.vec) <= 32;
+    const bool one = a.D / (2 * h.vec) <= 32, two = a.D / (2 * h.vec) <= 64;
     auto go = [&](auto kernel) {
         e = launch_pdl(kernel, dim3(grid), dim3(h.threads), h.smem, ctx->stream, a, h);
     };
@@ -385,9 +385,9 @@ template <typename T, bool BWD> qsml_status_t launch(Context* ctx, const RotaryA
             else
                 one ? go(k_norm_rotary<T, FULL, 1, P, BWD>) : go(k_norm_rotary<T, FULL, 2, P, BWD>);
         } else if (h.vec == 2) {
-            one ? go(k_norm_rotary<T, 2, 1, P, BWD>) : go(k_norm_rotary<T, 2, 4, P, BWD>);
+            one ? go(k_norm_rotary<T, 2, 1, P, BWD>) : two ? go(k_norm_rotary<T, 2, 2, P, BWD>) : go(k_norm_rotary<T, 2, 4, P, BWD>);
         } else {
-            one ? go(k_norm_rotary<T, 1, 1, P, BWD>) : go(k_norm_rotary<T, 1, 8, P, BWD>);
+            one ? go(k_norm_rotary<T, 1, 1, P, BWD>) : two ? go(k_norm_rotary<T, 1, 2, P, BWD>) : go(k_norm_rotary<T, 1, 8, P, BWD>);
         }
     };
     a.pairs ? pairing(std::true_type()) : pairing(std::false_type());
