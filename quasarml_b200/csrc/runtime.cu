@@ -296,7 +296,8 @@ qsml_status_t CachingAllocator::free(void* ptr, std::string* err) {
     size_t sz = it->second;
     live_.erase(it);
     live_bytes_ -= sz;
-    free_.emplace(sz, ptr);
+    // before the others of its size: the block last in use is the next one given out
+    free_.emplace_hint(free_.lower_bound(sz), sz, ptr);
     return QSML_OK;
 }
 
