@@ -27,8 +27,12 @@ using heads::Pack;
 using heads::to_f;
 using heads::View;
 
-// Threads of a CTA, at most; two CTAs a SM keep enough rows on their way.
-constexpr int most_threads(bool backward) { return backward ? 320 : 384; }
+// Threads of a CTA, at most, and CTAs a SM that registers are to be had for.  Forward: 80 registers, 81 us
+// of 16384 tokens of 40 heads of 128 in binary16 (4 x 192 threads 80, 5 x 160 82, 6 x 160 90, and 109 with two
+// rows on their way instead of one).  Backward: 128, without spills, 122 us (2 x 320 threads 154, 4 x 128
+// 131).
+constexpr int most_threads(bool backward) { return backward ? 160 : 384; }
+constexpr int least_ctas(bool backward) { return backward ? 3 : 2; }
 constexpr int kMaxAxes = 4;
 constexpr int kMaxD = 512;
 
@@ -171,7 +175,7 @@ struct Shape {
 
 // NC chunk pairs of V columns a lane.
 template <typename T, int V, int NC, bool PAIRS, bool BWD>
-__global__ void __launch_bounds__(most_threads(BWD), 2) k_norm_rotary(const __grid_constant__ RotaryArgs a, Shape sh) {
+__global__ void __launch_bounds__(most_threads(BWD), least_ctas(BWD)) k_norm_rotary(const __grid_constant__ RotaryArgs a, Shape sh) {
     extern __shared__ float4 shared[];  // cosines and sines [2][batch][2][pairs]; backward: then [slots][D] partial sums
     float* angle = reinterpret_cast<float*>(shared);
     pdl_begin();
