@@ -374,6 +374,65 @@ def test_the_same_bits_at_every_call_and_in_graphs(ctx, dt, sq, sk):
         ctx.set_stream(own)
 
 
+@DT
+@pytest.mark.parametrize("sq,sk,D", [(200, 200, 64), (200, 200, 128), (5, 300, 64), (90, 90, 36)])
+def test_what_is_no_number_stays_with_the_rows_that_see_it(ctx, dt, sq, sk, D):
+    """A query of NaN is NaN in its row alone, a key of NaN in the rows that see it; the others keep their bits."""
+    c = Case(dt, sq, sk, 2, 1, D, 50, 2)
+    clean, lse = run_forward(ctx, c)
+    row, key = sq // 2, sk - sq // 2
+    c.q[0, row, 0] = NAN
+    o, s = run_forward(ctx, c)
+    hit = np.zeros((1, sq, 2), bool)
+    hit[0, row, 0] = True
+    assert np.isnan(o[hit]).all() and np.array_equal(o[~hit], clean[~hit])
+    assert np.array_equal(np.isnan(s), hit.transpose(0, 2, 1))
+    c = Case(dt, sq, sk, 2, 1, D, 50, 2)
+    c.k[0, key] = NAN
+    o, s = run_forward(ctx, c)
+    sees = visible(sq, sk, sq, sk, 50, 2)[:, key]
+    assert sees.any() and not sees.all()
+    assert np.isnan(o[0, sees]).all() and np.array_equal(o[0, ~sees], clean[0, ~sees])
+    assert np.array_equal(s[0][:, ~sees], lse[0][:, ~sees])
+
+
+def test_two_contexts_at_once():
+    """Two contexts on streams of their own, in flight together, give what each gives alone."""
+    import torch
+    torch.cuda.set_device(0)
+    ctxs, streams = [abi.Context(0), abi.Context(0)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    work, want = [], []
+    for n, (c, s) in enumerate(zip(ctxs, streams)):
+        case = Case(np.float16, 700 + 60 * n, 700 + 60 * n, 4, 2, 128 if n else 64, 300, 5, B=2, seed=30 + n)
+        t = [dev(x) for x in (case.q, case.k, case.v, case.do)]
+        out = [torch.zeros_like(t[0]), torch.zeros(2, 4, case.sq, device="cuda")] + [torch.zeros_like(t[i]) for i in range(3)]
+        token = torch.zeros_like(t[0][:, :1])
+        how = case.how()
+
+        def call(ctx=c, t=t, out=out, token=token, how=how):
+            ctx.attention(d(t[0]), d(t[1]), d(t[2]), d(out[0]), lse=d(out[1]), **how)
+            ctx.attention_backward(*[d(x) for x in (t[0], t[1], t[2], out[0], out[1], t[3], out[2], out[3], out[4])], **how)
+            ctx.attention(d(t[0][:, -1:]), d(t[1]), d(t[2]), d(token), **how)
+        torch.cuda.synchronize()
+        c.set_stream(s.cuda_stream)
+        call()
+        c.synchronize()
+        want.append([host(x) for x in out + [token]])
+        for x in out + [token]:
+            x.zero_()
+        work.append((call, out + [token], case))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for call, _, _ in work:
+            call()
+    for c, (_, out, _), w in zip(ctxs, work, want):
+        c.synchronize()
+        for x, y in zip(out, w):
+            assert np.array_equal(host(x), y)
+    for c in ctxs:
+        c.close()
+
+
 def test_offsets_beyond_2_to_the_31(ctx):
     """A cache whose second sequence starts past 2^31 elements, read in place."""
     import torch
