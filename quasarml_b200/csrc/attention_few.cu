@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) k_attention_few(const __grid_constan
 }
 
 // The parts of a row joined in a fixed order: by a warp, or by eight with every eighth part each where
-// there are more than eight.
+// there are more than eight parts or few rows.
 constexpr int kMaxParts = 128, kJoinWarps = 8;
 template <typename T> __global__ void __launch_bounds__(32 * kJoinWarps) k_attention_join(const __grid_constant__ Problem p, Parts parts, int64_t rows, int per_row) {
     __shared__ float weight[kJoinWarps][kMaxParts], part[kJoinWarps][256];
@@ -338,8 +338,8 @@ int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, 
     const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (visible + least - 1) / least));
     // The time of n parts: waves of CTAs (whole ones, where all are alike), each of a part's keys and
-    // of what a CTA takes besides, as long as START keys (128 to 1024 measured: 16 sequences over up to 8192 keys
-    // 81, 79, 76, 85 us; 32 over 1000 43, 38, 38, 30; one over 32768 52, 42, 48, 35).
+    // of what a CTA takes besides, as long as START keys (128, 256, 512 and 1024 measured: 16 sequences over up to
+    // 8192 keys 81, 79, 76, 85 us; 32 over 1000 43, 38, 38, 30; one over 32768 52, 42, 48, 35).
     constexpr double START = 512.0;
     const double slots = static_cast<double>(ctx->num_sms) * resident;
     int64_t best = 1;
@@ -367,7 +367,7 @@ qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts) {
     if (parts.parts == 1) return QSML_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
     if (rows > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
-    const int per_row = parts.parts > kJoinWarps ? kJoinWarps : 1, at_once = kJoinWarps / per_row;
+    const int per_row = parts.parts > kJoinWarps || rows <= 4096 ? kJoinWarps : 1, at_once = kJoinWarps / per_row;
     const cudaError_t e = launch_pdl(p.f16 ? k_attention_join<__half> : k_attention_join<float>, dim3(static_cast<unsigned>((rows + at_once - 1) / at_once)),
                                      dim3(32 * kJoinWarps), 0, ctx->stream, p, parts, rows, per_row);
     if (e != cudaSuccess) return check_cuda(ctx, e, "k_attention_join");
