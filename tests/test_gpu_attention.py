@@ -245,6 +245,36 @@ def test_layouts(ctx, dt, D, permuted, off):
 
 
 @DT
+@pytest.mark.parametrize("sq", [1, 3, 140])
+def test_keys_shared_by_heads_and_read_backwards(ctx, dt, sq):
+    """kv heads of stride 0, and a cache whose tokens lie in descending order."""
+    import torch
+    c = Case(dt, sq, 140, 4, 2, 64, 50, 2, B=2)
+    c.k[:, :, 1], c.v[:, :, 1] = c.k[:, :, 0], c.v[:, :, 0]
+    q, do = dev(c.q), dev(c.do)
+    ro, eo, rl, el = c.forward()
+    k, v = (dev(x[:, :, :1]).expand(2, 140, 2, 64) for x in (c.k, c.v))
+    flipped = [dev(np.ascontiguousarray(x[:, ::-1])) for x in (c.k, c.v)]
+
+    def backwards(t):
+        view = d(t)
+        view.data += 139 * t.stride(1) * t.element_size()
+        view.stride[1] = -t.stride(1)
+        return view
+    for keys, values in ((d(k), d(v)), (backwards(flipped[0]), backwards(flipped[1]))):
+        o, lse = torch.full_like(q, NAN), torch.full((2, 4, sq), NAN, device="cuda")
+        ctx.attention(d(q), keys, values, d(o), lse=d(lse), **c.how())
+        grads = [torch.full_like(q, NAN)] + [torch.full((2, 140, 2, 64), NAN, dtype=q.dtype, device="cuda") for _ in range(2)]
+        ctx.attention_backward(d(q), keys, values, d(o), d(lse), d(do), *[d(x) for x in grads], **c.how())
+        ctx.synchronize()
+        near(host(o), ro, eo, "o")
+        near(host(lse), rl, el, "lse")
+        ref, err = c.backward(host(o), host(lse))
+        for x, r, e, what in zip(grads, ref, err, ("dq", "dk", "dv")):
+            near(host(x), r, e, what)
+
+
+@DT
 def test_shared_keys_of_broadcast_sequences(ctx, dt):
     """Sequences that share their keys and values (stride 0): gradients are each sequence's own."""
     import torch
