@@ -108,6 +108,7 @@ qsml_status_t forward_few(Context* ctx, const Problem& p);
 // Calls f with the least of the widths that hold D columns as a constant.
 template <typename F> qsml_status_t by_width(int D, F&& f) {
     if (D <= 64) return f(std::integral_constant<int, 64>());
+    if (D <= 96) return f(std::integral_constant<int, 96>());
     if (D <= 128) return f(std::integral_constant<int, 128>());
     return f(std::integral_constant<int, 256>());
 }

@@ -41,12 +41,12 @@ __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at,
     const T* p = reinterpret_cast<const T*>(v.p) + at;
     if (vec) {
         // a thread's loads are all on their way before the first is stored
-        constexpr int COLS = DP / V, N = S::BT * COLS / kThreads;
+        constexpr int COLS = DP / V, ALL = S::BT * COLS, N = (ALL + kThreads - 1) / kThreads;
         heads::Pack<T, V> x[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = threadIdx.x + i * kThreads, c = at % COLS * V, row = r0 + at / COLS;
-            const bool in = (row >= lo || row < sink) && row < hi && c < D;
+            const bool in = at < ALL && (row >= lo || row < sink) && row < hi && c < D;
 #pragma unroll
             for (int e = 0; e < V; ++e) heads::from_f(0.0f, x[i].v[e]);
             if (in) x[i] = *reinterpret_cast<const heads::Pack<T, V>*>(p + row * v.s + c);
@@ -54,6 +54,7 @@ __device__ __forceinline__ void load_tile(float* dst, const View& v, int64_t at,
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = threadIdx.x + i * kThreads, c = at % COLS * V, r = at / COLS;
+            if (ALL % kThreads && at >= ALL) break;
 #pragma unroll
             for (int e = 0; e < V; e += 4)
                 *reinterpret_cast<float4*>(dst + r * S::LD + c + e) =
@@ -97,8 +98,9 @@ template <int DP, int BT> __device__ __forceinline__ void dots(int D, const floa
         for (int j = 0; j < S::RT; ++j) acc[i][j] = sum2(s[i][j]);
 }
 
-// Columns of a thread's sums: 4 tx + 64 n + e.
+// Columns of a thread's sums: 4 tx + 64 n + e, and 2 tx + e of the last 32 where they are half of 64.
 template <int DP, int BT> struct Sum {
+    static constexpr int FOURS = DP / 64;
     P2 v[Shape<DP, BT>::RT][Shape<DP, BT>::CT / 2];
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -118,7 +120,7 @@ template <int DP, int BT> struct Sum {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int n = 0; n < DP / 64; ++n) {
+                for (int n = 0; n < FOURS; ++n) {
                     const float4 y = *reinterpret_cast<const float4*>(x + (k + e) * S::LD + 4 * tx + 64 * n);
 #pragma unroll
                     for (int i = 0; i < S::RT; ++i) {
@@ -126,17 +128,31 @@ template <int DP, int BT> struct Sum {
                         v[i][2 * n + 1] = fma2(both(w[i][e]), pack(y.z, y.w), v[i][2 * n + 1]);
                     }
                 }
+            if constexpr (DP % 64 != 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 y = *reinterpret_cast<const float2*>(x + (k + e) * S::LD + 2 * tx + 64 * FOURS);
+#pragma unroll
+                    for (int i = 0; i < S::RT; ++i) v[i][2 * FOURS] = fma2(both(w[i][e]), pack(y.x, y.y), v[i][2 * FOURS]);
+                }
+            }
         }
     }
     template <typename T> __device__ __forceinline__ void store(int i, T* row, float f, int D) const {
         const int tx = threadIdx.x & 15;
 #pragma unroll
-        for (int n = 0; n < DP / 64; ++n) {
+        for (int n = 0; n < FOURS; ++n) {
             const float2 a = unpack(v[i][2 * n]), b = unpack(v[i][2 * n + 1]);
             const float y[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (4 * tx + 64 * n + e < D) heads::from_f(y[e], row[4 * tx + 64 * n + e]);
+        }
+        if constexpr (DP % 64 != 0) {
+            const float2 a = unpack(v[i][2 * FOURS]);
+            const int c = 2 * tx + 64 * FOURS;
+            if (c < D) heads::from_f(a.x * f, row[c]);
+            if (c + 1 < D) heads::from_f(a.y * f, row[c + 1]);
         }
     }
 };
