@@ -10,8 +10,8 @@
 // Bound by the way from S over P and P V to the next S (2400 cycles, of which the exponentials
 // take 1024 and the products of 128 columns as many), which two CTAs on a SM walk in turn: each
 // has half of TMEM and of shared memory, with 128 columns one tile of K and one of V, the next
-// loaded while the other is in use.  Measured at 8192 tokens of 32 heads over 8, 128 columns:
-// 500 us, 1100 TFLOP/s.  One CTA with two tiles of queries that share the loads: 495, but 67 us
+// loaded while the other is in use.  Measured at 8192 tokens of 32 heads over 8, 128 columns, every
+// earlier key visible: 492 us, 1120 TFLOP/s.  One CTA with two tiles of queries that share the loads: 495, but 67 us
 // instead of 53 for one head of 4096 tokens; two buffers of S with 64 keys each: 609; a quarter
 // of the exponentials on the FMA pipe: no gain.
 // Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, the second warpgroup has the rows and
@@ -152,10 +152,6 @@ __global__ void __launch_bounds__(kThreads, 2)
             // S = Q K^T of step n, after O += P V of the one before: MMAs are executed in the order of
             // their issue, so P has been read when S is written over it.
             for (int n = 0; n <= steps && ok; ++n) {
-                if (n < steps) {
-                    ok = warp_wait(full(slot(2 * n)), turn(2 * n), abort_flag, limit);
-                    if (!ok) break;
-                }
                 if (n > 0) {
                     const int v = 2 * n - 1;
                     ok = warp_wait(full(slot(v)), turn(v), abort_flag, limit);
@@ -172,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (issue) mma_commit(empty(slot(v)));
                 }
                 if (n == steps) break;
+                ok = warp_wait(full(slot(2 * n)), turn(2 * n), abort_flag, limit);
+                if (!ok) break;
                 tc_fence_after();
                 mma_scores<DP, TILE>(issue, tmem, score_desc(q_tile), score_desc(ring(slot(2 * n))));
                 if (issue) {
