@@ -34,6 +34,10 @@ __device__ __forceinline__ bool sees(const Problem& a, int p, int j) {
     return j <= p && (a.window == 0 || p - j < a.window || j < a.sinks);
 }
 
+// Whether the query at position p sees one key alone: its weight is 1 whatever the score, and its dS is 0,
+// which P (dP - delta) is only but for their roundings.
+__device__ __forceinline__ bool sees_one(const Problem& a, int p) { return p == 0 || (a.window == 1 && a.sinks == 0); }
+
 // The keys that some query of positions [p0, p1] sees: the sinks [0, sink) and [lo, hi),
 // with sink <= lo.
 struct Keys {

@@ -331,7 +331,7 @@ __device__ __forceinline__ void gradients_of_keys(const Problem& p, int cta, con
                 const bool seen = whole || (q0 + q < seq.nq && sees(p, q0 + q + off, key));
                 const float e = seen ? exp2_fast((s[i][j] * p.scale - sl[q]) * kLog2e) : 0.0f;
                 sp[(ty * S::RT + i) * S::LP + q] = e;
-                sd[(ty * S::RT + i) * S::LP + q] = seen ? e * (d[i][j] - sdel[q]) : 0.0f;
+                sd[(ty * S::RT + i) * S::LP + q] = seen && !sees_one(p, q0 + q + off) ? e * (d[i][j] - sdel[q]) : 0.0f;
             }
         __syncthreads();
         dv.add(sp, sg);
@@ -393,7 +393,7 @@ __device__ __forceinline__ void gradients_of_queries(const Problem& p, int cta, 
                 const int q = q0 + ty * S::RT + i;
                 const bool seen = whole || (q < seq.nq && sees(p, q + off, k0 + tx + 16 * j));
                 const float e = seen ? exp2_fast((s[i][j] * p.scale - lse[i]) * kLog2e) : 0.0f;
-                sd[(ty * S::RT + i) * S::LP + tx + 16 * j] = seen ? e * (d[i][j] - del[i]) : 0.0f;
+                sd[(ty * S::RT + i) * S::LP + tx + 16 * j] = seen && !sees_one(p, q + off) ? e * (d[i][j] - del[i]) : 0.0f;
             }
         __syncthreads();
         dq.add(sd, sk);

@@ -36,7 +36,7 @@ struct Stats {
 };
 
 // A CTA takes 128 rows of a head (blocks below qblocks: of dout and o, then of v), 16 lanes a row.
-__global__ void __launch_bounds__(256) k_attention_prepare(const __grid_constant__ Problem p, Stats st, int qblocks) {
+__global__ void __launch_bounds__(256, 4) k_attention_prepare(const __grid_constant__ Problem p, Stats st, int qblocks) {
     pdl_begin();
     const int lane = threadIdx.x & 15, row = threadIdx.x >> 4;
     const bool of_q = static_cast<int>(blockIdx.x) < qblocks;
@@ -58,32 +58,35 @@ __global__ void __launch_bounds__(256) k_attention_prepare(const __grid_constant
         for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
         return s;
     };
-    constexpr int ROWS = TILE / 16;
-    uint4 x[ROWS], y[ROWS];
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const int r = first + row + 16 * k;
-        x[k] = y[k] = make_uint4(0, 0, 0, 0);
-        if (r < n && mine) {
-            x[k] = *at(of_q ? p.dout : p.v, r);
-            if (of_q) y[k] = *at(p.o, r);
-        }
-    }
     float most[2] = {0.0f, 0.0f};
+    constexpr int ROWS = 4;  // of a lane at once: with all eight two CTAs fit a SM, and their waves took 30 us
+    for (int r0 = first + row; r0 < first + TILE; r0 += 16 * ROWS) {
+        uint4 x[ROWS], y[ROWS];
+        float lse[ROWS];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const int r = first + row + 16 * k;
-        most[0] = fmaxf(most[0], sum(x[k], x[k]));
-        if (!of_q) continue;
-        most[1] = fmaxf(most[1], sum(y[k], y[k]));
-        const float delta = sum(x[k], y[k]);
-        if (lane == 0) {
-            const float lse = r < n ? p.lse[static_cast<int64_t>(bh) * p.Sq + r] : -INFINITY;
-            st.minus[bh * st.pitch + r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -kLog2e, SHIFT);
-            st.delta[bh * st.pitch + r] = delta;
+        for (int k = 0; k < ROWS; ++k) {
+            const int r = r0 + 16 * k;
+            lse[k] = of_q && lane == 0 && r < n ? p.lse[static_cast<int64_t>(bh) * p.Sq + r] : -INFINITY;
+            x[k] = y[k] = make_uint4(0, 0, 0, 0);
+            if (r < n && mine) {
+                x[k] = *at(of_q ? p.dout : p.v, r);
+                if (of_q) y[k] = *at(p.o, r);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int r = r0 + 16 * k;
+            most[0] = fmaxf(most[0], sum(x[k], x[k]));
+            if (!of_q) continue;
+            most[1] = fmaxf(most[1], sum(y[k], y[k]));
+            const float delta = sum(x[k], y[k]);
+            if (lane == 0) {
+                st.minus[bh * st.pitch + r] = lse[k] == -INFINITY ? -INFINITY : fmaf(lse[k], -kLog2e, SHIFT);
+                st.delta[bh * st.pitch + r] = delta;
+            }
         }
     }
-    // one atomic a CTA: 18000 on one word took 20 us
+    // one atomic a CTA
     __shared__ float largest[2][8];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -369,6 +372,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_st16(s_at + 16 * h, f);
             }
             arrive(p_ready(w));
+            if (sees_one(p, pos + TILE) || (pos <= 0 && pos > -TILE)) {  // queries whose dS is 0: all, or that at position 0
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                    if (sees_one(p, pos + 64 * w + e)) r[e] = 0;
+            }
             ok = warp_wait(dp_full, n & 1, abort_flag, limit);
             if (!ok) break;
             tc_fence_after();
@@ -612,6 +620,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 keep(r, (below(hi) & ~below(lo)) | below(sink), (below(hi - 32) & ~below(lo - 32)) | below(sink - 32));
             }
             weights(r, c, [&](int) { return both(minus); });
+            if (sees_one(p, pos)) {
+#pragma unroll
+                for (uint32_t& x : r) x = 0;
+            }
             ok = warp_wait(dp_full, n & 1, abort_flag, limit);
             if (!ok) break;
             tc_fence_after();

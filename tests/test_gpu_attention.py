@@ -334,6 +334,26 @@ def test_gradients_left_out(ctx, dt):
 
 
 @DT
+@pytest.mark.parametrize("size", [(1, 1, 4, 2, 64, 0, 0), (1, 1, 2, 1, 128, 0, 0), (200, 200, 2, 1, 64, 1, 0), (140, 260, 2, 2, 128, 1, 0),
+                                  (3, 3, 1, 1, 33, 1, 0)], ids=str)
+def test_a_row_of_one_key_has_no_gradient_but_its_value(ctx, dt, size):
+    """With one key its weight is 1 whatever the score: dq and dk are 0, dv is the sum of the group's dout."""
+    import torch
+    c = Case(dt, *size, B=2)
+    ro, _, rl, _ = c.forward()
+    t = [dev(x) for x in (c.q, c.k, c.v, ro.astype(dt), rl.astype(np.float32), c.do)]
+    out = [torch.full_like(t[i], NAN) for i in range(3)]
+    ctx.attention_backward(*[d(x) for x in t], *[d(x) for x in out], **c.how())
+    ctx.synchronize()
+    assert not host(out[0]).any() and not host(out[1]).any()
+    want = np.zeros(c.v.shape)
+    want[:, c.sk - c.sq:] = c.do.astype(F64).reshape(2, c.sq, c.hk, c.hq // c.hk, c.D).sum(3)
+    size = np.abs(c.do.astype(F64)).max() * (c.hq // c.hk)
+    # the weight is off by 2^-11 in F16, and by the scores' rounding against lse's
+    near(host(out[2]), want, size * ((2.0 ** -11 if dt == np.float16 else 0) + 400 * 2.0 ** -24), "dv")
+
+
+@DT
 def test_gradients_against_differences(ctx, dt):
     """sum(o * dout) along a direction: the binary64 forward pass's central difference against the
     gradients' product with that direction, whose rounding is that of F16's P and dS (2^-11 each of
