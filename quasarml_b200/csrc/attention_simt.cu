@@ -10,7 +10,8 @@
 // summed by one CTA over all queries that see it and all heads of its group, dq of a tile
 // of queries by another over its keys: seven products instead of five, no atomics.  Where the tiles
 // do not fill the device, each one's steps are split over CTAs whose sums are joined in order.
-// Bound by the FFMA pipe and by shared memory, a 16-byte load for 8 multiply-adds.
+// Bound by the FFMA pipe and by shared memory, a 16-byte load for 8 multiply-adds; two fifths of that pipe
+// at 2048 tokens of 8 heads over 2 of 128 (269 us, 32 TFLOP/s of visible pairs), with two CTAs a SM.
 #include <algorithm>
 #include <type_traits>
 
@@ -463,8 +464,8 @@ qsml_status_t launch(Context* ctx, K kernel, const char* name, size_t smem, int6
 }
 
 // f(width, tile) with constants: tiles of 64, or of 32 for more than 128 columns and where there are few
-// steps of 64, which take four times as long (SMALL a SM: 3 x 200 tokens of 6 heads over 3, binary32,
-// gradients 69 -> 40 us).
+// steps of 64 (up to SMALL a SM), which take four times as long: 64 tokens of one head of 128, binary32,
+// gradients 41 -> 26 us.  With 24 for SMALL 2 x 777 tokens take 282 us instead of 225.
 template <typename F> qsml_status_t by_shape(Context* ctx, const Problem& p, int64_t heads, F&& f) {
     constexpr int64_t SMALL = 8;
     const int64_t tq = (p.Sq + 63) / 64, tk = std::min<int64_t>((p.Sk + 63) / 64, p.window ? (static_cast<int64_t>(p.window) + p.sinks) / 64 + 2 : p.Sk);

@@ -14,8 +14,9 @@
 // dS is rounded to binary16 between two products.  It is computed times a power of two that
 // brings 2 |dout| |v|, which bounds it, to [2^14, 2^15], and which the sums are divided by.
 // A row whose keys are all in one tile takes delta = sum(P dP) instead of sum(dout o): with a few
-// keys the rounding of o would be the largest error of dq and dk (0.00033 of their norm for
-// 0.00022).
+// keys the rounding of o would be the largest error of dq and dk (alone 0.00033 of their norm, where
+// their own rounding is 0.00021).  Measured, 2 x 4096 tokens of 16 heads over 2 with 128 columns, window
+// 2048: 417 us, dkv 241 (a step 3560 cycles) and dq 184 (2600).
 #include <algorithm>
 
 #include "attention_tc.cuh"
