@@ -92,8 +92,8 @@ bool tc_takes_backward(const Problem& p);
 qsml_status_t backward_tc(Context* ctx, const Problem& p);
 // A row's keys in parts, row = (b Hq + h) Sq + query: each part's sum, maximum (base 2, scaled) and norm.
 struct Parts {
-    float* sum = nullptr;   // [rows][parts][D], not divided by l
-    float* stat = nullptr;  // [rows][parts][2]: m, l
+    float* sum = nullptr;   // [rows][parts][D], not divided by l; on 16 bytes
+    float* stat = nullptr;  // [rows][parts][2]: m, l, read as pairs; on 16 bytes
     int parts = 1;
 };
 // Room for them in ws, where there is more than one.

@@ -357,9 +357,11 @@ qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t n
     if (n == 1) return QSML_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * p.Sq;
     void* m = nullptr;
-    QSML_TRY_STATUS(ws->get(sizeof(float) * rows * n * (p.D + 2), &m));
-    out->sum = static_cast<float*>(m);
-    out->stat = out->sum + rows * n * p.D;
+    // the pairs of statistics first, so that they lie on 8 bytes and the sums on 16 whatever rows * n * D is
+    const int64_t stats = (rows * n * 2 + 3) / 4 * 4;
+    QSML_TRY_STATUS(ws->get(sizeof(float) * (stats + rows * n * p.D), &m));
+    out->stat = static_cast<float*>(m);
+    out->sum = out->stat + stats;
     return QSML_OK;
 }
 
