@@ -549,8 +549,10 @@ QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const 
  * dq has q's shape, dk and dv k's, strides as o's above.  Each may be NULL when it
  * is not wanted; rows and keys behind a sequence's last get 0.  What lies behind a
  * sequence's last query or key is not used; what is not finite before it reaches the
- * gradients of the tokens next to it, which may not see it.  F16: P and dS are rounded to F16
- * between the products, dS times a power of two that keeps it in range; where all
+ * gradients of the tokens next to it, which may not see it, but of no other sequence or kv
+ * head.  F16: P and dS are rounded to F16
+ * between the products, dS times a power of two that keeps it in range, from the largest
+ * finite |dout|, |o| and |v| of its sequence and head (for dk, of its group of heads); where all
  * the keys that a row sees are close together, sum(P dP) stands for the equal
  * sum(dout o), whose o has been rounded.  No sum depends on the order in which CTAs
  * finish: the same bits at every call. */

@@ -3,7 +3,7 @@
 // With P = exp(scale q k^T - lse), dP = dout v^T, dS = P (dP - delta):
 //   dq = scale dS k,   dk = scale dS^T q,   dv = P^T dout.
 // k_attention_prepare takes delta = sum(dout o) of each row, lse in base 2, and the largest
-// |dout|, |o| and |v|.  k_attention_dq goes over a tile of queries' keys, k_attention_dkv over
+// |dout|, |o| and |v| of each head.  k_attention_dq goes over a tile of queries' keys, k_attention_dkv over
 // the queries of all heads of the group that see a tile of keys: P and dP are computed in both,
 // seven products instead of five, and no sum is shared between CTAs.  The accumulators stay in
 // TMEM (dkv: S^T, dP^T, dV and dK of 128 columns fill it); P^T and dS^T (dq: dS) are left there
@@ -12,7 +12,9 @@
 // Bound by the tensor core and the exponentials in turn: of a tile of 128 x 128 with 128
 // columns, 2048 (dkv) and 1536 (dq) cycles of products, and 1024 of exponentials.
 // dS is rounded to binary16 between two products.  It is computed times a power of two that
-// brings 2 |dout| |v|, which bounds it, to [2^14, 2^15], and which the sums are divided by.
+// brings 2 |dout| |v|, which bounds it, to [2^14, 2^15], and which the sums are divided by: in dq that of
+// the head, in dkv that of the largest head of the group, whose terms share a sum.  Only rows that take part
+// and are finite count, so that no sequence or kv head costs another bits.
 // A row whose keys are all in one tile takes delta = sum(P dP) instead of sum(dout o): with a few
 // keys the rounding of o would be the largest error of dq and dk (alone 0.00033 of their norm, where
 // their own rounding is 0.00021).  Measured, 2 x 4096 tokens of 16 heads over 2 with 128 columns, window
@@ -32,7 +34,7 @@ constexpr float SHIFT = 14.0f;
 
 struct Stats {
     float *minus, *delta;  // [B * Hq, pitch]; minus: SHIFT - lse in base 2, -inf where a row sees nothing
-    unsigned* largest;    // bits of the largest squared norms of dout, o, v
+    unsigned *of_q, *of_v;  // bits of the largest squared norms: [B * Hq][2] of dout's and o's rows, [B * Hk] of v's
     int64_t pitch;
 };
 
@@ -44,7 +46,10 @@ __global__ void __launch_bounds__(256, 4) k_attention_prepare(const __grid_const
     const int i = of_q ? blockIdx.x : blockIdx.x - qblocks, H = of_q ? p.Hq : p.Hk;
     const int bh = i % (p.B * H), first = i / (p.B * H) * TILE, b = bh / H, h = bh - b * H;
     const Seq seq(p, b);
-    const int n = of_q ? seq.nq : seq.nk;
+    const int n = of_q ? seq.nq : seq.nk, off = seq.nk - seq.nq;
+    // rows that take part: queries that see a key, keys that a query sees
+    const Keys keys(p, seq.nk, off, seq.nk - 1);
+    const int from = of_q ? -off : keys.lo, sink = of_q ? 0 : keys.sink;
     const bool mine = lane * 8 < p.D;
     auto at = [&](const View& v, int r) { return reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(v.p) + b * v.b + h * v.h + r * v.s + lane * 8); };
     auto sum = [&](const uint4& x, const uint4& y) {
@@ -60,6 +65,7 @@ __global__ void __launch_bounds__(256, 4) k_attention_prepare(const __grid_const
         return s;
     };
     float most[2] = {0.0f, 0.0f};
+    auto larger = [](float m, float x) { return x < INFINITY ? fmaxf(m, x) : m; };  // of numbers
     constexpr int ROWS = 4;  // of a lane at once: with all eight two CTAs fit a SM, and their waves took 30 us
     for (int r0 = first + row; r0 < first + TILE; r0 += 16 * ROWS) {
         uint4 x[ROWS], y[ROWS];
@@ -77,9 +83,12 @@ __global__ void __launch_bounds__(256, 4) k_attention_prepare(const __grid_const
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
             const int r = r0 + 16 * k;
-            most[0] = fmaxf(most[0], sum(x[k], x[k]));
+            const bool takes_part = r >= from || r < sink;
+            const float xx = sum(x[k], x[k]);
+            if (takes_part) most[0] = larger(most[0], xx);
             if (!of_q) continue;
-            most[1] = fmaxf(most[1], sum(y[k], y[k]));
+            const float yy = sum(y[k], y[k]);
+            if (takes_part) most[1] = larger(most[1], yy);
             const float delta = sum(x[k], y[k]);
             if (lane == 0) {
                 st.minus[bh * st.pitch + r] = lse[k] == -INFINITY ? -INFINITY : fmaf(lse[k], -kLog2e, SHIFT);
@@ -102,13 +111,21 @@ __global__ void __launch_bounds__(256, 4) k_attention_prepare(const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, largest[threadIdx.x][i]);
         // bits of numbers that are not negative are in their order; the largest does not depend on it
-        if (m > 0.0f) atomicMax(st.largest + (of_q ? threadIdx.x : 2), __float_as_uint(m));
+        if (m > 0.0f) atomicMax(of_q ? st.of_q + 2 * static_cast<int64_t>(bh) + threadIdx.x : st.of_v + bh, __float_as_uint(m));
     }
 }
 
-// The power of two that dS is multiplied by: 2^15 at most after it.
-__device__ __forceinline__ float gain_of(const Stats& st) {
-    const float g = __uint_as_float(st.largest[0]), o = __uint_as_float(st.largest[1]), v = __uint_as_float(st.largest[2]);
+// The power of two that the dS of n query heads (of all sequences' heads) of a kv head is multiplied by: 2^15 at
+// most after it.
+__device__ __forceinline__ float gain_of(const Stats& st, int head, int n, int kv_head) {
+    float g = 0.0f, o = 0.0f;
+    const float v = __uint_as_float(st.of_v[kv_head]);
+#pragma unroll 4
+    for (int i = head; i < head + n; ++i) {
+        const uint2 m = reinterpret_cast<const uint2*>(st.of_q)[i];
+        g = fmaxf(g, __uint_as_float(m.x));
+        o = fmaxf(o, __uint_as_float(m.y));
+    }
     const float bound = sqrtf(g) * (sqrtf(o) + sqrtf(v));
     if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
     int e;
@@ -344,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = (warp - 4) >> 2, quarter = warp & 3, k = k0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t s_at = lanes + 64 * w, dp_at = lanes + TILE + 64 * w;
-        const float c = p.scale * kLog2e, gain = gain_of(st), ds_gain = gain * exp2f(-SHIFT);
+        const float c = p.scale * kLog2e, gain = gain_of(st, b * p.Hq + hk * p.G, p.G, b * p.Hk + hk), ds_gain = gain * exp2f(-SHIFT);
         const int last_key = min(k0 + TILE, seq.nk) - 1;
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
@@ -602,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane, q = q0 + lane_row;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t dp_at = lanes + 2 * TILE + 64 * w;
-        const float c = p.scale * kLog2e, gain = gain_of(st);
+        const float c = p.scale * kLog2e, gain = gain_of(st, bh, 1, b * p.Hk + hk);
         const int64_t at = (static_cast<int64_t>(b) * p.Hq + h) * st.pitch + q;
         const float minus = st.minus[at] - SHIFT + log2f(gain);  // P is wanted times the power of two alone
         float delta = st.delta[at];
@@ -737,12 +754,14 @@ qsml_status_t backward_tc(Context* ctx, const Problem& p) {
     Stats st;
     st.pitch = (p.Sq + TILE - 1) / TILE * static_cast<int64_t>(TILE);
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hq * st.pitch;
+    const int64_t norms = static_cast<int64_t>(p.B) * (2 * static_cast<int64_t>(p.Hq) + p.Hk);
     void* m = nullptr;
-    QSML_TRY_STATUS(ws.get(sizeof(float) * (2 * rows + 4), &m));
-    st.minus = static_cast<float*>(m);
+    QSML_TRY_STATUS(ws.get(sizeof(float) * (2 * rows + norms), &m));
+    st.minus = static_cast<float*>(m);  // rows is a multiple of 128
     st.delta = st.minus + rows;
-    st.largest = reinterpret_cast<unsigned*>(st.delta + rows);
-    QSML_TRY_STATUS(check_cuda(ctx, cudaMemsetAsync(st.largest, 0, 3 * sizeof(unsigned), ctx->stream), "qsml_attention_backward"));
+    st.of_q = reinterpret_cast<unsigned*>(st.delta + rows);
+    st.of_v = st.of_q + 2 * static_cast<int64_t>(p.B) * p.Hq;
+    QSML_TRY_STATUS(check_cuda(ctx, cudaMemsetAsync(st.of_q, 0, norms * sizeof(unsigned), ctx->stream), "qsml_attention_backward"));
     const int64_t qblocks = rows / TILE, vblocks = static_cast<int64_t>(p.B) * p.Hk * ((p.Sk + TILE - 1) / TILE);
     if (qblocks + vblocks > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention_backward: dimensions too large");
     const cudaError_t e = launch_pdl(k_attention_prepare, dim3(static_cast<unsigned>(qblocks + vblocks)), dim3(256), 0, ctx->stream, p, st,
