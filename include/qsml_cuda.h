@@ -533,10 +533,12 @@ QSML_API qsml_status_t qsml_norm_rotary_backward(qsml_ctx* ctx, const qsml_tdesc
  * sequence's last, give 0 and -inf.  What lies behind a sequence's last key is not
  * used, whatever its bits; a key that a row does not see, but rows next to it do
  * (by window or position), has to be finite in v.
- * Scores, sums and norms are binary32; F16 weights of the values (the
- * exponentials) are rounded to F16 between the two products, and the tensor core's
- * accumulator truncates: a sum of 8192 values of one sign loses 5e-5 of itself, of
- * 131072 8e-4.  Outputs may not overlap inputs or each other.  Workspace as for qsml_layer_norm_backward.
+ * Scores, sums and norms are binary32, weights below 2^-126 of a row's largest are 0; F16 weights of
+ * the values (the exponentials) are rounded to F16 between the two products.  The tensor core's
+ * accumulator truncates: a sum of 8192 values of one sign loses 5e-5 of itself.  Longer sums are added
+ * up from such parts in binary32 (beyond 4 million keys, with few queries, from longer ones).
+ * Outputs may not overlap inputs or each other.  Workspace as for qsml_layer_norm_backward; D floats a
+ * query and head of it where a query can see more than 8192 keys.
  * No reference counterpart. */
 QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k, const qsml_tdesc* v,
                                       const qsml_tdesc* q_lengths, const qsml_tdesc* k_lengths, float scale,
@@ -554,7 +556,8 @@ QSML_API qsml_status_t qsml_attention(qsml_ctx* ctx, const qsml_tdesc* q, const 
  * between the products, dS times a power of two that keeps it in range, from the largest
  * finite |dout|, |o| and |v| of its sequence and head (for dk, of its group of heads); where all
  * the keys that a row sees are close together, sum(P dP) stands for the equal
- * sum(dout o), whose o has been rounded.  No sum depends on the order in which CTAs
+ * sum(dout o), whose o has been rounded.  dk and dv, which add up the queries of a group's heads, and
+ * dq are summed in parts as o is.  No sum depends on the order in which CTAs
  * finish: the same bits at every call. */
 QSML_API qsml_status_t qsml_attention_backward(qsml_ctx* ctx, const qsml_tdesc* q, const qsml_tdesc* k,
                                                const qsml_tdesc* v, const qsml_tdesc* o, const qsml_tdesc* lse,

@@ -100,8 +100,9 @@ struct Parts {
 qsml_status_t get_parts(Context* ctx, Workspace* ws, const Problem& p, int64_t parts, Parts* out);
 // o and lse from the parts, in their order (attention_few.cu).
 qsml_status_t join_parts(Context* ctx, const Problem& p, const Parts& parts);
-// Parts of a row's keys for `groups` CTAs, of which a SM holds `resident`, each part of `least` keys or more.
-int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least);
+// Parts of a row's keys for `groups` CTAs, of which a SM holds `resident`, each part of `least` keys or more and,
+// as far as that many parts can be joined, of `longest` or less.
+int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least, int64_t longest);
 // Few queries over many keys: binary16 on the tensor cores, where few_tc_takes (attention_few_tc.cu).
 bool few_tc_takes(const Problem& p);
 qsml_status_t forward_few_tc(Context* ctx, const Problem& p);

@@ -298,7 +298,7 @@ template <typename T, int DP, int RT> qsml_status_t run(Context* ctx, const Prob
     QSML_TRY_STATUS(check_cuda(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, S::SMEM), name));
     const int R = p.Sq * p.G, row_tiles = (R + RT - 1) / RT;
     const int64_t groups = static_cast<int64_t>(row_tiles) * p.Hk * p.B;
-    const int64_t n = few_parts(ctx, p, groups, std::max(resident, 1), 2 * S::KT);
+    const int64_t n = few_parts(ctx, p, groups, std::max(resident, 1), 2 * S::KT, INT64_MAX);
     if (groups * n > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     Workspace ws(ctx);
     Parts parts;
@@ -333,7 +333,7 @@ bool few_queries(const Problem& p) {
     return rows <= 16 || (rows <= 64 && p.Sk >= 4 * rows);
 }
 
-int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least) {
+int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, int least, int64_t longest) {
     // no row sees more keys than these
     const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (visible + least - 1) / least));
@@ -342,12 +342,13 @@ int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, 
     // 8192 keys 81, 79, 76, 85 us; 32 over 1000 43, 38, 38, 30; one over 32768 52, 42, 48, 35).
     constexpr double START = 512.0;
     const double slots = static_cast<double>(ctx->num_sms) * resident;
-    int64_t best = 1;
+    const int64_t fewest = std::max<int64_t>(1, std::min<int64_t>(most, visible / longest + (visible % longest != 0)));
+    int64_t best = fewest;
     double least_time = 0.0;
-    for (int64_t n = 1; n <= most; ++n) {
+    for (int64_t n = fewest; n <= most; ++n) {
         const double waves = static_cast<double>(groups * n) / slots;
         const double time = (p.nk ? waves + 1.0 : std::ceil(waves)) * (static_cast<double>(visible) / n + START);
-        if (n == 1 || time < least_time) best = n, least_time = time;
+        if (n == fewest || time < least_time) best = n, least_time = time;
     }
     return best;
 }

@@ -251,7 +251,8 @@ template <int DP> qsml_status_t run(Context* ctx, const Problem& p) {
     const int64_t groups = static_cast<int64_t>(row_tiles) * p.Hk * p.B;
     // a SM holds three CTAs; parts for two leave room for the ends of long sequences (16 over 8192 keys:
     // 105 us, parts for three 119; one over 32768: 35 and 45)
-    const int64_t n = few_parts(ctx, p, groups, 2, kWarps * KT);
+    // a warp's accumulators take no more than 8192 keys: they truncate (32768 keys of one sign: 2e-4 of the sum)
+    const int64_t n = few_parts(ctx, p, groups, 2, kWarps * KT, kWarps * 8192);
     if (groups * n > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
     Workspace ws(ctx);
     Parts parts;

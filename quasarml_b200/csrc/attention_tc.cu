@@ -39,9 +39,9 @@ struct FwdMaps {
     HeadMap q, k, v;
 };
 
-template <int DP>
+template <int DP, bool LONG>
 __global__ void __launch_bounds__(kThreads, 2)
-    k_attention_tc(const __grid_constant__ Problem p, const __grid_constant__ FwdMaps maps, int tiles, int* status) {
+    k_attention_tc(const __grid_constant__ Problem p, const __grid_constant__ FwdMaps maps, int tiles, float* kept, int* status) {
     using L = Fwd<DP>;
     constexpr int BYTES = TileOf<DP>::BYTES, STAGES = L::STAGES, PARTS = L::PARTS;
     extern __shared__ unsigned char smem_raw[];
@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const Keys keys(p, seq.nk, q0 + off, min(q0 + TILE, seq.nq) - 1 + off);
     const Tiles list(keys, TILE);
     const int steps = q0 < seq.nq ? list.n : 0;
+    auto fresh = [](int n) { return LONG ? n % DRAIN == 0 : n == 0; };  // whether O begins with step n
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::FEW));
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                         ok = ok && warp_wait(p_full(part), (n - 1) & 1, abort_flag, limit);
                         if (!ok) break;
                         tc_fence_after();
-                        mma_sums<DP, N>(issue, tmem + TILE, tmem + part * N / 2, desc_on(x, part * N * 128), n > 1 || part > 0);
+                        mma_sums<DP, N>(issue, tmem + TILE, tmem + part * N / 2, desc_on(x, part * N * 128), !fresh(n - 1) || part > 0);
                     }
                     if (!ok) break;
                     if (issue) mma_commit(empty(slot(v)));
@@ -192,13 +193,19 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int pos = q + off;
         const int row_hi = q < seq.nq ? pos : -1, row_lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
         const int first_pos = q0 + off, last_pos = min(q0 + TILE, seq.nq) - 1 + off;
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f, m_kept = -INFINITY;  // m_kept: the maximum that the kept row goes by
+        auto kept_row = [&] { return kept_at(kept + (static_cast<int64_t>(bh) * tiles + q0 / TILE) * TILE * p.D, q - q0, 0); };
+        auto kept_factor = [&] { return m_kept == m ? 1.0f : exp2_fast((m_kept - m) * c); };
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
             const int k0 = list.tile(n) * TILE;
             ok = warp_wait(s_full, n & 1, abort_flag, limit);
             if (!ok) break;
             tc_fence_after();
+            if (LONG && n > 0 && fresh(n)) {  // P V of the steps before had been added when S came
+                keep_sums<DP>(o_at, kept_row(), p.D, n == DRAIN, kept_factor());
+                m_kept = m;
+            }
             uint32_t r[TILE];
 #pragma unroll
             for (int g = 0; g < TILE; g += 32) tmem_ld32_start(s_at + g, r + g);
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const float f = grow ? exp2_fast((m - top) * c) : 1.0f;
                 if (grow) m = top;
                 l *= f;
-                if (n > 0) {  // the P V before had been added when S came
+                if (!fresh(n)) {  // the P V before had been added when S came
 #pragma unroll
                     for (int d = 0; d < DP; d += 32) {
                         uint32_t o[32];
@@ -279,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             __half* to = q < p.Sq ? reinterpret_cast<__half*>(p.o.p) + b * p.o.b + q * p.o.s + h * p.o.h : nullptr;
             const bool any = l > 0.0f || isnan(l);
             if (begun)
-                store_row<DP>(o_at, any ? 1.0f / l : 0.0f, to, p.D);
+                store_row<DP>(o_at, any ? 1.0f / l : 0.0f, to, p.D, LONG && steps > DRAIN ? kept_row() : nullptr, LONG ? kept_factor() : 1.0f);
             else if (to)
                 zero_row(to, p.D);
             if (p.lse && q < p.Sq)
@@ -302,12 +309,15 @@ template <int DP> qsml_status_t forward(Context* ctx, const Problem& p) {
         !make_head_map(&maps.v, p.v, p.D, p.Sk, p.Hk, p.B))
         return set_error(ctx, QSML_E_CUDA, "qsml_attention: cuTensorMapEncodeTiled failed");
     const char* name = "k_attention_tc";
-    const auto kernel = k_attention_tc<DP>;
     const int tiles = (p.Sq + TILE - 1) / TILE;
     if (static_cast<int64_t>(tiles) * p.Hq * p.B > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");
+    Workspace ws(ctx);
+    float* kept = nullptr;
+    QSML_TRY_STATUS(get_kept(&ws, p, &kept));
+    const auto kernel = kept ? k_attention_tc<DP, true> : k_attention_tc<DP, false>;
     QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::SMEM)), name));
     const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * p.Hq * p.B)), dim3(kThreads), L::SMEM, ctx->stream, p, maps, tiles,
-                                     ctx->status);
+                                     kept, ctx->status);
     if (e != cudaSuccess) return check_cuda(ctx, e, name);
     return after_launch(ctx, name);
 }

@@ -7,6 +7,8 @@
 // A operand from TMEM, where the threads that compute them leave them as pairs of binary16.
 #pragma once
 
+#include <algorithm>
+
 #include "attention.cuh"
 #include "packed.cuh"
 #include "tcgen05.cuh"
@@ -179,14 +181,72 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)) != 0;
 }
 
-// A row of binary32 sums in TMEM, times f, as binary16 to `to` (null: nowhere), D columns.
-template <int DP> __device__ __forceinline__ void store_row(uint32_t taddr, float f, __half* to, int D) {
+// The accumulator truncates: a sum of 8192 numbers of one sign loses 5e-5 of itself, of 131072 9e-4 (an
+// output's rounding is 4.9e-4).  Sums over more than DRAIN tiles leave it every DRAIN tiles for binary32 sums
+// in memory, by kernels of their own (LONG): the others are 0.5 to 2 % slower with the branches, 32768 tokens
+// of 8 heads over 2 take 1.85 -> 1.89 ms, their gradients 6.8 -> 7.0.  A tile's are [D / 4][128 rows][4], so that a
+// warp's 16 bytes a lane lie together; only the row's own thread uses them.
+constexpr int DRAIN = 64;
+// Tiles of keys that a tile of queries meets, at most.
+inline int64_t most_key_tiles(const Problem& p) {
+    const int64_t all = (static_cast<int64_t>(p.Sk) + TILE - 1) / TILE;
+    return p.window ? std::min<int64_t>(all, p.window / TILE + 3 + (p.sinks + TILE - 1) / TILE) : all;
+}
+// Kept sums of all tiles of queries, [B][Hq][tiles], or null where none meets that many tiles of keys.
+inline qsml_status_t get_kept(Workspace* ws, const Problem& p, float** kept) {
+    *kept = nullptr;
+    if (most_key_tiles(p) <= DRAIN) return QSML_OK;
+    void* m = nullptr;
+    QSML_TRY_STATUS(ws->get(sizeof(float) * p.B * p.Hq * ((static_cast<size_t>(p.Sq) + TILE - 1) / TILE) * TILE * p.D, &m));
+    *kept = static_cast<float*>(m);
+    return QSML_OK;
+}
+// Column c (a multiple of 4) of a row of a tile's kept sums.
+__device__ __forceinline__ float* kept_at(float* tile, int row, int c) { return tile + c * TILE + row * 4; }
+// 32 columns of a row of sums in TMEM, of which n are in use, with g times what is kept of them (null: nothing).
+__device__ __forceinline__ void load_sums(uint32_t taddr, uint32_t (&r)[32], const float* kept, int n, float g) {
+    tmem_ld32_start(taddr, r);
+    tmem_wait(r);
+    if (kept) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 16) {  // in two batches: all at once cost registers that the steps use
+            float4 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e + 4 * i < n) y[i] = *reinterpret_cast<const float4*>(kept + (e + 4 * i) * TILE);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e + 4 * i < n) {
+                    const float z[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[e + 4 * i + k] = __float_as_uint(fmaf(z[k], g, __uint_as_float(r[e + 4 * i + k])));
+                }
+        }
+    }
+}
+// A row of sums, D columns from TMEM's, added to g times what is kept of it (first: nothing yet).
+template <int DP> __device__ __forceinline__ void keep_sums(uint32_t taddr, float* kept, int D, bool first, float g) {
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         if (c >= D) break;
         uint32_t r[32];
-        tmem_ld32_start(taddr + c, r);
-        tmem_wait(r);
+        load_sums(taddr + c, r, first ? nullptr : kept + c * TILE, D - c, g);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+            if (c + j < D)
+                *reinterpret_cast<float4*>(kept + (c + j) * TILE) =
+                    make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+    }
+}
+
+// A row of binary32 sums in TMEM, with g times what is kept of it (null: nothing), times f, as binary16 to `to`
+// (null: nowhere), D columns.
+template <int DP> __device__ __forceinline__ void store_row(uint32_t taddr, float f, __half* to, int D, const float* kept = nullptr, float g = 1.0f) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+        if (c >= D) break;
+        uint32_t r[32];
+        load_sums(taddr + c, r, kept ? kept + c * TILE : nullptr, D - c, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (to && c + 8 * j < D) {

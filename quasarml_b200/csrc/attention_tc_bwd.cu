@@ -174,16 +174,13 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// A row of sums in TMEM (none: zeros), times f, as binary32.
-template <int DP> __device__ __forceinline__ void store_sums(uint32_t at, bool any, float f, float* to, int D) {
+// A row of sums in TMEM (none: zeros), with what is kept of it (null: nothing), times f, as binary32.
+template <int DP> __device__ __forceinline__ void store_sums(uint32_t at, bool any, float f, float* to, int D, const float* kept) {
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         if (c >= D) break;
         uint32_t r[32];
-        if (any) {
-            tmem_ld32_start(at + c, r);
-            tmem_wait(r);
-        }
+        if (any) load_sums(at + c, r, kept ? kept + c * TILE : nullptr, D - c, 1.0f);
 #pragma unroll
         for (int j = 0; j < 32; j += 4)
             if (c + j < D)
@@ -199,9 +196,10 @@ struct BwdMaps {
 
 // The steps of a tile of keys (tiles of queries that see it, of all heads of the group) over several
 // CTAs: the tiles with sinks, which all later queries see, in `many` parts, the others in `few`.  A
-// part's dk and dv are binary32 tiles [128][D] each in `sum`, where its tile has more than one.
+// part's dk and dv are binary32 tiles [128][D] each in `sum`, where its tile has more than one; a part of
+// more than DRAIN steps keeps its sums in tiles of `kept` on the way.
 struct KeyParts {
-    float* sum;
+    float *sum, *kept;
     int many, few, sink_tiles, tiles;
     __host__ __device__ int64_t slots() const { return static_cast<int64_t>(sink_tiles) * many + static_cast<int64_t>(tiles - sink_tiles) * few; }
     __host__ __device__ int64_t slot(int tile) const {
@@ -216,7 +214,7 @@ template <int DP> struct Dkv {
     static constexpr size_t SMEM = 2 * size_t(TileOf<DP>::BYTES) + 2 * (STAGE + 1024) + 1024 + 8 * 16 + 16;
 };
 
-template <int DP>
+template <int DP, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attention_dkv(const __grid_constant__ Problem p, const __grid_constant__ BwdMaps maps, Stats st, KeyParts kp, int* status) {
     using L = Dkv<DP>;
@@ -271,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Queries qs(p, seq, k0, k0 + TILE);
     const int t0 = qs.lo / TILE, per = qs.hi > qs.lo ? (qs.hi + TILE - 1) / TILE - t0 : 0;  // tiles of queries a head
     const int share = (per * p.G + parts - 1) / parts, step0 = min(part * share, per * p.G), steps = min(share, per * p.G - step0);
+    auto fresh = [](int n) { return LONG ? n % DRAIN == 0 : n == 0; };  // whether the sums begin with step n
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
@@ -321,13 +320,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool issue = elect_one();
             bool ok = warp_wait(kv_full, 0, abort_flag, limit);
             const uint64_t kd = score_desc(k_tile), vd = score_desc(v_tile);
-            // x += a operand in two halves as they come, times a tile
+            // x += a operand in two halves as they come, times a tile.  Where the sums begin anew, warpgroup 0 has
+            // moved dV and warpgroup 1 dK before their P of the step was ready
             auto sums = [&](uint32_t d, uint32_t a, uint32_t tile, uint32_t bar, int n) {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     if (!warp_wait(bar + 8 * w, n & 1, abort_flag, limit)) return false;
                     tc_fence_after();
-                    mma_sums<DP, 64>(issue, d, a + 64 * w, desc_on(sum_desc<DP>(tile), w * 64 * 128), n > 0 || w > 0);
+                    mma_sums<DP, 64>(issue, d, a + 64 * w, desc_on(sum_desc<DP>(tile), w * 64 * 128), !fresh(n) || w > 0);
                 }
                 return true;
             };
@@ -363,11 +363,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t s_at = lanes + 64 * w, dp_at = lanes + TILE + 64 * w;
         const float c = p.scale * kLog2e, gain = gain_of(st, b * p.Hq + hk * p.G, p.G, b * p.Hk + hk), ds_gain = gain * exp2f(-SHIFT);
         const int last_key = min(k0 + TILE, seq.nk) - 1;
+        // a warpgroup each: dV and dK
+        const View& to = w ? p.dk : p.dv;
+        const uint32_t sums_at = lanes + 256 + w * DP;
+        const int64_t out_tile = (((static_cast<int64_t>(slot) * p.B + b) * p.Hk + hk) * 2 + w) * TILE * p.D;
+        auto kept_row = [&] { return kept_at(kp.kept + out_tile, k - k0, 0); };
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
             const int s = n & 1, q0 = (t0 + (step0 + n) % per) * TILE;
             const float *minus = stats + s * 256 + 64 * w, *delta = minus + 128;
             ok = warp_wait(s_full, n & 1, abort_flag, limit) && warp_wait(full(s), n >> 1 & 1, abort_flag, limit);
+            if (LONG && ok && n > 0 && fresh(n)) {  // dP^T comes after all sums of the step before
+                ok = warp_wait(dp_full, n & 1, abort_flag, limit);
+                if (!ok) break;
+                tc_fence_after();
+                keep_sums<DP>(sums_at, kept_row(), p.D, n == DRAIN, 1.0f);
+            }
             if (!ok) break;
             tc_fence_after();
             uint32_t r[64];
@@ -417,16 +428,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok && steps > 0) ok = warp_wait(sums_full, 0, abort_flag, limit);
         tc_fence_after();
-        // a warpgroup each: dV and dK
-        const View& to = w ? p.dk : p.dv;
+        const float* prior = LONG && steps > DRAIN ? kept_row() : nullptr;
+        const float f = w ? p.scale / gain : exp2f(-SHIFT);
         if (ok && parts > 1) {
-            float* row = kp.sum + (((static_cast<int64_t>(slot) * p.B + b) * p.Hk + hk) * 2 + w) * TILE * p.D + static_cast<int64_t>(k - k0) * p.D;
-            store_sums<DP>(lanes + 256 + w * DP, steps > 0, w ? p.scale / gain : exp2f(-SHIFT), row, p.D);
+            store_sums<DP>(sums_at, steps > 0, f, kp.sum + out_tile + static_cast<int64_t>(k - k0) * p.D, p.D, prior);
         } else if (ok && to.p) {
             __half* row = k < p.Sk ? reinterpret_cast<__half*>(to.p) + b * to.b + k * to.s + hk * to.h : nullptr;
             if (steps > 0) {
                 const bool live = k < seq.nk;
-                store_row<DP>(lanes + 256 + w * DP, w ? p.scale / gain : exp2f(-SHIFT), live ? row : nullptr, p.D);
+                store_row<DP>(sums_at, f, live ? row : nullptr, p.D, prior);
                 if (row && !live) zero_row(row, p.D);
             } else if (row) {
                 zero_row(row, p.D);
@@ -477,9 +487,9 @@ template <int DP> struct Dq {
     static_assert(SMEM <= 232448, "shared memory");
 };
 
-template <int DP>
+template <int DP, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attention_dq(const __grid_constant__ Problem p, const __grid_constant__ BwdMaps maps, Stats st, int tiles, int* status) {
+    k_attention_dq(const __grid_constant__ Problem p, const __grid_constant__ BwdMaps maps, Stats st, int tiles, float* kept, int* status) {
     using L = Dq<DP>;
     constexpr int BYTES = TileOf<DP>::BYTES;
     extern __shared__ unsigned char smem_raw[];
@@ -529,6 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Keys keys(p, seq.nk, q0 + off, min(q0 + TILE, seq.nq) - 1 + off);
     const Tiles list(keys, TILE);
     const int steps = q0 < seq.nq ? list.n : 0;
+    auto fresh = [](int n) { return LONG ? n % DRAIN == 0 : n == 0; };  // whether dQ begins with step n
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
@@ -596,12 +607,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             ok = ok && begin_s(0) && begin_dp(0) && (steps == 1 || begin_s(1));
             for (int n = 0; n < steps && ok; ++n) {
+                // both warpgroups have moved their columns of dQ
+                if (LONG && n > 0 && fresh(n)) ok = warp_wait(ds_ready(1), n & 1, abort_flag, limit);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     ok = ok && warp_wait(ds_ready(w), n & 1, abort_flag, limit);
                     if (!ok) break;
                     tc_fence_after();
-                    mma_sums<DP, 64>(issue, tmem + 3 * TILE, tmem + 2 * TILE + 64 * w, desc_on(sum_desc<DP>(slot(0, n)), w * 64 * 128), n > 0 || w > 0);
+                    mma_sums<DP, 64>(issue, tmem + 3 * TILE, tmem + 2 * TILE + 64 * w, desc_on(sum_desc<DP>(slot(0, n)), w * 64 * 128), !fresh(n) || w > 0);
                 }
                 if (!ok) break;
                 if (issue) mma_commit(empty(0, n));
@@ -625,10 +638,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         float delta = st.delta[at];
         const int pos = q + off, first_pos = q0 + off, last_pos = min(q0 + TILE, seq.nq) - 1 + off;
         const int row_hi = q < seq.nq ? pos : -1, row_lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
+        // a warpgroup has half of the columns of dQ
+        const int c0 = w * DP / 2, cols = min(p.D - c0, DP / 2);
+        const uint32_t dq_at = lanes + 3 * TILE + c0;
+        auto kept_row = [&] { return kept_at(kept + (static_cast<int64_t>(bh) * tiles + q0 / TILE) * TILE * p.D, lane_row, c0); };
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
             const int k0 = list.tile(n) * TILE;
             ok = warp_wait(s_full(n), n >> 1 & 1, abort_flag, limit);
+            if (LONG && ok && n > 0 && fresh(n)) {  // dP comes after the sums of the step before
+                ok = warp_wait(dp_full, n & 1, abort_flag, limit);
+                if (!ok) break;
+                tc_fence_after();
+                if (cols > 0) keep_sums<DP / 2>(dq_at, kept_row(), cols, n == DRAIN, 1.0f);
+            }
             if (!ok) break;
             tc_fence_after();
             uint32_t r[64];
@@ -676,15 +699,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok && steps > 0) ok = warp_wait(sums_full, 0, abort_flag, limit);
         tc_fence_after();
-        if (ok && p.dq.p) {  // a warpgroup stores half of the columns
+        if (ok && p.dq.p) {
             __half* row = q < p.Sq ? reinterpret_cast<__half*>(p.dq.p) + b * p.dq.b + q * p.dq.s + h * p.dq.h : nullptr;
-            const int c0 = w * DP / 2, n = min(p.D - c0, DP / 2);
             if (steps > 0) {
                 const bool live = q < seq.nq;
-                if (n > 0) store_row<DP / 2>(lanes + 3 * TILE + c0, p.scale / gain, live && row ? row + c0 : nullptr, n);
-                if (row && !live && n > 0) zero_row(row + c0, n);
-            } else if (row && n > 0) {
-                zero_row(row + c0, n);
+                if (cols > 0)
+                    store_row<DP / 2>(dq_at, p.scale / gain, live && row ? row + c0 : nullptr, cols, LONG && steps > DRAIN ? kept_row() : nullptr);
+                if (row && !live && cols > 0) zero_row(row + c0, cols);
+            } else if (row && cols > 0) {
+                zero_row(row + c0, cols);
             }
         }
     }
@@ -713,12 +736,16 @@ template <int DP> qsml_status_t backward(Context* ctx, const Problem& p, const S
         return set_error(ctx, QSML_E_CUDA, "qsml_attention_backward: cuTensorMapEncodeTiled failed");
     // first, as it takes the deltas of rows with few keys
     const int tq = (p.Sq + TILE - 1) / TILE, tk = (p.Sk + TILE - 1) / TILE;
-    if (p.dq.p || p.dk.p)
-        QSML_TRY_STATUS(launch(ctx, k_attention_dq<DP>, "k_attention_dq", Dq<DP>::SMEM, static_cast<int64_t>(tq) * p.Hq * p.B, p, maps, st, tq, ctx->status));
+    Workspace ws(ctx);
+    if (p.dq.p || p.dk.p) {
+        float* kept = nullptr;
+        if (p.dq.p) QSML_TRY_STATUS(get_kept(&ws, p, &kept));
+        QSML_TRY_STATUS(launch(ctx, kept ? k_attention_dq<DP, true> : k_attention_dq<DP, false>, "k_attention_dq", Dq<DP>::SMEM, static_cast<int64_t>(tq) * p.Hq * p.B, p, maps, st, tq, kept, ctx->status));
+    }
     if (!p.dk.p && !p.dv.p) return QSML_OK;
     // Parts of about as many steps each, so that the CTAs are three waves: with a tile a CTA the one with
     // the sinks took as long as all else (2 x 4096 tokens of 16 heads over 2, window 2048: 540 us).
-    KeyParts kp{nullptr, 1, 1, p.window ? std::min((p.sinks + TILE - 1) / TILE, tk) : 0, tk};
+    KeyParts kp{nullptr, nullptr, 1, 1, p.window ? std::min((p.sinks + TILE - 1) / TILE, tk) : 0, tk};
     const int64_t bh = static_cast<int64_t>(p.B) * p.Hk, most = static_cast<int64_t>(p.G) * tq;
     const int64_t usual = p.window ? std::min(most, static_cast<int64_t>(p.G) * (p.window / TILE + 2)) : most;
     const int64_t total = bh * (kp.sink_tiles * most + (tk - kp.sink_tiles) * usual);
@@ -726,14 +753,18 @@ template <int DP> qsml_status_t backward(Context* ctx, const Problem& p, const S
     auto parts = [&](int64_t steps) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, steps / chunk))); };
     kp.many = parts(most);
     kp.few = parts(usual);
-    Workspace ws(ctx);
     const bool split = kp.few > 1 || (kp.sink_tiles && kp.many > 1);
-    if (split) {
+    // the steps that a part may have
+    auto longest = [&](int64_t steps, int n) { return (steps + n - 1) / n; };
+    const int64_t reach = p.window ? std::min<int64_t>(most, static_cast<int64_t>(p.G) * (p.window / TILE + 3)) : most;
+    const bool drained = longest(reach, kp.few) > DRAIN || (kp.sink_tiles && longest(most, kp.many) > DRAIN);
+    for (float** to : {split ? &kp.sum : nullptr, drained ? &kp.kept : nullptr}) {
         void* m = nullptr;
+        if (!to) continue;
         QSML_TRY_STATUS(ws.get(sizeof(float) * kp.slots() * bh * 2 * TILE * p.D, &m));
-        kp.sum = static_cast<float*>(m);
+        *to = static_cast<float*>(m);
     }
-    QSML_TRY_STATUS(launch(ctx, k_attention_dkv<DP>, "k_attention_dkv", Dkv<DP>::SMEM, kp.slots() * bh, p, maps, st, kp, ctx->status));
+    QSML_TRY_STATUS(launch(ctx, drained ? k_attention_dkv<DP, true> : k_attention_dkv<DP, false>, "k_attention_dkv", Dkv<DP>::SMEM, kp.slots() * bh, p, maps, st, kp, ctx->status));
     if (!split) return QSML_OK;
     if (4 * tk * bh > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention_backward: dimensions too large");
     const int tiles = kp.few > 1 ? tk : kp.sink_tiles;
