@@ -22,7 +22,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename T, int DP, int RT> struct Shape {
     static constexpr int V = 16 / sizeof(T);
-    static constexpr int KT = sizeof(T) * DP >= 512 ? 32 : 64;  // keys a tile: two stages and three CTAs a SM
+    // keys a tile, in two stages: one CTA a SM for binary32 heads of 256 columns, two to five for the others
+    static constexpr int KT = sizeof(T) * DP >= 512 ? 32 : 64;
     static constexpr int LD = DP + V;  // elements between rows: lanes' 16-byte loads 8 by 8 in no bank
     static constexpr int TILE = KT * LD * sizeof(T);
     static constexpr size_t SMEM = 4 * TILE + sizeof(float) * (RT * DP + RT * KT + 3 * RT);
@@ -338,8 +339,10 @@ int64_t few_parts(Context* ctx, const Problem& p, int64_t groups, int resident, 
     const int64_t visible = p.window ? std::min<int64_t>(p.Sk, static_cast<int64_t>(p.window) + p.sinks + p.Sq) : p.Sk;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (visible + least - 1) / least));
     // The time of n parts: waves of CTAs (whole ones, where all are alike), each of a part's keys and
-    // of what a CTA takes besides, as long as START keys (128, 256, 512 and 1024 measured: 16 sequences over up to
-    // 8192 keys 81, 79, 76, 85 us; 32 over 1000 43, 38, 38, 30; one over 32768 52, 42, 48, 35).
+    // of what a CTA takes besides, as long as START keys (128, 256, 512 and 1024 measured, each call on keys out of
+    // L2: binary16 of 8 heads of 128, 16 sequences over 1 to 8192 keys 69, 67, 73, 73 us; 8 over 1 to 16384 62, 59, 57,
+    // 64; 64 over 1 to 2048 71, 71, 71, 65; 64 over 2048 of 16 heads of 64 102, 102, 90, 90; binary32, 5 over 1 to
+    // 8192 of 8 heads of 64 54, 56, 50, 67; one sequence, and 4 over 4096, the same with each).
     constexpr double START = 512.0;
     const double slots = static_cast<double>(ctx->num_sms) * resident;
     const int64_t fewest = std::max<int64_t>(1, std::min<int64_t>(most, visible / longest + (visible % longest != 0)));

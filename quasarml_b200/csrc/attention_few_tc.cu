@@ -8,8 +8,8 @@
 // permuted by the row so that ldmatrix meets no bank twice), so there is no barrier until the
 // warps' sums are joined at the end; parts of a row's keys are joined as in attention_few.cu.
 // P is 2^(s c - m c + 8), which keeps small weights in binary16's normal range.  Measured: 64 sequences
-// over 2048 keys of 16 heads of 64 (537 MB) 84 us, 0.97 of the copy's rate; 16 over 1 to 8192 keys of 8 heads
-// of 128 (304 MB) 77 us, with their first loads and last joins in the open.
+// over 2048 keys of 16 heads of 64 (537 MB) 90 us, 0.91 of the copy's rate; 16 over 1 to 8192 keys of 8 heads
+// of 128 (304 MB) 73 us, with their first loads and last joins in the open.
 #include <algorithm>
 
 #include "attention.cuh"
@@ -249,8 +249,8 @@ template <int DP> qsml_status_t run(Context* ctx, const Problem& p) {
     QSML_TRY_STATUS(check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), name));
     const int row_tiles = (p.Sq * p.G + 15) / 16;
     const int64_t groups = static_cast<int64_t>(row_tiles) * p.Hk * p.B;
-    // a SM holds three CTAs; parts for two leave room for the ends of long sequences (16 over 8192 keys:
-    // 105 us, parts for three 119; one over 32768: 35 and 45)
+    // A SM holds three CTAs; parts for two are fewer to join: one sequence over 8192 keys 18 us (parts for three
+    // 22), over 32768 33 (37), 4 over 4096 23 (24); but 16 over 8192 each 124 (90), whose last wave is short.
     // a warp's accumulators take no more than 8192 keys: they truncate (32768 keys of one sign: 2e-4 of the sum)
     const int64_t n = few_parts(ctx, p, groups, 2, kWarps * KT, kWarps * 8192);
     if (groups * n > INT32_MAX) return set_error(ctx, QSML_E_UNSUPPORTED, "qsml_attention: dimensions too large");

@@ -18,7 +18,8 @@
 // A row whose keys are all in one tile takes delta = sum(P dP) instead of sum(dout o): with a few
 // keys the rounding of o would be the largest error of dq and dk (alone 0.00033 of their norm, where
 // their own rounding is 0.00021).  Measured, 2 x 4096 tokens of 16 heads over 2 with 128 columns, window
-// 2048: 417 us, dkv 241 (a step 3560 cycles) and dq 184 (2600).
+// 2048: 424 us in short runs, dkv 241 (a step 3560 cycles) and dq 184 (2600); 467 back to back, under the power
+// cap.  With 128 columns both kernels reload spilled registers, dq 248 bytes and dkv 108.
 #include <algorithm>
 
 #include "attention_tc.cuh"

@@ -29,8 +29,9 @@ using heads::View;
 
 // Threads of a CTA, at most, and CTAs a SM that registers are to be had for.  Forward: 80 registers, 81 us
 // of 16384 tokens of 40 heads of 128 in binary16 (4 x 192 threads 80, 5 x 160 82, 6 x 160 90, and 109 with two
-// rows on their way instead of one).  Backward: 128, without spills, 122 us (2 x 320 threads 154, 4 x 128
-// 131).
+// rows on their way instead of one).  Backward: 128, for these heads without spills, 122 us (2 x 320 threads 154,
+// 4 x 128 131); the kernels of wide heads (binary32 beyond 256 columns, and those that no vector fits beyond 128)
+// spill 96 to 204 bytes.
 constexpr int most_threads(bool backward) { return backward ? 160 : 384; }
 constexpr int least_ctas(bool backward) { return backward ? 3 : 2; }
 constexpr int kMaxAxes = 4;
