@@ -208,3 +208,39 @@ def test_waits_that_run_out_in_long_sums():
     for x, y in zip(run(c, q, k, v, do, 0.125), want):
         assert torch.equal(x, y)
     c.close()
+
+
+def test_long_sums_in_two_graphs(ctx):
+    """Two captured graphs, replayed together with eager calls between, keep the bits: each has rows of its own."""
+    import torch
+    q, k, v, do = tensors(1, 260, 20000, 2, 1, 64, 8, positive=False)
+    want = run(ctx, q, k, v, do, 0.125)
+    lse, sets = [torch.empty(1, 2, 260, device="cuda") for _ in range(3)], [[torch.empty_like(x) for x in (q, q, k, v)] for _ in range(3)]
+
+    def call(n):
+        o, *g = sets[n]
+        ctx.attention(d(q), d(k), d(v), d(o), 0.125, lse=d(lse[n]))
+        ctx.attention_backward(d(q), d(k), d(v), d(o), d(lse[n]), d(do), *[d(x) for x in g], 0.125)
+    own, graphs, streams = ctx.stream(), [], [torch.cuda.Stream() for _ in range(2)]
+    try:
+        for n, s in enumerate(streams):
+            ctx.set_stream(s.cuda_stream)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                call(n)
+            graphs.append(graph)
+        ctx.set_stream(own)
+        for _ in range(3):
+            for t in sum(sets, []):
+                t.fill_(NAN)
+            torch.cuda.synchronize()
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            call(2)
+            torch.cuda.synchronize()
+            for out in sets:
+                for x, y in zip(out, want):
+                    assert torch.equal(x, y)
+    finally:
+        ctx.set_stream(own)
